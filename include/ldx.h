@@ -40,7 +40,7 @@ extern "C" {
 
 /* Message of the calling thread's most recent failure ("" if none). */
 const char* ldx_last_error(void);
-/* ABI version (13); bumped on any change to the structs below or the entry points. */
+/* ABI version (14); bumped on any change to the structs below or the entry points. */
 int ldx_abi_version(void);
 
 /* ---------------------------------------------------------------- conv3d -------
@@ -403,6 +403,125 @@ int ldx_group_norm_source_half(const void* x, int64_t x_batch_stride, int64_t x_
                                float* affine, void* y, int64_t y_batch_stride, int64_t y_channel_stride,
                                int64_t y_voxel_stride, void* workspace, size_t workspace_bytes,
                                void* stream);
+
+/* ------------------------------------------------------------ 8-bit operators -------
+ * No counterpart in the reference, whose networks run in 16 and 32 bits.
+ *
+ * An 8-bit tensor is OCP e4m3 codes (largest number 448, code 0x7f NaN, no infinity) and one
+ * scale byte b (E8M0, 2^(b - 127)) for each block; a value is code * 2^(b - 127). The writers
+ * below take the least b >= 1 with which the block's largest magnitude is at most 448 *
+ * 2^(b - 127) and round to nearest even. NaN stays NaN and is not counted in the magnitude;
+ * an infinity becomes a NaN code.
+ *
+ * 8-bit rows: LDX_BLOCK8 columns of a row share a scale. codes: (rows, pitch) bytes, 16-byte
+ * aligned, pitch a multiple of 16 and at least the features rounded up to whole blocks; the
+ * columns that fill the last block are zero codes. scales: (rows, pitch) bytes, 4-byte
+ * aligned, pitch a multiple of 4 and at least the number of blocks rounded up to 4. */
+#define LDX_BLOCK8 128
+#define LDX_PAGE8 64
+
+/* s = T(x + residual) (without a residual x itself); y = s / sqrt(mean(s^2) + eps) * gamma,
+ * statistics in fp32; rounded to T (y) or written as 8-bit rows (codes, scales): one of the
+ * two. sum (may be NULL) receives s and may be x or residual; y may be x. x, residual, sum
+ * and y are of type dtype (T) with contiguous features, any alignment; gamma fp32, eps at
+ * least 1e-30. Rows whose squares pass fp32 although their values do not are normalised from
+ * scaled squares. */
+typedef struct ldx_rms_norm_args {
+  int64_t rows;
+  int32_t features;
+  int32_t dtype;
+  const void* x; int64_t x_pitch;
+  const void* residual; int64_t residual_pitch;
+  void* sum; int64_t sum_pitch;
+  const float* gamma;
+  float eps;
+  void* y; int64_t y_pitch;
+  void* codes; int64_t codes_pitch;
+  void* scales; int64_t scales_pitch;
+} ldx_rms_norm_args;
+int ldx_rms_norm(const ldx_rms_norm_args* args, void* stream);
+
+/* 8-bit rows of a tensor as it is. */
+int ldx_quantize8(const void* x, int64_t x_pitch, int64_t rows, int32_t features, int32_t dtype, void* codes,
+                  int64_t codes_pitch, void* scales, int64_t scales_pitch, void* stream);
+
+/* y[m, o] = act(sum_k x[m, k] w[o, k] + bias[o] + residual[m, o]) of 8-bit rows x (rows) and w
+ * (out_features), both with their scales per 128 columns of k. fp32 sums, one rounding to
+ * dtype. An fp16 or bf16 y comes from the e4m3 matrix instruction, which adds products in
+ * groups of eight cut at 2^-13 of the group's largest: its sum is within 2^-10 of the sum of
+ * the terms' magnitudes (about 1.5e-5 of the result's size for ordinary data). An fp32 y is
+ * summed from the operands as bf16 values, which hold them exactly. residual and y are of
+ * type dtype; bias fp32. */
+typedef struct ldx_dense8_args {
+  int64_t rows;
+  int32_t features, out_features;
+  const void* x_codes; int64_t x_pitch;
+  const void* x_scales; int64_t x_scales_pitch;
+  const void* w_codes; int64_t w_pitch;
+  const void* w_scales; int64_t w_scales_pitch;
+  const float* bias;
+  const void* residual; int64_t residual_pitch;
+  int32_t act;
+  int32_t dtype;
+  void* y; int64_t y_pitch;
+} ldx_dense8_args;
+int ldx_dense8(const ldx_dense8_args* args, void* stream);
+
+/* A cache of keys and values in pages of LDX_PAGE8 tokens, each page with one scale for a
+ * head's keys and one for its values: k codes (pages, heads, 64, head_dim), v codes (pages,
+ * heads, head_dim, 64) -- a channel's tokens side by side, as the product with the
+ * probabilities reads them -- and scales (pages, heads). All contiguous, the codes 16-byte
+ * aligned. head_dim 32, 64, 128 or 256. A sequence's pages stand in its row of `table` (int32,
+ * device; `width` pages a row), its token t in page table[b][t / 64] at t % 64. */
+typedef struct ldx_cache8 {
+  void* k; void* v;
+  void* k_scales; void* v_scales;
+  int32_t pages, heads, head_dim;
+} ldx_cache8;
+
+/* Writes tokens 0..counts[b] (counts NULL: all `tokens`) of k and v (batch, token, head strides
+ * in elements, contiguous channels, type dtype) at positions starts[b].. of each sequence. A
+ * page that holds older tokens (before starts[b]) keeps the larger of its scale and the one
+ * that the new tokens ask for; where it rises the older codes are rounded to it. A page whose
+ * first token is written takes the new tokens' scale. Codes behind the last written token
+ * stay as they are. Sequences that write must not share a page. Nothing is written of a
+ * sequence with starts[b] < 0, past the table's width, or in a page that the cache does not
+ * have. */
+typedef struct ldx_cache8_append_args {
+  ldx_cache8 cache;
+  int32_t batch, tokens;
+  const void* k; int64_t k_stride[3];
+  const void* v; int64_t v_stride[3];
+  int32_t dtype;
+  const int32_t* table; int64_t table_pitch; int32_t width;
+  const int32_t* starts;
+  const int32_t* counts;
+} ldx_cache8_append_args;
+int ldx_cache8_append(const ldx_cache8_append_args* args, void* stream);
+
+/* o = softmax(q k^T * scale) v over a sequence's first lengths[b] tokens of the cache; with
+ * starts, query i sees no token behind starts[b] + i (causal for queries at starts[b]..). q and
+ * o: (batch, token, head) strides, contiguous channels, fp16 or bf16; q_heads a multiple of
+ * the cache's heads, query head j reads the cache's head j / (q_heads / heads). fp32 scores,
+ * softmax and sums; probabilities are rounded to fp16. A query that sees no token gets 0.
+ * Tokens that a query does not see do not touch its result, NaN among them. A page that the
+ * cache does not have gives NaN to the queries that see it, a length past the table to the
+ * whole sequence. Workspace: partial results where a sequence is split over workgroups,
+ * ldx_cache8_attention_workspace_bytes of them; with less nothing is split. */
+typedef struct ldx_cache8_attention_args {
+  ldx_cache8 cache;
+  int32_t batch, q_heads, q_len;
+  const void* q; int64_t q_stride[3];
+  void* o; int64_t o_stride[3];
+  int32_t dtype;
+  float scale;
+  const int32_t* table; int64_t table_pitch; int32_t width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  void* workspace; size_t workspace_bytes;
+} ldx_cache8_attention_args;
+size_t ldx_cache8_attention_workspace_bytes(const ldx_cache8_attention_args* args);
+int ldx_cache8_attention(const ldx_cache8_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -22,6 +22,8 @@ ACT_SILU = 2
 DTYPE_F16 = 0
 DTYPE_F32 = 1
 DTYPE_BF16 = 2
+BLOCK8 = 128                         # LDX_BLOCK8
+PAGE8 = 64                           # LDX_PAGE8
 GROUP_NORM_SCRATCH_BYTES = 4 << 20   # LDX_GROUP_NORM_SCRATCH_BYTES
 
 c_i32 = ctypes.c_int32
@@ -82,6 +84,67 @@ class SourceConvArgs(ctypes.Structure):
     ]
 
 
+class RmsNormArgs(ctypes.Structure):
+    """Mirror of ``ldx_rms_norm_args``."""
+
+    _fields_ = [
+        ("rows", c_i64), ("features", c_i32), ("dtype", c_i32),
+        ("x", c_vp), ("x_pitch", c_i64),
+        ("residual", c_vp), ("residual_pitch", c_i64),
+        ("sum", c_vp), ("sum_pitch", c_i64),
+        ("gamma", c_vp), ("eps", c_f32),
+        ("y", c_vp), ("y_pitch", c_i64),
+        ("codes", c_vp), ("codes_pitch", c_i64),
+        ("scales", c_vp), ("scales_pitch", c_i64),
+    ]
+
+
+class Dense8Args(ctypes.Structure):
+    """Mirror of ``ldx_dense8_args``."""
+
+    _fields_ = [
+        ("rows", c_i64), ("features", c_i32), ("out_features", c_i32),
+        ("x_codes", c_vp), ("x_pitch", c_i64), ("x_scales", c_vp), ("x_scales_pitch", c_i64),
+        ("w_codes", c_vp), ("w_pitch", c_i64), ("w_scales", c_vp), ("w_scales_pitch", c_i64),
+        ("bias", c_vp), ("residual", c_vp), ("residual_pitch", c_i64),
+        ("act", c_i32), ("dtype", c_i32),
+        ("y", c_vp), ("y_pitch", c_i64),
+    ]
+
+
+class Cache8Block(ctypes.Structure):
+    """Mirror of ``ldx_cache8``."""
+
+    _fields_ = [
+        ("k", c_vp), ("v", c_vp), ("k_scales", c_vp), ("v_scales", c_vp),
+        ("pages", c_i32), ("heads", c_i32), ("head_dim", c_i32),
+    ]
+
+
+class Cache8AppendArgs(ctypes.Structure):
+    """Mirror of ``ldx_cache8_append_args``."""
+
+    _fields_ = [
+        ("cache", Cache8Block), ("batch", c_i32), ("tokens", c_i32),
+        ("k", c_vp), ("k_stride", c_i64 * 3), ("v", c_vp), ("v_stride", c_i64 * 3), ("dtype", c_i32),
+        ("table", c_vp), ("table_pitch", c_i64), ("width", c_i32),
+        ("starts", c_vp), ("counts", c_vp),
+    ]
+
+
+class Cache8AttentionArgs(ctypes.Structure):
+    """Mirror of ``ldx_cache8_attention_args``."""
+
+    _fields_ = [
+        ("cache", Cache8Block), ("batch", c_i32), ("q_heads", c_i32), ("q_len", c_i32),
+        ("q", c_vp), ("q_stride", c_i64 * 3), ("o", c_vp), ("o_stride", c_i64 * 3),
+        ("dtype", c_i32), ("scale", c_f32),
+        ("table", c_vp), ("table_pitch", c_i64), ("width", c_i32),
+        ("lengths", c_vp), ("starts", c_vp),
+        ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # name -> (restype, argtypes); every function declared in include/ldx.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ldx_last_error": (ctypes.c_char_p, []),
@@ -131,9 +194,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ldx_group_norm_source_half": (c_i32, [c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_i64, c_i32, c_vp, c_vp,
                                            c_f32, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, ctypes.c_size_t,
                                            c_vp]),
+    "ldx_rms_norm": (c_i32, [ctypes.POINTER(RmsNormArgs), c_vp]),
+    "ldx_quantize8": (c_i32, [c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "ldx_dense8": (c_i32, [ctypes.POINTER(Dense8Args), c_vp]),
+    "ldx_cache8_append": (c_i32, [ctypes.POINTER(Cache8AppendArgs), c_vp]),
+    "ldx_cache8_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Cache8AttentionArgs)]),
+    "ldx_cache8_attention": (c_i32, [ctypes.POINTER(Cache8AttentionArgs), c_vp]),
 }
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 
 def _load() -> ctypes.CDLL:

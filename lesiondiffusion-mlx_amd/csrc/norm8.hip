@@ -1,0 +1,296 @@
+// Root-mean-square norm with the residual's addition, into the input's type or into 8-bit rows, and
+// the same 8-bit rows of a tensor as it is.
+//
+//   s = T(x + residual)            (stored where asked for; x itself without a residual)
+//   y = s / sqrt(mean(s^2) + eps) * gamma
+//   y rounded to T, or per row and 128 columns to e4m3 codes and a power of two (quant8.h)
+//
+// One pass: a row's values stay in registers between the sum of squares and the output.
+#include "quant8.h"
+
+namespace ldx {
+namespace {
+
+struct NormArgs {
+  const void* x; int64_t xp;
+  const void* r; int64_t rp;      // residual or null
+  void* s; int64_t sp;            // sum or null
+  const float* gamma; float eps;  // null gamma: no norm
+  void* y; int64_t yp;            // T output or null
+  uint8_t* codes; int64_t cp;     // 8-bit output
+  uint8_t* scales; int64_t ep;
+  int64_t rows;
+  int C, kb;                      // features; 128-column blocks
+};
+
+// Sum / largest over a row's threads: a wave, or the four waves of the workgroup through red.
+template <int TPR, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float* red) {
+  v = MAX ? wave_max(v) : wave_sum(v);
+  if constexpr (TPR > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 64; i++) v = MAX ? fmaxf(v, red[i]) : v + red[i];
+  }
+  return v;
+}
+
+// Values c .. c + 7 of a row, zero past C; with a residual, the rounded sum (also stored).
+template <typename T>
+__device__ __forceinline__ void take8(const NormArgs& a, const T* x, const T* r, T* s, int c, float (&f)[8]) {
+  if (c + 8 <= a.C) {
+    load8(x + c, f);
+    if (r) {
+      float g[8];
+      load8(r + c, g);
+#pragma unroll
+      for (int i = 0; i < 8; i++) f[i] = (float)(T)(f[i] + g[i]);
+      if (s) store8(s + c, f);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    f[i] = 0.f;
+    if (c + i < a.C) {
+      f[i] = (float)x[c + i];
+      if (r) {
+        f[i] = (float)(T)(f[i] + (float)r[c + i]);
+        if (s) s[c + i] = (T)f[i];
+      }
+    }
+  }
+}
+
+// The output of values c .. c + 7: a 16-lane row holds a block of 128.
+template <typename T, bool NORM, bool Q8>
+__device__ __forceinline__ void give8(const NormArgs& a, int64_t row, int c, float rstd, float (&f)[8]) {
+  if constexpr (NORM) {
+    if (c + 8 <= a.C) {
+      float g[8];
+      load8(a.gamma + c, g);
+#pragma unroll
+      for (int i = 0; i < 8; i++) f[i] = f[i] * rstd * g[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (c + i < a.C) f[i] = f[i] * rstd * a.gamma[c + i];
+    }
+  }
+  if constexpr (Q8) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(f[i]));
+    m = row16_max(m);
+    const int b = scale_byte(m);
+    const float inv = inverse_of(b);
+    if (c < a.kb * kBlock8) {
+      const i32x2 w = {encode4(f[0], f[1], f[2], f[3], inv), encode4(f[4], f[5], f[6], f[7], inv)};
+      *reinterpret_cast<i32x2*>(a.codes + row * a.cp + c) = w;
+      if (c % kBlock8 == 0) a.scales[row * a.ep + c / kBlock8] = (uint8_t)b;
+    }
+  } else {
+    T* y = (T*)a.y + row * a.yp;
+    if (c + 8 <= a.C) {
+      store8(y + c, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (c + i < a.C) y[c + i] = (T)f[i];
+    }
+  }
+}
+
+// 1 / sqrt(mean + eps) of a row from its sum of squares, for values that are first multiplied by g: 1
+// but where the squares pass fp32 although the values do not (bf16 and fp32 beyond 2^64 / sqrt(C));
+// there the power of two that brings the largest value to 1..4, and the squares are taken again.
+template <int TPR, typename Square>
+__device__ __forceinline__ float row_rstd(const NormArgs& a, float ss, float amax, float* red, float& g,
+                                          Square squares) {
+  g = 1.f;
+  if (!(ss <= 3.0e38f)) {   // uniform over the row's threads
+    amax = row_reduce<TPR, true>(amax, red);
+    if (amax < __builtin_inff()) {
+      g = inverse_of(min(max(__float_as_int(amax) >> 23, 1), 253));
+      ss = row_reduce<TPR, false>(squares(g), red);
+    }
+  }
+  return 1.0f / sqrtf(ss / a.C + a.eps * g * g);
+}
+
+template <int N>
+__device__ __forceinline__ void times(float (&f)[N], float g) {
+  if (g != 1.f)
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] *= g;
+}
+
+// TPR threads a row, NCH groups of eight consecutive values each; NCH = 0 takes rows of any length and
+// reads them twice.
+template <typename T, int TPR, int NCH, bool NORM, bool Q8>
+__global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
+  __shared__ float red[4];
+  constexpr int RPB = 256 / TPR;
+  const int t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (RPB > 1 && row >= a.rows) return;   // whole waves: rows of several waves fill the workgroup
+  const T* x = (const T*)a.x + row * a.xp;
+  const T* r = a.r ? (const T*)a.r + row * a.rp : nullptr;
+  T* s = a.s ? (T*)a.s + row * a.sp : nullptr;
+  if constexpr (NCH > 0) {
+    float f[NCH][8];
+    float ss = 0.f, amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < NCH; k++) take8(a, x, r, s, (k * TPR + t) * 8, f[k]);
+    float rstd = 1.f, g = 1.f;
+    if constexpr (NORM) {
+#pragma unroll
+      for (int k = 0; k < NCH; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          ss += f[k][i] * f[k][i];
+          amax = fmaxf(amax, fabsf(f[k][i]));
+        }
+      ss = row_reduce<TPR, false>(ss, red);
+      rstd = row_rstd<TPR>(a, ss, amax, red, g, [&](float by) {
+        float q = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; k++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) q += (f[k][i] * by) * (f[k][i] * by);
+        return q;
+      });
+#pragma unroll
+      for (int k = 0; k < NCH; k++) times(f[k], g);
+    }
+#pragma unroll
+    for (int k = 0; k < NCH; k++) give8<T, NORM, Q8>(a, row, (k * TPR + t) * 8, rstd, f[k]);
+  } else {
+    // Whole workgroup rounds, so that the lanes of a block of 128 stay together.
+    const int rounds = (a.kb * kBlock8 + TPR * 8 - 1) / (TPR * 8);
+    float rstd = 1.f, g = 1.f;
+    if constexpr (NORM) {
+      float ss = 0.f, amax = 0.f, f[8];
+      for (int k = 0; k < rounds; k++) {
+        take8(a, x, r, s, (k * TPR + t) * 8, f);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          ss += f[i] * f[i];
+          amax = fmaxf(amax, fabsf(f[i]));
+        }
+      }
+      ss = row_reduce<TPR, false>(ss, red);
+      // Read again: the sum that this thread stored, since it may have been stored over x or r.
+      const T* x2 = r && s ? s : x;
+      const T* r2 = r && s ? nullptr : r;
+      rstd = row_rstd<TPR>(a, ss, amax, red, g, [&](float by) {
+        float q = 0.f, h[8];
+        for (int k = 0; k < rounds; k++) {
+          take8<T>(a, x2, r2, nullptr, (k * TPR + t) * 8, h);
+#pragma unroll
+          for (int i = 0; i < 8; i++) q += (h[i] * by) * (h[i] * by);
+        }
+        return q;
+      });
+      for (int k = 0; k < rounds; k++) {
+        take8<T>(a, x2, r2, nullptr, (k * TPR + t) * 8, f);
+        times(f, g);
+        give8<T, NORM, Q8>(a, row, (k * TPR + t) * 8, rstd, f);
+      }
+    } else {
+      float f[8];
+      for (int k = 0; k < rounds; k++) {
+        take8(a, x, r, s, (k * TPR + t) * 8, f);
+        give8<T, NORM, Q8>(a, row, (k * TPR + t) * 8, rstd, f);
+      }
+    }
+  }
+  if constexpr (Q8)   // the bytes that pad a row's scales to four: 1.0
+    if (t < (int)(-a.kb & 3)) a.scales[row * a.ep + a.kb + t] = 127;
+}
+
+template <typename T, bool NORM, bool Q8>
+void launch(const NormArgs& a, hipStream_t st) {
+  const int n = Q8 ? a.kb * kBlock8 : a.C;
+  const dim3 wide((unsigned)a.rows), narrow((unsigned)((a.rows + 3) / 4)), block(256);
+  if (n <= 512)
+    hipLaunchKernelGGL((norm8_kernel<T, 64, 1, NORM, Q8>), narrow, block, 0, st, a);
+  else if (n <= 1024)
+    hipLaunchKernelGGL((norm8_kernel<T, 64, 2, NORM, Q8>), narrow, block, 0, st, a);
+  else if (n <= 2048)
+    hipLaunchKernelGGL((norm8_kernel<T, 256, 1, NORM, Q8>), wide, block, 0, st, a);
+  else if (n <= 4096)
+    hipLaunchKernelGGL((norm8_kernel<T, 256, 2, NORM, Q8>), wide, block, 0, st, a);
+  else if (n <= 8192)
+    hipLaunchKernelGGL((norm8_kernel<T, 256, 4, NORM, Q8>), wide, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((norm8_kernel<T, 256, 0, NORM, Q8>), wide, block, 0, st, a);
+}
+
+template <bool NORM, bool Q8>
+int launch_any(const NormArgs& a, int dtype, hipStream_t st, const char* what) {
+  if (dtype == LDX_DTYPE_F16) launch<f16, NORM, Q8>(a, st);
+  else if (dtype == LDX_DTYPE_BF16) launch<bf16, NORM, Q8>(a, st);
+  else launch<float, NORM, Q8>(a, st);
+  return check_launch(what);
+}
+
+// Rows of `rows` elements apart by `pitch` within one allocation that int64 byte offsets reach.
+int check_rows(const char* what, int64_t rows, int64_t features, int dtype) {
+  if (dtype != LDX_DTYPE_F16 && dtype != LDX_DTYPE_BF16 && dtype != LDX_DTYPE_F32)
+    return fail("%s: dtype %d is not LDX_DTYPE_F16, LDX_DTYPE_BF16 or LDX_DTYPE_F32", what, dtype);
+  if (rows < 1 || rows > 0x7fffffff) return fail("%s: %lld rows", what, (long long)rows);
+  if (features < 1 || features > (1 << 28)) return fail("%s: %lld features", what, (long long)features);
+  return LDX_OK;
+}
+
+int check_codes(const char* what, const void* codes, int64_t cp, const void* scales, int64_t ep, int kb) {
+  if (!scales) return fail("%s: null pointer", what);
+  if (cp < (int64_t)kb * kBlock8 || cp % 16 || ep < ((kb + 3) & ~3) || ep % 4)
+    return fail("%s: pitches %lld, %lld do not hold %d blocks of %d", what, (long long)cp, (long long)ep, kb, kBlock8);
+  if ((uintptr_t)codes % 16 || (uintptr_t)scales % 4) return fail("%s: codes or scales not aligned", what);
+  return LDX_OK;
+}
+
+}  // namespace
+}  // namespace ldx
+
+using namespace ldx;
+
+extern "C" int ldx_rms_norm(const ldx_rms_norm_args* p, void* stream) {
+  if (!p || !p->x || !p->gamma || (!p->y && !p->codes)) return fail("rms_norm: null pointer");
+  if (int rc = check_rows("rms_norm", p->rows, p->features, p->dtype)) return rc;
+  if (p->y && p->codes) return fail("rms_norm: one output, y or codes");
+  if (p->sum && !p->residual) return fail("rms_norm: a sum needs a residual");
+  const int C = p->features, kb = (C + kBlock8 - 1) / kBlock8;
+  if (p->x_pitch < C || (p->residual && p->residual_pitch < C) || (p->sum && p->sum_pitch < C) ||
+      (p->y && p->y_pitch < C))
+    return fail("rms_norm: row pitch below %d features", C);
+  if (!(p->eps >= 1e-30f && p->eps <= 1e30f)) return fail("rms_norm: eps %g", (double)p->eps);
+  if (p->codes)
+    if (int rc = check_codes("rms_norm", p->codes, p->codes_pitch, p->scales, p->scales_pitch, kb)) return rc;
+  const NormArgs a = {p->x, p->x_pitch, p->residual, p->residual_pitch, p->sum, p->sum_pitch, p->gamma, p->eps,
+                      p->y, p->y_pitch, (uint8_t*)p->codes, p->codes_pitch, (uint8_t*)p->scales, p->scales_pitch,
+                      p->rows, C, kb};
+  hipStream_t st = as_stream(stream);
+  return p->codes ? launch_any<true, true>(a, p->dtype, st, "rms_norm")
+                  : launch_any<true, false>(a, p->dtype, st, "rms_norm");
+}
+
+extern "C" int ldx_quantize8(const void* x, int64_t xp, int64_t rows, int32_t features, int32_t dtype, void* codes,
+                             int64_t cp, void* scales, int64_t ep, void* stream) {
+  if (!x || !codes) return fail("quantize8: null pointer");
+  if (int rc = check_rows("quantize8", rows, features, dtype)) return rc;
+  const int kb = (features + kBlock8 - 1) / kBlock8;
+  if (xp < features) return fail("quantize8: row pitch below %d features", features);
+  if (int rc = check_codes("quantize8", codes, cp, scales, ep, kb)) return rc;
+  NormArgs a = {};
+  a.x = x; a.xp = xp;
+  a.codes = (uint8_t*)codes; a.cp = cp;
+  a.scales = (uint8_t*)scales; a.ep = ep;
+  a.rows = rows; a.C = features; a.kb = kb;
+  return launch_any<false, true>(a, dtype, as_stream(stream), "quantize8");
+}

@@ -1,0 +1,84 @@
+// The 8-bit form of the norm, dense and cache operators: OCP e4m3 codes times a power of two per
+// block. The power is held in one byte b (E8M0: 2^(b - 127)), the least for which the block's largest
+// magnitude is at most 448, e4m3's largest number. A power of two costs a floating-point code none of
+// its relative precision, raising it later changes no code that stays normal, and it is the form that
+// the scale operand of the gfx950 matrix instructions takes.
+#pragma once
+
+#include "common.h"
+
+namespace ldx {
+
+constexpr int kBlock8 = LDX_BLOCK8;   // columns of a row that share a scale
+constexpr int kPage8 = LDX_PAGE8;     // tokens of a cache page
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// The scale byte of a block with largest magnitude amax = 1.m * 2^(E - 127): amax <= 1.75 * 2^(b - 119)
+// holds from b = E - 8 on where 1.m <= 1.75, from E - 7 where it is larger. All-zero and subnormal
+// blocks get 1 (2^-126); an infinite amax gets 247, under which infinities become NaN codes.
+__device__ __forceinline__ int scale_byte(float amax) {
+  const int bits = __float_as_int(amax);
+  const int b = (bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
+  return b > 1 ? b : 1;
+}
+
+// 2^(b - 127) and 2^(127 - b) for 1 <= b <= 253.
+__device__ __forceinline__ float scale_of(int b) { return __int_as_float(b << 23); }
+__device__ __forceinline__ float inverse_of(int b) { return __int_as_float((254 - b) << 23); }
+
+// Four values times the inverse scale as four codes (round to nearest even; v_cvt_pk_fp8_f32 gives
+// subnormal codes their correct rounding, and NaN codes for infinities and NaN).
+__device__ __forceinline__ int encode4(float a, float b, float c, float d, float inv) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
+}
+
+// Eight consecutive values of T from memory of any alignment (gfx950 reads unaligned vectors).
+template <typename T>
+struct Load8 {
+  T v[8];
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  Load8<T> u;
+  __builtin_memcpy(&u, p, sizeof(u));
+#pragma unroll
+  for (int i = 0; i < 8; i++) f[i] = (float)u.v[i];
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  Load8<T> u;
+#pragma unroll
+  for (int i = 0; i < 8; i++) u.v[i] = (T)f[i];
+  __builtin_memcpy(p, &u, sizeof(u));
+}
+
+// Largest of v over the 16 lanes of a DPP row, on every one of them.
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, dpp_f<0x128>(v));   // row_ror:8
+  v = fmaxf(v, dpp_f<0x124>(v));
+  v = fmaxf(v, dpp_f<0x122>(v));
+  return fmaxf(v, dpp_f<0x121>(v));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+  v = row16_max(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  v = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += dpp_f<0x128>(v);
+  v += dpp_f<0x124>(v);
+  v += dpp_f<0x122>(v);
+  v += dpp_f<0x121>(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  v = __int_as_float(a[0]) + __int_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return __int_as_float(b[0]) + __int_as_float(b[1]);
+}
+
+}  // namespace ldx

@@ -20,13 +20,15 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from ._lib import ACT_GELU, ACT_NONE, ACT_SILU, AttnArgs, ConvArgs, SourceConvArgs, check, lib
+from ._lib import (ACT_GELU, ACT_NONE, ACT_SILU, BLOCK8, PAGE8, AttnArgs, Cache8AppendArgs, Cache8AttentionArgs,
+                   Cache8Block, ConvArgs, Dense8Args, RmsNormArgs, SourceConvArgs, check, lib)
 
 __all__ = [
     "PackedWeight", "pack_weight", "pack_upsample_weight", "nax_conv3d", "conv3d", "dense",
     "group_norm_affine", "layer_norm", "attention", "flash_attention", "timestep_embedding",
     "silu", "upsample_nearest2", "resize_nearest", "output_extent", "count_flops", "squared_norms4",
-    "nearest_codebook4", "conv3d_half", "group_norm_half",
+    "nearest_codebook4", "conv3d_half", "group_norm_half", "Quantized8", "quantize8", "rms_norm", "dense8",
+    "Cache8", "cache8_append", "cache8_attention",
 ]
 
 
@@ -679,7 +681,7 @@ def _vq_rows(t: torch.Tensor, name: str) -> int:
 def squared_norms4(x: torch.Tensor) -> torch.Tensor:
     """Per-row ``T(sum float32(T(x * x)))`` of ``(rows, 4)`` vectors, the squared norm the
     reference keeps per codebook entry (mlx_model.py:775-778)."""
-    n = _vq_rows(x, "x")
+    n = _vq_rows(x)
     out = torch.empty(n, dtype=x.dtype, device=x.device)
     check(lib.ldx_vq_squared_norms4(_ptr(x), n, _VQ_DTYPES[x.dtype], _ptr(out), _stream()), "vq_squared_norms4")
     return out
@@ -796,3 +798,348 @@ def group_norm_half(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, *
                                          _ptr(bias), float(eps), _ptr(affine), _ptr(y), ys[0], ys[1], ys[2],
                                          _ptr(ws), int(ws.numel()), _stream()), "group_norm_source_half")
     return (y, affine) if return_affine else y
+
+
+# ------------------------------------------------------------------ 8-bit operators
+
+@dataclass
+class Quantized8:
+    """8-bit rows: e4m3 ``codes`` (..., features rounded up to whole blocks of 128, zero codes past
+    ``features``) and E8M0 ``scales`` (..., blocks rounded up to four), one per row and 128 columns; a
+    value is its code times its block's power of two. Both contiguous. What ``quantize8`` and
+    ``rms_norm(..., quantize=True)`` return and ``dense8`` takes on both sides (a weight is quantized
+    once, ``quantize8(weight)`` of the Torch-layout ``(O, C)``)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    features: int
+
+    @staticmethod
+    def empty(lead: tuple[int, ...], features: int, device: torch.device) -> "Quantized8":
+        kb = -(-features // BLOCK8)
+        return Quantized8(torch.empty((*lead, kb * BLOCK8), dtype=torch.float8_e4m3fn, device=device),
+                          torch.empty((*lead, -(-kb // 4) * 4), dtype=torch.float8_e8m0fnu, device=device), features)
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        return (*self.codes.shape[:-1], self.features)
+
+    def float(self) -> torch.Tensor:
+        """The values as fp32 (a test and debugging aid)."""
+        kb = self.codes.shape[-1] // BLOCK8
+        s = self.scales.float()[..., :kb, None]
+        v = self.codes.float().unflatten(-1, (kb, BLOCK8)) * s
+        return v.flatten(-2)[..., :self.features]
+
+
+def _launch8(fn, args, device: torch.device, what: str) -> None:
+    """One C call on ``device``'s current stream; the device is made current for it where it is not."""
+    if device.index == torch._C._cuda_getDevice():
+        check(fn(*args, _stream()), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream()), what)
+
+
+def _same_device(x: torch.Tensor, *others: tuple[torch.Tensor | None, str]) -> None:
+    for t, name in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, not on {x.device}")
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` as ``(rows, features)`` and its row pitch: rows evenly spaced, features contiguous (a copy
+    is made of one that is not)."""
+    f = int(t.shape[-1])
+    t2 = t if t.dim() == 2 else t.reshape(-1, f)
+    if f > 1 and t2.stride(1) != 1 or t2.shape[0] > 1 and t2.stride(0) < f:
+        t2 = t2.contiguous()
+    return t2, (t2.stride(0) if t2.shape[0] > 1 else f)
+
+
+def _rows_in_place(t: torch.Tensor, name: str) -> int:
+    """Row pitch of an output, which has to be viewable as ``(rows, features)``."""
+    f = int(t.shape[-1])
+    try:
+        t2 = t.view(-1, f)
+    except RuntimeError:
+        raise ValueError(f"{name}: rows must be evenly spaced") from None
+    if f > 1 and t2.stride(1) != 1 or t2.shape[0] > 1 and t2.stride(0) < f:
+        raise ValueError(f"{name}: features must be contiguous and rows must not overlap")
+    return t2.stride(0) if t2.shape[0] > 1 else f
+
+
+def _out_like(out: torch.Tensor | None, x: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device), int(x.shape[-1])
+    _require_cuda(out, name, x.dtype)
+    _same_device(x, (out, name))
+    if out.shape != x.shape:
+        raise ValueError(f"{name} shape {tuple(out.shape)} != {tuple(x.shape)}")
+    return out, _rows_in_place(out, name)
+
+
+def quantize8(x: torch.Tensor) -> Quantized8:
+    """fp16, bf16 or fp32 ``x`` as 8-bit rows: per row and 128 columns the least power of two with which
+    the largest magnitude does not pass 448, codes rounded to nearest even."""
+    _require_cuda(x, "x", tuple(ALL_DTYPES))
+    if x.dim() < 1 or not x.numel():
+        raise ValueError(f"quantize8: shape {tuple(x.shape)} holds no rows")
+    x2, pitch = _rows(x)
+    rows, f = x2.shape
+    q = Quantized8.empty(tuple(x.shape[:-1]), f, x.device)
+    _launch8(lib.ldx_quantize8, (x2.data_ptr(), pitch, rows, f, ALL_DTYPES[x.dtype], q.codes.data_ptr(),
+                                 q.codes.shape[-1], q.scales.data_ptr(), q.scales.shape[-1]), x.device, "quantize8")
+    return q
+
+
+def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, *, residual: torch.Tensor | None = None,
+             quantize: bool = False, out: torch.Tensor | None = None, sum_out: torch.Tensor | None = None):
+    """``s / sqrt(mean(s^2) + eps) * gamma`` over the last axis of fp16, bf16 or fp32 ``x``, ``s`` being
+    ``x``, or ``x + residual`` rounded to that type. Returns the norm in ``x``'s type (into ``out`` when
+    given, which may be ``x``), or as ``Quantized8`` rows with ``quantize``; with a ``residual`` the pair
+    ``(norm, s)``, ``s`` into ``sum_out`` when given, which may be ``x`` or ``residual``. Statistics in
+    fp32, one launch."""
+    _require_cuda(x, "x", tuple(ALL_DTYPES))
+    if x.dim() < 1 or not x.numel():
+        raise ValueError(f"rms_norm: shape {tuple(x.shape)} holds no rows")
+    f = int(x.shape[-1])
+    _require_cuda(gamma, "gamma", None)
+    if tuple(gamma.shape) != (f,):
+        raise ValueError(f"gamma shape {tuple(gamma.shape)} != ({f},)")
+    if quantize and out is not None:
+        raise ValueError("rms_norm: out and quantize exclude each other")
+    if sum_out is not None and residual is None:
+        raise ValueError("rms_norm: sum_out needs a residual")
+    if residual is not None:
+        _same_elem(residual, "residual", x.dtype)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual shape {tuple(residual.shape)} != {tuple(x.shape)}")
+    _same_device(x, (gamma, "gamma"), (residual, "residual"))
+    x2, xp = _rows(x)
+    g32 = _f32(gamma)
+    a = RmsNormArgs(rows=x2.shape[0], features=f, dtype=ALL_DTYPES[x.dtype], x=x2.data_ptr(), x_pitch=xp,
+                    gamma=g32.data_ptr(), eps=float(eps))
+    s = None
+    if residual is not None:
+        r2, a.residual_pitch = _rows(residual)
+        a.residual = r2.data_ptr()
+        s, a.sum_pitch = _out_like(sum_out, x, "sum_out")
+        a.sum = s.data_ptr()
+    if quantize:
+        y = Quantized8.empty(tuple(x.shape[:-1]), f, x.device)
+        a.codes, a.codes_pitch = y.codes.data_ptr(), y.codes.shape[-1]
+        a.scales, a.scales_pitch = y.scales.data_ptr(), y.scales.shape[-1]
+    else:
+        y, a.y_pitch = _out_like(out, x, "out")
+        a.y = y.data_ptr()
+        if s is not None and y.data_ptr() == a.sum:
+            raise ValueError("rms_norm: out and sum_out are the same tensor")
+    _launch8(lib.ldx_rms_norm, (ctypes.byref(a),), x.device, "rms_norm")
+    if out is not None:
+        _wrote(out)
+    if sum_out is not None:
+        _wrote(sum_out)
+    return y if residual is None else (y, s)
+
+
+def _rows8(q: Quantized8, name: str) -> int:
+    """Checks one operand of ``dense8`` and returns its rows."""
+    if not isinstance(q, Quantized8):
+        raise ValueError(f"{name} must be Quantized8 rows")
+    _require_cuda(q.codes, f"{name} codes", torch.float8_e4m3fn)
+    _require_cuda(q.scales, f"{name} scales", torch.float8_e8m0fnu)
+    kb = -(-q.features // BLOCK8)
+    if q.features < 1 or q.codes.shape[-1] != kb * BLOCK8 or q.scales.shape[-1] != -(-kb // 4) * 4 \
+            or q.codes.shape[:-1] != q.scales.shape[:-1]:
+        raise ValueError(f"{name}: codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} do not hold rows of "
+                         f"{q.features} features")
+    if not q.codes.is_contiguous() or not q.scales.is_contiguous():
+        raise ValueError(f"{name}: codes and scales must be contiguous")
+    return q.codes.numel() // (kb * BLOCK8)
+
+
+def dense8(x: Quantized8, weight: Quantized8, bias: torch.Tensor | None = None, *,
+           residual: torch.Tensor | None = None, act: str | None = None, out: torch.Tensor | None = None,
+           dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """``act(x @ weight^T + bias + residual)`` of 8-bit rows ``x`` (..., C) and an 8-bit weight (O, C),
+    fp32 sums and one rounding to ``dtype`` (fp16, bf16 or fp32; ``residual`` and ``out`` share it).
+    ``act`` is None, ``"gelu"`` or ``"silu"``. fp16 and bf16 results come from the e4m3 matrix
+    instruction, whose sums are within 2^-10 of the terms' magnitudes (about 1.5e-5 of the result for
+    ordinary data); fp32 results are summed to fp32 accuracy at half its rate."""
+    m, o = _rows8(x, "x"), _rows8(weight, "weight")
+    if weight.codes.dim() != 2:
+        raise ValueError(f"weight must be (O, C) rows, got {weight.shape}")
+    if x.features != weight.features:
+        raise ValueError(f"weight expects {weight.features} features, got {x.features}")
+    if dtype not in ALL_DTYPES:
+        raise ValueError(f"dtype must be fp16, bf16 or fp32, not {dtype}")
+    if act not in (None, "gelu", "silu"):
+        raise ValueError(f"act must be None, 'gelu' or 'silu', not {act!r}")
+    if not m or not o:
+        raise ValueError(f"dense8: {m} rows and {o} outputs")
+    lead = tuple(x.codes.shape[:-1])
+    bias32, batched = _bias32(bias, 1, o)
+    if batched:
+        raise ValueError(f"bias shape {tuple(bias.shape)} != ({o},)")
+    _same_device(x.codes, (x.scales, "x scales"), (weight.codes, "weight"), (weight.scales, "weight scales"),
+                 (bias32, "bias"), (residual, "residual"), (out, "out"))
+    if out is None:
+        out = torch.empty((*lead, o), dtype=dtype, device=x.codes.device)
+        yp, given = o, False
+    else:
+        _require_cuda(out, "out", dtype)
+        if tuple(out.shape) != (*lead, o):
+            raise ValueError(f"out shape {tuple(out.shape)} != {(*lead, o)}")
+        yp, given = _rows_in_place(out, "out"), True
+    a = Dense8Args(rows=m, features=x.features, out_features=o, x_codes=x.codes.data_ptr(),
+                   x_pitch=x.codes.shape[-1], x_scales=x.scales.data_ptr(), x_scales_pitch=x.scales.shape[-1],
+                   w_codes=weight.codes.data_ptr(), w_pitch=weight.codes.shape[-1],
+                   w_scales=weight.scales.data_ptr(), w_scales_pitch=weight.scales.shape[-1],
+                   bias=_ptr(bias32), act={None: ACT_NONE, "gelu": ACT_GELU, "silu": ACT_SILU}[act],
+                   dtype=ALL_DTYPES[dtype], y=out.data_ptr(), y_pitch=yp)
+    if residual is not None:
+        _same_elem(residual, "residual", dtype)
+        if tuple(residual.shape) != (*lead, o):
+            raise ValueError(f"residual shape {tuple(residual.shape)} != {(*lead, o)}")
+        r2, a.residual_pitch = _rows(residual)
+        a.residual = r2.data_ptr()
+    if count_flops.active is not None:
+        count_flops.active.dense += 2.0 * m * o * x.features
+    _launch8(lib.ldx_dense8, (ctypes.byref(a),), x.codes.device, "dense8")
+    if given:
+        _wrote(out)
+    return out
+
+
+@dataclass
+class Cache8:
+    """Keys and values in 8 bits, in pages of 64 tokens: e4m3 codes ``k`` (pages, heads, 64, D) and ``v``
+    (pages, heads, D, 64) and E8M0 scales ``k_scales``, ``v_scales`` (pages, heads), all contiguous. Pages
+    belong to no sequence by themselves: an int32 ``table`` (batch, pages per sequence) says which hold
+    a sequence's tokens, in order."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+    @staticmethod
+    def empty(pages: int, heads: int, head_dim: int, device: torch.device | str = "cuda") -> "Cache8":
+        codes = [torch.zeros(s, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+                 for s in ((pages, heads, PAGE8, head_dim), (pages, heads, head_dim, PAGE8))]
+        scales = [torch.full((pages, heads), 127, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+                  for _ in range(2)]
+        return Cache8(*codes, *scales)
+
+
+def _cache_block(cache: Cache8, what: str) -> Cache8Block:
+    if not isinstance(cache, Cache8):
+        raise ValueError(f"{what}: cache must be a Cache8")
+    k, v, ks, vs = cache.k, cache.v, cache.k_scales, cache.v_scales
+    _require_cuda(k, "cache k", torch.float8_e4m3fn)
+    _require_cuda(v, "cache v", torch.float8_e4m3fn)
+    _require_cuda(ks, "cache k_scales", torch.float8_e8m0fnu)
+    _require_cuda(vs, "cache v_scales", torch.float8_e8m0fnu)
+    if k.dim() != 4 or k.shape[2] != PAGE8:
+        raise ValueError(f"cache k must be (pages, heads, {PAGE8}, D), got {tuple(k.shape)}")
+    pages, heads, _, d = k.shape
+    if v.shape != (pages, heads, d, PAGE8) or ks.shape != (pages, heads) or vs.shape != (pages, heads):
+        raise ValueError(f"cache v {tuple(v.shape)} or scales {tuple(ks.shape)}, {tuple(vs.shape)} do not fit k "
+                         f"{tuple(k.shape)}")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("cache tensors must be contiguous")
+    _same_device(k, (v, "cache v"), (ks, "cache k_scales"), (vs, "cache v_scales"))
+    return Cache8Block(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, d)
+
+
+def _cache_ints(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> None:
+    _require_cuda(t, name, torch.int32)
+    _same_device(like, (t, name))
+    if tuple(t.shape) != shape or (t.dim() == 1 and shape[0] > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be contiguous int32 {shape}, got {tuple(t.shape)}")
+
+
+def _cache_table(table: torch.Tensor, batch: int, like: torch.Tensor) -> tuple[int, int]:
+    """``(pitch, width)`` of a page table (a column range of a wider one is fine)."""
+    _require_cuda(table, "table", torch.int32)
+    _same_device(like, (table, "table"))
+    if table.dim() != 2 or table.shape[0] != batch or not table.shape[1] or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"table must be int32 ({batch}, pages) with contiguous rows, got {tuple(table.shape)}")
+    width = int(table.shape[1])
+    return (table.stride(0) if batch > 1 else width), width
+
+
+def _head_strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(batch, token, head) strides of a ``(B, H, L, D)`` tensor with contiguous channels."""
+    st = t.stride()
+    if t.shape[3] > 1 and st[3] != 1:
+        raise ValueError(f"{name}: head_dim must be contiguous")
+    return st[0], st[2], st[1]
+
+
+def cache8_append(cache: Cache8, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, *,
+                  counts: torch.Tensor | None = None) -> None:
+    """Write ``k``, ``v`` (B, heads, L, D; fp16, bf16 or fp32, any strides with contiguous channels) into
+    ``cache`` at positions ``starts[b] ..`` of each sequence: its first ``counts[b]`` tokens (all ``L``
+    without). Each page of 64 tokens has one power of two for a head's keys and one for its values; it
+    rises with the largest token written, and older codes of the page are then rounded to it. Tokens
+    past the table's width, of a negative start or in a page that the cache does not have are left out;
+    sequences that write must not share pages. ``table``, ``starts`` and ``counts`` are int32 on the
+    device, so a captured graph appends where they say at each replay."""
+    block = _cache_block(cache, "cache8_append")
+    _require_cuda(k, "k", tuple(ALL_DTYPES))
+    _same_elem(v, "v", k.dtype)
+    _same_device(cache.k, (k, "k"), (v, "v"))
+    if k.dim() != 4 or k.shape != v.shape or k.shape[1] != block.heads or k.shape[3] != block.head_dim \
+            or not k.shape[0] or not k.shape[2]:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be (B, {block.heads}, L, {block.head_dim})")
+    b, _, n, _ = k.shape
+    pitch, width = _cache_table(table, b, cache.k)
+    _cache_ints(starts, "starts", (b,), cache.k)
+    if counts is not None:
+        _cache_ints(counts, "counts", (b,), cache.k)
+    a = Cache8AppendArgs(block, b, n, k.data_ptr(), _head_strides(k, "k"), v.data_ptr(), _head_strides(v, "v"),
+                         ALL_DTYPES[k.dtype], table.data_ptr(), pitch, width, starts.data_ptr(), _ptr(counts))
+    _launch8(lib.ldx_cache8_append, (ctypes.byref(a),), cache.k.device, "cache8_append")
+    for t in (cache.k, cache.v, cache.k_scales, cache.v_scales):
+        _wrote(t)
+
+
+def cache8_attention(q: torch.Tensor, cache: Cache8, table: torch.Tensor, lengths: torch.Tensor, scale: float, *,
+                     starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``softmax(q k^T * scale) v`` over the first ``lengths[b]`` tokens that ``cache`` holds of each
+    sequence. ``q`` is fp16 or bf16 ``(B, heads, L, D)``, its heads a multiple of the cache's (query head
+    ``j`` reads the cache's head ``j // group``). With ``starts`` query ``i`` sees tokens up to position
+    ``starts[b] + i`` (causal); without, all ``lengths[b]``. A query that sees no token gives 0; tokens that
+    it does not see, and pages behind the length, do not touch its result. A page that the cache does
+    not have, or a length past the table, gives NaN. Returns ``(B, heads, L, D)`` in ``q``'s type (into
+    ``out`` when given); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
+    block = _cache_block(cache, "cache8_attention")
+    _require_cuda(q, "q", tuple(ELEM_DTYPES))
+    _same_device(cache.k, (q, "q"), (out, "out"))
+    if q.dim() != 4 or q.shape[3] != block.head_dim or q.shape[1] % block.heads or not q.numel():
+        raise ValueError(f"q {tuple(q.shape)} must be (B, a multiple of {block.heads}, L, {block.head_dim})")
+    b, hq, lq, d = q.shape
+    pitch, width = _cache_table(table, b, cache.k)
+    _cache_ints(lengths, "lengths", (b,), cache.k)
+    if starts is not None:
+        _cache_ints(starts, "starts", (b,), cache.k)
+    given = out is not None
+    if given:
+        _same_elem(out, "out", q.dtype)
+        if out.shape != q.shape:
+            raise ValueError(f"out shape {tuple(out.shape)} != {tuple(q.shape)}")
+    else:
+        out = torch.empty((b, hq, lq, d), dtype=q.dtype, device=q.device)
+    a = Cache8AttentionArgs(block, b, hq, lq, q.data_ptr(), _head_strides(q, "q"), out.data_ptr(),
+                            _head_strides(out, "out"), ALL_DTYPES[q.dtype], float(scale), table.data_ptr(), pitch,
+                            width, lengths.data_ptr(), _ptr(starts))
+    ws_bytes = lib.ldx_cache8_attention_workspace_bytes(ctypes.byref(a))
+    if ws_bytes:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws_bytes
+    _launch8(lib.ldx_cache8_attention, (ctypes.byref(a),), q.device, "cache8_attention")
+    if given:
+        _wrote(out)
+    return out
