@@ -1,5 +1,7 @@
 // Products of 8-bit rows: y = act(x w^T + bias + residual), x and w e4m3 codes with a power of two per
 // row and 128 columns.
+#include <type_traits>
+
 #include "quant8.h"
 
 namespace ldx {
@@ -17,11 +19,39 @@ struct Dense8Args {
   int O, kb, act, dtype;
 };
 
-__device__ __forceinline__ float gelu_f(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f)); }
+// exp(-x) as 2^hi * (1 + lo), lo the part of x log2(e) that its rounding to hi left.
+__device__ __forceinline__ float exp_neg(float x) {
+  const float hi = x * -1.44269504f;
+  const float lo = __builtin_fmaf(x, -1.44269504f, -hi) - x * 1.92596299e-8f;
+  return __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.693147181f, 1.0f);
+}
+
+// GELU without the cancellation of 1 + erf for negative v: v Q(|v|) there and v (1 - Q(v)) otherwise,
+// Q(v) = erfc(v / sqrt 2) / 2 = t exp(p(t) - v^2 / 2) / 2, t = 1 / (1 + 0.4 v / sqrt 2), where p is a
+// least-squares Chebyshev fit of log(erfc(x) exp(x^2) / t) for x up to 12 (to 1.1e-7). Branchless: the
+// library's erff and expf in the eight-wide epilogue were 20 KB of code.
+__device__ __forceinline__ float gelu_f(float v) {
+  const float u = fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(u, 0.4f * 0.70710678f, 1.0f));
+  float p = -0.213728147f;
+  p = __builtin_fmaf(p, t, 0.955197486f);
+  p = __builtin_fmaf(p, t, -1.5495496f);
+  p = __builtin_fmaf(p, t, 1.07216591f);
+  p = __builtin_fmaf(p, t, -0.493939286f);
+  p = __builtin_fmaf(p, t, 0.321830446f);
+  p = __builtin_fmaf(p, t, 0.394323262f);
+  p = __builtin_fmaf(p, t, 1.00245476f);
+  p = __builtin_fmaf(p, t, -1.48875494f);
+  const float hu = 0.5f * u, sq = hu * u, rest = __builtin_fmaf(hu, u, -sq);   // v^2 / 2 = sq + rest
+  const float e = exp_neg(sq) * __builtin_amdgcn_exp2f((p - rest) * 1.44269504f);
+  const float q = 0.5f * t * e;
+  return v * (v < 0.f ? q : 1.0f - q);
+}
+
+__device__ __forceinline__ float silu8_f(float v) { return v * __builtin_amdgcn_rcpf(1.0f + exp_neg(v)); }
 
 __device__ __forceinline__ float act_f(float v, int act) {
   if (act == LDX_ACT_GELU) return gelu_f(v);
-  if (act == LDX_ACT_SILU) return v / (1.0f + expf(-v));
+  if (act == LDX_ACT_SILU) return silu8_f(v);
   return v;
 }
 
@@ -59,6 +89,42 @@ __device__ __forceinline__ void finish(const Dense8Args& a, int64_t m, int o, fl
   ((T*)a.y)[m * a.yp + o] = (T)act_f(v, a.act);
 }
 
+// Outputs o .. o + 7 of row m, as many as there are.
+template <typename T>
+__device__ __forceinline__ void finish8(const Dense8Args& a, int64_t m, int o, float (&v)[8]) {
+  T* y = (T*)a.y + m * a.yp + o;
+  if (o + 8 <= a.O) {
+    float f[8];
+    if (a.bias) {
+      load8(a.bias + o, f);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] += f[i];
+    }
+    if (a.res) {
+      load8((const T*)a.res + m * a.rp + o, f);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] += f[i];
+    }
+    if (a.act == LDX_ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = gelu_f(v[i]);
+    } else if (a.act == LDX_ACT_SILU) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = silu8_f(v[i]);
+    }
+    store8(y, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (o + i >= a.O) break;
+      float f = v[i];
+      if (a.bias) f += a.bias[o + i];
+      if (a.res) f += (float)((const T*)a.res)[m * a.rp + o + i];
+      y[i] = (T)act_f(f, a.act);
+    }
+  }
+}
+
 // One 16 x 16 tile a workgroup, its blocks of 128 dealt to the waves and their sums added in wave order.
 constexpr int kTileWaves = 4;
 
@@ -93,8 +159,265 @@ __global__ __launch_bounds__(64 * kTileWaves) void dense8_tile_kernel(Dense8Args
   if (m0 + tm < a.M && o0 + to < a.O) finish<T>(a, m0 + tm, o0 + to, v);
 }
 
+// ------------------------------------------------------------------------------ large products
+//
+// A workgroup of 2 x 2 waves takes 64 FN outputs x 64 FM rows, a wave 32 FN x 32 FM of them in 32 x 32
+// accumulators. The operands' rows of a block (128 bytes) come into LDS by DMA, a ring of two stages;
+// whole 128-byte lines, since 64-byte pieces arrive at 18 TB/s and lines at 24 (every CU loading from
+// L2). Of row r the 16-byte unit u stands at u ^ (r / 2 % 8), so that the 16 lanes which read one unit of
+// 16 rows meet all 64 banks once.
+//
+// With one wave a SIMD nothing else hides what a wave issues between its matrix instructions: the LDS
+// reads of the next half block go one by one between the products of this one, and with the second half's
+// the DMAs into the stage that all waves have then read.
+//
+// Scales come by DMA too, four blocks' bytes (a dword a row) at a time.
+
+constexpr int kHalf8 = kBlock8 / 2;
+
+template <int FN, int FM>
+struct BigTile {
+  static constexpr int TN = 64 * FN, TM = 64 * FM;
+  static constexpr int STAGE = (TN + TM) * kBlock8;
+  static constexpr int SCALES = (TN + TM) * 4;
+  static constexpr int DMAS = 2 * (FN + FM);      // 1 KB (8 rows) each, per wave and block
+  static constexpr int READS = 2 * (FN + FM);     // per half block
+  // The result leaves through LDS: a wave's JP x 32 rows of 32 FN outputs, padded by 16 bytes.
+  static constexpr int JP = FN == 4 ? 2 : 1, PITCH = 32 * FN + 4, OUT = 4 * JP * 32 * PITCH * 4;
+  static constexpr int RING = 2 * STAGE + 2 * SCALES;
+  static constexpr int LDS = RING > OUT ? RING : OUT;
+  static_assert(FM % JP == 0 && LDS <= 160 * 1024, "tile");
+};
+
+template <typename T, int FN, int FM>
+__global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned nt, unsigned mt) {
+  typedef BigTile<FN, FM> B;
+  constexpr bool EXACT = sizeof(T) == 4;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 31, h = lane >> 5, wn = wave >> 1, wm = wave & 1;
+  // Workgroups l and l + 8 share an XCD: each XCD gets a contiguous range of tiles, in which bands of
+  // four rows of tiles run along the outputs, so that what it holds at a time is near a square.
+  const unsigned tiles = nt * mt, l = blockIdx.x;
+  const unsigned x = l % 8, per = tiles / 8, extra = tiles % 8;
+  const unsigned idx = x * per + (x < extra ? x : extra) + l / 8;
+  constexpr unsigned BAND = 4;
+  const unsigned band = idx / (BAND * nt), first = band * BAND;
+  const unsigned high = mt - first < BAND ? mt - first : BAND, in = idx - band * BAND * nt;
+  const unsigned tm = first + in % high, tn = in / high;
+  const int64_t m0 = (int64_t)tm * B::TM;
+  const int o0 = (int)tn * B::TN;
+  const int mrows = (int)(a.M - m0 < B::TM ? a.M - m0 : B::TM), orows = a.O - o0 < B::TN ? a.O - o0 : B::TN;
+  // Rows past the operand's last read as zeros (the buffer ends there).
+  const i32x4 wr = dma_rsrc(a.w + o0 * a.wp, (unsigned)(orows * a.wp));
+  const i32x4 xr = dma_rsrc(a.x + m0 * a.xp, (unsigned)(mrows * a.xp));
+  const i32x4 wsr = dma_rsrc(a.ws + o0 * a.wsp, (unsigned)(orows * a.wsp));
+  const i32x4 xsr = dma_rsrc(a.xs + m0 * a.xsp, (unsigned)(mrows * a.xsp));
+  const unsigned base = lds_offset(lds);
+  // A lane's place in a DMA of eight rows; its unit depends on whether the eight is an odd one.
+  unsigned wv[2], xv[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const unsigned row = 8 * i + lane / 8, unit = (lane % 8) ^ (row / 2 % 8);
+    wv[i] = lane / 8 * (unsigned)a.wp + unit * 16;
+    xv[i] = lane / 8 * (unsigned)a.xp + unit * 16;
+  }
+  const unsigned wstep = 8 * (unsigned)a.wp, xstep = 8 * (unsigned)a.xp;
+  // DMA i of this wave for block k.
+  const auto dma = [&](int k, int i) {
+    const unsigned to = base + (k & 1) * B::STAGE, at = k * kBlock8;
+    if (i < 2 * FN) {
+      const unsigned e = wave * 2 * FN + i;
+      dma_buffer_b128(wr, wv[i & 1], e * wstep + at, to + e * 1024);
+    } else {
+      const unsigned e = wave * 2 * FM + i - 2 * FN;
+      dma_buffer_b128(xr, xv[i & 1], e * xstep + at, to + (B::TN / 8 + e) * 1024);
+    }
+  };
+  // Scales of blocks k .. k + 3.
+  const auto dma_scales = [&](int k) {
+    if (k & 3) return;
+    const unsigned to = base + 2 * B::STAGE + (k >> 2 & 1) * B::SCALES;
+#pragma unroll
+    for (int i = 0; i < FN + FM; i++) {
+      if (i % 4 != wave) continue;
+      const unsigned row = (unsigned)(i * 64 + lane);
+      if (i < FN) dma_buffer_b32(wsr, row * (unsigned)a.wsp, (unsigned)k, to + i * 256);
+      else dma_buffer_b32(xsr, (row - B::TN) * (unsigned)a.xsp, (unsigned)k, to + i * 256);
+    }
+  };
+
+  f32x16 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; i++)
+#pragma unroll
+    for (int j = 0; j < FM; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+
+  // Units 2 p + h (p = 0, 1 in the block's first half) of the lane's row of the wave's first fragments.
+  unsigned wu[4], xu[4];
+#pragma unroll
+  for (int p = 0; p < 4; p++) {
+    const unsigned u = (unsigned)r * kBlock8 + (((2 * p + h) ^ (r / 2 % 8)) * 16);
+    wu[p] = wn * FN * 32 * kBlock8 + u;
+    xu[p] = (B::TN + wm * FM * 32) * kBlock8 + u;
+  }
+  i32x8 fw[2][FN], fx[2][FM];
+  // LDS read i of half c of block k.
+  const auto read = [&](int k, int c, int i) {
+    const uint8_t* s = lds + (k & 1) * B::STAGE;
+    const int f = i / 2, p = i % 2;
+    const i32x4 v = *reinterpret_cast<const i32x4*>(f < FN ? s + wu[2 * c + p] + f * 32 * kBlock8
+                                                           : s + xu[2 * c + p] + (f - FN) * 32 * kBlock8);
+    i32x8& to = f < FN ? fw[c][f < FN ? f : 0] : fx[c][f < FN ? 0 : f - FN];
+#pragma unroll
+    for (int e = 0; e < 4; e++) to[4 * p + e] = v[e];
+  };
+  int sn[FN], sx[FM];
+  const auto scales = [&](int k) {
+    const int* s = reinterpret_cast<const int*>(lds + 2 * B::STAGE + (k >> 2 & 1) * B::SCALES);
+#pragma unroll
+    for (int i = 0; i < FN; i++) sn[i] = s[(wn * FN + i) * 32 + r];
+#pragma unroll
+    for (int j = 0; j < FM; j++) sx[j] = s[B::TN + (wm * FM + j) * 32 + r];
+  };
+  // Products of half c of block k; between them the reads of the half block after it and, with MORE in
+  // the second half, the DMAs of block k + 2.
+  const auto products = [&](int k, auto half, auto more) {
+    constexpr int c = decltype(half)::value;
+    constexpr bool MORE = c == 1 && decltype(more)::value;
+    constexpr int N = EXACT ? 4 : FN * FM;
+    const auto beside = [&](int s) {
+#pragma unroll
+      for (int i = s * B::READS / N; i < (s + 1) * B::READS / N; i++) read(k + c, 1 - c, i);
+      if constexpr (MORE)
+#pragma unroll
+        for (int i = s * B::DMAS / N; i < (s + 1) * B::DMAS / N; i++) dma(k + 2, i);
+    };
+    if constexpr (MORE) dma_scales(k + 2);
+    if constexpr (!EXACT) {
+#pragma unroll
+      for (int s = 0; s < N; s++) {
+        const int i = s / FM, j = s % FM;
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[c][i], fx[c][j], acc[i][j], 0, 0, 0, sn[i], 0,
+                                                                   sx[j]);
+        beside(s);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < 4; p++) {
+        bf16x8 bw[FN];
+#pragma unroll
+        for (int i = 0; i < FN; i++) bw[i] = widen8(fw[c][i][2 * p], fw[c][i][2 * p + 1], scale_of(sn[i] & 255));
+        beside(p);
+#pragma unroll
+        for (int j = 0; j < FM; j++) {
+          const bf16x8 bx = widen8(fx[c][j][2 * p], fx[c][j][2 * p + 1], scale_of(sx[j] & 255));
+#pragma unroll
+          for (int i = 0; i < FN; i++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bw[i], bx, acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+    // The products stay in this half block: without this the compiler sinks them past the branches below.
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+      for (int j = 0; j < FM; j++) asm volatile("" : "+a"(acc[i][j]));
+    if constexpr (c == 1) {
+      if ((k & 3) == 3) {
+        scales(k + 1);   // past the last block: old bytes, not used
+      } else {
+#pragma unroll
+        for (int i = 0; i < FN; i++) sn[i] = (int)((unsigned)sn[i] >> 8);
+#pragma unroll
+        for (int j = 0; j < FM; j++) sx[j] = (int)((unsigned)sx[j] >> 8);
+      }
+    }
+  };
+  constexpr std::integral_constant<int, 0> half0{};
+  constexpr std::integral_constant<int, 1> half1{};
+
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+    if (k < a.kb) {
+      dma_scales(k);
+#pragma unroll
+      for (int i = 0; i < B::DMAS; i++) dma(k, i);
+    }
+  if (a.kb > 1) vmcnt_wait<B::DMAS>();
+  else vmcnt_wait<0>();
+  ring_barrier();
+#pragma unroll
+  for (int i = 0; i < B::READS; i++) read(0, 0, i);
+  scales(0);
+  int k = 0;
+  for (; k + 2 < a.kb; k++) {
+    products(k, half0, std::true_type{});
+    vmcnt_wait<0>();   // block k + 1 has come, and behind the barrier every wave has read block k
+    ring_barrier();
+    products(k, half1, std::true_type{});
+  }
+  for (; k < a.kb; k++) {   // the last two, or one: the reads past the end take old bytes, not used
+    products(k, half0, std::false_type{});
+    vmcnt_wait<0>();
+    ring_barrier();
+    products(k, half1, std::false_type{});
+  }
+
+  // A lane holds outputs 8 q + 4 h + e of row r of each 32 x 32. Through LDS a wave takes whole rows of its
+  // 32 FN outputs, eight to a lane, in one rolled loop (the epilogue unrolled over the accumulators was
+  // so much code that a 256 x 256 tile spent 20 us in it).
+  ring_barrier();
+  float* out = reinterpret_cast<float*>(lds) + wave * B::JP * 32 * B::PITCH;
+#pragma unroll
+  for (int j0 = 0; j0 < FM; j0 += B::JP) {
+#pragma unroll
+    for (int j = 0; j < B::JP; j++)
+#pragma unroll
+      for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+          *reinterpret_cast<f32x4*>(out + (j * 32 + r) * B::PITCH + i * 32 + 8 * q + 4 * h) =
+              (f32x4){acc[i][j0 + j][4 * q], acc[i][j0 + j][4 * q + 1], acc[i][j0 + j][4 * q + 2], acc[i][j0 + j][4 * q + 3]};
+    __builtin_amdgcn_wave_barrier();
+    constexpr int PER = 4 * FN;   // lanes a row
+#pragma unroll 4
+    for (int row = lane / PER; row < B::JP * 32; row += 64 / PER) {
+      const float* f = out + row * B::PITCH + lane % PER * 8;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = f[e];
+      const int64_t m = m0 + (wm * FM + j0) * 32 + row;
+      if (m < a.M) finish8<T>(a, m, o0 + wn * FN * 32 + lane % PER * 8, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <typename T, int FN, int FM>
+void launch_big(const Dense8Args& a, hipStream_t st) {
+  typedef BigTile<FN, FM> B;
+  const unsigned nt = (unsigned)((a.O + B::TN - 1) / B::TN), mt = (unsigned)((a.M + B::TM - 1) / B::TM);
+  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(dense8_big_kernel<T, FN, FM>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, B::LDS);
+  (void)once;
+  hipLaunchKernelGGL((dense8_big_kernel<T, FN, FM>), dim3(nt * mt), dim3(256), B::LDS, st, a, nt, mt);
+}
+
 template <typename T>
 void launch(const Dense8Args& a, hipStream_t st) {
+  if (a.M > 64 && (a.wp | a.xp) < (1 << 22)) {
+    // Rounds of workgroups (one 256 x 256 tile a CU, two of 128 x 128) times what a round was measured to
+    // take, us: so much a block of 128 and so much to start and store.
+    const auto cdiv = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+    const double wide = cdiv(cdiv(a.M, 256) * cdiv(a.O, 256), 256) * (1.32 * a.kb + 13.0);
+    const double narrow = cdiv(cdiv(a.M, 128) * cdiv(a.O, 128), 512) * (0.93 * a.kb + 8.0);
+    if (wide < narrow) launch_big<T, 4, 4>(a, st);
+    else launch_big<T, 2, 2>(a, st);
+    return;
+  }
   const int64_t tiles = (a.M + 15) / 16 * ((a.O + 15) / 16);
   hipLaunchKernelGGL(dense8_tile_kernel<T>, dim3((unsigned)tiles), dim3(64 * kTileWaves), 0, st, a);
 }
@@ -121,6 +444,7 @@ extern "C" int ldx_dense8(const ldx_dense8_args* p, void* stream) {
   if (p->dtype != LDX_DTYPE_F16 && p->dtype != LDX_DTYPE_BF16 && p->dtype != LDX_DTYPE_F32)
     return fail("dense8: dtype %d is not LDX_DTYPE_F16, LDX_DTYPE_BF16 or LDX_DTYPE_F32", p->dtype);
   if (p->act != LDX_ACT_NONE && p->act != LDX_ACT_GELU && p->act != LDX_ACT_SILU) return fail("dense8: act %d", p->act);
+  // (the largest grid, of 16 x 16 tiles)
   if ((p->rows + 15) / 16 * ((p->out_features + 15) / 16) > 0x7fffffff)
     return fail("dense8: %lld x %d outputs are more than one launch takes", (long long)p->rows, p->out_features);
   const int kb = (p->features + kBlock8 - 1) / kBlock8;

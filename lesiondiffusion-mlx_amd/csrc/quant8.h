@@ -81,4 +81,12 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(b[0]) + __int_as_float(b[1]);
 }
 
+// Four bytes per lane from a buffer (byte offset voff + soff; out of range reads zeros) straight into
+// LDS at lds + 4 * lane; awaited like dma_buffer_b128.
+__device__ __forceinline__ void dma_buffer_b32(i32x4 rs, unsigned voff, unsigned soff, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(rs),
+               "s"(soff), "s"(lds)
+               : "memory");
+}
+
 }  // namespace ldx

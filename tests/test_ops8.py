@@ -407,6 +407,29 @@ def test_dense8_epilogue(pkg, dev, m, k, o, act, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize(("m", "k", "o", "act"), [(3000, 100, 3100, None), (2561, 700, 4360, "gelu"), (4100, 256, 2999, "silu")])
+def test_dense8_large(pkg, dev, m, k, o, act, t) -> None:
+    """Sizes that the largest tiles serve, ragged in both directions, against float64 products on the
+    device; the bound is the one above with the sum of the terms in the place of the eights' largest."""
+    x = pkg.ops.quantize8(rand((m, k), 1).to(dev))
+    w = pkg.ops.quantize8((rand((o, k), 2) / math.sqrt(k)).to(dev))
+    b, r = rand((o,), 3).to(dev), rand((m, o), 4, t).to(dev)
+    base = torch.full((m, o + 3), 7.0, dtype=t, device=dev)
+    got = pkg.ops.dense8(x, w, b, residual=r, act=act, out=base[:, 2:2 + o], dtype=t)
+    assert (base[:, :2] == 7).all() and (base[:, 2 + o:] == 7).all()
+    a, ww = wide(x).to(dev), wide(w).to(dev)
+    y = torch.mm(a, ww.t().contiguous()) + b.double() + r.double()
+    terms = torch.mm(a.abs(), ww.abs().t().contiguous())
+    bound = (7 * 2.0 ** (-13 if t != torch.float32 else -23) + (k / 8 + 20) * 2.0 ** -23) * terms
+    bound += 2.0 ** -23 * (y.abs() + b.double().abs() + r.double().abs())
+    z = activate(y, act)
+    allowed = 1.13 * bound + z.abs() * (half_step(t) + 8 * 2.0 ** -23) + tiny(t) + (2.0 ** -23 * y.abs() if act else 0)
+    err = (got.double() - z).abs()
+    assert (err <= allowed).all(), (err / allowed).max()
+
+
+@gpu
 @pytest.mark.parametrize("m", [4, 100, 600])
 def test_dense8_scales_differ_by_block(pkg, dev, m) -> None:
     """Blocks of very unlike sizes, zero blocks and rows among them: each product takes its own scales."""
