@@ -127,7 +127,8 @@ struct Attend8Args {
   const int32_t* table; int64_t tp; int width;
   const int32_t* lengths;
   const int32_t* starts;
-  int splits;
+  int splits, chunk;     // parts of a sequence; least pages of a part
+  int tile;              // rows of a workgroup
   float* part;           // splits > 1: [b][h][row][split] of D sums, then of (m, l)
 };
 
@@ -160,11 +161,48 @@ __device__ __forceinline__ void codes_as(int lo, int hi, bf16x8& r) {
   r = (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// The largest of three numbers, NaN ignored where there is another. (fmaxf of a product's results costs a
+// second instruction for each, which would quiet a signalling NaN.)
+__device__ __forceinline__ float max3_f(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Entry p of a page table by a scalar load, whose result is awaited where it is used. (As a vector load of
+// one address its value is moved to a scalar, and so awaited, where it is loaded.)
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+__device__ __forceinline__ int table_entry(const int32_t* table, int p) { return ((scalar_ints)(uintptr_t)table)[p]; }
+
+// A page's scale byte, loaded by every lane (none is 0 that the compiler does not know) for the same reason.
+__device__ __forceinline__ int scale_entry(const uint8_t* scales, int64_t at, int none) { return scales[at + none]; }
+
 // The keys that a query sees: limit = min(length, start + i + 1) with starts, the length without.
 __device__ __forceinline__ int key_limit(const Attend8Args& a, int len, int64_t start, int row) {
   if (!a.starts) return len;
   const int64_t c = start + row / a.G + 1;
   return (int)(c < 0 ? 0 : c < len ? c : len);
+}
+
+// The softmax scale's size, in powers of two (1 for a scale of 0); its sign, or 0, is the queries'.
+__device__ __forceinline__ float soft_scale(const Attend8Args& a) { return a.scale == 0.f ? 1.f : fabsf(a.scale); }
+
+// That and the keys' scale go onto the scores inside the exponential. Kept a number larger than 0, so that
+// a masked score stays minus infinity and a score of 0 stays 0.
+__device__ __forceinline__ float score_scale(float c, int byte) {
+  return fminf(fmaxf(c * scale_of(byte), 1.1754944e-38f), 3.0e38f);
+}
+
+// Channels at .. at + 7 of a query, with the softmax scale's sign.
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::V query8(const Attend8Args& a, const T* q, int at, bool real) {
+  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (real) load8(q + at, f);
+  const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;
+  typename Vec8<T>::V v;
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = (T)(f[e] * sign);
+  return v;
 }
 
 // The 0x80 bit of every byte of w that holds a NaN code.
@@ -179,16 +217,22 @@ __device__ __forceinline__ unsigned nan_bytes(int w) {
 //
 // The scales stay out of the operands: the keys' goes into the softmax scale, the values' onto each page's
 // sum as it is added to the running one, so that probabilities (at most 1) are what fp16 rounds.
+//
+// What bounds it while tokens are produced one by one is reading the cache. A wave holds one page's keys
+// and one page's values and always has one of the two on its way: the next page's keys are asked for when
+// the scores are done, the next values when the sums are. (Two whole pages in registers left one wave a
+// SIMD at head width 128.) The loads go through buffer descriptors that end at the page, or at nothing
+// behind the last page, so that every round issues the same loads and waits for the older half only.
 constexpr int kAttendWaves = 4;
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kAttendWaves) void attend8_kernel(Attend8Args a) {
+__global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_kernel(Attend8Args a) {
   typedef typename Vec8<T>::V V8;
   constexpr int ND = D / 16;              // channel tiles
   constexpr int NK = D / 32;              // products per key tile
   __shared__ float sm[kAttendWaves][16], sl[kAttendWaves][16];
   __shared__ float sacc[kAttendWaves][16][D + 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int b = blockIdx.z, split = blockIdx.x, tiles = (a.rows + 15) / 16;
   const int h = blockIdx.y / tiles, row0 = blockIdx.y % tiles * 16;
   const int row = row0 + r;
@@ -201,134 +245,214 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend8_kernel(Attend8Args 
   const int least = key_limit(a, len, start, row0);                                // the tile's first row
   const int most = key_limit(a, len, start, min(row0 + 15, a.rows - 1));           // and its last
   const int npages = (most + kPage8 - 1) / kPage8;
-  const int chunk = (npages + a.splits - 1) / a.splits;
-  const int p0 = split * chunk, p1 = min(p0 + chunk, npages);
+  const int chunk = max((npages + a.splits - 1) / a.splits, a.chunk);
+  const int p0 = a.splits > 1 ? split * chunk : 0, p1 = a.splits > 1 ? min(p0 + chunk, npages) : npages;
+  if (p0 >= p1 && split > 0) return;   // the join knows that there is no such part
 
+  const float c = soft_scale(a);
   V8 q[NK];
-  if (real) {
+  {
     const T* qp = (const T*)a.q + b * a.qs[0] + (int64_t)(row / a.G) * a.qs[1] + (int64_t)(h * a.G + row % a.G) * a.qs[2];
     // D >= 64: the products 2 j and 2 j + 1 take channels 64 j + 16 g + 0..7 and + 8..15, so that a
     // key's bytes are read 16 at a time.
 #pragma unroll
-    for (int j = 0; j < NK; j++) {
-      const int c = D == 32 ? 8 * g : 64 * (j / 2) + 16 * g + 8 * (j % 2);
-      __builtin_memcpy(&q[j], qp + c, 16);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < NK; j++) q[j] = V8{};
+    for (int j = 0; j < NK; j++) q[j] = query8<T>(a, qp, D == 32 ? 8 * g : 64 * (j / 2) + 16 * g + 8 * (j % 2), real);
   }
 
-  f32x4 acc[ND];
+  float acc[ND][4];   // single numbers: as vectors, every branch that changes them copies them
 #pragma unroll
-  for (int d = 0; d < ND; d++) acc[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[d][i] = 0.f;
   float m = -__builtin_inff(), l = 0.f;
+  uint64_t poison = 0;   // bit 4 d + i: acc[d][i] holds a NaN value that its query sees
 
-  for (int p = p0 + wave; p < p1; p += kAttendWaves) {
-    int page = a.table[b * a.tp + p];
+  const int32_t* table = a.table + b * a.tp;
+  const unsigned koff = (unsigned)(16 * (r >> 2) + (r & 3)) * D + (D == 32 ? 8 : 16) * g;
+  const unsigned voff = (unsigned)r * kPage8 + 16 * g;
+  i32x4 kc[D == 32 ? 2 : D / 16];   // a page's keys (head width 32: two tiles of 8 bytes in one)
+  i32x4 vc[ND];
+  int ks, vs;
+  // Where page p of the sequence stands (its head's place in the cache), and whether the cache has it.
+  struct Place {
+    int64_t at;
+    bool missing;
+  };
+  int none = 0;
+  asm volatile("" : "+v"(none));
+  const auto place = [&](int page) {
     const bool missing = (unsigned)page >= (unsigned)a.pages;
-    if (missing) page = 0;
-    const int64_t at = (int64_t)page * a.H + h;
-    const uint8_t* kp = a.k + at * (kPage8 * D);
-    const uint8_t* vp = a.v + at * (kPage8 * D);
-    const float vscale = scale_of(a.vs[at]);
-    const float kscale = missing ? __builtin_nanf("") : a.scale * scale_of(a.ks[at]);
+    return Place{(int64_t)(missing ? 0 : page) * a.H + h, missing};
+  };
+  const auto load_k = [&](Place t, int p) {
+    const __amdgpu_buffer_rsrc_t kr = make_rsrc(a.k + t.at * (kPage8 * D), p < p1 ? (unsigned)(kPage8 * D) : 0u);
+    ks = scale_entry(a.ks, t.at, none);
+    if constexpr (D == 32) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(kr, koff, 4 * i * D, 0);
+        kc[i / 2][i % 2 * 2] = (int)w[0];
+        kc[i / 2][i % 2 * 2 + 1] = (int)w[1];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < NK / 2; j++) kc[i * (NK / 2) + j] = buffer_load16<i32x4>(kr, koff, 4 * i * D + 64 * j);
+    }
+  };
+  const auto load_v = [&](Place t, int p) {
+    const __amdgpu_buffer_rsrc_t vr = make_rsrc(a.v + t.at * (kPage8 * D), p < p1 ? (unsigned)(kPage8 * D) : 0u);
+    vs = scale_entry(a.vs, t.at, none);
+#pragma unroll
+    for (int d = 0; d < ND; d++) vc[d] = buffer_load16<i32x4>(vr, voff, d * 16 * kPage8);
+  };
+
+  // Page numbers are known two rounds ahead; behind the last page the last one's is read again.
+  const int last = max(p1 - 1, 0);
+  const auto entry = [&](int p) { return table_entry(table, min(p, last)); };
+  int p = p0 + wave;
+  Place now = place(entry(p)), next = place(entry(p + kAttendWaves));
+  int after = entry(p + 2 * kAttendWaves);
+  load_k(now, p);
+  load_v(now, p);
+  for (; p < p1; p += kAttendWaves) {
+    const float grow = score_scale(c, ks);
     const int base = p * kPage8 + 16 * g;   // the lane's first token
     float s[16];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      f32x4 c = {0.f, 0.f, 0.f, 0.f};
-      const uint8_t* kr = kp + (16 * (r >> 2) + 4 * t + (r & 3)) * D;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      V8 kv;
       if constexpr (D == 32) {
-        const i32x2 w = *reinterpret_cast<const i32x2*>(kr + 8 * g);
-        V8 kv;
-        codes_as(w[0], w[1], kv);
-        c = mfma_q(kv, q[0], c);
+        codes_as(kc[t / 2][t % 2 * 2], kc[t / 2][t % 2 * 2 + 1], kv);
+        o = mfma_q(kv, q[0], o);
       } else {
 #pragma unroll
         for (int j = 0; j < NK / 2; j++) {
-          const i32x4 w = *reinterpret_cast<const i32x4*>(kr + 64 * j + 16 * g);
-          V8 kv;
+          const i32x4 w = kc[t * (NK / 2) + j];
           codes_as(w[0], w[1], kv);
-          c = mfma_q(kv, q[2 * j], c);
+          o = mfma_q(kv, q[2 * j], o);
           codes_as(w[2], w[3], kv);
-          c = mfma_q(kv, q[2 * j + 1], c);
+          o = mfma_q(kv, q[2 * j + 1], o);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; i++) s[4 * t + i] = c[i] * kscale;
+      for (int i = 0; i < 4; i++) s[4 * t + i] = o[i];
+      __builtin_amdgcn_sched_barrier(0);   // one tile's widened codes at a time
     }
+    load_k(next, p + kAttendWaves);
+    __builtin_amdgcn_sched_barrier(0);
+    const float vscale = scale_of(vs);
+    if (now.missing && p * kPage8 < limit) l = __builtin_nanf("");   // page 0 was read in its place
     const bool cut = p * kPage8 + kPage8 > least;   // some query does not see the whole page
     if (cut) {
+      int left = limit - base;
+      pin_value(left);
 #pragma unroll
       for (int i = 0; i < 16; i++)
-        if (base + i >= limit) s[i] = -__builtin_inff();
+        if (i >= left) s[i] = -__builtin_inff();
     }
     float mx = s[0];
 #pragma unroll
-    for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+    for (int i = 1; i < 15; i += 2) mx = max3_f(mx, s[i], s[i + 1]);
+    mx = max3_f(mx, s[15], s[15]);
     const auto x16 = __builtin_amdgcn_permlane16_swap(__float_as_int(mx), __float_as_int(mx), false, false);
-    mx = fmaxf(__int_as_float(x16[0]), __int_as_float(x16[1]));
+    mx = max3_f(__int_as_float(x16[0]), __int_as_float(x16[1]), __int_as_float(x16[1]));
     const auto x32 = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
-    mx = fmaxf(__int_as_float(x32[0]), __int_as_float(x32[1]));
-    const float mn = fmaxf(m, mx);
+    const float mn = max3_f(m, __int_as_float(x32[0]) * grow, __int_as_float(x32[1]) * grow);
     const float ref = mn == -__builtin_inff() ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = mn;
-    l *= alpha;
-    f16x8 pr[2];
+    if (__any(mn != m)) {
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+      l *= alpha;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const float e = __builtin_amdgcn_exp2f(s[i] - ref);
-      l += e;
-      pr[i / 8][i % 8] = (f16)e;
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[d][i] *= alpha;
+      m = mn;
+    }
+    f16x8 pr[2];
+    // Eight at a time, summed as they come (left alone, the sums are made behind the products below).
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * u + i], grow, -ref));
+        sum[i & 1] += e;
+        pr[u][i] = (f16)e;
+      }
+      l += sum[0] + sum[1];
+      pin_value(l);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (cut) {
+      // Tokens behind the sequence are whatever was there: zero them. Tokens that only some of the queries
+      // see may be NaN, and zero times NaN is not zero: their codes are zeroed too, and a product of their
+      // places with 1 for each token seen says which sums they belong in (one bit each, applied last).
+      const int left = len - base;
+      unsigned nan = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int n = left - 4 * i;
+        const int keep = n >= 4 ? -1 : n <= 0 ? 0 : (int)(0xffffffffu >> (32 - 8 * n));
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          vc[d][i] &= keep;
+          nan |= nan_bytes(vc[d][i]);
+        }
+      }
+      if (__any(nan != 0)) {
+        f16x8 seen[2];
+#pragma unroll
+        for (int i = 0; i < 16; i++) seen[i / 8][i % 8] = base + i < limit ? (f16)1.f : (f16)0.f;
+        const __amdgpu_buffer_rsrc_t vr = make_rsrc(a.v + now.at * (kPage8 * D), (unsigned)(kPage8 * D));
+#pragma unroll 1
+        for (int d = 0; d < ND; d++) {
+          const i32x4 w = buffer_load16<i32x4>(vr, voff, d * 16 * kPage8);
+          f16x8 mk[2];
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            mk[i / 8][i % 8] = i < left && ((nan_bytes(w[i / 4]) >> (8 * (i % 4))) & 0x80) ? (f16)1.f : (f16)0.f;
+          const f32x4 marks = mfma16(mk[1], seen[1], mfma16(mk[0], seen[0], (f32x4){0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (marks[i] > 0.f) poison |= 1ull << (4 * d + i);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            int w = vc[d][i];
+            pin_value(w);   // computed anew: kept from above, the bytes' bits double the registers
+            vc[d][i] = w & ~(int)((nan_bytes(w) >> 7) * 255u);
+          }
+      }
     }
 #pragma unroll
     for (int d = 0; d < ND; d++) {
-      i32x4 w = *reinterpret_cast<const i32x4*>(vp + (16 * d + r) * kPage8 + 16 * g);
-      bool poisoned = false;
-      f16x8 seen[2];
-      if (cut) {
-        // Tokens behind the sequence are whatever was there: zero them. Tokens that only some of the
-        // queries see may be NaN, and zero times NaN is not zero: they are taken out of the product, and
-        // a product of their places with 1 for each token seen says which sums they belong in.
-        const int left = len - base;
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int n = left - 4 * i;
-          if (n < 4) w[i] = n <= 0 ? 0 : w[i] & (int)(0xffffffffu >> (32 - 8 * n));
-          nan = nan || nan_bytes(w[i]) != 0;
-        }
-        poisoned = __any(nan);
-      }
-      f32x4 c = {0.f, 0.f, 0.f, 0.f};
-      f32x4 marks = {0.f, 0.f, 0.f, 0.f};
-      if (poisoned) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) seen[i / 8][i % 8] = base + i < limit ? (f16)1.f : (f16)0.f;
-        f16x8 mk[2];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const unsigned nb = nan_bytes(w[i]);
-#pragma unroll
-          for (int j = 0; j < 4; j++) mk[i / 2][i % 2 * 4 + j] = (nb >> (8 * j)) & 0x80 ? (f16)1.f : (f16)0.f;
-          w[i] &= ~(int)((nb >> 7) * 255u);
-        }
-        marks = mfma16(mk[0], seen[0], marks);
-        marks = mfma16(mk[1], seen[1], marks);
-      }
       f16x8 v0, v1;
-      codes_as(w[0], w[1], v0);
-      codes_as(w[2], w[3], v1);
-      c = mfma16(v0, pr[0], c);
-      c = mfma16(v1, pr[1], c);
+      codes_as(vc[d][0], vc[d][1], v0);
+      codes_as(vc[d][2], vc[d][3], v1);
+      const f32x4 o = mfma16(v1, pr[1], mfma16(v0, pr[0], (f32x4){0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (poisoned && marks[i] > 0.f) c[i] = __builtin_nanf("");
-        acc[d][i] = acc[d][i] * alpha + c[i] * vscale;
-      }
+      for (int i = 0; i < 4; i++) acc[d][i] += o[i] * vscale;
+      if (d % 2) __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(next, p + kAttendWaves);
+    __builtin_amdgcn_sched_barrier(0);
+    now = next;
+    next = place(after);
+    after = entry(p + 3 * kAttendWaves);
+  }
+
+  if (poison) {
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (poison >> (4 * d + i) & 1) acc[d][i] = __builtin_nanf("");
   }
   // l over the four lane groups of a query, then the waves' states through LDS.
   const auto l16 = __builtin_amdgcn_permlane16_swap(__float_as_int(l), __float_as_int(l), false, false);
@@ -340,7 +464,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend8_kernel(Attend8Args 
     sl[wave][r] = l;
   }
 #pragma unroll
-  for (int d = 0; d < ND; d++) *reinterpret_cast<f32x4*>(&sacc[wave][r][16 * d + 4 * g]) = acc[d];
+  for (int d = 0; d < ND; d++) *reinterpret_cast<f32x4*>(&sacc[wave][r][16 * d + 4 * g]) = (f32x4){acc[d][0], acc[d][1], acc[d][2], acc[d][3]};
   __syncthreads();
   const int64_t bh = (int64_t)b * a.H + h;
   for (int e = threadIdx.x; e < 16 * D / 4; e += 64 * kAttendWaves) {
@@ -376,50 +500,446 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend8_kernel(Attend8Args 
   }
 }
 
-// Joins the splits of a row: a thread takes four channels.
+// ------------------------------------------------------------------- many queries of a cache head
+//
+// A workgroup takes 128 rows (queries x grouped heads), a wave 32 of them, and shares each page through
+// LDS as 16-bit operands, so that a code is widened once for all of them. S^T = K Q^T and O^T += V^T P^T
+// on 32 x 32 x 16 products: lane l holds query column l % 32, h = l / 32. Row 8 q + 4 h + i of a 32-token
+// key tile is its token 16 h + 4 q + i, so that the scores a lane receives are 16 tokens in a row and the
+// probabilities go into the second product as they lie, against eight tokens side by side of the turned
+// values.
+//
+// LDS holds the operands in fragment order (a lane's 16 bytes at its place), the fragments padded so that
+// 16 widening lanes, which write to several fragments at once, meet all banks once; two page buffers, one
+// barrier a page. The next page's codes are asked for before a page's products and widened behind them.
+//
+// A page's scales stay out of the 16-bit values, as above: the keys' goes with the softmax's into the
+// exponential's argument (whose sign goes into the queries), the values' onto the page's sums.
+constexpr int kWideRows = 128;
+
+__device__ __forceinline__ f32x16 mfma_w(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma_w(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// 16 lanes widen the keys' pieces j of 256 / D tokens and the values' four pieces of four channels: a key
+// fragment's pad moves its 16-byte places by 256 / D a piece, a value fragment's by 4, and its
+// second half of tokens by 4 again.
+template <int D>
+struct WideLds {
+  static constexpr int KF = 1024 + 4096 / D, VH = 512 + 64, VF = 2 * 512 + 64;
+  static constexpr int KEYS = 2 * (D / 16) * KF, BUF = KEYS + 4 * (D / 32) * VF;
+};
+
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Args a, int64_t total) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t at = e / (D / 4);
-  if (at >= total) return;
-  const int c = (int)(e % (D / 4)) * 4;
-  const float* ml = a.part + total * a.splits * D + at * a.splits * 2;
-  float mt = -__builtin_inff();
-  for (int s = 0; s < a.splits; s++)
-    if (ml[2 * s + 1] != 0.f) mt = fmaxf(mt, ml[2 * s]);
-  float lt = 0.f;
-  f32x4 ot = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; s++) {
-    if (ml[2 * s + 1] == 0.f) continue;   // a split without a token that the row sees
-    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - mt);
-    lt += ml[2 * s + 1] * f;
-    ot += *reinterpret_cast<const f32x4*>(a.part + (at * a.splits + s) * D + c) * f;
-  }
-  const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  const int64_t bh = at / a.rows;
-  const int row = (int)(at % a.rows), h = (int)(bh % a.H);
-  T* op = (T*)a.o + bh / a.H * a.os[0] + (int64_t)(row / a.G) * a.os[1] + (int64_t)(h * a.G + row % a.G) * a.os[2] + c;
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_wide_kernel(Attend8Args a) {
+  typedef typename Vec8<T>::V V8;
+  constexpr int NJ = D / 16;               // products per key tile
+  constexpr int NT = D / 32;               // channel tiles
+  constexpr int RAW = D / 64;              // 16-byte pieces of a page's keys (values) a thread widens
+  typedef WideLds<D> L;
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ int flags[2];                 // the last page of each buffer that holds a NaN value code
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
+  const int b = blockIdx.z, split = blockIdx.x, tiles = (a.rows + kWideRows - 1) / kWideRows;
+  const int h = blockIdx.y / tiles, row0 = (tiles - 1 - blockIdx.y % tiles) * kWideRows;   // causal: longest first
+  const int wrow = row0 + 32 * wave, row = wrow + r;
+  const bool real = row < a.rows;
+  const int raw = a.lengths[b];
+  const bool too_long = raw > (int64_t)a.width * kPage8;
+  const int len = too_long || raw < 0 ? 0 : raw;
+  const int64_t start = a.starts ? a.starts[b] : 0;
+  const int limit = real ? key_limit(a, len, start, row) : 0;
+  const int least = wrow < a.rows ? key_limit(a, len, start, wrow) : 0;                             // of the wave
+  const int wmost = wrow < a.rows ? key_limit(a, len, start, min(wrow + 31, a.rows - 1)) : 0;
+  const int tleast = key_limit(a, len, start, row0);                                                // of the tile
+  const int most = key_limit(a, len, start, min(row0 + kWideRows, a.rows) - 1);
+  const int npages = (most + kPage8 - 1) / kPage8;
+  const int chunk = max((npages + a.splits - 1) / a.splits, a.chunk);
+  const int p0 = a.splits > 1 ? split * chunk : 0, p1 = a.splits > 1 ? min(p0 + chunk, npages) : npages;
+  if (p0 >= p1 && split > 0) return;   // the join knows that there is no such part
+
+  const float c = soft_scale(a);
+  V8 q[NJ];
+  {
+    const T* qp = (const T*)a.q + b * a.qs[0] + (int64_t)(row / a.G) * a.qs[1] + (int64_t)(h * a.G + row % a.G) * a.qs[2];
 #pragma unroll
-  for (int i = 0; i < 4; i++) op[i] = (T)(ot[i] * inv);
+    for (int j = 0; j < NJ; j++) q[j] = query8<T>(a, qp, 16 * j + 8 * hh, real);
+  }
+  float acc[NT][16];   // single numbers: as vectors, every branch that changes them copies them
+#pragma unroll
+  for (int d = 0; d < NT; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;
+  uint64_t poison[(NT + 3) / 4] = {};   // 16 bits a channel tile: sums that hold a NaN value their query sees
+
+  const int32_t* table = a.table + b * a.tp;
+  int none = 0;
+  asm volatile("" : "+v"(none));
+  const auto entry = [&](int p) { return table_entry(table, min(p, p1 - 1)); };
+  const auto place = [&](int page) { return (int64_t)((unsigned)page >= (unsigned)a.pages ? 0 : page) * a.H + h; };
+
+  i32x4 kraw[RAW], vraw[RAW];
+  int ks, vs;
+  // A thread's pieces of a page: keys in rows of D bytes, values in rows of 64.
+  const auto load = [&](int64_t at) {
+    ks = scale_entry(a.ks, at, none);
+    vs = scale_entry(a.vs, at, none);
+    const i32x4* kp = reinterpret_cast<const i32x4*>(a.k + at * (kPage8 * D));
+    const i32x4* vp = reinterpret_cast<const i32x4*>(a.v + at * (kPage8 * D));
+#pragma unroll
+    for (int i = 0; i < RAW; i++) {
+      kraw[i] = kp[tid + 256 * i];
+      vraw[i] = vp[tid + 256 * i];
+    }
+  };
+  // Widen page p's pieces into buffer p & 1.
+  const auto widen = [&](int p) {
+    uint8_t* kb = lds + (p & 1) * L::BUF;
+    uint8_t* vb = kb + L::KEYS;
+    const bool cut = p * kPage8 + kPage8 > tleast;
+#pragma unroll
+    for (int i = 0; i < RAW; i++) {
+      const int e = tid + 256 * i, key = e / (D / 16), j = e % (D / 16);
+      const int t = key & 31, at = 8 * (t >> 2 & 3) + 4 * (t >> 4) + (t & 3);   // the token's row of its tile
+      V8 w;
+      uint8_t* f = kb + ((key >> 5) * NJ + j) * L::KF + at * 16;
+      codes_as(kraw[i][0], kraw[i][1], w);
+      *reinterpret_cast<V8*>(f) = w;
+      codes_as(kraw[i][2], kraw[i][3], w);
+      *reinterpret_cast<V8*>(f + 512) = w;
+    }
+#pragma unroll
+    for (int i = 0; i < RAW; i++) {
+      const int e = tid + 256 * i, d = e >> 2, part = e & 3;   // channel; 16 tokens from 16 part on
+      if (cut) {   // tokens behind the sequence and NaN codes as zero; see the streaming kernel
+        const int left = len - p * kPage8 - 16 * part;
+        unsigned nan = 0;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const int n = left - 4 * x;
+          int w = vraw[i][x] & (n >= 4 ? -1 : n <= 0 ? 0 : (int)(0xffffffffu >> (32 - 8 * n)));
+          const unsigned nb = nan_bytes(w);
+          nan |= nb;
+          vraw[i][x] = w & ~(int)((nb >> 7) * 255u);
+        }
+        if (nan) flags[p & 1] = p;
+      }
+      f16x8 w;
+      uint8_t* f = vb + ((d >> 5) * 4 + (part >> 1) * 2) * L::VF + (part & 1) * L::VH + (d & 31) * 16;
+      codes_as(vraw[i][0], vraw[i][1], w);
+      *reinterpret_cast<f16x8*>(f) = w;
+      codes_as(vraw[i][2], vraw[i][3], w);
+      *reinterpret_cast<f16x8*>(f + L::VF) = w;
+    }
+  };
+
+  const auto attend = [&](int p, bool missing, int ksb, int vsb) {
+    const uint8_t* kb = lds + (p & 1) * L::BUF + lane * 16;
+    const uint8_t* vb = lds + (p & 1) * L::BUF + L::KEYS + hh * L::VH + r * 16;
+    f32x16 sv[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) sv[t][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) sv[t] = mfma_w(*reinterpret_cast<const V8*>(kb + (t * NJ + j) * L::KF), q[j], sv[t]);
+      if (j % 2) __builtin_amdgcn_sched_barrier(0);   // bounds the operands read ahead
+    }
+    float s[2][16];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[t][e] = sv[t][e];
+    const int base = p * kPage8 + 16 * hh;   // score e of tile t is token base + 32 t + e
+    if (missing && p * kPage8 < limit) l = __builtin_nanf("");   // page 0 was read in its place
+    if (p * kPage8 + kPage8 > least) {
+      int left = limit - base;
+      pin_value(left);
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+          if (32 * t + e >= left) s[t][e] = -__builtin_inff();
+    }
+    float mx = max3_f(s[0][0], s[1][0], s[0][1]);
+    mx = max3_f(mx, s[1][1], s[1][1]);
+#pragma unroll
+    for (int e = 2; e < 16; e++) mx = max3_f(mx, s[0][e], s[1][e]);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
+    const float kc = score_scale(c, ksb);
+    const float mn = max3_f(m, __int_as_float(x[0]) * kc, __int_as_float(x[1]) * kc);
+    const float ref = mn == -__builtin_inff() ? 0.f : mn;
+    if (__any(mn != m)) {
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[d][e] *= alpha;
+      m = mn;
+    }
+    f16x8 pr[2][2];
+    // Eight at a time, summed as they come: left alone, the sums are made behind the products below, and
+    // all 32 probabilities stay in fp32 until then.
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + e], kc, -ref));
+          sum[e & 1] += w;
+          pr[t][u][e] = (f16)w;
+        }
+        l += sum[0] + sum[1];
+        pin_value(l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    const float vscale = scale_of(vsb);
+#pragma unroll
+    for (int d = 0; d < NT; d++) {
+      f32x16 o;
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+          o = mfma_w(*reinterpret_cast<const f16x8*>(vb + (d * 4 + t * 2 + u) * L::VF), pr[t][u], o);
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[d][e] += o[e] * vscale;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Which sums a page's NaN values belong in: their places times 1 for each token that a query sees.
+  const auto mark = [&](int p, int64_t at) {
+    const uint8_t* vp = a.v + at * (kPage8 * D) + r * kPage8 + 16 * hh;
+#pragma unroll 1
+    for (int d = 0; d < NT; d++) {
+      f32x16 marks;
+#pragma unroll
+      for (int e = 0; e < 16; e++) marks[e] = 0.f;
+#pragma unroll 1
+      for (int tu = 0; tu < 4; tu++) {
+        const i32x2 w = *reinterpret_cast<const i32x2*>(vp + d * 32 * kPage8 + 32 * (tu / 2) + 8 * (tu % 2));
+        const int base = p * kPage8 + 16 * hh + 32 * (tu / 2) + 8 * (tu % 2);
+        f16x8 mk, seen;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          mk[e] = base + e < len && ((nan_bytes(w[e / 4]) >> (8 * (e % 4))) & 0x80) ? (f16)1.f : (f16)0.f;
+          seen[e] = base + e < limit ? (f16)1.f : (f16)0.f;
+        }
+        marks = mfma_w(mk, seen, marks);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (marks[e] > 0.f) poison[d / 4] |= 1ull << (16 * (d % 4) + e);
+    }
+  };
+
+  if (tid < 2) flags[tid] = -1;
+  __syncthreads();
+  if (p0 < p1) {
+    int page = entry(p0), next = entry(p0 + 1);
+    int64_t at = place(page);
+    load(at);
+    widen(p0);
+    for (int p = p0; p < p1; p++) {
+      const int ksb = __builtin_amdgcn_readfirstlane(ks), vsb = __builtin_amdgcn_readfirstlane(vs);
+      const int64_t nat = place(next);
+      const int after = entry(p + 2);
+      if (p + 1 < p1) load(nat);
+      // Page p stands in its buffer, and every wave is done with the other one. (__syncthreads would wait
+      // for the codes asked for above.)
+      ring_barrier();
+      if (p * kPage8 < wmost) {
+        attend(p, (unsigned)page >= (unsigned)a.pages, ksb, vsb);
+        if (p * kPage8 + kPage8 > tleast && flags[p & 1] == p) mark(p, at);
+      }
+      if (p + 1 < p1) widen(p + 1);
+      page = next;
+      next = after;
+      at = nat;
+    }
+  }
+
+#pragma unroll
+  for (int d = 0; d < NT; d++)
+    if (poison[d / 4])
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (poison[d / 4] >> (16 * (d % 4) + e) & 1) acc[d][e] = __builtin_nanf("");
+  const auto l32 = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
+  l = __int_as_float(l32[0]) + __int_as_float(l32[1]);
+  if (too_long) l = __builtin_nanf("");
+  if (!real) return;
+  if (a.splits > 1) {
+    const int64_t bh = (int64_t)b * a.H + h, place8 = (bh * a.rows + row) * a.splits + split;
+    const int64_t all = (int64_t)gridDim.z * a.H * a.rows * a.splits;
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+      for (int g = 0; g < 4; g++)
+        *reinterpret_cast<f32x4*>(a.part + place8 * D + 32 * d + 8 * g + 4 * hh) =
+            (f32x4){acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+    if (hh == 0) {
+      a.part[all * D + 2 * place8] = m == -__builtin_inff() ? 0.f : m;
+      a.part[all * D + 2 * place8 + 1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* op = (T*)a.o + b * a.os[0] + (int64_t)(row / a.G) * a.os[1] + (int64_t)(h * a.G + row % a.G) * a.os[2];
+#pragma unroll
+  for (int d = 0; d < NT; d++)
+#pragma unroll
+    for (int g = 0; g < 2; g++) {   // halves exchanged between a row's two lanes: eight channels each
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(acc[d][8 * g + e]),
+                                                        __float_as_int(acc[d][8 * g + 4 + e]), false, false);
+        f[e] = __int_as_float(x[0]) * inv;
+        f[4 + e] = __int_as_float(x[1]) * inv;
+      }
+      store8(op + 32 * d + 16 * g + 8 * hh, f);
+    }
 }
 
 template <typename T, int D>
-void launch_d(const Attend8Args& a, int batch, hipStream_t st) {
-  const dim3 grid((unsigned)a.splits, (unsigned)(a.H * ((a.rows + 15) / 16)), (unsigned)batch);
-  hipLaunchKernelGGL((attend8_kernel<T, D>), grid, dim3(64 * kAttendWaves), 0, st, a);
-  if (a.splits > 1) {
-    const int64_t total = (int64_t)batch * a.H * a.rows;
-    hipLaunchKernelGGL((attend8_merge_kernel<T, D>), dim3((unsigned)((total * (D / 4) + 255) / 256)), dim3(256), 0, st, a,
-                       total);
+int launch_wide(const Attend8Args& a, dim3 grid, hipStream_t st) {
+  constexpr int LDS = 2 * WideLds<D>::BUF;
+  const auto kern = attend8_wide_kernel<T, D>;
+  if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+    return check_launch("cache8_attention: set LDS size");
+  hipLaunchKernelGGL(kern, grid, dim3(256), LDS, st, a);
+  return LDX_OK;
+}
+
+// Parts that a sequence of npages has (of a.splits possible ones), at least one.
+__device__ __forceinline__ int part_count(const Attend8Args& a, int npages) {
+  const int chunk = max((npages + a.splits - 1) / a.splits, a.chunk);
+  return max((npages + chunk - 1) / chunk, 1);
+}
+
+// The output of four channels of a row.
+template <typename T>
+__device__ __forceinline__ void put4(const Attend8Args& a, int b, int h, int row, int channel, f32x4 o, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* op = (T*)a.o + b * a.os[0] + (int64_t)(row / a.G) * a.os[1] + (int64_t)(h * a.G + row % a.G) * a.os[2] + channel;
+#pragma unroll
+  for (int i = 0; i < 4; i++) op[i] = (T)(o[i] * inv);
+}
+
+// Parts that a row's sequence was given.
+__device__ __forceinline__ int parts_of(const Attend8Args& a, int b, int row) {
+  const int raw = a.lengths[b];
+  const int len = raw < 0 || raw > (int64_t)a.width * kPage8 ? 0 : raw;
+  // The last row of a workgroup's tile says how many pages it reads.
+  const int most = key_limit(a, len, a.starts ? a.starts[b] : 0, min((row / a.tile + 1) * a.tile, a.rows) - 1);
+  return part_count(a, (most + kPage8 - 1) / kPage8);
+}
+
+// Joins the parts of rows, few parts (at most kFewParts): a thread takes four channels of a row.
+constexpr int kFewParts = 8;
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attend8_join_kernel(Attend8Args a, int64_t total) {
+  constexpr int PER = D / 4;
+  const int64_t at = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER, bh = at / a.rows;
+  if (at >= total) return;
+  const int b = (int)(bh / a.H), h = (int)(bh % a.H), row = (int)(at % a.rows), c = threadIdx.x % PER;
+  const int parts = parts_of(a, b, row);
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part + total * a.splits * D) + at * a.splits;
+  float mt = -__builtin_inff();
+  for (int s = 0; s < parts; s++)
+    if (ml[s][1] != 0.f) mt = fmaxf(mt, ml[s][0]);   // a part without a token that the row sees has sum 0
+  float lt = 0.f;
+  f32x4 ot = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < parts; s++) {
+    const float f = ml[s][1] != 0.f ? __builtin_amdgcn_exp2f(ml[s][0] - mt) : 0.f;
+    lt += ml[s][1] * f;
+    ot += *reinterpret_cast<const f32x4*>(a.part + (at * a.splits + s) * D + 4 * c) * f;
   }
+  put4<T>(a, b, h, row, 4 * c, ot, lt);
+}
+
+// Joins the parts of a row, a workgroup each: the parts' weights side by side, then a thread takes four
+// channels of every (1024 / D)-th part and the threads of a channel are joined through LDS.
+constexpr int kMostParts = 1024;
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Args a) {
+  constexpr int PER = D / 4, LANES = 256 / PER;
+  __shared__ float weight[kMostParts];
+  __shared__ f32x4 so[LANES][PER];
+  __shared__ float red[8];
+  const int64_t total = gridDim.x, at = blockIdx.x, bh = at / a.rows;
+  const int b = (int)(bh / a.H), h = (int)(bh % a.H), row = (int)(at % a.rows), tid = threadIdx.x;
+  const int parts = parts_of(a, b, row);
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part + total * a.splits * D) + at * a.splits;
+  float mt = -__builtin_inff();
+  for (int s = tid; s < parts; s += 256) {
+    const f32x2 e = ml[s];
+    if (e[1] != 0.f) mt = fmaxf(mt, e[0]);   // a part without a token that the row sees has sum 0
+  }
+  mt = wave_max(mt);
+  if ((tid & 63) == 0) red[tid >> 6] = mt;
+  __syncthreads();
+  mt = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float lt = 0.f;
+  for (int s = tid; s < parts; s += 256) {
+    const f32x2 e = ml[s];
+    const float f = e[1] != 0.f ? __builtin_amdgcn_exp2f(e[0] - mt) : 0.f;
+    weight[s] = f;
+    lt += e[1] * f;
+  }
+  lt = wave_sum(lt);
+  if ((tid & 63) == 0) red[4 + (tid >> 6)] = lt;
+  __syncthreads();
+  lt = red[4] + red[5] + red[6] + red[7];
+  const int c = tid % PER, lane = tid / PER;
+  f32x4 ot = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = lane; s < parts; s += LANES)
+    ot += *reinterpret_cast<const f32x4*>(a.part + (at * a.splits + s) * D + 4 * c) * weight[s];
+  so[lane][c] = ot;
+  __syncthreads();
+  if (lane) return;
+#pragma unroll
+  for (int s = 1; s < LANES; s++) ot += so[s][c];
+  put4<T>(a, b, h, row, 4 * c, ot, lt);
+}
+
+template <typename T, int D>
+int launch_d(const Attend8Args& a, int batch, hipStream_t st) {
+  const dim3 grid((unsigned)a.splits, (unsigned)(a.H * ((a.rows + a.tile - 1) / a.tile)), (unsigned)batch);
+  if (a.tile == 16) {
+    hipLaunchKernelGGL((attend8_kernel<T, D>), grid, dim3(64 * kAttendWaves), 0, st, a);
+  } else if constexpr (D >= 64) {
+    if (int rc = launch_wide<T, D>(a, grid, st)) return rc;
+  }
+  const int64_t total = (int64_t)batch * a.H * a.rows;
+  constexpr int ROWS = 1024 / D;   // of a workgroup
+  if (a.splits > kFewParts)
+    hipLaunchKernelGGL((attend8_merge_kernel<T, D>), dim3((unsigned)total), dim3(256), 0, st, a);
+  else if (a.splits > 1)
+    hipLaunchKernelGGL((attend8_join_kernel<T, D>), dim3((unsigned)((total + ROWS - 1) / ROWS)), dim3(256), 0, st, a, total);
+  return check_launch("cache8_attention");
 }
 
 template <typename T>
-void launch_t(const Attend8Args& a, int D, int batch, hipStream_t st) {
-  if (D == 32) launch_d<T, 32>(a, batch, st);
-  else if (D == 64) launch_d<T, 64>(a, batch, st);
-  else if (D == 128) launch_d<T, 128>(a, batch, st);
-  else launch_d<T, 256>(a, batch, st);
+int launch_t(const Attend8Args& a, int D, int batch, hipStream_t st) {
+  if (D == 32) return launch_d<T, 32>(a, batch, st);
+  if (D == 64) return launch_d<T, 64>(a, batch, st);
+  if (D == 128) return launch_d<T, 128>(a, batch, st);
+  return launch_d<T, 256>(a, batch, st);
 }
 
 int check_cache(const char* what, const ldx_cache8& c) {
@@ -431,15 +951,43 @@ int check_cache(const char* what, const ldx_cache8& c) {
   return LDX_OK;
 }
 
-// Workgroups that a sequence's pages are spread over: enough that the launch fills the card.
-int split_count(const ldx_cache8_attention_args* p) {
-  const int64_t rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
-  const int64_t groups = (int64_t)p->batch * p->cache.heads * ((rows + 15) / 16);
-  int64_t s = 1024 / groups;
-  const int64_t most = (p->width + kAttendWaves - 1) / kAttendWaves;
-  if (s > most) s = most;
-  if (s > 64) s = 64;
-  return s < 1 ? 1 : (int)s;
+// How a call is laid out. The host knows only how many pages a table's row holds; the kernels divide the
+// pages that a sequence has.
+struct Plan {
+  bool wide;    // pages shared through LDS by 128 rows of a cache head, or streamed by 16
+  int splits;   // parts that a sequence's pages may be spread over
+};
+
+constexpr int kLeastChunk = 8;   // pages of a part at least: two for each streaming wave. (8 and 16: 4 sequences
+                                 // of 8,000 tokens 20 and 22 us, 8 of 5,000 at head width 256 22 and 28)
+
+Plan plan_of(const ldx_cache8_attention_args* p) {
+  const int D = p->cache.head_dim;
+  const int64_t heads = (int64_t)p->batch * p->cache.heads, rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
+  const int64_t most = (p->width + kLeastChunk - 1) / kLeastChunk;
+  Plan plan;
+  // A page of 16 rows costs a streaming wave about 0.6 / 1.5 / 3.0 us at head width 64 / 128 / 256 (0.38 at 32,
+  // and as much shared, so that is not done), shared 0.5 / 0.9 / 2.3, and sharing 10 to 20 us more at the start and end. From these sums
+  // of pages on it was ahead (4,096 queries of 4 heads behind 8,192 tokens 103 -> 84 / 262 -> 139 us at 64 /
+  // 128, 512 queries of 16 heads 200 -> 151 at 256; below, 4,096 queries behind 256 tokens 35 and 41 at 64).
+  const int64_t work = heads * ((rows + 15) / 16) * p->width;
+  plan.wide = rows >= kWideRows && work >= (D == 32 ? INT64_MAX : D == 64 ? 100000 : D == 128 ? 18000 : 9000);
+  int64_t s = 1;
+  if (plan.wide) {
+    // Rounds of workgroups on the CUs' places, the pages of a round, and what a part more costs to join.
+    const int64_t groups = heads * ((rows + kWideRows - 1) / kWideRows), places = D == 64 ? 768 : D == 128 ? 512 : 256;
+    double best = 1e30;
+    for (int64_t i = 1; i <= kFewParts && i <= most; i++) {
+      const double cost = (double)((groups * i + places - 1) / places) * ((p->width + i - 1) / i) + 3.0 * i;
+      if (cost < best) best = cost, s = i;
+    }
+  } else {
+    // Two workgroups a CU (256 to 1,024 parts in all were within a tenth for most calls, more slower).
+    s = 512 / (heads * ((rows + 15) / 16));
+    if (s > most) s = most;
+  }
+  plan.splits = (int)(s < 1 ? 1 : s > kMostParts ? kMostParts : s);
+  return plan;
 }
 
 size_t split_bytes(const ldx_cache8_attention_args* p, int splits) {
@@ -458,6 +1006,9 @@ int check_attention(const ldx_cache8_attention_args* p) {
   if (p->q_heads < 1 || p->q_heads % p->cache.heads)
     return fail("cache8_attention: %d query heads over %d cache heads", p->q_heads, p->cache.heads);
   const int64_t rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
+  if (rows * p->cache.heads * p->batch > 0x7fffffff)
+    return fail("cache8_attention: %d x %d queries of %d heads are more than one launch takes", p->batch, p->q_len,
+                p->q_heads);
   if ((rows + 15) / 16 * p->cache.heads > 65535)
     return fail("cache8_attention: %d queries of %d heads are more than one launch takes", p->q_len, p->q_heads);
   if (p->table_pitch < p->width) return fail("cache8_attention: table pitch below %d", p->width);
@@ -494,23 +1045,23 @@ extern "C" int ldx_cache8_append(const ldx_cache8_append_args* p, void* stream) 
 }
 
 extern "C" size_t ldx_cache8_attention_workspace_bytes(const ldx_cache8_attention_args* p) {
-  return check_attention(p) == LDX_OK ? split_bytes(p, split_count(p)) : 0;
+  return check_attention(p) == LDX_OK ? split_bytes(p, plan_of(p).splits) : 0;
 }
 
 extern "C" int ldx_cache8_attention(const ldx_cache8_attention_args* p, void* stream) {
   if (int rc = check_attention(p)) return rc;
-  int splits = split_count(p);
-  if (splits > 1 && (!p->workspace || p->workspace_bytes < split_bytes(p, splits))) splits = 1;
-  if (splits > 1 && (uintptr_t)p->workspace % 16) return fail("cache8_attention: workspace not aligned");
+  Plan plan = plan_of(p);
+  if (plan.splits > 1 && (!p->workspace || p->workspace_bytes < split_bytes(p, plan.splits))) plan.splits = 1;
+  if (plan.splits > 1 && (uintptr_t)p->workspace % 16) return fail("cache8_attention: workspace not aligned");
   const int G = p->q_heads / p->cache.heads;
   const Attend8Args a = {(const uint8_t*)p->cache.k, (const uint8_t*)p->cache.v, (const uint8_t*)p->cache.k_scales,
                          (const uint8_t*)p->cache.v_scales, p->cache.pages, p->cache.heads,
                          p->q, {p->q_stride[0], p->q_stride[1], p->q_stride[2]},
                          p->o, {p->o_stride[0], p->o_stride[1], p->o_stride[2]},
                          G, p->q_len, G * p->q_len, p->scale * 1.4426950408889634f,
-                         p->table, p->table_pitch, p->width, p->lengths, p->starts, splits, (float*)p->workspace};
+                         p->table, p->table_pitch, p->width, p->lengths, p->starts, plan.splits, kLeastChunk,
+                         plan.wide ? kWideRows : 16, (float*)p->workspace};
   hipStream_t st = as_stream(stream);
-  if (p->dtype == LDX_DTYPE_F16) launch_t<f16>(a, p->cache.head_dim, p->batch, st);
-  else launch_t<bf16>(a, p->cache.head_dim, p->batch, st);
-  return check_launch("cache8_attention");
+  return p->dtype == LDX_DTYPE_F16 ? launch_t<f16>(a, p->cache.head_dim, p->batch, st)
+                                   : launch_t<bf16>(a, p->cache.head_dim, p->batch, st);
 }

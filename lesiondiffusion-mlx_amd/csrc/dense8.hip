@@ -397,29 +397,29 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
 }
 
 template <typename T, int FN, int FM>
-void launch_big(const Dense8Args& a, hipStream_t st) {
+int launch_big(const Dense8Args& a, hipStream_t st) {
   typedef BigTile<FN, FM> B;
   const unsigned nt = (unsigned)((a.O + B::TN - 1) / B::TN), mt = (unsigned)((a.M + B::TM - 1) / B::TM);
-  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(dense8_big_kernel<T, FN, FM>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, B::LDS);
-  (void)once;
-  hipLaunchKernelGGL((dense8_big_kernel<T, FN, FM>), dim3(nt * mt), dim3(256), B::LDS, st, a, nt, mt);
+  const auto kern = dense8_big_kernel<T, FN, FM>;
+  if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, B::LDS) != hipSuccess)
+    return check_launch("dense8: set LDS size");
+  hipLaunchKernelGGL(kern, dim3(nt * mt), dim3(256), B::LDS, st, a, nt, mt);
+  return check_launch("dense8");
 }
 
 template <typename T>
-void launch(const Dense8Args& a, hipStream_t st) {
+int launch(const Dense8Args& a, hipStream_t st) {
   if (a.M > 64 && (a.wp | a.xp) < (1 << 22)) {
     // Rounds of workgroups (one 256 x 256 tile a CU, two of 128 x 128) times what a round was measured to
     // take, us: so much a block of 128 and so much to start and store.
     const auto cdiv = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
     const double wide = cdiv(cdiv(a.M, 256) * cdiv(a.O, 256), 256) * (1.32 * a.kb + 13.0);
     const double narrow = cdiv(cdiv(a.M, 128) * cdiv(a.O, 128), 512) * (0.93 * a.kb + 8.0);
-    if (wide < narrow) launch_big<T, 4, 4>(a, st);
-    else launch_big<T, 2, 2>(a, st);
-    return;
+    return wide < narrow ? launch_big<T, 4, 4>(a, st) : launch_big<T, 2, 2>(a, st);
   }
   const int64_t tiles = (a.M + 15) / 16 * ((a.O + 15) / 16);
   hipLaunchKernelGGL(dense8_tile_kernel<T>, dim3((unsigned)tiles), dim3(64 * kTileWaves), 0, st, a);
+  return check_launch("dense8");
 }
 
 int check_operand(const char* name, const void* codes, int64_t cp, const void* scales, int64_t sp, int kb) {
@@ -457,8 +457,5 @@ extern "C" int ldx_dense8(const ldx_dense8_args* p, void* stream) {
                         p->bias, p->residual, p->residual_pitch, p->y, p->y_pitch, p->rows, p->out_features, kb,
                         p->act, p->dtype};
   hipStream_t st = as_stream(stream);
-  if (p->dtype == LDX_DTYPE_F16) launch<f16>(a, st);
-  else if (p->dtype == LDX_DTYPE_BF16) launch<bf16>(a, st);
-  else launch<float>(a, st);
-  return check_launch("dense8");
+  return p->dtype == LDX_DTYPE_F16 ? launch<f16>(a, st) : p->dtype == LDX_DTYPE_BF16 ? launch<bf16>(a, st) : launch<float>(a, st);
 }

@@ -12,6 +12,7 @@ namespace ldx {
 constexpr int kBlock8 = LDX_BLOCK8;   // columns of a row that share a scale
 constexpr int kPage8 = LDX_PAGE8;     // tokens of a cache page
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 

@@ -169,7 +169,7 @@ def test_cache8_attention_refuses(pkg, bad) -> None:
 def test_cpu_tensors_are_refused(pkg) -> None:
     ops = pkg.ops
     x = torch.zeros(2, 8)
-    q = ops.Quantized8.empty((2,), 8, torch.device("cpu"))
+    q = ops.Quantized8.empty((2,), 8, x)
     cache = ops.Cache8.empty(2, 1, 32, device="cpu")
     ints = torch.zeros(1, dtype=torch.int32)
     for call in (lambda: ops.quantize8(x), lambda: ops.rms_norm(x, torch.ones(8)), lambda: ops.dense8(q, q),
@@ -651,11 +651,21 @@ def filled(pkg, dev, b, heads, d, width, seed=0, lengths=None):
     return cache, Pages(cache), table
 
 
-def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, seed=0, scale=None):
+# Columns of a page table with which 128 rows and more of one cache head share pages through LDS (the host
+# decides by the table's width); a table that is longer than its sequences is what serving keeps anyway.
+LONG = {64: 14000, 128: 2600, 256: 1300}
+
+
+def longer(table: torch.Tensor, width: int | None) -> torch.Tensor:
+    """``table`` followed by columns that name no page."""
+    return table if width is None else torch.nn.functional.pad(table, (0, width - table.shape[1]), value=-1)
+
+
+def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, seed=0, scale=None, long=None):
     scale = d ** -0.5 if scale is None else scale
     cache, ref, table = filled(pkg, dev, b, heads, d, width, seed, lengths)
     q = rand((b, heads * group, lq, d), seed + 7, t)
-    got = pkg.ops.cache8_attention(q.to(dev), cache, table.to(dev), lengths.to(dev), scale,
+    got = pkg.ops.cache8_attention(q.to(dev), cache, longer(table, long).to(dev), lengths.to(dev), scale,
                                    starts=None if starts is None else starts.to(dev))
     assert got.dtype == t and got.shape == q.shape
     want, allowed = attention_reference(ref, q, table, lengths, scale, starts)
@@ -688,6 +698,26 @@ def test_attention_causal(pkg, dev, heads, group, lq, d, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize(("heads", "group", "lq"), [(1, 1, 128), (2, 1, 129), (1, 3, 50), (2, 4, 65)])
+def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
+    """128 rows of a cache head and more: the last tile with one row, or full; lengths and starts as above."""
+    attention_case(pkg, dev, t, 7, heads, group, d, lq, ints(0, 1, 63, 64, 65, 300, 448), None, 7, seed=d + lq, long=LONG[d])
+    starts = ints(0, 1, 100, -3, 250, 63)
+    lengths = ints(lq, lq + 1, 100 + lq, lq, 250 + max(lq // 2, 1), 63 + lq)
+    attention_case(pkg, dev, t, 6, heads, group, d, lq, lengths, starts, 8, seed=d + lq, long=LONG[d])
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_of_many_rows_in_parts(pkg, dev, d) -> None:
+    """Sequences of unequal lengths spread over several workgroups, some of which find nothing to do."""
+    attention_case(pkg, dev, torch.float16, 3, 1, 2, d, 70, ints(5000, 700, 1), None, 80, long=LONG[d])
+    attention_case(pkg, dev, torch.bfloat16, 3, 1, 1, d, 200, ints(5000, 700, 200), ints(4800, 500, 0), 80, long=LONG[d])
+
+
+@gpu
 @pytest.mark.parametrize(("b", "heads", "group", "d", "n"), [(1, 1, 1, 64, 20000), (2, 2, 8, 128, 9001), (1, 1, 4, 256, 5000)])
 def test_attention_long(pkg, dev, b, heads, group, d, n) -> None:
     lengths = ints(*[n - 77 * i for i in range(b)])
@@ -702,11 +732,16 @@ def test_attention_scores_far_apart(pkg, dev, lq) -> None:
     attention_case(pkg, dev, torch.float16, 2, 2, 2, 64, lq, ints(300, 129), None, 5, scale=3.0)
     attention_case(pkg, dev, torch.bfloat16, 2, 2, 2, 128, lq, ints(300, 129), ints(200, 100), 5, scale=-2.0)
     attention_case(pkg, dev, torch.float16, 2, 1, 2, 64, lq, ints(300, 129), None, 5, scale=0.0)
+    if lq == 100:
+        attention_case(pkg, dev, torch.float16, 2, 2, 2, 64, lq, ints(300, 129), None, 5, scale=3.0, long=LONG[64])
+        attention_case(pkg, dev, torch.bfloat16, 2, 2, 2, 128, lq, ints(300, 129), ints(200, 100), 5, scale=-2.0, long=LONG[128])
+        attention_case(pkg, dev, torch.float16, 2, 1, 2, 64, lq, ints(300, 129), None, 5, scale=0.0, long=LONG[64])
 
 
 @gpu
-@pytest.mark.parametrize(("lq", "d"), [(1, 64), (9, 64), (70, 128), (200, 64), (130, 256)])
-def test_attention_loud_page_of_small_weight(pkg, dev, lq, d) -> None:
+@pytest.mark.parametrize(("lq", "d", "long"), [(1, 64, None), (9, 64, None), (70, 128, None), (200, 64, LONG[64]),
+                                               (130, 128, LONG[128]), (130, 256, LONG[256])])
+def test_attention_loud_page_of_small_weight(pkg, dev, lq, d, long) -> None:
     """A page whose values are 2^30 times the others' but whose keys nobody attends to: the small values
     of the others come out as they are."""
     cache, _, table = filled(pkg, dev, 1, 1, d, 4, seed=3)
@@ -717,20 +752,22 @@ def test_attention_loud_page_of_small_weight(pkg, dev, lq, d) -> None:
     pkg.ops.cache8_append(cache, k, v, table.to(dev), ints(0).to(dev))
     ref = Pages(cache)
     lengths = ints(256)
-    got = pkg.ops.cache8_attention(q, cache, table.to(dev), lengths.to(dev), 1.0).cpu().double()
+    got = pkg.ops.cache8_attention(q, cache, longer(table, long).to(dev), lengths.to(dev), 1.0).cpu().double()
     want, _ = attention_reference(ref, q.cpu(), table, lengths, 1.0, None)
     # equal probabilities of 1: their rounding is exact, the sums are fp32
     assert ((got - want).abs() <= want.abs() * half_step(torch.float16) + 300 * 2.0 ** -23 * 4).all()
 
 
 @gpu
-@pytest.mark.parametrize(("lq", "group", "d"), [(4, 1, 64), (70, 1, 64), (33, 4, 128), (200, 1, 32), (100, 2, 256)])
-def test_attention_nan_in_tokens_that_a_query_does_not_see(pkg, dev, lq, group, d) -> None:
+@pytest.mark.parametrize(("lq", "group", "d", "long"), [
+    (4, 1, 64, None), (70, 1, 64, None), (33, 4, 128, None), (200, 1, 32, None), (100, 2, 256, None),
+    (200, 1, 64, LONG[64]), (130, 2, 128, LONG[128]), (300, 1, 256, LONG[256])])
+def test_attention_nan_in_tokens_that_a_query_does_not_see(pkg, dev, lq, group, d, long) -> None:
     """A NaN key and a NaN value: queries before them are untouched, queries from them on are NaN (in that
     channel, for a value)."""
-    cache, _, table = filled(pkg, dev, 1, 1, d, 6, seed=1)
+    cache, _, table = filled(pkg, dev, 1, 1, d, 7, seed=1)
     q = rand((1, group, lq, d), 2, torch.float16).to(dev)
-    args = (table.to(dev), ints(100 + lq).to(dev), d ** -0.5)
+    args = (longer(table, long).to(dev), ints(100 + lq).to(dev), d ** -0.5)
     starts = ints(100).to(dev)
     clean = pkg.ops.cache8_attention(q, cache, *args, starts=starts)
     at = 100 + lq // 2
@@ -748,33 +785,33 @@ def test_attention_nan_in_tokens_that_a_query_does_not_see(pkg, dev, lq, group, 
 
 
 @gpu
-@pytest.mark.parametrize("lq", [1, 90])
-def test_attention_says_when_a_page_or_a_length_is_wrong(pkg, dev, lq) -> None:
+@pytest.mark.parametrize(("lq", "long"), [(1, None), (90, None), (150, LONG[64])])
+def test_attention_says_when_a_page_or_a_length_is_wrong(pkg, dev, lq, long) -> None:
     cache, _, table = filled(pkg, dev, 4, 2, 64, 5, seed=1)
     q = rand((4, 2, lq, 64), 2, torch.float16).to(dev)
     lengths = ints(320, 320, 130, 320)
-    good = pkg.ops.cache8_attention(q, cache, table.to(dev), lengths.to(dev), 0.1)
+    good = pkg.ops.cache8_attention(q, cache, longer(table, long).to(dev), lengths.to(dev), 0.1)
     table[1, 3], table[2, 3], table[3, 1] = 1 << 30, -7, -1      # sequence 2 does not reach its bad page
-    got = pkg.ops.cache8_attention(q, cache, table.to(dev), lengths.to(dev), 0.1)
+    got = pkg.ops.cache8_attention(q, cache, longer(table, long).to(dev), lengths.to(dev), 0.1)
     assert torch.equal(got[[0, 2]], good[[0, 2]]) and got[[1, 3]].isnan().all()
-    got = pkg.ops.cache8_attention(q, cache, table.to(dev), ints(320, -4, 321, 1 << 30).to(dev), 0.1)
+    got = pkg.ops.cache8_attention(q, cache, longer(table, long).to(dev), ints(320, -4, (long or 5) * 64 + 1, 1 << 30).to(dev), 0.1)
     assert torch.equal(got[0], good[0]) and (got[1] == 0).all() and got[2:].isnan().all()
 
 
 @gpu
-@pytest.mark.parametrize("lq", [1, 70])
-def test_attention_layouts(pkg, dev, lq) -> None:
+@pytest.mark.parametrize(("lq", "width"), [(1, 9), (70, 9), (140, LONG[64])])
+def test_attention_layouts(pkg, dev, lq, width) -> None:
     """Head-interleaved q and out, a table that is part of a wider one, out given."""
     cache, _, table = filled(pkg, dev, 2, 2, 64, 5, seed=1)
     q = rand((2, 4, lq, 64), 2, torch.bfloat16).to(dev)
     lengths = ints(300, 90).to(dev)
-    want = pkg.ops.cache8_attention(q, cache, table.to(dev), lengths, 0.1)
+    want = pkg.ops.cache8_attention(q, cache, longer(table, width - 4).to(dev), lengths, 0.1)
     inter = q.transpose(1, 2).contiguous().transpose(1, 2)
     buf = torch.zeros(2, lq, 4, 64 + 3, dtype=torch.bfloat16, device=dev)
     out = buf[..., 1:65].transpose(1, 2)
-    widetable = torch.full((2, 9), -1, dtype=torch.int32)
+    widetable = torch.full((2, width), -1, dtype=torch.int32)
     widetable[:, 2:7] = table
-    got = pkg.ops.cache8_attention(inter, cache, widetable.to(dev)[:, 2:7], lengths, 0.1, out=out)
+    got = pkg.ops.cache8_attention(inter, cache, widetable.to(dev)[:, 2:width - 2], lengths, 0.1, out=out)
     assert got is out and torch.equal(out, want)
     assert (buf[..., 0] == 0).all() and (buf[..., 65:] == 0).all()
 
