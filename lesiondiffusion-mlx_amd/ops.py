@@ -853,7 +853,7 @@ def _launch8(fn, args: tuple, device: int, what: str) -> None:
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype | tuple | None, device: int) -> None:
     """``t`` is a tensor of ``dtype`` (one of several, or any with None) on device ``device`` (any with -1)."""
-    if type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == device:
+    if type(t) is torch.Tensor and t.dtype is dtype and (t.get_device() == device if device >= 0 else t.is_cuda):
         return
     _require_cuda(t, name, dtype)
     if device >= 0 and t.get_device() != device:
