@@ -451,7 +451,7 @@ int ldx_quantize8(const void* x, int64_t x_pitch, int64_t rows, int32_t features
  * groups of eight cut at 2^-13 of the group's largest: its sum is within 2^-10 of the sum of
  * the terms' magnitudes (about 1.5e-5 of the result's size for ordinary data). An fp32 y is
  * summed from the operands as bf16 values, which hold them exactly. residual and y are of
- * type dtype; bias fp32. */
+ * type dtype; bias fp32. At most 2^22 features; pitches of codes and scales at most 2^22. */
 typedef struct ldx_dense8_args {
   int64_t rows;
   int32_t features, out_features;

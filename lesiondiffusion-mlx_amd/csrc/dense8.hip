@@ -64,31 +64,6 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float s) {
   return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// D(16 x 16) += A(16 x 128) B(128 x 16) of one block of 128: lane l holds 32 codes of A row l % 16 and of
-// B column l % 16 and the scale bytes of that row and column (all four quarters of k share them, so the
-// order of k within the block is free as long as A and B agree); D column l % 16, rows 4 (l / 16) + i.
-// EXACT: the same from bf16 operands, whose products the instruction adds within 24 bits.
-template <bool EXACT>
-__device__ __forceinline__ f32x4 block16(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
-  if constexpr (!EXACT) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
-  } else {
-    const float fa = scale_of(sa), fb = scale_of(sb);
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(a[2 * i], a[2 * i + 1], fa),
-                                                  widen8(b[2 * i], b[2 * i + 1], fb), c, 0, 0, 0);
-    return c;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void finish(const Dense8Args& a, int64_t m, int o, float v) {
-  if (a.bias) v += a.bias[o];
-  if (a.res) v += (float)((const T*)a.res)[m * a.rp + o];
-  ((T*)a.y)[m * a.yp + o] = (T)act_f(v, a.act);
-}
-
 // Outputs o .. o + 7 of row m, as many as there are.
 template <typename T>
 __device__ __forceinline__ void finish8(const Dense8Args& a, int64_t m, int o, float (&v)[8]) {
@@ -125,38 +100,167 @@ __device__ __forceinline__ void finish8(const Dense8Args& a, int64_t m, int o, f
   }
 }
 
-// One 16 x 16 tile a workgroup, its blocks of 128 dealt to the waves and their sums added in wave order.
-constexpr int kTileWaves = 4;
+// The tile of workgroup l of nt x mt. Workgroups l and l + 8 share an XCD: each XCD gets a contiguous range
+// of tiles, in which bands of four rows of tiles run along the outputs, so that what it holds at a time is
+// near a square.
+__device__ __forceinline__ void tile_of(unsigned l, unsigned nt, unsigned mt, unsigned& tm, unsigned& tn) {
+  const unsigned tiles = nt * mt, x = l % 8, per = tiles / 8, extra = tiles % 8;
+  const unsigned idx = x * per + (x < extra ? x : extra) + l / 8;
+  constexpr unsigned BAND = 4;
+  const unsigned band = idx / (BAND * nt), first = band * BAND;
+  const unsigned high = mt - first < BAND ? mt - first : BAND, in = idx - band * BAND * nt;
+  tm = first + in % high;
+  tn = in / high;
+}
 
-template <typename T>
-__global__ __launch_bounds__(64 * kTileWaves) void dense8_tile_kernel(Dense8Args a) {
+// ----------------------------------------------------------------------------------- few tiles
+//
+// Where few tiles launch, a block's turn (DMA, barrier, LDS reads, a handful of products) is bound by its
+// latencies, not by any rate. Here a workgroup's W waves take blocks of k of their own: each has a ring of
+// S blocks (32 FN outputs + 32 FM rows of 128 bytes, swizzled as below), no barrier until the end, and the
+// sums of the whole tile, which are added through LDS in wave order.
+// (64 x 4,096 x 4,096 7.4 us, 18 with the shared blocks of the next kernel; 77 x 768 x 512 4.6 and 5.7.)
+template <int FN, int FM, int W, int S>
+struct SplitTile {
+  static constexpr int TN = 32 * FN, TM = 32 * FM;
+  static constexpr int DATA = (TN + TM) * kBlock8, SLOT = DATA + 512;   // 64 dwords of scales each
+  static constexpr int DMAS = 4 * (FN + FM) + 2;
+  static constexpr int PITCH = TN + 4, OUT = W * TM * PITCH * 4;
+  static constexpr int RING = W * S * SLOT, LDS = RING > OUT ? RING : OUT;
+  static_assert(LDS <= 160 * 1024, "tile");
+};
+
+template <typename T, int FN, int FM, int W, int S>
+__global__ __launch_bounds__(64 * W) void dense8_split_kernel(Dense8Args a, unsigned nt, unsigned mt) {
+  typedef SplitTile<FN, FM, W, S> B;
   constexpr bool EXACT = sizeof(T) == 4;
-  __shared__ float part[kTileWaves][16][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const unsigned no = (unsigned)(a.O + 15) / 16;
-  const int64_t m0 = (int64_t)(blockIdx.x / no) * 16;
-  const int o0 = (int)(blockIdx.x % no) * 16;
-  const int64_t m = m0 + r < a.M ? m0 + r : a.M - 1;
-  const int o = o0 + r < a.O ? o0 + r : a.O - 1;
-  const uint8_t* w = a.w + o * a.wp + 16 * g;
-  const uint8_t* x = a.x + m * a.xp + 16 * g;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int k = wave; k < a.kb; k += kTileWaves) {
-    i32x8 A, B;
-    reinterpret_cast<i32x4*>(&A)[0] = *reinterpret_cast<const i32x4*>(w + k * kBlock8);
-    reinterpret_cast<i32x4*>(&A)[1] = *reinterpret_cast<const i32x4*>(w + k * kBlock8 + 64);
-    reinterpret_cast<i32x4*>(&B)[0] = *reinterpret_cast<const i32x4*>(x + k * kBlock8);
-    reinterpret_cast<i32x4*>(&B)[1] = *reinterpret_cast<const i32x4*>(x + k * kBlock8 + 64);
-    acc = block16<EXACT>(A, B, acc, a.ws[o * a.wsp + k], a.xs[m * a.xsp + k]);
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+  unsigned tm, tn;
+  tile_of(blockIdx.x, nt, mt, tm, tn);
+  const int64_t m0 = (int64_t)tm * B::TM;
+  const int o0 = (int)tn * B::TN;
+  const int mrows = (int)(a.M - m0 < B::TM ? a.M - m0 : B::TM), orows = a.O - o0 < B::TN ? a.O - o0 : B::TN;
+  // Rows past the operand's last read as zeros (the buffer ends there).
+  const i32x4 wr = dma_rsrc(a.w + o0 * a.wp, (unsigned)(orows * a.wp));
+  const i32x4 xr = dma_rsrc(a.x + m0 * a.xp, (unsigned)(mrows * a.xp));
+  const i32x4 wsr = dma_rsrc(a.ws + o0 * a.wsp, (unsigned)(orows * a.wsp));
+  const i32x4 xsr = dma_rsrc(a.xs + m0 * a.xsp, (unsigned)(mrows * a.xsp));
+  uint8_t* ring = lds + wave * S * B::SLOT;
+  const unsigned base = lds_offset(ring);
+  unsigned wv[2], xv[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const unsigned row = 8 * i + lane / 8, unit = (lane % 8) ^ (row / 2 % 8);
+    wv[i] = lane / 8 * (unsigned)a.wp + unit * 16;
+    xv[i] = lane / 8 * (unsigned)a.xp + unit * 16;
   }
+  const int steps = (a.kb - wave + W - 1) / W;   // blocks wave, wave + W, ..
+  const auto fetch = [&](int i) {
+    const unsigned k = wave + W * i, to = base + i % S * B::SLOT, at = k * kBlock8;
+    dma_buffer_b32(wsr, lane * (unsigned)a.wsp, k & ~3u, to + B::DATA);
+    dma_buffer_b32(xsr, lane * (unsigned)a.xsp, k & ~3u, to + B::DATA + 256);
 #pragma unroll
-  for (int i = 0; i < 4; i++) part[wave][r][4 * g + i] = acc[i];
+    for (int e = 0; e < 4 * FN; e++) dma_buffer_b128(wr, wv[e & 1], e * 8 * (unsigned)a.wp + at, to + e * 1024);
+#pragma unroll
+    for (int e = 0; e < 4 * FM; e++) dma_buffer_b128(xr, xv[e & 1], e * 8 * (unsigned)a.xp + at, to + (4 * FN + e) * 1024);
+  };
+  f32x16 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; i++)
+#pragma unroll
+    for (int j = 0; j < FM; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+  unsigned unit[4];
+#pragma unroll
+  for (int p = 0; p < 4; p++) unit[p] = (unsigned)r * kBlock8 + (((2 * p + h) ^ (r / 2 % 8)) * 16);
+
+#pragma unroll
+  for (int i = 0; i < S; i++)
+    if (i < steps) fetch(i);
+  for (int i = 0; i < steps; i++) {
+    if (S > 1 && i + S <= steps) vmcnt_wait<(S - 1) * B::DMAS>();   // block i has come, S - 1 are on their way
+    else vmcnt_wait<0>();
+    asm volatile("" ::: "memory");
+    const uint8_t* s = ring + i % S * B::SLOT;
+    i32x8 fr[2][FN + FM];
+    int sc[FN + FM];
+#pragma unroll
+    for (int f = 0; f < FN + FM; f++) {
+#pragma unroll
+      for (int p = 0; p < 4; p++) {
+        const i32x4 v = *reinterpret_cast<const i32x4*>(s + f * 32 * kBlock8 + unit[p]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) fr[p / 2][f][p % 2 * 4 + e] = v[e];
+      }
+      const int row = f < FN ? f * 32 + r : 64 + (f - FN) * 32 + r;
+      sc[f] = reinterpret_cast<const int*>(s + B::DATA)[row] >> (8 * ((wave + W * i) & 3));
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // the reads have returned: the slot is free
+    asm volatile("" ::: "memory");
+    if (i + S < steps) fetch(i + S);
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+#pragma unroll
+      for (int f = 0; f < FN; f++)
+#pragma unroll
+        for (int j = 0; j < FM; j++) {
+          if constexpr (!EXACT) {
+            acc[f][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fr[c][f], fr[c][FN + j], acc[f][j], 0, 0, 0, sc[f],
+                                                                       0, sc[FN + j]);
+          } else {
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+              acc[f][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  widen8(fr[c][f][2 * p], fr[c][f][2 * p + 1], scale_of(sc[f] & 255)),
+                  widen8(fr[c][FN + j][2 * p], fr[c][FN + j][2 * p + 1], scale_of(sc[FN + j] & 255)), acc[f][j], 0, 0, 0);
+          }
+        }
+#pragma unroll
+    for (int f = 0; f < FN; f++)
+#pragma unroll
+      for (int j = 0; j < FM; j++) asm volatile("" : "+a"(acc[f][j]));
+  }
+
+  ring_barrier();
+  float* out = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int f = 0; f < FN; f++)
+#pragma unroll
+    for (int j = 0; j < FM; j++)
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        *reinterpret_cast<f32x4*>(out + (wave * B::TM + j * 32 + r) * B::PITCH + f * 32 + 8 * q + 4 * h) =
+            (f32x4){acc[f][j][4 * q], acc[f][j][4 * q + 1], acc[f][j][4 * q + 2], acc[f][j][4 * q + 3]};
   __syncthreads();
-  const int tm = threadIdx.x >> 4, to = threadIdx.x & 15;
-  float v = part[0][tm][to];
+  for (int e = threadIdx.x; e < B::TM * 4 * FN; e += 64 * W) {
+    const int row = e / (4 * FN), col = e % (4 * FN) * 8;
+    if (row >= mrows || col >= orows) continue;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 1; i < kTileWaves; i++) v += part[i][tm][to];
-  if (m0 + tm < a.M && o0 + to < a.O) finish<T>(a, m0 + tm, o0 + to, v);
+    for (int w = 0; w < W; w++) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(out + (w * B::TM + row) * B::PITCH + col);
+      const f32x4 lo = p[0], hi = p[1];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        v[i] += lo[i];
+        v[4 + i] += hi[i];
+      }
+    }
+    finish8<T>(a, m0 + row, o0 + col, v);
+  }
+}
+
+template <typename T, int FN, int FM, int W, int S>
+int launch_split(const Dense8Args& a, hipStream_t st) {
+  typedef SplitTile<FN, FM, W, S> B;
+  const unsigned nt = (unsigned)((a.O + B::TN - 1) / B::TN), mt = (unsigned)((a.M + B::TM - 1) / B::TM);
+  const auto kern = dense8_split_kernel<T, FN, FM, W, S>;
+  if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, B::LDS) != hipSuccess)
+    return check_launch("dense8: set LDS size");
+  hipLaunchKernelGGL(kern, dim3(nt * mt), dim3(64 * W), B::LDS, st, a, nt, mt);
+  return check_launch("dense8");
 }
 
 // ------------------------------------------------------------------------------ large products
@@ -175,7 +279,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void dense8_tile_kernel(Dense8Args
 
 constexpr int kHalf8 = kBlock8 / 2;
 
-template <int FN, int FM>
+template <int FN, int FM, int S>
 struct BigTile {
   static constexpr int TN = 64 * FN, TM = 64 * FM;
   static constexpr int STAGE = (TN + TM) * kBlock8;
@@ -184,27 +288,21 @@ struct BigTile {
   static constexpr int READS = 2 * (FN + FM);     // per half block
   // The result leaves through LDS: a wave's JP x 32 rows of 32 FN outputs, padded by 16 bytes.
   static constexpr int JP = FN == 4 ? 2 : 1, PITCH = 32 * FN + 4, OUT = 4 * JP * 32 * PITCH * 4;
-  static constexpr int RING = 2 * STAGE + 2 * SCALES;
+  static constexpr int GROUPS = S == 2 ? 2 : 4;   // of four blocks' scales; S / 4 + 2 are in use at a time
+  static constexpr int RING = S * STAGE + GROUPS * SCALES;
   static constexpr int LDS = RING > OUT ? RING : OUT;
   static_assert(FM % JP == 0 && LDS <= 160 * 1024, "tile");
 };
 
-template <typename T, int FN, int FM>
+template <typename T, int FN, int FM, int S>
 __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned nt, unsigned mt) {
-  typedef BigTile<FN, FM> B;
+  typedef BigTile<FN, FM, S> B;
   constexpr bool EXACT = sizeof(T) == 4;
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5, wn = wave >> 1, wm = wave & 1;
-  // Workgroups l and l + 8 share an XCD: each XCD gets a contiguous range of tiles, in which bands of
-  // four rows of tiles run along the outputs, so that what it holds at a time is near a square.
-  const unsigned tiles = nt * mt, l = blockIdx.x;
-  const unsigned x = l % 8, per = tiles / 8, extra = tiles % 8;
-  const unsigned idx = x * per + (x < extra ? x : extra) + l / 8;
-  constexpr unsigned BAND = 4;
-  const unsigned band = idx / (BAND * nt), first = band * BAND;
-  const unsigned high = mt - first < BAND ? mt - first : BAND, in = idx - band * BAND * nt;
-  const unsigned tm = first + in % high, tn = in / high;
+  unsigned tm, tn;
+  tile_of(blockIdx.x, nt, mt, tm, tn);
   const int64_t m0 = (int64_t)tm * B::TM;
   const int o0 = (int)tn * B::TN;
   const int mrows = (int)(a.M - m0 < B::TM ? a.M - m0 : B::TM), orows = a.O - o0 < B::TN ? a.O - o0 : B::TN;
@@ -225,7 +323,7 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
   const unsigned wstep = 8 * (unsigned)a.wp, xstep = 8 * (unsigned)a.xp;
   // DMA i of this wave for block k.
   const auto dma = [&](int k, int i) {
-    const unsigned to = base + (k & 1) * B::STAGE, at = k * kBlock8;
+    const unsigned to = base + (k % S) * B::STAGE, at = k * kBlock8;
     if (i < 2 * FN) {
       const unsigned e = wave * 2 * FN + i;
       dma_buffer_b128(wr, wv[i & 1], e * wstep + at, to + e * 1024);
@@ -237,7 +335,7 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
   // Scales of blocks k .. k + 3.
   const auto dma_scales = [&](int k) {
     if (k & 3) return;
-    const unsigned to = base + 2 * B::STAGE + (k >> 2 & 1) * B::SCALES;
+    const unsigned to = base + S * B::STAGE + (k / 4 % B::GROUPS) * B::SCALES;
 #pragma unroll
     for (int i = 0; i < FN + FM; i++) {
       if (i % 4 != wave) continue;
@@ -266,7 +364,7 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
   i32x8 fw[2][FN], fx[2][FM];
   // LDS read i of half c of block k.
   const auto read = [&](int k, int c, int i) {
-    const uint8_t* s = lds + (k & 1) * B::STAGE;
+    const uint8_t* s = lds + (k % S) * B::STAGE;
     const int f = i / 2, p = i % 2;
     const i32x4 v = *reinterpret_cast<const i32x4*>(f < FN ? s + wu[2 * c + p] + f * 32 * kBlock8
                                                            : s + xu[2 * c + p] + (f - FN) * 32 * kBlock8);
@@ -276,14 +374,14 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
   };
   int sn[FN], sx[FM];
   const auto scales = [&](int k) {
-    const int* s = reinterpret_cast<const int*>(lds + 2 * B::STAGE + (k >> 2 & 1) * B::SCALES);
+    const int* s = reinterpret_cast<const int*>(lds + S * B::STAGE + (k / 4 % B::GROUPS) * B::SCALES);
 #pragma unroll
     for (int i = 0; i < FN; i++) sn[i] = s[(wn * FN + i) * 32 + r];
 #pragma unroll
     for (int j = 0; j < FM; j++) sx[j] = s[B::TN + (wm * FM + j) * 32 + r];
   };
   // Products of half c of block k; between them the reads of the half block after it and, with MORE in
-  // the second half, the DMAs of block k + 2.
+  // the second half, the DMAs of block k + S.
   const auto products = [&](int k, auto half, auto more) {
     constexpr int c = decltype(half)::value;
     constexpr bool MORE = c == 1 && decltype(more)::value;
@@ -293,9 +391,9 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
       for (int i = s * B::READS / N; i < (s + 1) * B::READS / N; i++) read(k + c, 1 - c, i);
       if constexpr (MORE)
 #pragma unroll
-        for (int i = s * B::DMAS / N; i < (s + 1) * B::DMAS / N; i++) dma(k + 2, i);
+        for (int i = s * B::DMAS / N; i < (s + 1) * B::DMAS / N; i++) dma(k + S, i);
     };
-    if constexpr (MORE) dma_scales(k + 2);
+    if constexpr (MORE) dma_scales(k + S);
     if constexpr (!EXACT) {
 #pragma unroll
       for (int s = 0; s < N; s++) {
@@ -340,28 +438,30 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
   constexpr std::integral_constant<int, 1> half1{};
 
 #pragma unroll
-  for (int k = 0; k < 2; k++)
+  for (int k = 0; k < S; k++)
     if (k < a.kb) {
       dma_scales(k);
 #pragma unroll
       for (int i = 0; i < B::DMAS; i++) dma(k, i);
     }
-  if (a.kb > 1) vmcnt_wait<B::DMAS>();
+  if (a.kb >= S) vmcnt_wait<(S - 1) * B::DMAS>();
   else vmcnt_wait<0>();
   ring_barrier();
 #pragma unroll
   for (int i = 0; i < B::READS; i++) read(0, 0, i);
   scales(0);
   int k = 0;
-  for (; k + 2 < a.kb; k++) {
+  for (; k + S < a.kb; k++) {
     products(k, half0, std::true_type{});
-    vmcnt_wait<0>();   // block k + 1 has come, and behind the barrier every wave has read block k
+    // Block k + 1 has come (S - 2 more are on their way), and behind the barrier every wave has read block k.
+    vmcnt_wait<(S - 2) * B::DMAS>();
     ring_barrier();
     products(k, half1, std::true_type{});
   }
-  for (; k < a.kb; k++) {   // the last two, or one: the reads past the end take old bytes, not used
+  for (; k < a.kb; k++) {   // the last S: the reads past the end take old bytes, not used
     products(k, half0, std::false_type{});
-    vmcnt_wait<0>();
+    if (S > 2 && k + S == a.kb) vmcnt_wait<(S - 2) * B::DMAS>();
+    else vmcnt_wait<0>();
     ring_barrier();
     products(k, half1, std::false_type{});
   }
@@ -396,35 +496,58 @@ __global__ __launch_bounds__(256) void dense8_big_kernel(Dense8Args a, unsigned 
   }
 }
 
-template <typename T, int FN, int FM>
+template <typename T, int FN, int FM, int S>
 int launch_big(const Dense8Args& a, hipStream_t st) {
-  typedef BigTile<FN, FM> B;
+  typedef BigTile<FN, FM, S> B;
   const unsigned nt = (unsigned)((a.O + B::TN - 1) / B::TN), mt = (unsigned)((a.M + B::TM - 1) / B::TM);
-  const auto kern = dense8_big_kernel<T, FN, FM>;
+  const auto kern = dense8_big_kernel<T, FN, FM, S>;
   if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, B::LDS) != hipSuccess)
     return check_launch("dense8: set LDS size");
   hipLaunchKernelGGL(kern, dim3(nt * mt), dim3(256), B::LDS, st, a, nt, mt);
   return check_launch("dense8");
 }
 
+// Which kernel: the one of least estimated time. A call's time was measured as a sum of a fixed part, one
+// for each round of workgroups (places: as many as the CUs hold at once), for each block of a workgroup's
+// steps in a round, and for the workgroups and their steps by how full the rounds are -- fitted to 130 random
+// shapes (1 to 8,192 rows, 64 to 8,192 features and outputs) per kernel; the choices are within 0.5 % (16-bit
+// results) and 1.3 % (fp32) of the fastest on average, 19 % at most. us.
+struct Cost {
+  float fixed, round, step, work, tile;   // the last two per full round
+};
+
+inline double estimate(const Cost& c, int64_t M, int64_t O, int kb, int tm, int tn, int places, int waves) {
+  const double tiles = (double)((M + tm - 1) / tm) * (double)((O + tn - 1) / tn), full = tiles / places;
+  const double rounds = (double)(int64_t)(full + 0.999999), steps = (kb + waves - 1) / waves;
+  return c.fixed + c.round * rounds + c.step * rounds * steps + c.work * full * steps + c.tile * full;
+}
+
 template <typename T>
 int launch(const Dense8Args& a, hipStream_t st) {
-  if (a.M > 64 && (a.wp | a.xp) < (1 << 22)) {
-    // Rounds of workgroups (one 256 x 256 tile a CU, two of 128 x 128) times what a round was measured to
-    // take, us: so much a block of 128 and so much to start and store.
-    const auto cdiv = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
-    const double wide = cdiv(cdiv(a.M, 256) * cdiv(a.O, 256), 256) * (1.32 * a.kb + 13.0);
-    const double narrow = cdiv(cdiv(a.M, 128) * cdiv(a.O, 128), 512) * (0.93 * a.kb + 8.0);
-    return wide < narrow ? launch_big<T, 4, 4>(a, st) : launch_big<T, 2, 2>(a, st);
+  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr Cost big4 = EXACT ? Cost{9.80f, 2.11f, 2.267f, 0.298f, 14.97f} : Cost{10.78f, 1.97f, 0.981f, 0.299f, 9.03f};
+  constexpr Cost big2 = EXACT ? Cost{5.22f, 0.f, 0.740f, 0.654f, 9.33f} : Cost{5.16f, 0.f, 0.411f, 0.546f, 4.85f};
+  constexpr Cost big1 = EXACT ? Cost{4.06f, 0.f, 0.366f, 0.169f, 2.83f} : Cost{3.51f, 0.62f, 0.208f, 0.174f, 1.50f};
+  constexpr Cost split2 = EXACT ? Cost{3.21f, 1.27f, 1.010f, 0.092f, 1.56f} : Cost{3.10f, 1.60f, 0.677f, 0.192f, 0.80f};
+  constexpr Cost split1 = EXACT ? Cost{3.66f, 0.f, 0.468f, 0.267f, 1.16f} : Cost{3.65f, 0.01f, 0.339f, 0.327f, 0.91f};
+  const double t[5] = {estimate(split1, a.M, a.O, a.kb, 32, 32, 512, 4), estimate(split2, a.M, a.O, a.kb, 64, 64, 256, 4),
+                       estimate(big1, a.M, a.O, a.kb, 64, 64, 512, 1), estimate(big2, a.M, a.O, a.kb, 128, 128, 512, 1),
+                       estimate(big4, a.M, a.O, a.kb, 256, 256, 256, 1)};
+  int best = 0;
+  for (int i = 1; i < 5; i++)
+    if (t[i] < t[best]) best = i;
+  switch (best) {
+    case 0: return launch_split<T, 1, 1, 4, 2>(a, st);
+    case 1: return launch_split<T, 2, 2, 4, 2>(a, st);
+    case 2: return launch_big<T, 1, 1, 4>(a, st);
+    case 3: return launch_big<T, 2, 2, 2>(a, st);
+    default: return launch_big<T, 4, 4, 2>(a, st);
   }
-  const int64_t tiles = (a.M + 15) / 16 * ((a.O + 15) / 16);
-  hipLaunchKernelGGL(dense8_tile_kernel<T>, dim3((unsigned)tiles), dim3(64 * kTileWaves), 0, st, a);
-  return check_launch("dense8");
 }
 
 int check_operand(const char* name, const void* codes, int64_t cp, const void* scales, int64_t sp, int kb) {
   if (!codes || !scales) return fail("dense8: null pointer");
-  if (cp < (int64_t)kb * kBlock8 || cp % 16 || sp < ((kb + 3) & ~3) || sp % 4)
+  if (cp < (int64_t)kb * kBlock8 || cp > (1 << 22) || cp % 16 || sp < ((kb + 3) & ~3) || sp > (1 << 22) || sp % 4)
     return fail("dense8: %s pitches %lld, %lld do not hold %d blocks of %d", name, (long long)cp, (long long)sp, kb,
                 kBlock8);
   if ((uintptr_t)codes % 16 || (uintptr_t)scales % 4) return fail("dense8: %s codes or scales not aligned", name);
@@ -438,14 +561,13 @@ using namespace ldx;
 
 extern "C" int ldx_dense8(const ldx_dense8_args* p, void* stream) {
   if (!p || !p->y) return fail("dense8: null pointer");
-  if (p->rows < 1 || p->rows > 0x7fffffff || p->features < 1 || p->features > (1 << 28) || p->out_features < 1 ||
+  if (p->rows < 1 || p->rows > 0x7fffffff || p->features < 1 || p->features > (1 << 22) || p->out_features < 1 ||
       p->out_features > (1 << 28))
     return fail("dense8: %lld rows, %d features, %d outputs", (long long)p->rows, p->features, p->out_features);
   if (p->dtype != LDX_DTYPE_F16 && p->dtype != LDX_DTYPE_BF16 && p->dtype != LDX_DTYPE_F32)
     return fail("dense8: dtype %d is not LDX_DTYPE_F16, LDX_DTYPE_BF16 or LDX_DTYPE_F32", p->dtype);
   if (p->act != LDX_ACT_NONE && p->act != LDX_ACT_GELU && p->act != LDX_ACT_SILU) return fail("dense8: act %d", p->act);
-  // (the largest grid, of 16 x 16 tiles)
-  if ((p->rows + 15) / 16 * ((p->out_features + 15) / 16) > 0x7fffffff)
+  if ((p->rows + 31) / 32 * ((p->out_features + 31) / 32) > 0x7fffffff)   // the largest grid
     return fail("dense8: %lld x %d outputs are more than one launch takes", (long long)p->rows, p->out_features);
   const int kb = (p->features + kBlock8 - 1) / kBlock8;
   if (int rc = check_operand("x", p->x_codes, p->x_pitch, p->x_scales, p->x_scales_pitch, kb)) return rc;

@@ -117,6 +117,8 @@ def test_quantize8_refuses(pkg) -> None:
     {"rows": 0}, {"features": 0}, {"out_features": 0}, {"dtype": 4}, {"act": 3}, {"x_codes": None}, {"w_scales": None},
     {"y": None}, {"x_pitch": 128}, {"w_pitch": 264}, {"x_scales_pitch": 3}, {"w_codes": 24}, {"x_scales": 2},
     {"y_pitch": 4}, {"residual": 16, "residual_pitch": 4}, {"rows": 0x7fffffff, "out_features": 1 << 20, "y_pitch": 1 << 20},
+    {"features": 1 << 22 | 1, "x_pitch": 1 << 23, "w_pitch": 1 << 23, "x_scales_pitch": 1 << 20, "w_scales_pitch": 1 << 20},
+    {"w_pitch": (1 << 22) + 16}, {"w_scales_pitch": (1 << 22) + 4},
 ])
 def test_dense8_refuses(pkg, bad) -> None:
     a = pkg._lib.Dense8Args(rows=3, features=200, out_features=5, x_codes=16, x_pitch=256, x_scales=16, x_scales_pitch=4,
@@ -427,6 +429,35 @@ def test_dense8_large(pkg, dev, m, k, o, act, t) -> None:
     allowed = 1.13 * bound + z.abs() * (half_step(t) + 8 * 2.0 ** -23) + tiny(t) + (2.0 ** -23 * y.abs() if act else 0)
     err = (got.double() - z).abs()
     assert (err <= allowed).all(), (err / allowed).max()
+
+
+@gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize(("m", "k", "o"), [
+    (34, 2385, 552), (103, 1465, 5093), (600, 1300, 1100), (1301, 1123, 3148), (8000, 1250, 8100)])
+def test_dense8_tiles(pkg, dev, m, k, o, t) -> None:
+    """Long rows at sizes for every tile, blocks of very unlike scales: all rows of some outputs and all
+    outputs of some rows, the last ones among them, against the bound of the small cases."""
+    gen = torch.Generator().manual_seed(m)
+    blocks = -(-k // 128)
+    x, w = rand((m, k), 1), rand((o, k), 2)
+    x *= torch.exp2(torch.randint(-6, 7, (m, blocks), generator=gen).float()).repeat_interleave(128, 1)[:, :k]
+    w *= torch.exp2(torch.randint(-6, 7, (o, blocks), generator=gen).float()).repeat_interleave(128, 1)[:, :k]
+    xq, wq = pkg.ops.quantize8(x.to(dev)), pkg.ops.quantize8(w.to(dev))
+    got = pkg.ops.dense8(xq, wq, dtype=t).double()
+    a, ww = wide(xq).to(dev), wide(wq).to(dev)
+    rows = torch.cat((torch.randperm(m, generator=gen)[:40], torch.tensor([0, m - 1]))).to(dev)
+    cols = torch.cat((torch.randperm(o, generator=gen)[:40], torch.tensor([0, o - 1]))).to(dev)
+    for xs, ws, part in ((a, ww[cols], got[:, cols]), (a[rows], ww, got[rows])):
+        y = torch.mm(xs, ws.t().contiguous())
+        allowed = dense_bound(xs, ws, k, t)
+        # Rounding to fp16 makes infinities of what is half a step (16) and more above its largest, 65504.
+        top = 65520 if t == torch.float16 else math.inf
+        inf = part.isinf()
+        assert (y.abs() + allowed >= top)[inf].all() and (part[inf] * y[inf] > 0).all()
+        assert (y.abs() - allowed < top)[~inf].all()
+        allowed += y.abs() * half_step(t) + tiny(t)
+        assert ((part - y).abs() <= allowed)[~inf].all(), ((part - y).abs() / allowed)[~inf].max()
 
 
 @gpu
