@@ -145,19 +145,20 @@ __device__ __forceinline__ f32x4 mfma_q(f16x8 a, f16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mfma_q(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-// Eight codes as they stand (scale 1): e4m3's values fit fp16 and bf16 exactly.
-__device__ __forceinline__ void codes_as(int lo, int hi, f16x8& r) {
-  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
-  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
-  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
-  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+// Eight codes times s, a power of two; as they stand, and within 2^-15 .. 2^7, e4m3's values fit fp16 and
+// bf16 exactly.
+__device__ __forceinline__ void codes_as(int lo, int hi, float s, f16x8& r) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, true);
   r = (f16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-__device__ __forceinline__ void codes_as(int lo, int hi, bf16x8& r) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+__device__ __forceinline__ void codes_as(int lo, int hi, float s, bf16x8& r) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
   r = (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -191,6 +192,24 @@ __device__ __forceinline__ float soft_scale(const Attend8Args& a) { return a.sca
 // a masked score stays minus infinity and a score of 0 stays 0.
 __device__ __forceinline__ float score_scale(float c, int byte) {
   return fminf(fmaxf(c * scale_of(byte), 1.1754944e-38f), 3.0e38f);
+}
+
+// A query's reference for its exponentials follows its maximum only where that passes it by kSlack (in powers of
+// two): the sums are seldom multiplied then, and probabilities up to 2^8 are as exact in fp16 as those up to 1.
+constexpr float kSlack = 8.f;
+
+// l and eight probabilities: as the products take them, in fp16 (their sum in fp32), so that rounding moves
+// both sides of the quotient alike. Two at a time: half the additions of fp32 numbers.
+__device__ __forceinline__ float sum8(f16x8 p, float l) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    l = __builtin_amdgcn_fdot2((f16x2){p[i], p[i + 1]}, (f16x2){(f16)1.f, (f16)1.f}, l, false);
+  return l;
+}
+
+// A value page's scale, any E8M0 byte (append writes 1 to 254); 1 for 255, NaN, whose queries get NaN by their sum.
+__device__ __forceinline__ float page_scale(int byte) {
+  return byte == 255 ? 1.f : byte ? scale_of(byte) : __int_as_float(0x00400000);
 }
 
 // Channels at .. at + 7 of a query, with the softmax scale's sign.
@@ -318,6 +337,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
   load_v(now, p);
   for (; p < p1; p += kAttendWaves) {
     const float grow = score_scale(c, ks);
+    const bool none_k = ks == 255;
     const int base = p * kPage8 + 16 * g;   // the lane's first token
     float s[16];
 #pragma unroll
@@ -325,15 +345,15 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
       V8 kv;
       if constexpr (D == 32) {
-        codes_as(kc[t / 2][t % 2 * 2], kc[t / 2][t % 2 * 2 + 1], kv);
+        codes_as(kc[t / 2][t % 2 * 2], kc[t / 2][t % 2 * 2 + 1], 1.f, kv);
         o = mfma_q(kv, q[0], o);
       } else {
 #pragma unroll
         for (int j = 0; j < NK / 2; j++) {
           const i32x4 w = kc[t * (NK / 2) + j];
-          codes_as(w[0], w[1], kv);
+          codes_as(w[0], w[1], 1.f, kv);
           o = mfma_q(kv, q[2 * j], o);
-          codes_as(w[2], w[3], kv);
+          codes_as(w[2], w[3], 1.f, kv);
           o = mfma_q(kv, q[2 * j + 1], o);
         }
       }
@@ -343,8 +363,8 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
     }
     load_k(next, p + kAttendWaves);
     __builtin_amdgcn_sched_barrier(0);
-    const float vscale = scale_of(vs);
-    if (now.missing && p * kPage8 < limit) l = __builtin_nanf("");   // page 0 was read in its place
+    const float vscale = page_scale(vs);
+    if ((now.missing || none_k || vs == 255) && p * kPage8 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
     const bool cut = p * kPage8 + kPage8 > least;   // some query does not see the whole page
     if (cut) {
       int left = limit - base;
@@ -361,8 +381,9 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
     mx = max3_f(__int_as_float(x16[0]), __int_as_float(x16[1]), __int_as_float(x16[1]));
     const auto x32 = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
     const float mn = max3_f(m, __int_as_float(x32[0]) * grow, __int_as_float(x32[1]) * grow);
-    const float ref = mn == -__builtin_inff() ? 0.f : mn;
-    if (__any(mn != m)) {
+    float ref = m == -__builtin_inff() ? 0.f : m;
+    if (__any(mn > m + kSlack)) {
+      ref = mn == -__builtin_inff() ? 0.f : mn;
       const float alpha = __builtin_amdgcn_exp2f(m - ref);
       l *= alpha;
 #pragma unroll
@@ -372,17 +393,11 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
       m = mn;
     }
     f16x8 pr[2];
-    // Eight at a time, summed as they come (left alone, the sums are made behind the products below).
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-      float sum[2] = {0.f, 0.f};
+    for (int u = 0; u < 2; u++) {   // eight at a time; left alone, the sums are made behind the products below
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * u + i], grow, -ref));
-        sum[i & 1] += e;
-        pr[u][i] = (f16)e;
-      }
-      l += sum[0] + sum[1];
+      for (int i = 0; i < 8; i++) pr[u][i] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * u + i], grow, -ref));
+      l = sum8(pr[u], l);
       pin_value(l);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -432,8 +447,8 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
 #pragma unroll
     for (int d = 0; d < ND; d++) {
       f16x8 v0, v1;
-      codes_as(vc[d][0], vc[d][1], v0);
-      codes_as(vc[d][2], vc[d][3], v1);
+      codes_as(vc[d][0], vc[d][1], 1.f, v0);
+      codes_as(vc[d][2], vc[d][3], 1.f, v1);
       const f32x4 o = mfma16(v1, pr[1], mfma16(v0, pr[0], (f32x4){0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
       for (int i = 0; i < 4; i++) acc[d][i] += o[i] * vscale;
@@ -567,7 +582,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
 #pragma unroll
     for (int j = 0; j < NJ; j++) q[j] = query8<T>(a, qp, 16 * j + 8 * hh, real);
   }
-  float acc[NT][16];   // single numbers: as vectors, every branch that changes them copies them
+  f32x16 acc[NT];
 #pragma unroll
   for (int d = 0; d < NT; d++)
 #pragma unroll
@@ -595,8 +610,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       vraw[i] = vp[tid + 256 * i];
     }
   };
-  // Widen page p's pieces into buffer p & 1.
-  const auto widen = [&](int p) {
+  // Values are widened times 2^(scale - unit), exact in fp16 (codes are 2^-9 .. 448) where that is 2^-15 .. 2^7,
+  // and summed in that unit, at first the first page's scale. A page further off makes its scale the unit,
+  // but never one more than 2^70 below the largest so far: the sums would pass fp32.
+  int unit = 0, top = 0;   // of the page widened last; the largest
+  const auto unit_for = [&](int byte) {
+    if (byte == 255 || (byte - unit >= -15 && byte - unit <= 7)) return;   // 255: its queries get NaN
+    unit = max(max(byte, top - 70), 1);
+    top = max(top, unit);
+  };
+  const auto times = [&](float f) {
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[d][e] *= f;
+  };
+  // Widen page p's pieces into buffer p & 1, the values times vf.
+  const auto widen = [&](int p, float vf) {
     uint8_t* kb = lds + (p & 1) * L::BUF;
     uint8_t* vb = kb + L::KEYS;
     const bool cut = p * kPage8 + kPage8 > tleast;
@@ -606,9 +636,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       const int t = key & 31, at = 8 * (t >> 2 & 3) + 4 * (t >> 4) + (t & 3);   // the token's row of its tile
       V8 w;
       uint8_t* f = kb + ((key >> 5) * NJ + j) * L::KF + at * 16;
-      codes_as(kraw[i][0], kraw[i][1], w);
+      codes_as(kraw[i][0], kraw[i][1], 1.f, w);
       *reinterpret_cast<V8*>(f) = w;
-      codes_as(kraw[i][2], kraw[i][3], w);
+      codes_as(kraw[i][2], kraw[i][3], 1.f, w);
       *reinterpret_cast<V8*>(f + 512) = w;
     }
 #pragma unroll
@@ -629,14 +659,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       }
       f16x8 w;
       uint8_t* f = vb + ((d >> 5) * 4 + (part >> 1) * 2) * L::VF + (part & 1) * L::VH + (d & 31) * 16;
-      codes_as(vraw[i][0], vraw[i][1], w);
+      codes_as(vraw[i][0], vraw[i][1], vf, w);
       *reinterpret_cast<f16x8*>(f) = w;
-      codes_as(vraw[i][2], vraw[i][3], w);
+      codes_as(vraw[i][2], vraw[i][3], vf, w);
       *reinterpret_cast<f16x8*>(f + L::VF) = w;
     }
   };
 
-  const auto attend = [&](int p, bool missing, int ksb, int vsb) {
+  int sums = 0;   // the unit of the lane's sums: a page that its query does not see leaves them alone
+  const auto attend = [&](int p, bool missing, int ksb, int punit, bool moved) {
     const uint8_t* kb = lds + (p & 1) * L::BUF + lane * 16;
     const uint8_t* vb = lds + (p & 1) * L::BUF + L::KEYS + hh * L::VH + r * 16;
     f32x16 sv[2];
@@ -656,7 +687,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
 #pragma unroll
       for (int e = 0; e < 16; e++) s[t][e] = sv[t][e];
     const int base = p * kPage8 + 16 * hh;   // score e of tile t is token base + 32 t + e
-    if (missing && p * kPage8 < limit) l = __builtin_nanf("");   // page 0 was read in its place
+    if (missing && p * kPage8 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
     if (p * kPage8 + kPage8 > least) {
       int left = limit - base;
       pin_value(left);
@@ -673,47 +704,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
     const float kc = score_scale(c, ksb);
     const float mn = max3_f(m, __int_as_float(x[0]) * kc, __int_as_float(x[1]) * kc);
-    const float ref = mn == -__builtin_inff() ? 0.f : mn;
-    if (__any(mn != m)) {
-      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    float ref = m == -__builtin_inff() ? 0.f : m;
+    if (moved || __any(mn > m + kSlack)) {
+      ref = mn == -__builtin_inff() ? 0.f : mn;
+      float alpha = __builtin_amdgcn_exp2f(m - ref);
       l *= alpha;
-#pragma unroll
-      for (int d = 0; d < NT; d++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) acc[d][e] *= alpha;
+      if (p * kPage8 < limit) {
+        alpha *= scale_of(max(127 + sums - punit, 0));
+        sums = punit;
+      }
+      times(alpha);
       m = mn;
     }
     f16x8 pr[2][2];
-    // Eight at a time, summed as they come: left alone, the sums are made behind the products below, and
-    // all 32 probabilities stay in fp32 until then.
+    // Eight at a time: left alone, all 32 probabilities stay in fp32 until the products below.
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + e], kc, -ref));
-          sum[e & 1] += w;
-          pr[t][u][e] = (f16)w;
-        }
-        l += sum[0] + sum[1];
+        for (int e = 0; e < 8; e++) pr[t][u][e] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + e], kc, -ref));
+        l = sum8(pr[t][u], l);
         pin_value(l);
         __builtin_amdgcn_sched_barrier(0);
       }
-    const float vscale = scale_of(vsb);
 #pragma unroll
     for (int d = 0; d < NT; d++) {
-      f32x16 o;
-#pragma unroll
-      for (int e = 0; e < 16; e++) o[e] = 0.f;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int u = 0; u < 2; u++)
-          o = mfma_w(*reinterpret_cast<const f16x8*>(vb + (d * 4 + t * 2 + u) * L::VF), pr[t][u], o);
-#pragma unroll
-      for (int e = 0; e < 16; e++) acc[d][e] += o[e] * vscale;
+          acc[d] = mfma_w(*reinterpret_cast<const f16x8*>(vb + (d * 4 + t * 2 + u) * L::VF), pr[t][u], acc[d]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -749,9 +770,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
     int page = entry(p0), next = entry(p0 + 1);
     int64_t at = place(page);
     load(at);
-    widen(p0);
+    const int first = __builtin_amdgcn_readfirstlane(vs);
+    unit = top = max(first == 255 ? 127 : first, 1);
+    sums = unit;
+    widen(p0, scale_of(max(127 + first - unit, 1)));
+    int was = unit;
     for (int p = p0; p < p1; p++) {
-      const int ksb = __builtin_amdgcn_readfirstlane(ks), vsb = __builtin_amdgcn_readfirstlane(vs);
+      const int ksb = __builtin_amdgcn_readfirstlane(ks), vsb = __builtin_amdgcn_readfirstlane(vs), punit = unit;
       const int64_t nat = place(next);
       const int after = entry(p + 2);
       if (p + 1 < p1) load(nat);
@@ -759,10 +784,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       // for the codes asked for above.)
       ring_barrier();
       if (p * kPage8 < wmost) {
-        attend(p, (unsigned)page >= (unsigned)a.pages, ksb, vsb);
+        attend(p, (unsigned)page >= (unsigned)a.pages || ksb == 255 || vsb == 255, ksb, punit, punit != was);
         if (p * kPage8 + kPage8 > tleast && flags[p & 1] == p) mark(p, at);
       }
-      if (p + 1 < p1) widen(p + 1);
+      if (p + 1 < p1) {
+        const int nvs = __builtin_amdgcn_readfirstlane(vs);
+        unit_for(nvs);
+        widen(p + 1, scale_of(max(127 + nvs - unit, 1)));
+      }
+      was = punit;
       page = next;
       next = after;
       at = nat;
@@ -775,6 +805,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
 #pragma unroll
       for (int e = 0; e < 16; e++)
         if (poison[d / 4] >> (16 * (d % 4) + e) & 1) acc[d][e] = __builtin_nanf("");
+  times(scale_of(sums));
   const auto l32 = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
   l = __int_as_float(l32[0]) + __int_as_float(l32[1]);
   if (too_long) l = __builtin_nanf("");

@@ -851,9 +851,13 @@ def _launch8(fn, args: tuple, device: int, what: str) -> None:
         check(rc, what)
 
 
+_ELEM, _ALL = tuple(ELEM_DTYPES), tuple(ALL_DTYPES)
+
+
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype | tuple | None, device: int) -> None:
     """``t`` is a tensor of ``dtype`` (one of several, or any with None) on device ``device`` (any with -1)."""
-    if type(t) is torch.Tensor and t.dtype is dtype and (t.get_device() == device if device >= 0 else t.is_cuda):
+    if type(t) is torch.Tensor and (t.dtype is dtype or dtype.__class__ is tuple and t.dtype in dtype) \
+            and (t.get_device() == device if device >= 0 else t.is_cuda):
         return
     _require_cuda(t, name, dtype)
     if device >= 0 and t.get_device() != device:
@@ -898,7 +902,7 @@ def _out_like(out: torch.Tensor | None, x: torch.Tensor, name: str) -> tuple[tor
 def quantize8(x: torch.Tensor) -> Quantized8:
     """fp16, bf16 or fp32 ``x`` as 8-bit rows: per row and 128 columns the least power of two with which
     the largest magnitude does not pass 448, codes rounded to nearest even."""
-    _require_cuda(x, "x", tuple(ALL_DTYPES))
+    _need(x, "x", _ALL, -1)
     n = x.numel()
     if x.dim() < 1 or not n:
         raise ValueError(f"quantize8: shape {tuple(x.shape)} holds no rows")
@@ -917,7 +921,7 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, *, residua
     given, which may be ``x``), or as ``Quantized8`` rows with ``quantize``; with a ``residual`` the pair
     ``(norm, s)``, ``s`` into ``sum_out`` when given, which may be ``x`` or ``residual``. Statistics in
     fp32, one launch."""
-    _require_cuda(x, "x", tuple(ALL_DTYPES))
+    _need(x, "x", _ALL, -1)
     n, dev, shape = x.numel(), x.get_device(), x.shape
     if not shape or not n:
         raise ValueError(f"rms_norm: shape {tuple(shape)} holds no rows")
@@ -1104,7 +1108,7 @@ def cache8_append(cache: Cache8, k: torch.Tensor, v: torch.Tensor, table: torch.
     sequences that write must not share pages. ``table``, ``starts`` and ``counts`` are int32 on the
     device, so a captured graph appends where they say at each replay."""
     block, dev = _cache_block(cache, "cache8_append")
-    _need(k, "k", tuple(ALL_DTYPES), dev)
+    _need(k, "k", _ALL, dev)
     _need(v, "v", k.dtype, dev)
     shape = k.shape
     if len(shape) != 4 or shape != v.shape or shape[1] != block.heads or shape[3] != block.head_dim or not shape[0] \
@@ -1129,7 +1133,7 @@ def cache8_attention(q: torch.Tensor, cache: Cache8, table: torch.Tensor, length
     not have, or a length past the table, gives NaN. Returns ``(B, heads, L, D)`` in ``q``'s type (into
     ``out`` when given); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
     block, dev = _cache_block(cache, "cache8_attention")
-    _need(q, "q", tuple(ELEM_DTYPES), dev)
+    _need(q, "q", _ELEM, dev)
     shape = q.shape
     if len(shape) != 4 or shape[3] != block.head_dim or shape[1] % block.heads or not q.numel():
         raise ValueError(f"q {tuple(shape)} must be (B, a multiple of {block.heads}, L, {block.head_dim})")

@@ -656,14 +656,18 @@ def attention_reference(ref, q, table, lengths, scale, starts):
         safe = torch.where(l > 0, l, 1.0)
         out[i] = p @ vz / safe
         mass = p @ vz.abs() / safe
-        # probabilities rounded to fp16 (2^-11; below 2^-14 half of 2^-24), scores off by `off`, fp32
-        # sums of n terms, the hardware's exponential (2^-22)
-        under = 2.0 ** -25 * (seen.double() @ vz.abs()) / safe
-        allowed[i] = mass * (2.0 ** -11 + 2.2 * off + (n + 80) * 2.0 ** -23) + under
+        # Probabilities p rounded to fp16 are p (1 + e) + u, |e| <= 2^-11, |u| <= 2^-25 (below 2^-14). Both
+        # sums of sum p v / sum p take the rounded ones: with o the exact result, the quotient is off by
+        # sum (p e + u) (v - o) / sum p (1 + e), at most 2^-11 (mass + |o|) and 2^-25 (sum |v| + n |o|) / sum p,
+        # times 1 + 2^-10 for the divisor. Scores are off by `off`, fp32 sums of n terms, the hardware's
+        # exponential (2^-22).
+        o = out[i].abs()
+        under = 2.0 ** -25 * (seen.double() @ vz.abs() + seen.sum(-1, keepdim=True) * o) / safe
+        allowed[i] = ((mass + o) * 2.0 ** -11 + under) * (1 + 2.0 ** -10) + mass * (2.2 * off + (n + 80) * 2.0 ** -23)
     return out, allowed
 
 
-def filled(pkg, dev, b, heads, d, width, seed=0, lengths=None):
+def filled(pkg, dev, b, heads, d, width, seed=0, lengths=None, spread=9):
     """A cache with codes everywhere (NaN codes behind the lengths), its float64 form and its table."""
     g = torch.Generator().manual_seed(seed)
     table = tables(b, width, seed=seed)
@@ -671,7 +675,7 @@ def filled(pkg, dev, b, heads, d, width, seed=0, lengths=None):
     n = width * 64
     k, v = torch.randn(b, heads, n, d, generator=g), torch.randn(b, heads, n, d, generator=g)
     k *= torch.exp2(torch.randint(-2, 2, (b, heads, width, 1), generator=g).float()).repeat_interleave(64, 2)
-    v *= torch.exp2(torch.randint(-9, 9, (b, heads, width, 1), generator=g).float()).repeat_interleave(64, 2)
+    v *= torch.exp2(torch.randint(-spread, spread, (b, heads, width, 1), generator=g).float()).repeat_interleave(64, 2)
     pkg.ops.cache8_append(cache, k.to(dev), v.to(dev), table.to(dev), torch.zeros(b, dtype=torch.int32, device=dev))
     if lengths is not None:
         for i, n in enumerate(lengths.tolist()):
@@ -692,9 +696,9 @@ def longer(table: torch.Tensor, width: int | None) -> torch.Tensor:
     return table if width is None else torch.nn.functional.pad(table, (0, width - table.shape[1]), value=-1)
 
 
-def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, seed=0, scale=None, long=None):
+def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, seed=0, scale=None, long=None, spread=9):
     scale = d ** -0.5 if scale is None else scale
-    cache, ref, table = filled(pkg, dev, b, heads, d, width, seed, lengths)
+    cache, ref, table = filled(pkg, dev, b, heads, d, width, seed, lengths, spread)
     q = rand((b, heads * group, lq, d), seed + 7, t)
     got = pkg.ops.cache8_attention(q.to(dev), cache, longer(table, long).to(dev), lengths.to(dev), scale,
                                    starts=None if starts is None else starts.to(dev))
@@ -738,6 +742,45 @@ def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
     starts = ints(0, 1, 100, -3, 250, 63)
     lengths = ints(lq, lq + 1, 100 + lq, lq, 250 + max(lq // 2, 1), 63 + lq)
     attention_case(pkg, dev, t, 6, heads, group, d, lq, lengths, starts, 8, seed=d + lq, long=LONG[d])
+
+
+@gpu
+@pytest.mark.parametrize("lq", [2, 140])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_value_scales_far_apart(pkg, dev, d, lq) -> None:
+    """Pages of values up to 2^60 apart, in both orders."""
+    long = LONG[d] if lq > 100 else None
+    attention_case(pkg, dev, torch.bfloat16, 2, 1, 1, d, lq, ints(1000, 640), None, 16, long=long, spread=30)
+    attention_case(pkg, dev, torch.bfloat16, 2, 1, 1, d, lq, ints(1000, 640), ints(1000 - lq, 500), 16, seed=5, long=long, spread=30)
+
+
+@gpu
+@pytest.mark.parametrize("lq", [3, 130])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_queries_before_a_page_do_not_feel_its_scale(pkg, dev, d, lq) -> None:
+    """A page's scale, however large, or NaN, reaches only the queries that see the page."""
+    long = LONG[d] if lq > 100 else None
+    cache, _, table = filled(pkg, dev, 1, 2, d, 8)
+    q = rand((1, 2, lq, d), 3, torch.bfloat16).to(dev)
+    first = 256 - lq // 2   # half of the queries see page 4
+    run = lambda: pkg.ops.cache8_attention(q, cache, longer(table, long).to(dev), ints(448).to(dev), 0.1, starts=ints(first).to(dev))
+    want, page = run(), int(table[0, 4])
+    assert want.isfinite().all()
+    for scales in (cache.v_scales, cache.k_scales):
+        was = scales.clone()
+        for byte in (240, 255, 0):
+            scales.view(torch.uint8)[page, 0] = byte
+            got = run()
+            assert torch.equal(got[:, 1], want[:, 1]) and torch.equal(got[:, 0, :256 - first], want[:, 0, :256 - first])
+            seen = got[:, 0, 256 - first:]
+            if byte == 255:
+                assert seen.isnan().all()
+            elif byte == 0 or scales is cache.v_scales:   # (keys of 448 * 2^113 and 64 channels of 4: scores pass fp32)
+                assert not seen.isnan().any()
+            if byte == 240 and scales is cache.v_scales:
+                assert (seen.abs() > 2.0 ** 80).any()
+        scales.copy_(was)
+    assert torch.equal(run(), want)
 
 
 @gpu
