@@ -38,8 +38,9 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
   return v;
 }
 
-// Values c .. c + 7 of a row, zero past C; with a residual, the rounded sum (also stored).
-template <typename T>
+// Values c .. c + 7 of a row, zero past C; with a residual, the rounded sum (also stored, past the caches
+// where it is not read again).
+template <bool STREAM = true, typename T>
 __device__ __forceinline__ void take8(const NormArgs& a, const T* x, const T* r, T* s, int c, float (&f)[8]) {
   if (c + 8 <= a.C) {
     load8(x + c, f);
@@ -48,7 +49,10 @@ __device__ __forceinline__ void take8(const NormArgs& a, const T* x, const T* r,
       load8(r + c, g);
 #pragma unroll
       for (int i = 0; i < 8; i++) f[i] = (float)(T)(f[i] + g[i]);
-      if (s) store8(s + c, f);
+      if (s) {
+        if constexpr (STREAM) stream8(s + c, f);
+        else store8(s + c, f);
+      }
     }
     return;
   }
@@ -89,13 +93,13 @@ __device__ __forceinline__ void give8(const NormArgs& a, int64_t row, int c, flo
     const float inv = inverse_of(b);
     if (c < a.kb * kBlock8) {
       const i32x2 w = {encode4(f[0], f[1], f[2], f[3], inv), encode4(f[4], f[5], f[6], f[7], inv)};
-      *reinterpret_cast<i32x2*>(a.codes + row * a.cp + c) = w;
+      __builtin_nontemporal_store(w, reinterpret_cast<i32x2*>(a.codes + row * a.cp + c));
       if (c % kBlock8 == 0) a.scales[row * a.ep + c / kBlock8] = (uint8_t)b;
     }
   } else {
     T* y = (T*)a.y + row * a.yp;
     if (c + 8 <= a.C) {
-      store8(y + c, f);
+      stream8(y + c, f);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++)
@@ -106,7 +110,8 @@ __device__ __forceinline__ void give8(const NormArgs& a, int64_t row, int c, flo
 
 // 1 / sqrt(mean + eps) of a row from its sum of squares, for values that are first multiplied by g: 1
 // but where the squares pass fp32 although the values do not (bf16 and fp32 beyond 2^64 / sqrt(C));
-// there the power of two that brings the largest value to 1..4, and the squares are taken again.
+// there the power of two that brings the largest value to 1..4, and the squares are taken again. (Squares
+// below fp32 are nothing beside eps, 1e-30 at least.)
 template <int TPR, typename Square>
 __device__ __forceinline__ float row_rstd(const NormArgs& a, float ss, float amax, float* red, float& g,
                                           Square squares) {
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
     if constexpr (NORM) {
       float ss = 0.f, amax = 0.f, f[8];
       for (int k = 0; k < rounds; k++) {
-        take8(a, x, r, s, (k * TPR + t) * 8, f);
+        take8<false>(a, x, r, s, (k * TPR + t) * 8, f);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           ss += f[i] * f[i];
@@ -189,14 +194,14 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
       rstd = row_rstd<TPR>(a, ss, amax, red, g, [&](float by) {
         float q = 0.f, h[8];
         for (int k = 0; k < rounds; k++) {
-          take8<T>(a, x2, r2, nullptr, (k * TPR + t) * 8, h);
+          take8(a, x2, r2, (T*)nullptr, (k * TPR + t) * 8, h);
 #pragma unroll
           for (int i = 0; i < 8; i++) q += (h[i] * by) * (h[i] * by);
         }
         return q;
       });
       for (int k = 0; k < rounds; k++) {
-        take8<T>(a, x2, r2, nullptr, (k * TPR + t) * 8, f);
+        take8(a, x2, r2, (T*)nullptr, (k * TPR + t) * 8, f);
         times(f, g);
         give8<T, NORM, Q8>(a, row, (k * TPR + t) * 8, rstd, f);
       }

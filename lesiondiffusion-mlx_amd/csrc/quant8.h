@@ -56,6 +56,18 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
   __builtin_memcpy(p, &u, sizeof(u));
 }
 
+// The same past the caches' retention, for results that leave the kernel: they go out while it works, where
+// dirty lines wait in the XCDs' caches for the launch's end.
+template <typename T>
+__device__ __forceinline__ void stream8(T* p, const float (&f)[8]) {
+  typedef T V __attribute__((ext_vector_type(8)));
+  typedef V Unaligned __attribute__((aligned(sizeof(T))));
+  V v;
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = (T)f[i];
+  __builtin_nontemporal_store(v, reinterpret_cast<Unaligned*>(p));
+}
+
 // Largest of v over the 16 lanes of a DPP row, on every one of them.
 __device__ __forceinline__ float row16_max(float v) {
   v = fmaxf(v, dpp_f<0x128>(v));   // row_ror:8
