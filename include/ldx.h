@@ -484,7 +484,7 @@ typedef struct ldx_cache8 {
  * page that holds older tokens (before starts[b]) keeps the larger of its scale and the one
  * that the new tokens ask for; where it rises the older codes are rounded to it. A page whose
  * first token is written takes the new tokens' scale. Codes behind the last written token
- * stay as they are. Sequences that write must not share a page. Nothing is written of a
+ * stay as they are. A page that is written stands once in the table. Nothing is written of a
  * sequence with starts[b] < 0, past the table's width, or in a page that the cache does not
  * have. */
 typedef struct ldx_cache8_append_args {
@@ -503,10 +503,12 @@ int ldx_cache8_append(const ldx_cache8_append_args* args, void* stream);
  * starts, query i sees no token behind starts[b] + i (causal for queries at starts[b]..). q and
  * o: (batch, token, head) strides, contiguous channels, fp16 or bf16; q_heads a multiple of
  * the cache's heads, query head j reads the cache's head j / (q_heads / heads). fp32 scores,
- * softmax and sums; probabilities are rounded to fp16. A query that sees no token gets 0.
- * Tokens that a query does not see do not touch its result, NaN among them. A page that the
- * cache does not have gives NaN to the queries that see it, a length past the table to the
- * whole sequence. Workspace: partial results where a sequence is split over workgroups,
+ * softmax and sums; probabilities are rounded to fp16, in both of the quotient's sums. A query
+ * that sees no token gets 0. Tokens that a query does not see do not touch its result, NaN
+ * among them. A page that the cache does not have, or with a scale of NaN, gives NaN to the
+ * queries that see it, a length past the table to the whole sequence. Where pages' value scales
+ * are more than 2^70 apart, what is below 2^-90 of the largest values may be lost. o may be q.
+ * Workspace: partial results where a sequence is split over workgroups,
  * ldx_cache8_attention_workspace_bytes of them; with less nothing is split. */
 typedef struct ldx_cache8_attention_args {
   ldx_cache8 cache;

@@ -252,8 +252,8 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
   __shared__ float sm[kAttendWaves][16], sl[kAttendWaves][16];
   __shared__ float sacc[kAttendWaves][16][D + 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int b = blockIdx.z, split = blockIdx.x, tiles = (a.rows + 15) / 16;
-  const int h = blockIdx.y / tiles, row0 = blockIdx.y % tiles * 16;
+  const int b = blockIdx.z, split = blockIdx.x % a.splits, tiles = (a.rows + 15) / 16, tile = blockIdx.x / a.splits;
+  const int h = tile / tiles, row0 = tile % tiles * 16;
   const int row = row0 + r;
   const bool real = row < a.rows;
   const int raw = a.lengths[b];
@@ -557,8 +557,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int flags[2];                 // the last page of each buffer that holds a NaN value code
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
-  const int b = blockIdx.z, split = blockIdx.x, tiles = (a.rows + kWideRows - 1) / kWideRows;
-  const int h = blockIdx.y / tiles, row0 = (tiles - 1 - blockIdx.y % tiles) * kWideRows;   // causal: longest first
+  const int b = blockIdx.z, split = blockIdx.x % a.splits, tiles = (a.rows + kWideRows - 1) / kWideRows;
+  const int tile = blockIdx.x / a.splits;
+  const int h = tile / tiles, row0 = (tiles - 1 - tile % tiles) * kWideRows;   // causal: longest first
   const int wrow = row0 + 32 * wave, row = wrow + r;
   const bool real = row < a.rows;
   const int raw = a.lengths[b];
@@ -950,7 +951,7 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Args a) {
 
 template <typename T, int D>
 int launch_d(const Attend8Args& a, int batch, hipStream_t st) {
-  const dim3 grid((unsigned)a.splits, (unsigned)(a.H * ((a.rows + a.tile - 1) / a.tile)), (unsigned)batch);
+  const dim3 grid((unsigned)a.splits * (unsigned)(a.H * ((a.rows + a.tile - 1) / a.tile)), 1, (unsigned)batch);
   if (a.tile == 16) {
     hipLaunchKernelGGL((attend8_kernel<T, D>), grid, dim3(64 * kAttendWaves), 0, st, a);
   } else if constexpr (D >= 64) {
@@ -1040,8 +1041,6 @@ int check_attention(const ldx_cache8_attention_args* p) {
   if (rows * p->cache.heads * p->batch > 0x7fffffff)
     return fail("cache8_attention: %d x %d queries of %d heads are more than one launch takes", p->batch, p->q_len,
                 p->q_heads);
-  if ((rows + 15) / 16 * p->cache.heads > 65535)
-    return fail("cache8_attention: %d queries of %d heads are more than one launch takes", p->q_len, p->q_heads);
   if (p->table_pitch < p->width) return fail("cache8_attention: table pitch below %d", p->width);
   if (!(p->scale > -1e30f && p->scale < 1e30f)) return fail("cache8_attention: scale %g", (double)p->scale);
   return LDX_OK;

@@ -511,8 +511,8 @@ int launch_big(const Dense8Args& a, hipStream_t st) {
 // Which kernel: the one of least estimated time. A call's time was measured as a sum of a fixed part, one
 // for each round of workgroups (places: as many as the CUs hold at once), for each block of a workgroup's
 // steps in a round, and for the workgroups and their steps by how full the rounds are -- fitted to 130 random
-// shapes (1 to 8,192 rows, 64 to 8,192 features and outputs) per kernel; the choices are within 0.5 % (16-bit
-// results) and 1.3 % (fp32) of the fastest on average, 19 % at most. us.
+// shapes (1 to 8,192 rows, 64 to 8,192 features and outputs) per kernel; the choices are within 0.6 % (16-bit
+// results) and 1.2 % (fp32) of the fastest on average, 20 % at most. us.
 struct Cost {
   float fixed, round, step, work, tile;   // the last two per full round
 };

@@ -1098,6 +1098,15 @@ def _head_strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     return b, l, h
 
 
+def _distinct(t: torch.Tensor, name: str) -> None:
+    """No two values of ``t`` stand in one place (sizes within strides, from the innermost axis out)."""
+    span = 1
+    for stride, size in sorted((stride, size) for stride, size in zip(t.stride(), t.shape) if size > 1):
+        if stride < span:
+            raise ValueError(f"{name} of strides {t.stride()} overlaps itself")
+        span = stride * size
+
+
 def cache8_append(cache: Cache8, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, *,
                   counts: torch.Tensor | None = None) -> None:
     """Write ``k``, ``v`` (B, heads, L, D; fp16, bf16 or fp32, any strides with contiguous channels) into
@@ -1105,7 +1114,7 @@ def cache8_append(cache: Cache8, k: torch.Tensor, v: torch.Tensor, table: torch.
     without). Each page of 64 tokens has one power of two for a head's keys and one for its values; it
     rises with the largest token written, and older codes of the page are then rounded to it. Tokens
     past the table's width, of a negative start or in a page that the cache does not have are left out;
-    sequences that write must not share pages. ``table``, ``starts`` and ``counts`` are int32 on the
+    a page that is written stands once in the table. ``table``, ``starts`` and ``counts`` are int32 on the
     device, so a captured graph appends where they say at each replay."""
     block, dev = _cache_block(cache, "cache8_append")
     _need(k, "k", _ALL, dev)
@@ -1131,7 +1140,7 @@ def cache8_attention(q: torch.Tensor, cache: Cache8, table: torch.Tensor, length
     ``starts[b] + i`` (causal); without, all ``lengths[b]``. A query that sees no token gives 0; tokens that
     it does not see, and pages behind the length, do not touch its result. A page that the cache does
     not have, or a length past the table, gives NaN. Returns ``(B, heads, L, D)`` in ``q``'s type (into
-    ``out`` when given); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
+    ``out`` when given, which may be ``q``); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
     block, dev = _cache_block(cache, "cache8_attention")
     _need(q, "q", _ELEM, dev)
     shape = q.shape
@@ -1143,6 +1152,8 @@ def cache8_attention(q: torch.Tensor, cache: Cache8, table: torch.Tensor, length
         _need(out, "out", q.dtype, dev)
         if out.shape != shape:
             raise ValueError(f"out shape {tuple(out.shape)} != {tuple(shape)}")
+        if not out.is_contiguous():
+            _distinct(out, "out")
     else:
         out = q.new_empty(shape)
     a = Cache8AttentionArgs(block, b, hq, lq, q.data_ptr(), _head_strides(q, "q"), out.data_ptr(),

@@ -745,6 +745,26 @@ def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("d", [32, 64])
+def test_attention_of_a_million_rows(pkg, dev, d) -> None:
+    """More tiles of rows than a launch's second axis takes."""
+    attention_case(pkg, dev, torch.bfloat16, 1, 1, 32, d, 33000, ints(70), None, 2)
+
+
+@gpu
+@pytest.mark.parametrize("lq", [1, 3, 200])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_attention_in_place(pkg, dev, d, lq) -> None:
+    long = LONG.get(d) if lq > 100 else None
+    cache, _, table = filled(pkg, dev, 2, 2, d, 30)
+    q = rand((2, lq, 4, d), 3, torch.bfloat16).to(dev).transpose(1, 2)
+    args = cache, longer(table, long).to(dev), ints(1900, 640).to(dev), 0.1
+    want = pkg.ops.cache8_attention(q, *args)
+    got = pkg.ops.cache8_attention(q, *args, out=q)
+    assert got is q and torch.equal(got, want)
+
+
+@gpu
 @pytest.mark.parametrize("lq", [2, 140])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attention_value_scales_far_apart(pkg, dev, d, lq) -> None:
@@ -906,6 +926,8 @@ def test_cache_refuses_on_the_device(pkg, dev) -> None:
                  lambda: ops.cache8_attention(q, cache, table, n, NAN),
                  lambda: ops.cache8_attention(q, bad_v, table, n, 1.0),
                  lambda: ops.cache8_attention(q, cache, table, n, 1.0, out=q[:, :, :2]),
+                 lambda: ops.cache8_attention(q, cache, table, n, 1.0, out=q[:, :, :1].expand(-1, -1, 3, -1)),
+                 lambda: ops.cache8_attention(q, cache, table, n, 1.0, out=q.flatten().as_strided(q.shape, (384, 64, 64, 1))),
                  lambda: ops.cache8_attention(q, cache, table, n, 1.0, starts=n.cpu()),
                  lambda: ops.cache8_append(cache, q, q[:, :, :1], table, n),
                  lambda: ops.cache8_append(cache, q, q.float(), table, n),
