@@ -1017,6 +1017,11 @@ Plan plan_of(const ldx_cache8_attention_args* p) {
     // Two workgroups a CU (256 to 1,024 parts in all were within a tenth for most calls, more slower).
     s = 512 / (heads * ((rows + 15) / 16));
     if (s > most) s = most;
+    // Parts cost a second launch to join, 3 us on the device and 4 on the host. A whole sequence's pages take a
+    // workgroup 0.17 / 0.2 / 0.4 / 0.8 us each at head width 32 / 64 / 128 / 256: up to these many it is ahead or
+    // near it (one token behind 1,500 at 64 10.0 us in parts, 9.5 whole, behind 2,000 10.5 and 10.9, 3,000 11.2
+    // and 13.7; called one by one 19.4 and 15.4; behind 1,000 at 128 12.1 and 11.5, 2,000 13.0 and 17.0).
+    if (p->width <= (D <= 64 ? 32 : D == 128 ? 20 : 10)) s = 1;
   }
   plan.splits = (int)(s < 1 ? 1 : s > kMostParts ? kMostParts : s);
   return plan;

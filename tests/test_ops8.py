@@ -812,7 +812,7 @@ def test_attention_of_many_rows_in_parts(pkg, dev, d) -> None:
 
 
 @gpu
-@pytest.mark.parametrize(("b", "heads", "group", "d", "n"), [(1, 1, 1, 64, 20000), (2, 2, 8, 128, 9001), (1, 1, 4, 256, 5000)])
+@pytest.mark.parametrize(("b", "heads", "group", "d", "n"), [(2, 1, 2, 32, 9000), (1, 1, 1, 64, 20000), (2, 2, 8, 128, 9001), (1, 1, 4, 256, 5000)])
 def test_attention_long(pkg, dev, b, heads, group, d, n) -> None:
     lengths = ints(*[n - 77 * i for i in range(b)])
     attention_case(pkg, dev, torch.float16, b, heads, group, d, 1, lengths, None, -(-n // 64) + 1)
