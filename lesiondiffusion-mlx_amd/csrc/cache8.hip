@@ -12,7 +12,7 @@ struct AppendArgs {
   uint8_t* scales[2];    // (pages, H)
   const void* src[2];
   int64_t st[2][3];      // batch, token, head strides of the new keys / values
-  int pages, H, D, tokens;
+  int pages, H, tokens;
   const int32_t* table; int64_t tp; int width;
   const int32_t* starts;
   const int32_t* counts;
@@ -28,11 +28,13 @@ __device__ __forceinline__ int recode4(int w, int from, int to) {
 }
 
 // One page's new tokens of one head, keys or values: their largest magnitude, the page's scale, the
-// codes. Values go through LDS, where they are turned channel by token.
-template <typename T>
+// codes. A thread keeps its D / 32 groups of eight channels of a token between the two. Values go through
+// LDS, where they are turned channel by token (rows of 68 bytes: the groups of a token meet different banks).
+template <typename T, int D>
 __global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
+  constexpr int UNITS = D / 8, MOST = D / 32, PITCH = kPage8 + 4;
   __shared__ float red[4];
-  __shared__ __align__(16) uint8_t turned[256 * 64];
+  __shared__ __align__(16) uint8_t turned[D * PITCH];
   const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, tid = threadIdx.x;
   const int start = a.starts[b];
   const int n = a.counts ? min(a.counts[b], a.tokens) : a.tokens;
@@ -42,62 +44,72 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
   if (first >= end || slot >= a.width) return;
   const int page = a.table[b * a.tp + slot];
   if ((unsigned)page >= (unsigned)a.pages) return;
+  uint8_t* scale = a.scales[which] + (int64_t)page * a.H + h;
+  uint8_t* codes = a.codes[which] + ((int64_t)page * a.H + h) * D * kPage8;
+  const int was = *scale;
   const int lo = (int)max(start - first, (int64_t)0), hi = (int)min(end - first, (int64_t)kPage8);
-  const int units = a.D / 8, chunks = (hi - lo) * units;   // eight channels of a token each
-  const T* src = (const T*)a.src[which] + b * a.st[which][0] + (first + lo - start) * a.st[which][1] + h * a.st[which][2];
+  const int chunks = (hi - lo) * UNITS;
   const int64_t tok = a.st[which][1];
+  const T* src = (const T*)a.src[which] + b * a.st[which][0] + (first + lo - start) * tok + h * a.st[which][2];
+  float f[MOST][8];
   float amax = 0.f;
-  for (int c = tid; c < chunks; c += 256) {
-    float f[8];
-    load8(src + c / units * tok + c % units * 8, f);
 #pragma unroll
-    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(f[i]));
+  for (int j = 0; j < MOST; j++) {
+    const int c = tid + 256 * j;
+    if (c < chunks) {
+      load8(src + c / UNITS * tok + c % UNITS * 8, f[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) f[j][i] = 0.f;
+    }
   }
+#pragma unroll
+  for (int j = 0; j < MOST; j++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(f[j][i]));
   amax = wave_max(amax);
   if ((tid & 63) == 0) red[tid >> 6] = amax;
-  __syncthreads();
+  __syncthreads();   // behind it every thread has read the old scale, too
   amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  uint8_t* scale = a.scales[which] + (int64_t)page * a.H + h;
-  uint8_t* codes = a.codes[which] + ((int64_t)page * a.H + h) * a.D * kPage8;
-  const int was = *scale;
   int to = scale_byte(amax);
   const bool rises = lo > 0 && to > was;
   if (lo > 0 && to < was) to = was;
   const float inv = inverse_of(min(to, 253));
-  __syncthreads();   // every thread has read the old scale
   if (tid == 0) *scale = (uint8_t)to;
   if (which == 0) {
     if (rises)
-      for (int c = tid; c < lo * a.D / 4; c += 256) {
+      for (int c = tid; c < lo * D / 4; c += 256) {
         int* w = reinterpret_cast<int*>(codes) + c;
         *w = recode4(*w, was, to);
       }
-    for (int c = tid; c < chunks; c += 256) {
-      float f[8];
-      load8(src + c / units * tok + c % units * 8, f);
-      const i32x2 w = {encode4(f[0], f[1], f[2], f[3], inv), encode4(f[4], f[5], f[6], f[7], inv)};
-      *reinterpret_cast<i32x2*>(codes + (lo + c / units) * a.D + c % units * 8) = w;
+#pragma unroll
+    for (int j = 0; j < MOST; j++) {
+      const int c = tid + 256 * j;
+      if (c >= chunks) break;
+      const i32x2 w = {encode4(f[j][0], f[j][1], f[j][2], f[j][3], inv), encode4(f[j][4], f[j][5], f[j][6], f[j][7], inv)};
+      *reinterpret_cast<i32x2*>(codes + (lo + c / UNITS) * D + c % UNITS * 8) = w;
     }
     return;
   }
-  for (int c = tid; c < chunks; c += 256) {
-    float f[8];
-    load8(src + c / units * tok + c % units * 8, f);
-    const int w0 = encode4(f[0], f[1], f[2], f[3], inv), w1 = encode4(f[4], f[5], f[6], f[7], inv);
-    uint8_t* t = turned + c % units * 8 * kPage8 + lo + c / units;
+#pragma unroll
+  for (int j = 0; j < MOST; j++) {
+    const int c = tid + 256 * j;
+    if (c >= chunks) break;
+    const int w0 = encode4(f[j][0], f[j][1], f[j][2], f[j][3], inv), w1 = encode4(f[j][4], f[j][5], f[j][6], f[j][7], inv);
+    uint8_t* t = turned + c % UNITS * 8 * PITCH + lo + c / UNITS;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      t[i * kPage8] = (uint8_t)(w0 >> (8 * i));
-      t[(i + 4) * kPage8] = (uint8_t)(w1 >> (8 * i));
+      t[i * PITCH] = (uint8_t)(w0 >> (8 * i));
+      t[(i + 4) * PITCH] = (uint8_t)(w1 >> (8 * i));
     }
   }
   __syncthreads();
   // Four tokens of a channel at a time: older ones (re-coded where the scale rises) below lo, new ones
   // up to hi, the rest as it is.
   const int g0 = rises ? 0 : lo / 4, g1 = (hi + 3) / 4, per = g1 - g0;
-  for (int c = tid; c < a.D * per; c += 256) {
-    const int at = c / per * kPage8 + (g0 + c % per) * 4, t0 = (g0 + c % per) * 4;
-    int w = *reinterpret_cast<const int*>(turned + at);
+  for (int c = tid; c < D * per; c += 256) {
+    const int d = c / per, t0 = (g0 + c % per) * 4, at = d * kPage8 + t0;
+    int w = *reinterpret_cast<const int*>(turned + d * PITCH + t0);
     if (t0 < lo || t0 + 4 > hi) {
       const int old = *reinterpret_cast<const int*>(codes + at);
       const int kept = rises ? recode4(old, was, to) : old;
@@ -112,6 +124,14 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
     }
     *reinterpret_cast<int*>(codes + at) = w;
   }
+}
+
+template <typename T>
+void launch_append(const AppendArgs& a, int D, dim3 grid, hipStream_t st) {
+  if (D == 32) hipLaunchKernelGGL((append8_kernel<T, 32>), grid, dim3(256), 0, st, a);
+  else if (D == 64) hipLaunchKernelGGL((append8_kernel<T, 64>), grid, dim3(256), 0, st, a);
+  else if (D == 128) hipLaunchKernelGGL((append8_kernel<T, 128>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((append8_kernel<T, 256>), grid, dim3(256), 0, st, a);
 }
 
 // ------------------------------------------------------------------------------------- attention
@@ -1068,14 +1088,14 @@ extern "C" int ldx_cache8_append(const ldx_cache8_append_args* p, void* stream) 
                   {(uint8_t*)p->cache.k_scales, (uint8_t*)p->cache.v_scales},
                   {p->k, p->v},
                   {{p->k_stride[0], p->k_stride[1], p->k_stride[2]}, {p->v_stride[0], p->v_stride[1], p->v_stride[2]}},
-                  p->cache.pages, p->cache.heads, p->cache.head_dim, p->tokens,
+                  p->cache.pages, p->cache.heads, p->tokens,
                   p->table, p->table_pitch, p->width, p->starts, p->counts};
   const unsigned slots = (unsigned)((p->tokens + 2 * (int64_t)kPage8 - 2) / kPage8);
   const dim3 grid(slots, 2 * (unsigned)p->cache.heads, (unsigned)p->batch);
   hipStream_t st = as_stream(stream);
-  if (p->dtype == LDX_DTYPE_F16) hipLaunchKernelGGL(append8_kernel<f16>, grid, dim3(256), 0, st, a);
-  else if (p->dtype == LDX_DTYPE_BF16) hipLaunchKernelGGL(append8_kernel<bf16>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(append8_kernel<float>, grid, dim3(256), 0, st, a);
+  if (p->dtype == LDX_DTYPE_F16) launch_append<f16>(a, p->cache.head_dim, grid, st);
+  else if (p->dtype == LDX_DTYPE_BF16) launch_append<bf16>(a, p->cache.head_dim, grid, st);
+  else launch_append<float>(a, p->cache.head_dim, grid, st);
   return check_launch("cache8_append");
 }
 
