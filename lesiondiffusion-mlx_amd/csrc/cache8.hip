@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
       const int c = tid + 256 * j;
       if (c >= chunks) break;
       const i32x2 w = {encode4(f[j][0], f[j][1], f[j][2], f[j][3], inv), encode4(f[j][4], f[j][5], f[j][6], f[j][7], inv)};
-      *reinterpret_cast<i32x2*>(codes + (lo + c / UNITS) * D + c % UNITS * 8) = w;
+      __builtin_nontemporal_store(w, reinterpret_cast<i32x2*>(codes + (lo + c / UNITS) * D + c % UNITS * 8));
     }
     return;
   }
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
       }
       w = (int)m;
     }
-    *reinterpret_cast<int*>(codes + at) = w;
+    __builtin_nontemporal_store(w, reinterpret_cast<int*>(codes + at));
   }
 }
 
