@@ -513,27 +513,37 @@ int launch_big(const Dense8Args& a, hipStream_t st) {
 // steps in a round, and for the workgroups and their steps by how full the rounds are -- fitted to 130 random
 // shapes (1 to 8,192 rows, 64 to 8,192 features and outputs) per kernel; the choices are within 0.6 % (16-bit
 // results) and 1.2 % (fp32) of the fastest on average, 20 % at most. us.
+// An activation adds to a round, and to the tiles of the two large ones, what one wave a SIMD takes for all of
+// its tile's results: without that 2.8 % from the fastest on average, 54 % at most, with it 1.1 and 31 (GELU).
 struct Cost {
   float fixed, round, step, work, tile;   // the last two per full round
+  float act, act_tile;
 };
 
-inline double estimate(const Cost& c, int64_t M, int64_t O, int kb, int tm, int tn, int places, int waves) {
+inline double estimate(const Cost& c, bool act, int64_t M, int64_t O, int kb, int tm, int tn, int places, int waves) {
   const double tiles = (double)((M + tm - 1) / tm) * (double)((O + tn - 1) / tn), full = tiles / places;
   const double rounds = (double)(int64_t)(full + 0.999999), steps = (kb + waves - 1) / waves;
-  return c.fixed + c.round * rounds + c.step * rounds * steps + c.work * full * steps + c.tile * full;
+  return c.fixed + c.round * rounds + c.step * rounds * steps + c.work * full * steps + c.tile * full +
+         (act ? c.act * rounds + c.act_tile * full : 0.0);
 }
 
 template <typename T>
 int launch(const Dense8Args& a, hipStream_t st) {
   constexpr bool EXACT = sizeof(T) == 4;
-  constexpr Cost big4 = EXACT ? Cost{9.80f, 2.11f, 2.267f, 0.298f, 14.97f} : Cost{10.78f, 1.97f, 0.981f, 0.299f, 9.03f};
-  constexpr Cost big2 = EXACT ? Cost{5.22f, 0.f, 0.740f, 0.654f, 9.33f} : Cost{5.16f, 0.f, 0.411f, 0.546f, 4.85f};
-  constexpr Cost big1 = EXACT ? Cost{4.06f, 0.f, 0.366f, 0.169f, 2.83f} : Cost{3.51f, 0.62f, 0.208f, 0.174f, 1.50f};
-  constexpr Cost split2 = EXACT ? Cost{3.21f, 1.27f, 1.010f, 0.092f, 1.56f} : Cost{3.10f, 1.60f, 0.677f, 0.192f, 0.80f};
-  constexpr Cost split1 = EXACT ? Cost{3.66f, 0.f, 0.468f, 0.267f, 1.16f} : Cost{3.65f, 0.01f, 0.339f, 0.327f, 0.91f};
-  const double t[5] = {estimate(split1, a.M, a.O, a.kb, 32, 32, 512, 4), estimate(split2, a.M, a.O, a.kb, 64, 64, 256, 4),
-                       estimate(big1, a.M, a.O, a.kb, 64, 64, 512, 1), estimate(big2, a.M, a.O, a.kb, 128, 128, 512, 1),
-                       estimate(big4, a.M, a.O, a.kb, 256, 256, 256, 1)};
+  const bool act = a.act != LDX_ACT_NONE;
+  constexpr Cost big4 = EXACT ? Cost{9.80f, 2.11f, 2.267f, 0.298f, 14.97f, 15.5f, 3.4f}
+                              : Cost{10.78f, 1.97f, 0.981f, 0.299f, 9.03f, 15.5f, 3.4f};
+  constexpr Cost big2 = EXACT ? Cost{5.22f, 0.f, 0.740f, 0.654f, 9.33f, 2.8f, 4.4f}
+                              : Cost{5.16f, 0.f, 0.411f, 0.546f, 4.85f, 2.8f, 4.4f};
+  constexpr Cost big1 = EXACT ? Cost{4.06f, 0.f, 0.366f, 0.169f, 2.83f, 0.9f, 0.3f}
+                              : Cost{3.51f, 0.62f, 0.208f, 0.174f, 1.50f, 0.9f, 0.3f};
+  constexpr Cost split2 = EXACT ? Cost{3.21f, 1.27f, 1.010f, 0.092f, 1.56f, 0.9f, 0.1f}
+                              : Cost{3.10f, 1.60f, 0.677f, 0.192f, 0.80f, 0.9f, 0.1f};
+  constexpr Cost split1 = EXACT ? Cost{3.66f, 0.f, 0.468f, 0.267f, 1.16f, 0.5f, 0.f}
+                              : Cost{3.65f, 0.01f, 0.339f, 0.327f, 0.91f, 0.5f, 0.f};
+  const double t[5] = {estimate(split1, act, a.M, a.O, a.kb, 32, 32, 512, 4), estimate(split2, act, a.M, a.O, a.kb, 64, 64, 256, 4),
+                       estimate(big1, act, a.M, a.O, a.kb, 64, 64, 512, 1), estimate(big2, act, a.M, a.O, a.kb, 128, 128, 512, 1),
+                       estimate(big4, act, a.M, a.O, a.kb, 256, 256, 256, 1)};
   int best = 0;
   for (int i = 1; i < 5; i++)
     if (t[i] < t[best]) best = i;
