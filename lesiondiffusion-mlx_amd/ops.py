@@ -681,7 +681,7 @@ def _vq_rows(t: torch.Tensor, name: str) -> int:
 def squared_norms4(x: torch.Tensor) -> torch.Tensor:
     """Per-row ``T(sum float32(T(x * x)))`` of ``(rows, 4)`` vectors, the squared norm the
     reference keeps per codebook entry (mlx_model.py:775-778)."""
-    n = _vq_rows(x)
+    n = _vq_rows(x, "x")
     out = torch.empty(n, dtype=x.dtype, device=x.device)
     check(lib.ldx_vq_squared_norms4(_ptr(x), n, _VQ_DTYPES[x.dtype], _ptr(out), _stream()), "vq_squared_norms4")
     return out
