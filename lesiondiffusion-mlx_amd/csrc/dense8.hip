@@ -28,10 +28,11 @@ __device__ __forceinline__ float exp_neg(float x) {
 
 // GELU without the cancellation of 1 + erf for negative v: v Q(|v|) there and v (1 - Q(v)) otherwise,
 // Q(v) = erfc(v / sqrt 2) / 2 = t exp(p(t) - v^2 / 2) / 2, t = 1 / (1 + 0.4 v / sqrt 2), where p is a
-// least-squares Chebyshev fit of log(erfc(x) exp(x^2) / t) for x up to 12 (to 1.1e-7). Branchless: the
-// library's erff and expf in the eight-wide epilogue were 20 KB of code.
+// least-squares Chebyshev fit of log(erfc(x) exp(x^2) / t) for x up to 12 (to 1.1e-7; beyond 64 Q is 0 and v
+// itself must not be squared). Branchless: the library's erff and expf in the eight-wide epilogue were 20 KB
+// of code.
 __device__ __forceinline__ float gelu_f(float v) {
-  const float u = fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(u, 0.4f * 0.70710678f, 1.0f));
+  const float u = fminf(fabsf(v), 64.f), t = __builtin_amdgcn_rcpf(__builtin_fmaf(u, 0.4f * 0.70710678f, 1.0f));
   float p = -0.213728147f;
   p = __builtin_fmaf(p, t, 0.955197486f);
   p = __builtin_fmaf(p, t, -1.5495496f);
@@ -47,7 +48,9 @@ __device__ __forceinline__ float gelu_f(float v) {
   return v * (v < 0.f ? q : 1.0f - q);
 }
 
-__device__ __forceinline__ float silu8_f(float v) { return v * __builtin_amdgcn_rcpf(1.0f + exp_neg(v)); }
+__device__ __forceinline__ float silu8_f(float v) {
+  return v * __builtin_amdgcn_rcpf(1.0f + exp_neg(fminf(fmaxf(v, -120.f), 120.f)));   // beyond: 0 and v
+}
 
 __device__ __forceinline__ float act_f(float v, int act) {
   if (act == LDX_ACT_GELU) return gelu_f(v);
@@ -267,7 +270,7 @@ int launch_split(const Dense8Args& a, hipStream_t st) {
 // ------------------------------------------------------------------------------ large products
 //
 // A workgroup of 2 x 2 waves takes 64 FN outputs x 64 FM rows, a wave 32 FN x 32 FM of them in 32 x 32
-// accumulators. The operands' rows of a block (128 bytes) come into LDS by DMA, a ring of two stages;
+// accumulators. The operands' rows of a block (128 bytes) come into LDS by DMA, a ring of S stages;
 // whole 128-byte lines, since 64-byte pieces arrive at 18 TB/s and lines at 24 (every CU loading from
 // L2). Of row r the 16-byte unit u stands at u ^ (r / 2 % 8), so that the 16 lanes which read one unit of
 // 16 rows meet all 64 banks once.
@@ -277,6 +280,10 @@ int launch_split(const Dense8Args& a, hipStream_t st) {
 // the DMAs into the stage that all waves have then read.
 //
 // Scales come by DMA too, four blocks' bytes (a dword a row) at a time.
+//
+// 8,192 x 4,096 x 8,192 in bf16 207 to 233 us (2.66 to 2.36 PF/s) in 256 x 256 tiles, of which a block's
+// turn is 1.28 us and the result's way out 9 us a tile; 2,048^3 12.7 us in 128 x 128 tiles. fp32 results, on
+// bf16 instructions, 422 and 25.6 us.
 
 constexpr int kHalf8 = kBlock8 / 2;
 

@@ -461,6 +461,22 @@ def test_dense8_tiles(pkg, dev, m, k, o, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", [2, 700])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_dense8_activations_of_large_values(pkg, dev, act, m, t) -> None:
+    """Values whose squares or exponentials leave fp32, infinities and NaN."""
+    top = 6e4 if t == torch.float16 else 3e38
+    b = torch.tensor([math.inf, NAN, top, -top, 1e4, -1e4, 90.0, -90.0, 0.0] * 40)
+    x = pkg.ops.quantize8(torch.zeros(m, 130, device=dev))
+    w = pkg.ops.quantize8(torch.ones(b.numel(), 130, device=dev))
+    y = pkg.ops.dense8(x, w, b.to(dev), act=act, dtype=t).cpu()
+    want = torch.tensor([math.inf, NAN, top, 0.0, 1e4, 0.0, 90.0, 0.0, 0.0] * 40).to(t)
+    assert torch.equal(y.isnan(), want.isnan().expand(m, -1))
+    assert torch.equal(y.nan_to_num(nan=1.0), want.nan_to_num(nan=1.0).expand(m, -1))
+
+
+@gpu
 @pytest.mark.parametrize("m", [4, 100, 600])
 def test_dense8_scales_differ_by_block(pkg, dev, m) -> None:
     """Blocks of very unlike sizes, zero blocks and rows among them: each product takes its own scales."""
