@@ -5,7 +5,9 @@
 //   y = s / sqrt(mean(s^2) + eps) * gamma
 //   y rounded to T, or per row and 128 columns to e4m3 codes and a power of two (quant8.h)
 //
-// One pass: a row's values stay in registers between the sum of squares and the output.
+// One pass: a row's values stay in registers between the sum of squares and the output (beyond 8,192 columns
+// they are read twice), a wave a row up to 1,024 columns and a workgroup beyond. Bound by memory: 16,384 rows
+// of 4,096 in bf16 with residual and 8-bit rows 71 us (6.6 TB/s, part of it from the cache), plain 40 us.
 #include "quant8.h"
 
 namespace ldx {
