@@ -555,9 +555,9 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
 // sums themselves. (Scaled and added behind each page's products: 2,048 causal queries of 8 x 4 heads of 128
 // at the end of 8,192 tokens 396 us, so 348, 890 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 140 and 129.)
 //
-// What bounds it is issue: the products and what lies between them cost a SIMD their sum (a page of 32 rows at
-// head width 64 takes 1,560 cycles, of them 512 in products and 820 in 32 exponentials, their arguments,
-// maxima, sums and conversions), with two waves a SIMD as with three or four, and the same with 64 rows a wave
+// What bounds it is issue: at head width 64 a page of 32 rows takes a SIMD 1,560 cycles, of which products 512
+// and 32 exponentials, their arguments, maxima, sums and conversions 880, only 150 of them at once -- with two
+// waves a SIMD as with three or four, with a raised priority around the products, and with 64 rows a wave
 // whose products and exponentials alternate.
 constexpr int kWideRows = 128;
 
