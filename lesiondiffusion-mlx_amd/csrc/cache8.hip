@@ -1072,7 +1072,7 @@ int check_attention(const ldx_cache8_attention_args* p) {
   if (p->q_heads < 1 || p->q_heads % p->cache.heads)
     return fail("cache8_attention: %d query heads over %d cache heads", p->q_heads, p->cache.heads);
   const int64_t rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
-  if (rows * p->cache.heads * p->batch > 0x7fffffff)
+  if (rows * p->cache.heads * p->batch > 0x7fffffff || (rows + 15) / 16 * p->cache.heads > 1 << 23)   // 2^31 threads
     return fail("cache8_attention: %d x %d queries of %d heads are more than one launch takes", p->batch, p->q_len,
                 p->q_heads);
   if (p->table_pitch < p->width) return fail("cache8_attention: table pitch below %d", p->width);
@@ -1090,7 +1090,7 @@ extern "C" int ldx_cache8_append(const ldx_cache8_append_args* p, void* stream) 
   if (int rc = check_cache("cache8_append", p->cache)) return rc;
   if (p->dtype != LDX_DTYPE_F16 && p->dtype != LDX_DTYPE_BF16 && p->dtype != LDX_DTYPE_F32)
     return fail("cache8_append: dtype %d is not LDX_DTYPE_F16, LDX_DTYPE_BF16 or LDX_DTYPE_F32", p->dtype);
-  if (p->batch < 1 || p->batch > 65535 || p->tokens < 1 || p->width < 1 || p->width > (1 << 24))
+  if (p->batch < 1 || p->batch > 65535 || p->tokens < 1 || p->tokens > 1 << 28 || p->width < 1 || p->width > (1 << 24))
     return fail("cache8_append: batch %d, %d tokens, %d pages a sequence", p->batch, p->tokens, p->width);
   if (p->table_pitch < p->width) return fail("cache8_append: table pitch below %d", p->width);
   AppendArgs a = {{(uint8_t*)p->cache.k, (uint8_t*)p->cache.v},

@@ -527,8 +527,11 @@ struct Cost {
   float act, act_tile;
 };
 
+constexpr int64_t kMostTiles = 1 << 23;   // of a launch: 2^31 threads
+
 inline double estimate(const Cost& c, bool act, int64_t M, int64_t O, int kb, int tm, int tn, int places, int waves) {
   const double tiles = (double)((M + tm - 1) / tm) * (double)((O + tn - 1) / tn), full = tiles / places;
+  if (tiles > (double)kMostTiles && tm < 256) return 1e30;
   const double rounds = (double)(int64_t)(full + 0.999999), steps = (kb + waves - 1) / waves;
   return c.fixed + c.round * rounds + c.step * rounds * steps + c.work * full * steps + c.tile * full +
          (act ? c.act * rounds + c.act_tile * full : 0.0);
@@ -585,7 +588,7 @@ extern "C" int ldx_dense8(const ldx_dense8_args* p, void* stream) {
   if (p->dtype != LDX_DTYPE_F16 && p->dtype != LDX_DTYPE_BF16 && p->dtype != LDX_DTYPE_F32)
     return fail("dense8: dtype %d is not LDX_DTYPE_F16, LDX_DTYPE_BF16 or LDX_DTYPE_F32", p->dtype);
   if (p->act != LDX_ACT_NONE && p->act != LDX_ACT_GELU && p->act != LDX_ACT_SILU) return fail("dense8: act %d", p->act);
-  if ((p->rows + 31) / 32 * ((p->out_features + 31) / 32) > 0x7fffffff)   // the largest grid
+  if ((p->rows + 255) / 256 * ((p->out_features + 255) / 256) > kMostTiles)
     return fail("dense8: %lld x %d outputs are more than one launch takes", (long long)p->rows, p->out_features);
   const int kb = (p->features + kBlock8 - 1) / kBlock8;
   if (int rc = check_operand("x", p->x_codes, p->x_pitch, p->x_scales, p->x_scales_pitch, kb)) return rc;

@@ -142,8 +142,8 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
   __shared__ float red[4];
   constexpr int RPB = 256 / TPR;
   const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  if (RPB > 1 && row >= a.rows) return;   // whole waves: rows of several waves fill the workgroup
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + threadIdx.x / TPR;
+  if (row >= a.rows) return;   // whole waves
   const T* x = (const T*)a.x + row * a.xp;
   const T* r = a.r ? (const T*)a.r + row * a.rp : nullptr;
   T* s = a.s ? (T*)a.s + row * a.sp : nullptr;
@@ -222,7 +222,9 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
 template <typename T, bool NORM, bool Q8>
 void launch(const NormArgs& a, hipStream_t st) {
   const int n = Q8 ? a.kb * kBlock8 : a.C;
-  const dim3 wide((unsigned)a.rows), narrow((unsigned)((a.rows + 3) / 4)), block(256);
+  // (A launch's axis takes 2^32 threads.)
+  const auto grid = [](int64_t n) { return n <= 1 << 22 ? dim3((unsigned)n) : dim3(1 << 22, (unsigned)((n + (1 << 22) - 1) >> 22)); };
+  const dim3 wide = grid(a.rows), narrow = grid((a.rows + 3) / 4), block(256);
   if (n <= 512)
     hipLaunchKernelGGL((norm8_kernel<T, 64, 1, NORM, Q8>), narrow, block, 0, st, a);
   else if (n <= 1024)

@@ -117,6 +117,7 @@ def test_quantize8_refuses(pkg) -> None:
     {"rows": 0}, {"features": 0}, {"out_features": 0}, {"dtype": 4}, {"act": 3}, {"x_codes": None}, {"w_scales": None},
     {"y": None}, {"x_pitch": 128}, {"w_pitch": 264}, {"x_scales_pitch": 3}, {"w_codes": 24}, {"x_scales": 2},
     {"y_pitch": 4}, {"residual": 16, "residual_pitch": 4}, {"rows": 0x7fffffff, "out_features": 1 << 20, "y_pitch": 1 << 20},
+    {"rows": 0x7fffffff, "out_features": 300, "y_pitch": 300},
     {"features": 1 << 22 | 1, "x_pitch": 1 << 23, "w_pitch": 1 << 23, "x_scales_pitch": 1 << 20, "w_scales_pitch": 1 << 20},
     {"w_pitch": (1 << 22) + 16}, {"w_scales_pitch": (1 << 22) + 4},
 ])
@@ -135,7 +136,7 @@ def _cache_args(lib, **kw):
 
 
 @pytest.mark.parametrize("bad", [
-    {"pages": 0}, {"heads": 0}, {"head_dim": 48}, {"head_dim": 512}, {"k_scales": None}, {"tokens": 0}, {"batch": 0},
+    {"pages": 0}, {"heads": 0}, {"head_dim": 48}, {"head_dim": 512}, {"k_scales": None}, {"tokens": 0}, {"tokens": (1 << 28) + 1}, {"batch": 0},
     {"batch": 70000}, {"width": 0}, {"table_pitch": 0}, {"table": None}, {"starts": None}, {"dtype": 9}, {"src": None},
 ])
 def test_cache8_append_refuses(pkg, bad) -> None:
@@ -153,7 +154,7 @@ def test_cache8_append_refuses(pkg, bad) -> None:
 @pytest.mark.parametrize("bad", [
     {"pages": 0}, {"head_dim": 16}, {"q_heads": 3}, {"q_heads": 0}, {"q_len": 0}, {"batch": 0}, {"width": 0},
     {"width": 1 << 25, "table_pitch": 1 << 25}, {"table_pitch": 0}, {"lengths": None}, {"dtype": 1}, {"scale": NAN},
-    {"src": None}, {"q_len": 1 << 30},
+    {"src": None}, {"q_len": 1 << 30}, {"q_len": 1 << 27},
 ])
 def test_cache8_attention_refuses(pkg, bad) -> None:
     lib = pkg._lib
@@ -286,6 +287,19 @@ def test_rms_norm_of_values_whose_squares_overflow(pkg, dev, c, size, t) -> None
     got = pkg.ops.rms_norm(x.to(dev), torch.ones(c, device=dev), 1e-6).cpu().double()
     rel = norm_relative(c)
     assert ((got - y).abs() <= y.abs() * (half_step(t) * (1 + rel) + rel) + tiny(t)).all()
+
+
+@gpu
+def test_quantize8_of_many_rows(pkg, dev) -> None:
+    """More rows than one axis of a launch takes."""
+    n = (1 << 26) + 1001
+    x = torch.randn(n, 3, device=dev).half()
+    q = pkg.ops.quantize8(x)
+    for lo in (0, (1 << 24) - 8, (1 << 26) - 500, n - 700):
+        part = pkg.ops.quantize8(x[lo:lo + 700])
+        m = part.codes.shape[0]
+        assert torch.equal(part.codes.view(torch.uint8), q.codes[lo:lo + m].view(torch.uint8))
+        assert torch.equal(part.scales.view(torch.uint8), q.scales[lo:lo + m].view(torch.uint8))
 
 
 @gpu
