@@ -775,6 +775,25 @@ def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
 
 
 @gpu
+def test_cache_beyond_4_gib(pkg, dev) -> None:
+    """Pages whose offsets pass 32 bits, written and read like the first ones."""
+    heads, d, far, width = 4, 128, 140000, 20
+    small, big = pkg.ops.Cache8.empty(width, heads, d, dev), pkg.ops.Cache8.empty(far, heads, d, dev)
+    low = torch.arange(width, dtype=torch.int32, device=dev)[None]
+    high = far - 1 - 7 * low
+    k, v = rand((1, heads, 1200, d), 1).to(dev), rand((1, heads, 1200, d), 2).to(dev)
+    for cache, table in ((small, low), (big, high)):
+        pkg.ops.cache8_append(cache, k, v, table, ints(3).to(dev))
+    for mine, theirs in zip((small.k, small.v, small.k_scales, small.v_scales), (big.k, big.v, big.k_scales, big.v_scales)):
+        assert torch.equal(mine.view(torch.uint8), theirs.view(torch.uint8)[high[0].long()])
+    for lq, long in ((1, None), (150, LONG[d])):
+        q = rand((1, 8, lq, d), 3, torch.bfloat16).to(dev)
+        n = ints(1203).to(dev)
+        got = pkg.ops.cache8_attention(q, big, longer(high, long), n, 0.1)
+        assert torch.equal(got, pkg.ops.cache8_attention(q, small, longer(low, long), n, 0.1))
+
+
+@gpu
 @pytest.mark.parametrize("d", [32, 64])
 def test_attention_of_a_million_rows(pkg, dev, d) -> None:
     """More tiles of rows than a launch's second axis takes."""
