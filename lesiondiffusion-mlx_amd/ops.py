@@ -804,7 +804,8 @@ def group_norm_half(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, *
 
 # Small calls are bound by this host path too: each check below is one comparison on the way through, and
 # the helpers that name what is wrong run only where one failed (a token's norm with residual and 8-bit rows
-# 14.7 -> 10.9 us on the host, a dense8 call 11.7 -> 8.8, a cache8_append 12.9 -> 8.6).
+# 14.7 -> 10.9 us on the host, three allocations and the launch 8 of them; a dense8 call 11.7 -> 8.8, a
+# cache8_append 12.9 -> 8.6).
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
