@@ -966,8 +966,10 @@ def _rows8(q: Quantized8, name: str, device: int) -> tuple[torch.Tensor, torch.T
     if not isinstance(q, Quantized8):
         raise ValueError(f"{name} must be Quantized8 rows")
     codes, scales, f = q.codes, q.scales, q.features
-    _need(codes, f"{name} codes", E4M3, device)
-    _need(scales, f"{name} scales", E8M0, codes.get_device())
+    if not (type(codes) is type(scales) is torch.Tensor and codes.dtype is E4M3 and scales.dtype is E8M0
+            and codes.get_device() == scales.get_device() >= 0 and (device < 0 or codes.get_device() == device)):
+        _need(codes, f"{name} codes", E4M3, device)
+        _need(scales, f"{name} scales", E8M0, codes.get_device())
     kb = -(-f // BLOCK8)
     cs, ss = codes.shape, scales.shape
     if f < 1 or not cs or not ss or cs[-1] != kb * BLOCK8 or ss[-1] != -(-kb // 4) * 4 or cs[:-1] != ss[:-1]:
@@ -1057,11 +1059,13 @@ def _cache_block(cache: Cache8, what: str) -> tuple[Cache8Block, int]:
     if not isinstance(cache, Cache8):
         raise ValueError(f"{what}: cache must be a Cache8")
     k, v, ks, vs = cache.k, cache.v, cache.k_scales, cache.v_scales
-    _need(k, "cache k", E4M3, -1)
+    if not (type(k) is type(v) is type(ks) is type(vs) is torch.Tensor and k.dtype is v.dtype is E4M3
+            and ks.dtype is vs.dtype is E8M0 and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() >= 0):
+        _need(k, "cache k", E4M3, -1)
+        _need(v, "cache v", E4M3, k.get_device())
+        _need(ks, "cache k_scales", E8M0, k.get_device())
+        _need(vs, "cache v_scales", E8M0, k.get_device())
     dev, shape = k.get_device(), k.shape
-    _need(v, "cache v", E4M3, dev)
-    _need(ks, "cache k_scales", E8M0, dev)
-    _need(vs, "cache v_scales", E8M0, dev)
     if len(shape) != 4 or shape[2] != PAGE8:
         raise ValueError(f"cache k must be (pages, heads, {PAGE8}, D), got {tuple(shape)}")
     pages, heads, _, d = shape
