@@ -555,7 +555,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
 // The keys' scale goes with the softmax's into the exponential's argument (whose sign goes into the queries).
 // The values' goes into their widening, exactly (see `unit` below), so that the products add to the running
 // sums themselves. (Scaled and added behind each page's products: 2,048 causal queries of 8 x 4 heads of 128
-// at the end of 8,192 tokens 396 us, so 348, 890 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 140 and 129.)
+// at the end of 8,192 tokens 396 us, so 348 to 365, 870 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 140 and 129.)
 //
 // What bounds it is issue: at head width 64 a page of 32 rows takes a SIMD 1,560 cycles, of which products 512
 // and 32 exponentials, their arguments, maxima, sums and conversions 880, only 150 of them at once -- with two
@@ -651,6 +651,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
     unit = max(max(byte, top - 70), 1);
     top = max(top, unit);
   };
+  // What a page's values are widened by (1 for a scale of NaN: queries that do not see the page must not get
+  // zero times infinity).
+  const auto widen_by = [&](int byte) { return byte == 255 ? 1.f : scale_of(max(127 + byte - unit, 1)); };
   const auto times = [&](float f) {
 #pragma unroll
     for (int d = 0; d < NT; d++)
@@ -805,7 +808,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
     const int first = __builtin_amdgcn_readfirstlane(vs);
     unit = top = max(first == 255 ? 127 : first, 1);
     sums = unit;
-    widen(p0, scale_of(max(127 + first - unit, 1)));
+    widen(p0, widen_by(first));
     int was = unit;
     for (int p = p0; p < p1; p++) {
       const int ksb = __builtin_amdgcn_readfirstlane(ks), vsb = __builtin_amdgcn_readfirstlane(vs), punit = unit;
@@ -822,7 +825,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       if (p + 1 < p1) {
         const int nvs = __builtin_amdgcn_readfirstlane(vs);
         unit_for(nvs);
-        widen(p + 1, scale_of(max(127 + nvs - unit, 1)));
+        widen(p + 1, widen_by(nvs));
       }
       was = punit;
       page = next;

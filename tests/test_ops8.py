@@ -850,6 +850,16 @@ def test_attention_queries_before_a_page_do_not_feel_its_scale(pkg, dev, d, lq) 
                 assert (seen.abs() > 2.0 ** 80).any()
         scales.copy_(was)
     assert torch.equal(run(), want)
+    # A scale of NaN beside scales of 1, in a later page and in the first, which half of the queries do not see.
+    cache.v_scales.view(torch.uint8).fill_(127)
+    for page, first in ((int(table[0, 4]), first), (int(table[0, 0]), -(lq // 2))):
+        want = run()
+        cache.v_scales.view(torch.uint8)[page, 1] = 255
+        got = run()
+        cache.v_scales.view(torch.uint8)[page, 1] = 127
+        at = lq // 2
+        assert want.isfinite().all() and torch.equal(got[:, 0], want[:, 0]) and torch.equal(got[:, 1, :at], want[:, 1, :at])
+        assert got[:, 1, at:].isnan().all()
 
 
 @gpu
