@@ -841,13 +841,16 @@ class Quantized8:
         return v.flatten(-2)[..., :self.features]
 
 
+_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _launch8(fn, args: tuple, device: int, what: str) -> None:
     """One C call on the current stream of device ``device``, made current for it where it is not."""
-    if device == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if device == _device():
+        rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+            rc = fn(*args, _raw_stream(device))
     if rc:
         check(rc, what)
 
@@ -857,7 +860,7 @@ _ELEM, _ALL = tuple(ELEM_DTYPES), tuple(ALL_DTYPES)
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype | tuple | None, device: int) -> None:
     """``t`` is a tensor of ``dtype`` (one of several, or any with None) on device ``device`` (any with -1)."""
-    if type(t) is torch.Tensor and (t.dtype is dtype or dtype.__class__ is tuple and t.dtype in dtype) \
+    if type(t) is torch.Tensor and (t.dtype is dtype or dtype is None or dtype.__class__ is tuple and t.dtype in dtype) \
             and (t.get_device() == device if device >= 0 else t.is_cuda):
         return
     _require_cuda(t, name, dtype)
@@ -961,8 +964,8 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, *, residua
     return y if residual is None else (y, s)
 
 
-def _rows8(q: Quantized8, name: str, device: int) -> tuple[torch.Tensor, torch.Tensor, int, int, int]:
-    """Checks one operand of ``dense8``: its codes and scales, their pitches, and its rows."""
+def _rows8(q: Quantized8, name: str, device: int) -> tuple[torch.Tensor, torch.Tensor, int, int, tuple]:
+    """Checks one operand of ``dense8``: its codes and scales, their pitches, and its leading axes."""
     if not isinstance(q, Quantized8):
         raise ValueError(f"{name} must be Quantized8 rows")
     codes, scales, f = q.codes, q.scales, q.features
@@ -971,12 +974,14 @@ def _rows8(q: Quantized8, name: str, device: int) -> tuple[torch.Tensor, torch.T
         _need(codes, f"{name} codes", E4M3, device)
         _need(scales, f"{name} scales", E8M0, codes.get_device())
     kb = -(-f // BLOCK8)
-    cs, ss = codes.shape, scales.shape
-    if f < 1 or not cs or not ss or cs[-1] != kb * BLOCK8 or ss[-1] != -(-kb // 4) * 4 or cs[:-1] != ss[:-1]:
-        raise ValueError(f"{name}: codes {tuple(cs)} and scales {tuple(ss)} do not hold rows of {f} features")
+    cp, sp = kb * BLOCK8, -(-kb // 4) * 4
+    cs = codes.shape
+    lead = cs[:-1]
+    if f < 1 or not cs or cs[-1] != cp or scales.shape != (*lead, sp):
+        raise ValueError(f"{name}: codes {tuple(cs)} and scales {tuple(scales.shape)} do not hold rows of {f} features")
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{name}: codes and scales must be contiguous")
-    return codes, scales, cs[-1], ss[-1], codes.numel() // cs[-1]
+    return codes, scales, cp, sp, lead
 
 
 _ACTS = {None: ACT_NONE, "gelu": ACT_GELU, "silu": ACT_SILU}
@@ -990,11 +995,12 @@ def dense8(x: Quantized8, weight: Quantized8, bias: torch.Tensor | None = None, 
     ``act`` is None, ``"gelu"`` or ``"silu"``. fp16 and bf16 results come from the e4m3 matrix
     instruction, whose sums are within 2^-10 of the terms' magnitudes (about 1.5e-5 of the result for
     ordinary data); fp32 results are summed to fp32 accuracy at half its rate."""
-    xc, xs, xp, xsp, m = _rows8(x, "x", -1)
+    xc, xs, xp, xsp, lead = _rows8(x, "x", -1)
     dev = xc.get_device()
-    wc, ws, wp, wsp, o = _rows8(weight, "weight", dev)
-    if wc.dim() != 2:
+    wc, ws, wp, wsp, outs = _rows8(weight, "weight", dev)
+    if len(outs) != 1:
         raise ValueError(f"weight must be (O, C) rows, got {weight.shape}")
+    m, o = math.prod(lead), outs[0]
     if x.features != weight.features:
         raise ValueError(f"weight expects {weight.features} features, got {x.features}")
     if dtype not in ALL_DTYPES:
@@ -1003,7 +1009,7 @@ def dense8(x: Quantized8, weight: Quantized8, bias: torch.Tensor | None = None, 
         raise ValueError(f"act must be None, 'gelu' or 'silu', not {act!r}")
     if not m or not o:
         raise ValueError(f"dense8: {m} rows and {o} outputs")
-    shape = (*xc.shape[:-1], o)
+    shape = (*lead, o)
     if bias is not None:
         _need(bias, "bias", None, dev)
         if bias.shape != (o,):
