@@ -7,7 +7,7 @@
 //
 // One pass: a row's values stay in registers between the sum of squares and the output (beyond 8,192 columns
 // they are read twice), a wave a row up to 1,024 columns and a workgroup beyond. Bound by memory: 16,384 rows
-// of 4,096 in bf16 with residual and 8-bit rows 71 us (6.6 TB/s, part of it from the cache), plain 40 us.
+// of 4,096 in bf16 with residual and 8-bit rows 73 us (6.4 TB/s, part of it from the cache), plain 40 us.
 #include "quant8.h"
 
 namespace ldx {
@@ -23,19 +23,21 @@ struct NormArgs {
   uint8_t* scales; int64_t ep;
   int64_t rows;
   int C, kb;                      // features; 128-column blocks
+  double per_C;                   // 1 / C
 };
 
-// Sum / largest over a row's threads: a wave, or the four waves of the workgroup through red.
-template <int TPR, bool MAX>
-__device__ __forceinline__ float row_reduce(float v, float* red) {
-  v = MAX ? wave_max(v) : wave_sum(v);
+// Sum (float, double) / largest over a row's threads: a wave, or the four waves of the workgroup through red.
+template <int TPR, bool MAX, typename F>
+__device__ __forceinline__ F row_reduce(F v, double* red) {
+  if constexpr (MAX) v = wave_max(v);
+  else v = wave_sum(v);
   if constexpr (TPR > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = red[0];
+    v = (F)red[0];
 #pragma unroll
-    for (int i = 1; i < TPR / 64; i++) v = MAX ? fmaxf(v, red[i]) : v + red[i];
+    for (int i = 1; i < TPR / 64; i++) v = MAX ? (F)fmax(v, (F)red[i]) : v + (F)red[i];
   }
   return v;
 }
@@ -71,19 +73,57 @@ __device__ __forceinline__ void take8(const NormArgs& a, const T* x, const T* r,
   }
 }
 
+// 1 / sqrt of a row as two numbers, to 2^-45.
+struct Root {
+  float hi, lo;
+};
+
+// f rstd g to 2^-40 as the nearest fp32 number y and what is left.
+__device__ __forceinline__ Root product(float f, Root rstd, float g) {
+  const float t = f * rstd.hi, y = t * g;
+  const float e = __builtin_fmaf(f, rstd.lo, __builtin_fmaf(f, rstd.hi, -t));
+  const float r = __builtin_fmaf(e, g, __builtin_fmaf(t, g, -y)), z = y + r;
+  return fabsf(y) < __builtin_inff() ? Root{z, r - (z - y)} : Root{y, 0.f};
+}
+
+// The product as the neighbour with an odd last bit where it lies between two fp32 numbers: rounded again,
+// to a code or past a scale's limit, it goes where the exact product would.
+__device__ __forceinline__ float product_odd(float f, Root rstd, float g) {
+  const Root y = product(f, rstd, g);
+  const int z = __float_as_int(y.hi), away = (unsigned)(z ^ __float_as_int(y.lo)) >> 31;   // 1: the product is nearer 0
+  return y.lo != 0.f ? __int_as_float((z - away) | 1) : y.hi;
+}
+
 // The output of values c .. c + 7: a 16-lane row holds a block of 128.
 template <typename T, bool NORM, bool Q8>
-__device__ __forceinline__ void give8(const NormArgs& a, int64_t row, int c, float rstd, float (&f)[8]) {
+__device__ __forceinline__ void give8(const NormArgs& a, int64_t row, int c, Root rstd, float (&f)[8]) {
   if constexpr (NORM) {
+    float g[8], x[8];
     if (c + 8 <= a.C) {
-      float g[8];
       load8(a.gamma + c, g);
-#pragma unroll
-      for (int i = 0; i < 8; i++) f[i] = f[i] * rstd * g[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (c + i < a.C) f[i] = f[i] * rstd * a.gamma[c + i];
+      for (int i = 0; i < 8; i++) g[i] = c + i < a.C ? a.gamma[c + i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      x[i] = f[i];
+      f[i] = x[i] * rstd.hi * g[i];   // within three last places of the product: enough for 16 bits
+    }
+    if constexpr (Q8) {
+      // What codes and scales round at has 19 zero bits at its end: only values within three of such a number
+      // need more (a wave in 100; zeros do, too). Of 67 million codes about 8 then differ from exact
+      // arithmetic's (what fp32 sums of squares leave), 43 without, for 2 us of 71.
+      unsigned least = ~0u;
+#pragma unroll
+      for (int i = 0; i < 8; i++) least = min(least, ((unsigned)__float_as_int(f[i]) + 3u) << 13);
+      if (__any(c < a.C && least <= 6u << 13)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = product_odd(x[i], rstd, g[i]);
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) f[i] = product(x[i], rstd, g[i]).hi;
     }
   }
   if constexpr (Q8) {
@@ -115,17 +155,20 @@ __device__ __forceinline__ void give8(const NormArgs& a, int64_t row, int c, flo
 // there the power of two that brings the largest value to 1..4, and the squares are taken again. (Squares
 // below fp32 are nothing beside eps, 1e-30 at least.)
 template <int TPR, typename Square>
-__device__ __forceinline__ float row_rstd(const NormArgs& a, float ss, float amax, float* red, float& g,
-                                          Square squares) {
+__device__ __forceinline__ Root row_rstd(const NormArgs& a, double ss, float amax, double* red, float& g,
+                                         Square squares) {
   g = 1.f;
-  if (!(ss <= 3.0e38f)) {   // uniform over the row's threads
+  if (!(ss <= 3.0e38)) {   // uniform over the row's threads
     amax = row_reduce<TPR, true>(amax, red);
     if (amax < __builtin_inff()) {
       g = inverse_of(min(max(__float_as_int(amax) >> 23, 1), 253));
-      ss = row_reduce<TPR, false>(squares(g), red);
+      ss = row_reduce<TPR, false>((double)squares(g), red);
     }
   }
-  return 1.0f / sqrtf(ss / a.C + a.eps * g * g);
+  const double v = ss * a.per_C + (double)a.eps * g * g, r = __builtin_amdgcn_rsqf((float)v);
+  const double s = r + 0.5 * r * (1.0 - v * r * r);   // a step of Newton's from fp32's root
+  const float hi = (float)s;
+  return v < __builtin_inf() ? Root{hi, (float)(s - hi)} : Root{(float)r, 0.f};
 }
 
 template <int N>
@@ -139,7 +182,7 @@ __device__ __forceinline__ void times(float (&f)[N], float g) {
 // reads them twice.
 template <typename T, int TPR, int NCH, bool NORM, bool Q8>
 __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
-  __shared__ float red[4];
+  __shared__ double red[4];
   constexpr int RPB = 256 / TPR;
   const int t = threadIdx.x % TPR;
   const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + threadIdx.x / TPR;
@@ -152,7 +195,8 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
     float ss = 0.f, amax = 0.f;
 #pragma unroll
     for (int k = 0; k < NCH; k++) take8(a, x, r, s, (k * TPR + t) * 8, f[k]);
-    float rstd = 1.f, g = 1.f;
+    Root rstd = {1.f, 0.f};
+    float g = 1.f;
     if constexpr (NORM) {
 #pragma unroll
       for (int k = 0; k < NCH; k++)
@@ -161,8 +205,7 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
           ss += f[k][i] * f[k][i];
           amax = fmaxf(amax, fabsf(f[k][i]));
         }
-      ss = row_reduce<TPR, false>(ss, red);
-      rstd = row_rstd<TPR>(a, ss, amax, red, g, [&](float by) {
+      rstd = row_rstd<TPR>(a, row_reduce<TPR, false>((double)ss, red), amax, red, g, [&](float by) {
         float q = 0.f;
 #pragma unroll
         for (int k = 0; k < NCH; k++)
@@ -178,7 +221,8 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
   } else {
     // Whole workgroup rounds, so that the lanes of a block of 128 stay together.
     const int rounds = (a.kb * kBlock8 + TPR * 8 - 1) / (TPR * 8);
-    float rstd = 1.f, g = 1.f;
+    Root rstd = {1.f, 0.f};
+    float g = 1.f;
     if constexpr (NORM) {
       float ss = 0.f, amax = 0.f, f[8];
       for (int k = 0; k < rounds; k++) {
@@ -189,11 +233,10 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
           amax = fmaxf(amax, fabsf(f[i]));
         }
       }
-      ss = row_reduce<TPR, false>(ss, red);
       // Read again: the sum that this thread stored, since it may have been stored over x or r.
       const T* x2 = r && s ? s : x;
       const T* r2 = r && s ? nullptr : r;
-      rstd = row_rstd<TPR>(a, ss, amax, red, g, [&](float by) {
+      rstd = row_rstd<TPR>(a, row_reduce<TPR, false>((double)ss, red), amax, red, g, [&](float by) {
         float q = 0.f, h[8];
         for (int k = 0; k < rounds; k++) {
           take8(a, x2, r2, (T*)nullptr, (k * TPR + t) * 8, h);
@@ -283,7 +326,7 @@ extern "C" int ldx_rms_norm(const ldx_rms_norm_args* p, void* stream) {
     if (int rc = check_codes("rms_norm", p->codes, p->codes_pitch, p->scales, p->scales_pitch, kb)) return rc;
   const NormArgs a = {p->x, p->x_pitch, p->residual, p->residual_pitch, p->sum, p->sum_pitch, p->gamma, p->eps,
                       p->y, p->y_pitch, (uint8_t*)p->codes, p->codes_pitch, (uint8_t*)p->scales, p->scales_pitch,
-                      p->rows, C, kb};
+                      p->rows, C, kb, 1.0 / C};
   hipStream_t st = as_stream(stream);
   return p->codes ? launch_any<true, true>(a, p->dtype, st, "rms_norm")
                   : launch_any<true, false>(a, p->dtype, st, "rms_norm");

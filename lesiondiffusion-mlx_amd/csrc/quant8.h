@@ -83,6 +83,26 @@ __device__ __forceinline__ float wave_max(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
   return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
 }
+// v's counterpart under a DPP row operation, and v and its partner half a row pair (a wave) away.
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  const i32x2 w = __builtin_bit_cast(i32x2, v);
+  const i32x2 r = {__builtin_amdgcn_update_dpp(0, w[0], CTRL, 0xf, 0xf, false),
+                   __builtin_amdgcn_update_dpp(0, w[1], CTRL, 0xf, 0xf, false)};
+  return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  v += dpp_d<0x128>(v);
+  v += dpp_d<0x124>(v);
+  v += dpp_d<0x122>(v);
+  v += dpp_d<0x121>(v);
+  i32x2 w = __builtin_bit_cast(i32x2, v);
+  const auto a0 = __builtin_amdgcn_permlane16_swap(w[0], w[0], false, false), a1 = __builtin_amdgcn_permlane16_swap(w[1], w[1], false, false);
+  v = __builtin_bit_cast(double, (i32x2){(int)a0[0], (int)a1[0]}) + __builtin_bit_cast(double, (i32x2){(int)a0[1], (int)a1[1]});
+  w = __builtin_bit_cast(i32x2, v);
+  const auto b0 = __builtin_amdgcn_permlane32_swap(w[0], w[0], false, false), b1 = __builtin_amdgcn_permlane32_swap(w[1], w[1], false, false);
+  return __builtin_bit_cast(double, (i32x2){(int)b0[0], (int)b1[0]}) + __builtin_bit_cast(double, (i32x2){(int)b0[1], (int)b1[1]});
+}
 __device__ __forceinline__ float wave_sum(float v) {
   v += dpp_f<0x128>(v);
   v += dpp_f<0x124>(v);
