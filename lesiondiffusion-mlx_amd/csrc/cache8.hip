@@ -220,6 +220,25 @@ __device__ __forceinline__ float score_scale(float c, int byte) {
 // two): the sums are seldom multiplied then, and probabilities up to 2^8 are as exact in fp16 as those up to 1.
 constexpr float kSlack = 8.f;
 
+// A score times its scale goes into the exponential unrounded, its reference does not: what the reference's rounding
+// left out, up to 2^-24 of it, moves all probabilities of a query by one factor, which beyond scores of 2^28 leaves
+// fp16. Pages that may hold scores of kFarScore (by the queries' sums of magnitudes and the largest code) have them
+// multiplied, and rounded, first.
+constexpr float kFarScore = 4194304.f;
+__device__ __forceinline__ bool far_page(float most, float grow) { return most * grow > kFarScore; }
+
+// The wave's largest score at a scale of 1, or more: 448 times the sum of a query's magnitudes, of which a lane holds
+// one of `lanes` parts.
+template <typename V, int N>
+__device__ __forceinline__ float most_score(const V (&q)[N], int lanes) {
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; j++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum += fabsf((float)q[j][e]);
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(wave_max(sum) * (448.f * lanes))));
+}
+
 // l and eight probabilities: as the products take them, in fp16 (their sum in fp32), so that rounding moves
 // both sides of the quotient alike. Two at a time: half the additions of fp32 numbers.
 __device__ __forceinline__ float sum8(f16x8 p, float l) {
@@ -359,8 +378,9 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
   int after = entry(p + 2 * kAttendWaves);
   load_k(now, p);
   load_v(now, p);
+  const float most_q = most_score(q, 4);
   for (; p < p1; p += kAttendWaves) {
-    const float grow = score_scale(c, ks);
+    float grow = score_scale(c, ks);
     const bool none_k = ks == 255;
     const int base = p * kPage8 + 16 * g;   // the lane's first token
     float s[16];
@@ -390,12 +410,14 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
     const float vscale = page_scale(vs);
     if ((now.missing || none_k || vs == 255) && p * kPage8 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
     const bool cut = p * kPage8 + kPage8 > least;   // some query does not see the whole page
-    if (cut) {
+    const bool far = __any(far_page(most_q, grow));
+    if (cut || far) {
       int left = limit - base;
       pin_value(left);
+      const float first = far ? grow : 1.f;
 #pragma unroll
-      for (int i = 0; i < 16; i++)
-        if (i >= left) s[i] = -__builtin_inff();
+      for (int i = 0; i < 16; i++) s[i] = i < left ? s[i] * first : -__builtin_inff();
+      grow = far ? 1.f : grow;
     }
     float mx = s[0];
 #pragma unroll
@@ -406,7 +428,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
     const auto x32 = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
     const float mn = max3_f(m, __int_as_float(x32[0]) * grow, __int_as_float(x32[1]) * grow);
     float ref = m == -__builtin_inff() ? 0.f : m;
-    if (__any(mn > m + kSlack)) {
+    if (__any(mn - m > kSlack)) {
       ref = mn == -__builtin_inff() ? 0.f : mn;
       const float alpha = __builtin_amdgcn_exp2f(m - ref);
       l *= alpha;
@@ -614,6 +636,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
 #pragma unroll
     for (int j = 0; j < NJ; j++) q[j] = query8<T>(a, qp, 16 * j + 8 * hh, real);
   }
+  float most_q = 0.f;
   f32x16 acc[NT];
 #pragma unroll
   for (int d = 0; d < NT; d++)
@@ -723,24 +746,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       for (int e = 0; e < 16; e++) s[t][e] = sv[t][e];
     const int base = p * kPage8 + 16 * hh;   // score e of tile t is token base + 32 t + e
     if (missing && p * kPage8 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
-    if (p * kPage8 + kPage8 > least) {
+    float kc = score_scale(c, ksb);
+    const bool far = far_page(most_q, kc);
+    if (p * kPage8 + kPage8 > least || far) {
       int left = limit - base;
       pin_value(left);
+      const float first = far ? kc : 1.f;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int e = 0; e < 16; e++)
-          if (32 * t + e >= left) s[t][e] = -__builtin_inff();
+        for (int e = 0; e < 16; e++) s[t][e] = 32 * t + e < left ? s[t][e] * first : -__builtin_inff();
+      kc = far ? 1.f : kc;
     }
     float mx = max3_f(s[0][0], s[1][0], s[0][1]);
     mx = max3_f(mx, s[1][1], s[1][1]);
 #pragma unroll
     for (int e = 2; e < 16; e++) mx = max3_f(mx, s[0][e], s[1][e]);
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
-    const float kc = score_scale(c, ksb);
     const float mn = max3_f(m, __int_as_float(x[0]) * kc, __int_as_float(x[1]) * kc);
     float ref = m == -__builtin_inff() ? 0.f : m;
-    if (moved || __any(mn > m + kSlack)) {
+    if (moved || __any(mn - m > kSlack)) {
       ref = mn == -__builtin_inff() ? 0.f : mn;
       float alpha = __builtin_amdgcn_exp2f(m - ref);
       l *= alpha;
@@ -805,6 +830,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
     int page = entry(p0), next = entry(p0 + 1);
     int64_t at = place(page);
     load(at);
+    most_q = most_score(q, 2);
     const int first = __builtin_amdgcn_readfirstlane(vs);
     unit = top = max(first == 255 ? 127 : first, 1);
     sums = unit;

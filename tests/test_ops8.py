@@ -892,6 +892,32 @@ def test_attention_scores_far_apart(pkg, dev, lq) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("lq", "d", "long"), [(1, 32, None), (3, 64, None), (20, 128, None), (2, 256, None), (130, 64, LONG[64]),
+                                               (130, 128, LONG[128]), (130, 256, LONG[256])])
+def test_attention_of_huge_scores(pkg, dev, lq, d, long, t) -> None:
+    """Scores of 2^20 to 2^37, whose last place is up to 2^14: the key of the largest takes all, and no product's
+    rounding carries its probability out of fp16."""
+    n = 500
+    cache = pkg.ops.Cache8.empty(10, 2, d, dev)
+    table = tables(1, 8)
+    k, v = rand((1, 2, n, d), 1, scale=100.0), rand((1, 2, n, d), 2)
+    pkg.ops.cache8_append(cache, k.to(dev), v.to(dev), table.to(dev), ints(0).to(dev))
+    kk, vv = Pages(cache).read(table[0], n)
+    best = torch.randint(0, n, (lq,), generator=torch.Generator().manual_seed(3))
+    q = torch.stack([kk[h, best] * 100 for h in range(2)])[None].to(t)    # towards one key each
+    for scale in (2.0 ** -4, 1.0, 37.3, 1000.0):
+        s = q[0].double() @ kk.transpose(1, 2) * scale
+        off = (d + 6) * 2.0 ** -23 * (q[0].double().abs() @ kk.abs().transpose(1, 2) * scale).amax(-1)
+        top = s.topk(2, -1)
+        # The largest is ahead by more than fp32 scores are off, and by more than fp16 probabilities reach.
+        assert (top.values[..., 0] - top.values[..., 1] > 2 * off + 40).all()
+        want = torch.stack([vv[h, top.indices[h, :, 0]] for h in range(2)])
+        got = pkg.ops.cache8_attention(q.to(dev), cache, longer(table, long).to(dev), ints(n).to(dev), scale).cpu().double()
+        assert ((got[0] - want).abs() <= want.abs() * (half_step(t) + 2.0 ** -20) + tiny(t)).all(), scale
+
+
+@gpu
 @pytest.mark.parametrize(("lq", "d", "long"), [(1, 64, None), (9, 64, None), (70, 128, None), (200, 64, LONG[64]),
                                                (130, 128, LONG[128]), (130, 256, LONG[256])])
 def test_attention_loud_page_of_small_weight(pkg, dev, lq, d, long) -> None:
