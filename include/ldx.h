@@ -503,11 +503,12 @@ int ldx_cache8_append(const ldx_cache8_append_args* args, void* stream);
  * starts, query i sees no token behind starts[b] + i (causal for queries at starts[b]..). q and
  * o: (batch, token, head) strides, contiguous channels, fp16 or bf16; q_heads a multiple of
  * the cache's heads, query head j reads the cache's head j / (q_heads / heads). fp32 scores,
- * softmax and sums; probabilities are rounded to fp16, in both of the quotient's sums. A query
+ * softmax and sums; probabilities are rounded to fp16, in both of the quotient's sums: to 2^-11 of
+ * themselves, and those below 2^-21 of a query's largest to 2^-32 of it. A query
  * that sees no token gets 0. Tokens that a query does not see do not touch its result, NaN
  * among them. A page that the cache does not have, or with a scale of NaN, gives NaN to the
  * queries that see it, a length past the table to the whole sequence. Where pages' value scales
- * are more than 2^70 apart, what is below 2^-90 of the largest values may be lost. o may be q.
+ * are more than 2^63 apart, what is below 2^-83 of the largest values may be lost. o may be q.
  * Workspace: partial results where a sequence is split over workgroups,
  * ldx_cache8_attention_workspace_bytes of them; with less nothing is split. */
 typedef struct ldx_cache8_attention_args {

@@ -216,14 +216,17 @@ __device__ __forceinline__ float score_scale(float c, int byte) {
   return fminf(fmaxf(c * scale_of(byte), 1.1754944e-38f), 3.0e38f);
 }
 
-// A query's reference for its exponentials follows its maximum only where that passes it by kSlack (in powers of
-// two): the sums are seldom multiplied then, and probabilities up to 2^8 are as exact in fp16 as those up to 1.
-constexpr float kSlack = 8.f;
+// A query's reference for its exponentials is 2^kRaise below its maximum, and follows it only where that passes it by
+// kSlack more (in powers of two): the sums are seldom multiplied then. Probabilities reach 2^15, and fp16 holds those
+// from 2^-21 of the largest on to 2^-11 of themselves and smaller ones to 2^-32 of it, so that many small ones beside
+// a dominant one keep their weight (with the maximum as the reference 2^-14 and 2^-25: 100,000 keys at 2^-23.6 of the
+// first one weighed a quarter less). What is summed is kept kLower times as large, so that the values' range is fp32's.
+constexpr float kSlack = 8.f, kRaise = 7.f, kLower = 0x1p-7f;
 
 // A score times its scale goes into the exponential unrounded, its reference does not: what the reference's rounding
 // left out, up to 2^-24 of it, moves all probabilities of a query by one factor, which beyond scores of 2^28 leaves
 // fp16. Pages that may hold scores of kFarScore (by the queries' sums of magnitudes and the largest code) have them
-// multiplied, and rounded, first.
+// multiplied, and rounded, first, and have no slack (7 less is rounded, too: to 8 less, or to nothing from 2^27 on).
 constexpr float kFarScore = 4194304.f;
 __device__ __forceinline__ bool far_page(float most, float grow) { return most * grow > kFarScore; }
 
@@ -276,7 +279,7 @@ __device__ __forceinline__ unsigned nan_bytes(int w) {
 // reads the turned values, and the probabilities go into the second product as they lie.
 //
 // The scales stay out of the operands: the keys' goes into the softmax scale, the values' onto each page's
-// sum as it is added to the running one, so that probabilities (at most 2^kSlack) are what fp16 rounds.
+// sum as it is added to the running one, so that probabilities are what fp16 rounds.
 //
 // What bounds it while tokens are produced one by one is reading the cache. A wave holds one page's keys
 // and one page's values and always has one of the two on its way: the next page's keys are asked for when
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
     }
     load_k(next, p + kAttendWaves);
     __builtin_amdgcn_sched_barrier(0);
-    const float vscale = page_scale(vs);
+    const float vscale = page_scale(vs) * kLower;
     if ((now.missing || none_k || vs == 255) && p * kPage8 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
     const bool cut = p * kPage8 + kPage8 > least;   // some query does not see the whole page
     const bool far = __any(far_page(most_q, grow));
@@ -426,9 +429,10 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
     const auto x16 = __builtin_amdgcn_permlane16_swap(__float_as_int(mx), __float_as_int(mx), false, false);
     mx = max3_f(__int_as_float(x16[0]), __int_as_float(x16[1]), __int_as_float(x16[1]));
     const auto x32 = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
-    const float mn = max3_f(m, __int_as_float(x32[0]) * grow, __int_as_float(x32[1]) * grow);
+    const float mn = max3_f(m, __builtin_fmaf(__int_as_float(x32[0]), grow, -kRaise),
+                            __builtin_fmaf(__int_as_float(x32[1]), grow, -kRaise));
     float ref = m == -__builtin_inff() ? 0.f : m;
-    if (__any(mn - m > kSlack)) {
+    if (__any(mn - m > (far ? 0.f : kSlack))) {
       ref = mn == -__builtin_inff() ? 0.f : mn;
       const float alpha = __builtin_amdgcn_exp2f(m - ref);
       l *= alpha;
@@ -439,14 +443,16 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
       m = mn;
     }
     f16x8 pr[2];
+    float lp = 0.f;   // the page's own sum, so that small ones do not go one by one into a large one
 #pragma unroll
     for (int u = 0; u < 2; u++) {   // eight at a time; left alone, the sums are made behind the products below
 #pragma unroll
       for (int i = 0; i < 8; i++) pr[u][i] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * u + i], grow, -ref));
-      l = sum8(pr[u], l);
-      pin_value(l);
+      lp = sum8(pr[u], lp);
+      pin_value(lp);
       __builtin_amdgcn_sched_barrier(0);
     }
+    l += lp;
     if (cut) {
       // Tokens behind the sequence are whatever was there: zero them. Tokens that only some of the queries
       // see may be NaN, and zero times NaN is not zero: their codes are zeroed too, and a product of their
@@ -519,7 +525,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
   const auto l16 = __builtin_amdgcn_permlane16_swap(__float_as_int(l), __float_as_int(l), false, false);
   l = __int_as_float(l16[0]) + __int_as_float(l16[1]);
   const auto l32 = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
-  l = __int_as_float(l32[0]) + __int_as_float(l32[1]);
+  l = (__int_as_float(l32[0]) + __int_as_float(l32[1])) * kLower;
   if (g == 0) {
     sm[wave][r] = m;
     sl[wave][r] = l;
@@ -667,11 +673,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
   };
   // Values are widened times 2^(scale - unit), exact in fp16 (codes are 2^-9 .. 448) where that is 2^-15 .. 2^7,
   // and summed in that unit, at first the first page's scale. A page further off makes its scale the unit,
-  // but never one more than 2^70 below the largest so far: the sums would pass fp32.
+  // but never one more than 2^63 below the largest so far: the sums (2^15 times 448 x 2^7 and up to 2^30 tokens)
+  // would pass fp32.
   int unit = 0, top = 0;   // of the page widened last; the largest
   const auto unit_for = [&](int byte) {
     if (byte == 255 || (byte - unit >= -15 && byte - unit <= 7)) return;   // 255: its queries get NaN
-    unit = max(max(byte, top - 70), 1);
+    unit = max(max(byte, top - 63), 1);
     top = max(top, unit);
   };
   // What a page's values are widened by (1 for a scale of NaN: queries that do not see the page must not get
@@ -763,9 +770,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
 #pragma unroll
     for (int e = 2; e < 16; e++) mx = max3_f(mx, s[0][e], s[1][e]);
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
-    const float mn = max3_f(m, __int_as_float(x[0]) * kc, __int_as_float(x[1]) * kc);
+    const float mn = max3_f(m, __builtin_fmaf(__int_as_float(x[0]), kc, -kRaise),
+                            __builtin_fmaf(__int_as_float(x[1]), kc, -kRaise));
     float ref = m == -__builtin_inff() ? 0.f : m;
-    if (moved || __any(mn - m > kSlack)) {
+    if (moved || __any(mn - m > (far ? 0.f : kSlack))) {
       ref = mn == -__builtin_inff() ? 0.f : mn;
       float alpha = __builtin_amdgcn_exp2f(m - ref);
       l *= alpha;
@@ -777,6 +785,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       m = mn;
     }
     f16x8 pr[2][2];
+    float lp = 0.f;
     // Eight at a time: left alone, all 32 probabilities stay in fp32 until the products below.
 #pragma unroll
     for (int t = 0; t < 2; t++)
@@ -784,10 +793,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       for (int u = 0; u < 2; u++) {
 #pragma unroll
         for (int e = 0; e < 8; e++) pr[t][u][e] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + e], kc, -ref));
-        l = sum8(pr[t][u], l);
-        pin_value(l);
+        lp = sum8(pr[t][u], lp);
+        pin_value(lp);
         __builtin_amdgcn_sched_barrier(0);
       }
+    l += lp;
 #pragma unroll
     for (int d = 0; d < NT; d++) {
 #pragma unroll
@@ -866,9 +876,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
 #pragma unroll
       for (int e = 0; e < 16; e++)
         if (poison[d / 4] >> (16 * (d % 4) + e) & 1) acc[d][e] = __builtin_nanf("");
-  times(scale_of(sums));
+  times(scale_of(sums) * kLower);
   const auto l32 = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
-  l = __int_as_float(l32[0]) + __int_as_float(l32[1]);
+  l = (__int_as_float(l32[0]) + __int_as_float(l32[1])) * kLower;
   if (too_long) l = __builtin_nanf("");
   if (!real) return;
   if (a.splits > 1) {

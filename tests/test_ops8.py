@@ -918,6 +918,41 @@ def test_attention_of_huge_scores(pkg, dev, lq, d, long, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("x", [15.3, 18.7, 20.5, 22.5, 23.6, 25.2])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize(("b", "n", "lq", "d", "long", "adds"), [
+    (1, 100_000, 1, 64, None, 300), (600, 8_000, 1, 64, None, 300), (300, 8_000, 2, 128, None, 300), (600, 8_000, 1, 32, None, 300),
+    (600, 4_000, 1, 256, None, 300), (1, 30_000, 130, 64, LONG[64], 2200), (1, 30_000, 130, 128, LONG[128], 2200),
+    (1, 30_000, 130, 256, LONG[256], 2200)])
+def test_attention_keeps_the_weight_of_a_long_tail(pkg, dev, b, n, lq, d, long, adds, first, x) -> None:
+    """One key, the first or the last, that outweighs each of ``n`` others by 2^x; their values are 1, its own 0
+    in half of the channels and -1 in the others."""
+    width, at = -(-(n + 1) // 64), 0 if first else n
+    cache = pkg.ops.Cache8.empty(width, 1, d, dev)
+    k, v = torch.zeros(1, 1, n + 1, d), torch.ones(1, 1, n + 1, d)
+    k[0, 0, at], v[0, 0, at, :d // 2], v[0, 0, at, d // 2:] = 16.0, 0.0, -1.0
+    table = torch.arange(width, dtype=torch.int32)[None]
+    pkg.ops.cache8_append(cache, k.to(dev), v.to(dev), table.to(dev), ints(0).to(dev))
+    p = 2.0 ** -x
+    l = 1 + n * p
+    o = torch.tensor([n * p / l, (n * p - 1) / l]).double().repeat_interleave(d // 2)
+    mass = torch.tensor([n * p / l, (n * p + 1) / l]).double().repeat_interleave(d // 2)
+    # Probabilities are rounded to fp16 2^7 times as large, p (1 + e) + u, |e| <= 2^-11, |u| <= 2^-25 / 2^7 (see
+    # attention_reference); the dominant one, a power of two, exactly. Exponents of at most 28 are off by 2^-23 of
+    # their size and the exponential by 2^-22: 2^-18 in all. fp32 sums of at most `adds` additions in a row (a
+    # product's sixteens, pages, waves and parts).
+    off = n * (p * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -32) * (1 - o) / l * (1 + 2.0 ** -10)
+    allowed = off + adds * 2.0 ** -24 * (mass + o.abs())
+    for t in (torch.float16, torch.bfloat16):
+        q = torch.ones(b, 1, lq, d, dtype=t, device=dev)
+        got = pkg.ops.cache8_attention(q, cache, longer(table, long).expand(b, -1).contiguous().to(dev),
+                                       torch.full((b,), n + 1, dtype=torch.int32, device=dev), x * math.log(2.0) / (16 * d))
+        err = (got.cpu().double() - o).abs()
+        bar = allowed * (1 + half_step(t)) + o.abs() * half_step(t) + tiny(t)
+        assert (err <= bar).all(), (err / bar).amax((0, 1, 2))
+
+
+@gpu
 @pytest.mark.parametrize(("lq", "d", "long"), [(1, 64, None), (9, 64, None), (70, 128, None), (200, 64, LONG[64]),
                                                (130, 128, LONG[128]), (130, 256, LONG[256])])
 def test_attention_loud_page_of_small_weight(pkg, dev, lq, d, long) -> None:
