@@ -76,7 +76,8 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
   int to = scale_byte(amax);
   const bool rises = lo > 0 && to > was;
   if (lo > 0 && to < was) to = was;
-  const float inv = inverse_of(min(to, 253));
+  // (254, which no append writes by itself, may be an older page's: its inverse, 2^-127, is a subnormal number.)
+  const float inv = to < 254 ? inverse_of(to) : __int_as_float(0x00400000);
   if (tid == 0) *scale = (uint8_t)to;
   if (which == 0) {
     if (rises)

@@ -662,6 +662,31 @@ def test_append_of_nan_zero_and_strided_tokens(pkg, dev) -> None:
     ref.equals(cache)
 
 
+@gpu
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("byte", [0, 1, 253, 254, 255])
+def test_append_behind_tokens_of_any_scale(pkg, dev, d, byte) -> None:
+    """A page that holds tokens under any E8M0 byte, also those that no append writes: the new ones are written
+    under the larger scale; a page of NaN stays one, with its older codes."""
+    old = torch.randint(0, 127, (2, 3, 2, 64, d), dtype=torch.uint8, generator=torch.Generator().manual_seed(d))
+    for size in (0.0, 2.0 ** -126, 1.0, 3.0e38):
+        cache = pkg.ops.Cache8.empty(3, 2, d, dev)
+        cache.k.view(torch.uint8).copy_(old[0])
+        cache.v.view(torch.uint8).copy_(old[1].transpose(2, 3))
+        for s in (cache.k_scales, cache.v_scales):
+            s.view(torch.uint8).fill_(byte)
+        ref, table, starts = Pages(cache), ints(1).reshape(1, 1), ints(13)
+        k, v = (rand((1, 2, 9, d), i).clamp(-1, 1) * size for i in (1, 2))
+        ref.append(k, v, table, starts)
+        pkg.ops.cache8_append(cache, k.to(dev), v.to(dev), table.to(dev), starts.to(dev))
+        if byte < 255:
+            ref.equals(cache)
+            continue
+        assert (cache.k_scales.view(torch.uint8)[1] == 255).all() and (cache.v_scales.view(torch.uint8)[1] == 255).all()
+        assert torch.equal(cache.k.view(torch.uint8)[1, :, :13].cpu(), old[0, 1, :, :13])
+        assert torch.equal(cache.v.view(torch.uint8)[1, :, :, :13].cpu(), old[1, 1, :, :13].transpose(1, 2))
+
+
 def attention_reference(ref, q, table, lengths, scale, starts):
     """(result, error allowed before the rounding to q's type) in float64."""
     b, hq, lq, d = q.shape
