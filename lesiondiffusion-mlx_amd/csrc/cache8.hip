@@ -211,10 +211,14 @@ __device__ __forceinline__ int key_limit(const Attend8Args& a, int len, int64_t 
 // The softmax scale's size, in powers of two (1 for a scale of 0); its sign, or 0, is the queries'.
 __device__ __forceinline__ float soft_scale(const Attend8Args& a) { return a.scale == 0.f ? 1.f : fabsf(a.scale); }
 
-// That and the keys' scale go onto the scores inside the exponential. Kept a number larger than 0, so that
-// a masked score stays minus infinity and a score of 0 stays 0.
+// A page's scale, any E8M0 byte (append writes 1 to 254); infinity for 255.
+__device__ __forceinline__ float any_scale(int byte) { return byte ? scale_of(byte) : __int_as_float(0x00400000); }
+
+// That and the keys' scale go onto the scores inside the exponential. Kept a number larger than 0, so that a masked
+// score stays minus infinity and a score of 0 stays 0; least scales make it a subnormal number, which the fused
+// multiply-add takes as it is.
 __device__ __forceinline__ float score_scale(float c, int byte) {
-  return fminf(fmaxf(c * scale_of(byte), 1.1754944e-38f), 3.0e38f);
+  return fminf(fmaxf(c * any_scale(byte), 1.4e-45f), 3.0e38f);
 }
 
 // A query's reference for its exponentials is 2^kRaise below its maximum, and follows it only where that passes it by
@@ -252,10 +256,8 @@ __device__ __forceinline__ float sum8(f16x8 p, float l) {
   return l;
 }
 
-// A value page's scale, any E8M0 byte (append writes 1 to 254); 1 for 255, NaN, whose queries get NaN by their sum.
-__device__ __forceinline__ float page_scale(int byte) {
-  return byte == 255 ? 1.f : byte ? scale_of(byte) : __int_as_float(0x00400000);
-}
+// A value page's scale; 1 for 255, NaN, whose queries get NaN by their sum.
+__device__ __forceinline__ float page_scale(int byte) { return byte == 255 ? 1.f : any_scale(byte); }
 
 // Channels at .. at + 7 of a query, with the softmax scale's sign.
 template <typename T>

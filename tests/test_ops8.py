@@ -978,6 +978,25 @@ def test_attention_keeps_the_weight_of_a_long_tail(pkg, dev, b, n, lq, d, long, 
 
 
 @gpu
+@pytest.mark.parametrize("byte", [0, 1, 2, 20])
+@pytest.mark.parametrize(("lq", "d", "long"), [(1, 32, None), (2, 64, None), (3, 128, None), (1, 256, None), (150, 64, LONG[64]),
+                                               (130, 128, LONG[128]), (130, 256, LONG[256])])
+def test_attention_of_keys_at_the_least_scales(pkg, dev, lq, d, long, byte) -> None:
+    """Keys near 2^-126 under any E8M0 byte and queries near bf16's other end, whose scores are ordinary."""
+    cache, _, table = filled(pkg, dev, 1, 1, d, 3)
+    g = torch.Generator().manual_seed(1)
+    cache.k_scales.view(torch.uint8).fill_(byte)
+    codes = torch.tensor([0x48, 0xc8, 0x38, 0xb8, 0x30, 0], dtype=torch.uint8)        # 4, -4, 1, -1, 0.5, 0
+    cache.k.view(torch.uint8).copy_(codes[torch.randint(0, 6, cache.k.shape, generator=g)])
+    q = ((torch.randint(0, 2, (1, 1, lq, d), generator=g) * 2.0 - 1) * 2.0 ** 117).to(torch.bfloat16)
+    for scale in (2.0 ** -8, 0.4, 3.0):
+        got = pkg.ops.cache8_attention(q.to(dev), cache, longer(table, long).to(dev), ints(190).to(dev), scale).cpu().double()
+        want, allowed = attention_reference(Pages(cache), q, table, ints(190), scale, None)
+        bar = allowed * (1 + half_step(q.dtype)) + want.abs() * half_step(q.dtype) + tiny(q.dtype)
+        assert ((got - want).abs() <= bar).all(), (scale, ((got - want).abs() / bar).max())
+
+
+@gpu
 @pytest.mark.parametrize(("lq", "d", "long"), [(1, 64, None), (9, 64, None), (70, 128, None), (200, 64, LONG[64]),
                                                (130, 128, LONG[128]), (130, 256, LONG[256])])
 def test_attention_loud_page_of_small_weight(pkg, dev, lq, d, long) -> None:
