@@ -48,8 +48,11 @@ __device__ __forceinline__ float gelu_f(float v) {
   return v * (v < 0.f ? q : 1.0f - q);
 }
 
+// v / (1 + exp(-v)); 0 from where exp(-v) passes fp32, v = -88.72 (values of 3e-37 and less). The divisor is quartered:
+// from v = -87.34 on its reciprocal is no normal number, and v_rcp_f32 gives 0 for such.
 __device__ __forceinline__ float silu8_f(float v) {
-  return v * __builtin_amdgcn_rcpf(1.0f + exp_neg(fminf(fmaxf(v, -120.f), 120.f)));   // beyond: 0 and v
+  const float e = exp_neg(fminf(fmaxf(v, -120.f), 120.f));   // beyond: 0 and v
+  return v * (0.25f * __builtin_amdgcn_rcpf(__builtin_fmaf(0.25f, e, 0.25f)));
 }
 
 __device__ __forceinline__ float act_f(float v, int act) {

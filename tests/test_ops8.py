@@ -491,6 +491,20 @@ def test_dense8_activations_of_large_values(pkg, dev, act, m, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", [2, 700])
+def test_dense8_silu_where_its_exponential_is_large(pkg, dev, m, t) -> None:
+    """Down to where exp(-v) passes fp32 (v = -88.72); from -87.34 on 1 / (1 + exp(-v)) is below fp32's normal
+    numbers. A few fp32 steps (as in dense_case) and the rounding to ``t``."""
+    b = torch.tensor([-80.0, -87.0, -87.3, -87.4, -88.0, -88.5, -88.7, -1e-30, 3e-30] * 9)
+    x = pkg.ops.quantize8(torch.zeros(m, 130, device=dev))
+    w = pkg.ops.quantize8(torch.ones(b.numel(), 130, device=dev))
+    y = pkg.ops.dense8(x, w, b.to(dev), act="silu", dtype=t).cpu().double()
+    want = b.double() / (1 + torch.exp(-b.double()))
+    assert ((y - want).abs() <= want.abs() * (half_step(t) + 8 * 2.0 ** -23) + tiny(t)).all(), y[0] / want
+
+
+@gpu
 @pytest.mark.parametrize("m", [4, 100, 600])
 def test_dense8_scales_differ_by_block(pkg, dev, m) -> None:
     """Blocks of very unlike sizes, zero blocks and rows among them: each product takes its own scales."""
