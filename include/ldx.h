@@ -421,7 +421,7 @@ int ldx_group_norm_source_half(const void* x, int64_t x_batch_stride, int64_t x_
 #define LDX_PAGE8 64
 
 /* s = T(x + residual) (without a residual x itself); y = s / sqrt(mean(s^2) + eps) * gamma,
- * statistics in fp32; rounded to T (y) or written as 8-bit rows (codes, scales): one of the
+ * squares summed in fp32, at most 32 at a time, and those sums in fp64; rounded to T (y) or written as 8-bit rows (codes, scales): one of the
  * two. sum (may be NULL) receives s and may be x or residual; y may be x. x, residual, sum
  * and y are of type dtype (T) with contiguous features, any alignment; gamma fp32, eps at
  * least 1e-30. Rows whose squares pass fp32 although their values do not are normalised from

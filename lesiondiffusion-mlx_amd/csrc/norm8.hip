@@ -224,26 +224,33 @@ __global__ __launch_bounds__(256) void norm8_kernel(NormArgs a) {
     Root rstd = {1.f, 0.f};
     float g = 1.f;
     if constexpr (NORM) {
-      float ss = 0.f, amax = 0.f, f[8];
+      // Eights in fp32 and their sum in fp64, however many there are.
+      double ss = 0.0;
+      float amax = 0.f, f[8];
       for (int k = 0; k < rounds; k++) {
         take8<false>(a, x, r, s, (k * TPR + t) * 8, f);
+        float q = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          ss += f[i] * f[i];
+          q += f[i] * f[i];
           amax = fmaxf(amax, fabsf(f[i]));
         }
+        ss += q;
       }
       // Read again: the sum that this thread stored, since it may have been stored over x or r.
       const T* x2 = r && s ? s : x;
       const T* r2 = r && s ? nullptr : r;
-      rstd = row_rstd<TPR>(a, row_reduce<TPR, false>((double)ss, red), amax, red, g, [&](float by) {
-        float q = 0.f, h[8];
+      rstd = row_rstd<TPR>(a, row_reduce<TPR, false>(ss, red), amax, red, g, [&](float by) {
+        double all = 0.0;
+        float h[8];
         for (int k = 0; k < rounds; k++) {
           take8(a, x2, r2, (T*)nullptr, (k * TPR + t) * 8, h);
+          float q = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; i++) q += (h[i] * by) * (h[i] * by);
+          all += q;
         }
-        return q;
+        return all;
       });
       for (int k = 0; k < rounds; k++) {
         take8(a, x2, r2, (T*)nullptr, (k * TPR + t) * 8, f);

@@ -923,8 +923,8 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, *, residua
     """``s / sqrt(mean(s^2) + eps) * gamma`` over the last axis of fp16, bf16 or fp32 ``x``, ``s`` being
     ``x``, or ``x + residual`` rounded to that type. Returns the norm in ``x``'s type (into ``out`` when
     given, which may be ``x``), or as ``Quantized8`` rows with ``quantize``; with a ``residual`` the pair
-    ``(norm, s)``, ``s`` into ``sum_out`` when given, which may be ``x`` or ``residual``. Statistics in
-    fp32, one launch."""
+    ``(norm, s)``, ``s`` into ``sum_out`` when given, which may be ``x`` or ``residual``. Squares are
+    summed in fp32, at most 32 at a time, and those sums in fp64; ``eps`` is at least 1e-30. One launch."""
     _need(x, "x", _ALL, -1)
     n, dev, shape = x.numel(), x.get_device(), x.shape
     if not shape or not n:

@@ -290,6 +290,28 @@ def test_rms_norm_of_values_whose_squares_overflow(pkg, dev, c, size, t) -> None
 
 
 @gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("c", [8193, 65536, (1 << 20) + 3, (1 << 24) + 1])
+def test_rms_norm_of_long_rows(pkg, dev, c, t) -> None:
+    """A row's error does not grow with its length: eight squares at a time are summed in fp32 (at most eight
+    roundings, half of which reach the root), the eights in fp64; root, quotient and products take four more."""
+    rel = (8 / 2 + 4) * 2.0 ** -24
+    gamma = (1 + rand((c,), 4, scale=0.1)).to(dev)
+    x = torch.stack((torch.full((c,), 1.1), rand((c,), 5), rand((c,), 6) ** 3))
+    if t != torch.float16:
+        x[2] *= 1e19      # squares and their sum leave fp32
+    x = x.to(t).to(dev)
+    d = x.double()
+    y = d / torch.sqrt((d * d).mean(-1, keepdim=True) + 1e-6) * gamma.double()
+    err = (pkg.ops.rms_norm(x, gamma).double() - y).abs()
+    bar = y.abs() * (half_step(t) * (1 + rel) + rel) + tiny(t)
+    assert (err <= bar).all(), (err / bar).amax(1)
+    r = rand((3, c), 7, t).to(dev)
+    got, s = pkg.ops.rms_norm(x, gamma, residual=r)
+    assert torch.equal(s, (x.float() + r.float()).to(t)) and torch.equal(got, pkg.ops.rms_norm(s, gamma))
+
+
+@gpu
 def test_quantize8_of_many_rows(pkg, dev) -> None:
     """More rows than one axis of a launch takes."""
     n = (1 << 26) + 1001
