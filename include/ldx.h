@@ -510,7 +510,7 @@ int ldx_cache8_append(const ldx_cache8_append_args* args, void* stream);
  * queries that see it, a length past the table to the whole sequence. Where pages' value scales
  * are more than 2^63 apart, what is below 2^-83 of the largest values may be lost. o may be q.
  * Workspace: partial results where a sequence is split over workgroups,
- * ldx_cache8_attention_workspace_bytes of them; with less nothing is split. */
+ * ldx_cache8_attention_workspace_bytes of them, 256 MiB at most; with less nothing is split. */
 typedef struct ldx_cache8_attention_args {
   ldx_cache8 cache;
   int32_t batch, q_heads, q_len;

@@ -1066,6 +1066,15 @@ struct Plan {
 constexpr int kLeastChunk = 8;   // pages of a part at least: two for each streaming wave. (8 and 16: 4 sequences
                                  // of 8,000 tokens 20 and 22 us, 8 of 5,000 at head width 256 22 and 28)
 
+size_t split_bytes(const ldx_cache8_attention_args* p, int splits) {
+  if (splits < 2) return 0;
+  const size_t rows = (size_t)p->q_len * (p->q_heads / p->cache.heads);
+  return (size_t)p->batch * p->cache.heads * rows * splits * (p->cache.head_dim + 2) * sizeof(float);
+}
+
+// What partial results may take at most. (It bounds the join's launch, too.)
+constexpr size_t kMostPartBytes = (size_t)256 << 20;
+
 Plan plan_of(const ldx_cache8_attention_args* p) {
   const int D = p->cache.head_dim;
   const int64_t heads = (int64_t)p->batch * p->cache.heads, rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
@@ -1079,11 +1088,16 @@ Plan plan_of(const ldx_cache8_attention_args* p) {
   plan.wide = rows >= kWideRows && work >= (D == 32 ? INT64_MAX : D == 64 ? 100000 : D == 128 ? 18000 : 9000);
   int64_t s = 1;
   if (plan.wide) {
-    // Rounds of workgroups on the CUs' places, the pages of a round, and what a part more costs to join.
+    // Rounds of workgroups on the CUs' places, the pages of a round, and what a part more costs: 3 pages of a round
+    // to join, or what it writes and the join reads, at 4.5 TB/s and 2.2 us a page of a round. (With 3 pages for any
+    // number of rows calls that fill the card anyway were split: of 40 random ones 35 are faster so, 0.85 of the time
+    // on average, 16 x 1,769 queries of 12 x 8 heads of 128 4,039 -> 2,431 us without 4.2 GB; four are 4 to 9 % slower.)
     const int64_t groups = heads * ((rows + kWideRows - 1) / kWideRows), places = D == 64 ? 768 : D == 128 ? 512 : 256;
+    const double traffic = 8e-7 * (double)(heads * rows) * (D + 2), part = traffic > 3.0 ? traffic : 3.0;
     double best = 1e30;
     for (int64_t i = 1; i <= kFewParts && i <= most; i++) {
-      const double cost = (double)((groups * i + places - 1) / places) * ((p->width + i - 1) / i) + 3.0 * i;
+      if (split_bytes(p, (int)i) > kMostPartBytes) break;
+      const double cost = (double)((groups * i + places - 1) / places) * ((p->width + i - 1) / i) + part * i;
       if (cost < best) best = cost, s = i;
     }
   } else {
@@ -1098,12 +1112,6 @@ Plan plan_of(const ldx_cache8_attention_args* p) {
   }
   plan.splits = (int)(s < 1 ? 1 : s > kMostParts ? kMostParts : s);
   return plan;
-}
-
-size_t split_bytes(const ldx_cache8_attention_args* p, int splits) {
-  if (splits < 2) return 0;
-  const size_t rows = (size_t)p->q_len * (p->q_heads / p->cache.heads);
-  return (size_t)p->batch * p->cache.heads * rows * splits * (p->cache.head_dim + 2) * sizeof(float);
 }
 
 int check_attention(const ldx_cache8_attention_args* p) {

@@ -169,6 +169,29 @@ def test_cache8_attention_refuses(pkg, bad) -> None:
     refused(pkg, lib.lib.ldx_cache8_attention(ctypes.byref(a), None), "cache8_attention")
 
 
+def test_attention_workspace_is_bounded(pkg) -> None:
+    """Partial results are at most 256 MiB, whatever a call's size, and nothing where the queries fill the card many
+    times over; long sequences of few queries are still spread over workgroups."""
+    lib = pkg._lib
+
+    def parts(batch, heads, group, q_len, d, width):
+        a = lib.Cache8AttentionArgs(cache=_cache_args(lib, heads=heads, head_dim=d), batch=batch, q_heads=heads * group,
+                                    q_len=q_len, q=16, o=16, scale=1.0, table=16, table_pitch=width, width=width, lengths=16)
+        n = lib.lib.ldx_cache8_attention_workspace_bytes(ctypes.byref(a))
+        per = batch * heads * group * q_len * (d + 2) * 4
+        assert n % per == 0 and n <= 256 << 20, (batch, heads, group, q_len, d, width, n)
+        return max(n // per, 1)
+
+    assert parts(16, 8, 4, 4000, 64, 126) == parts(64, 8, 4, 4096, 64, 64) == parts(16, 8, 8, 15900, 256, 440) == 1
+    assert parts(1, 4, 4, 2000, 64, 157) > 1 and parts(1, 8, 1, 1, 128, 128) > 1 and parts(1, 1, 1, 128, 64, 20000) > 1
+    gen = torch.Generator().manual_seed(1)
+    log = lambda lo, hi: int(math.exp(math.log(lo) + torch.rand((), generator=gen).item() * math.log(hi / lo)))
+    for _ in range(3000):
+        d = [32, 64, 128, 256][log(1, 16) % 4]
+        batch, heads, group = log(1, 2000), log(1, 64), log(1, 16)
+        parts(batch, heads, group, max(1, min(log(1, 100_000), 0x7fffffff // (batch * heads * group))), d, log(1, 1 << 24))
+
+
 def test_cpu_tensors_are_refused(pkg) -> None:
     ops = pkg.ops
     x = torch.zeros(2, 8)
