@@ -856,6 +856,7 @@ def _launch8(fn, args: tuple, device: int, what: str) -> None:
 
 
 _ELEM, _ALL = tuple(ELEM_DTYPES), tuple(ALL_DTYPES)
+_MOST = 0x7fffffff   # what a size in the C structs holds (ctypes drops the bits above)
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype | tuple | None, device: int) -> None:
@@ -910,8 +911,10 @@ def quantize8(x: torch.Tensor) -> Quantized8:
     n = x.numel()
     if x.dim() < 1 or not n:
         raise ValueError(f"quantize8: shape {tuple(x.shape)} holds no rows")
-    x2, pitch = _rows(x)
     f = x.shape[-1]
+    if f > _MOST:
+        raise ValueError(f"quantize8: {f} features")
+    x2, pitch = _rows(x)
     q = Quantized8.empty(x.shape[:-1], f, x)
     _launch8(lib.ldx_quantize8, (x2.data_ptr(), pitch, n // f, f, ALL_DTYPES[x.dtype], q.codes.data_ptr(),
                                  q.codes.shape[-1], q.scales.data_ptr(), q.scales.shape[-1]), x.get_device(), "quantize8")
@@ -930,6 +933,8 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, *, residua
     if not shape or not n:
         raise ValueError(f"rms_norm: shape {tuple(shape)} holds no rows")
     f = shape[-1]
+    if f > _MOST:
+        raise ValueError(f"rms_norm: {f} features")
     _need(gamma, "gamma", None, dev)
     if gamma.shape != (f,):
         raise ValueError(f"gamma shape {tuple(gamma.shape)} != ({f},)")
@@ -1098,6 +1103,8 @@ def _cache_table(table: torch.Tensor, batch: int, device: int) -> tuple[int, int
     if len(shape) != 2 or shape[0] != batch or not shape[1] or (shape[1] > 1 and table.stride(1) != 1) \
             or (batch > 1 and table.stride(0) < shape[1]):
         raise ValueError(f"table must be int32 ({batch}, pages) with contiguous rows, got {tuple(shape)}")
+    if shape[1] > _MOST:
+        raise ValueError(f"table of {shape[1]} pages a sequence")
     return table.data_ptr(), (table.stride(0) if batch > 1 else shape[1]), shape[1]
 
 
@@ -1135,6 +1142,8 @@ def cache8_append(cache: Cache8, k: torch.Tensor, v: torch.Tensor, table: torch.
             or not shape[2]:
         raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must be (B, {block.heads}, L, {block.head_dim})")
     b, _, n, _ = shape
+    if b > _MOST or n > _MOST:
+        raise ValueError(f"cache8_append: {b} x {n} tokens")
     a = Cache8AppendArgs(block, b, n, k.data_ptr(), _head_strides(k, "k"), v.data_ptr(), _head_strides(v, "v"),
                          ALL_DTYPES[k.dtype], *_cache_table(table, b, dev), _cache_ints(starts, "starts", b, dev),
                          None if counts is None else _cache_ints(counts, "counts", b, dev))
@@ -1158,6 +1167,8 @@ def cache8_attention(q: torch.Tensor, cache: Cache8, table: torch.Tensor, length
     if len(shape) != 4 or shape[3] != block.head_dim or shape[1] % block.heads or not q.numel():
         raise ValueError(f"q {tuple(shape)} must be (B, a multiple of {block.heads}, L, {block.head_dim})")
     b, hq, lq, _ = shape
+    if b > _MOST or hq > _MOST or lq > _MOST:
+        raise ValueError(f"cache8_attention: {b} x {hq} x {lq} queries")
     given = out is not None
     if given:
         _need(out, "out", q.dtype, dev)

@@ -209,6 +209,32 @@ def test_cpu_tensors_are_refused(pkg) -> None:
         ops.cache8_attention(x, x, ints, ints, 1.0)
 
 
+def test_sizes_beyond_the_abi_fields_are_refused(pkg, monkeypatch) -> None:
+    """Features, tokens, batches and table widths that the C structs' 32 bits do not hold, none of which a call may
+    take for the rest of them; tensors without memory stand in for those of a device."""
+    ops = pkg.ops
+    monkeypatch.setattr(ops, "_need", lambda *a: None)
+    meta = lambda *shape, t=torch.float16: torch.empty(shape, dtype=t, device="meta")
+    huge = (1 << 32) + 8
+    ints32 = lambda *shape: meta(*shape, t=torch.int32)
+    codes, scales = meta(2, 1, 64, 32, t=torch.float8_e4m3fn), meta(2, 1, t=torch.float8_e8m0fnu)
+    cache = ops.Cache8(codes, codes.view(2, 1, 32, 64), scales, scales)
+    monkeypatch.setattr(ops, "_cache_block", lambda c, what: (pkg._lib.Cache8Block(16, 16, 1, 1, 2, 1, 32), 0))
+    kv = meta(1, 1, 1, 32).expand(1, 1, huge, 32)
+    many = meta(1, 1, 1, 32).expand(huge, 1, 1, 32)
+    one = meta(1, 1, 1, 32)
+    for word, call in (
+            ("features", lambda: ops.quantize8(meta(1, huge))), ("features", lambda: ops.rms_norm(meta(1, huge), meta(huge))),
+            ("tokens", lambda: ops.cache8_append(cache, kv, kv, ints32(1, 1), ints32(1))),
+            ("tokens", lambda: ops.cache8_append(cache, many, many, ints32(huge, 1), ints32(huge))),
+            ("pages", lambda: ops.cache8_append(cache, one, one, ints32(1, huge), ints32(1))),
+            ("pages", lambda: ops.cache8_attention(one, cache, ints32(1, huge), ints32(1), 1.0)),
+            ("queries", lambda: ops.cache8_attention(kv, cache, ints32(1, 1), ints32(1), 1.0, out=kv)),
+            ("queries", lambda: ops.cache8_attention(many, cache, ints32(huge, 1), ints32(huge), 1.0, out=many))):
+        with pytest.raises(ValueError, match=word):
+            call()
+
+
 # ------------------------------------------------------------------ 8-bit rows and the norm
 
 SHAPES = [(1, 1), (3, 7), (1, 128), (2, 129), (5, 512), (4, 513), (7, 1000), (3, 1024), (2, 2047), (2, 4096), (1, 5001),
