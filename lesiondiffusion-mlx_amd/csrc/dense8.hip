@@ -61,7 +61,8 @@ __device__ __forceinline__ float act_f(float v, int act) {
   return v;
 }
 
-// Eight codes with their scale (its power of two, as fp32) as bf16 values: both fit exactly.
+// Eight codes with their scale (its power of two, as fp32, of whose bits the conversion takes the byte: 0 is 2^-127 and
+// 255 NaN) as bf16 values, which hold them exactly from 2^-130 to 2^128; digits below 2^-133 are rounded off.
 __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float s) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false);
   const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);

@@ -999,7 +999,8 @@ def dense8(x: Quantized8, weight: Quantized8, bias: torch.Tensor | None = None, 
     fp32 sums and one rounding to ``dtype`` (fp16, bf16 or fp32; ``residual`` and ``out`` share it).
     ``act`` is None, ``"gelu"`` or ``"silu"``. fp16 and bf16 results come from the e4m3 matrix
     instruction, whose sums are within 2^-10 of the terms' magnitudes (about 1.5e-5 of the result for
-    ordinary data); fp32 results are summed to fp32 accuracy at half its rate."""
+    ordinary data); fp32 results are summed to fp32 accuracy at half its rate: round those where a 16-bit
+    result has to have it, too."""
     xc, xs, xp, xsp, lead = _rows8(x, "x", -1)
     dev = xc.get_device()
     wc, ws, wp, wsp, outs = _rows8(weight, "weight", dev)

@@ -594,6 +594,35 @@ def test_dense8_scales_differ_by_block(pkg, dev, m) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize(("m", "o"), [(3, 40), (150, 140), (1500, 700)])
+def test_dense8_of_any_scale_byte(pkg, dev, m, o, t) -> None:
+    """Bytes that quantize8 does not write: 0 (2^-127) and 254 are powers of two like the others, 255 is NaN for its
+    row or output."""
+    k = 300
+    x, w = pkg.ops.quantize8(rand((m, k), 1).to(dev)), pkg.ops.quantize8(rand((o, k), 2).to(dev))
+    xs, ws, xc, wc = (q.view(torch.uint8) for q in (x.scales, w.scales, x.codes, w.codes))
+    xs[:, :3], ws[:, :3] = 120, 125
+    # Small rows times large outputs; codes of at most 1 where the scale is 2^127 (bf16 has no larger number).
+    one = torch.tensor(0x38, dtype=torch.uint8, device=dev)
+    xs[0, :3], xs[1, :3], xs[2, 1] = 0, 3, 255
+    wc[4:7] = torch.minimum(wc[4:7] & 0x7f, one)
+    ws[4, :3], ws[5, :3], ws[6, :3], ws[7, 2] = 254, 240, 250, 255
+    got = pkg.ops.dense8(x, w, dtype=t).cpu().double()
+    a, ww = wide(x), wide(w)
+    assert got[2].isnan().all() and got[:, 7].isnan().all()
+    a[2], ww[7] = 0, 0
+    y, terms = a @ ww.t(), a.abs() @ ww.abs().t()
+    allowed = dense_bound(a, ww, k, t) + y.abs() * half_step(t) + tiny(t)
+    if t == torch.float32:   # operands as bf16 values: those below 2^-126 to half of their last place, 2^-133
+        allowed += 2.0 ** -134 * (ww.abs().sum(1) + a.abs().sum(1)[:, None])
+    # Held to what stays in fp32 on the way and in t at the end.
+    keep = (terms < 2.0 ** 127) & (y.abs() + allowed < (65504 if t == torch.float16 else 2.0 ** 127))
+    keep[2], keep[:, 7] = False, False
+    assert keep[:2].sum() > 70 and keep[:, 5].any() and ((got - y).abs() <= allowed)[keep].all(), ((got - y).abs() / allowed)[keep].max()
+
+
+@gpu
 def test_dense8_nan_stays_in_its_row_and_column(pkg, dev) -> None:
     for m, o in ((5, 40), (140, 150)):
         x, w = rand((m, 256), 1), rand((o, 256), 2)
