@@ -40,7 +40,7 @@ extern "C" {
 
 /* Message of the calling thread's most recent failure ("" if none). */
 const char* ldx_last_error(void);
-/* ABI version (14); bumped on any change to the structs below or the entry points. */
+/* ABI version (15); bumped on any change to the structs below or the entry points. */
 int ldx_abi_version(void);
 
 /* ---------------------------------------------------------------- conv3d -------
@@ -467,6 +467,15 @@ typedef struct ldx_dense8_args {
   void* y; int64_t y_pitch;
 } ldx_dense8_args;
 int ldx_dense8(const ldx_dense8_args* args, void* stream);
+/* The kernel that such a call takes, on the host alone (pointers are looked at, not read): tiles
+ * of 32 or 64 rows and outputs whose waves take blocks of features of their own, or of 64, 128
+ * or 256 whose waves share them. */
+#define LDX_DENSE8_OWN_32 0
+#define LDX_DENSE8_OWN_64 1
+#define LDX_DENSE8_SHARED_64 2
+#define LDX_DENSE8_SHARED_128 3
+#define LDX_DENSE8_SHARED_256 4
+int ldx_dense8_kernel(const ldx_dense8_args* args);
 
 /* A cache of keys and values in pages of LDX_PAGE8 tokens, each page with one scale for a
  * head's keys and one for its values: k codes (pages, heads, 64, head_dim), v codes (pages,
@@ -526,6 +535,9 @@ typedef struct ldx_cache8_attention_args {
 } ldx_cache8_attention_args;
 size_t ldx_cache8_attention_workspace_bytes(const ldx_cache8_attention_args* args);
 int ldx_cache8_attention(const ldx_cache8_attention_args* args, void* stream);
+/* Rows (queries x heads of a cache head) that a workgroup of such a call takes, on the host
+ * alone: 16, each wave reading pages of its own, or 128, which share them. */
+int ldx_cache8_attention_rows(const ldx_cache8_attention_args* args);
 
 #ifdef __cplusplus
 }

@@ -197,12 +197,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ldx_rms_norm": (c_i32, [ctypes.POINTER(RmsNormArgs), c_vp]),
     "ldx_quantize8": (c_i32, [c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp]),
     "ldx_dense8": (c_i32, [ctypes.POINTER(Dense8Args), c_vp]),
+    "ldx_dense8_kernel": (c_i32, [ctypes.POINTER(Dense8Args)]),
     "ldx_cache8_append": (c_i32, [ctypes.POINTER(Cache8AppendArgs), c_vp]),
     "ldx_cache8_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Cache8AttentionArgs)]),
+    "ldx_cache8_attention_rows": (c_i32, [ctypes.POINTER(Cache8AttentionArgs)]),
     "ldx_cache8_attention": (c_i32, [ctypes.POINTER(Cache8AttentionArgs), c_vp]),
 }
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 
 def _load() -> ctypes.CDLL:

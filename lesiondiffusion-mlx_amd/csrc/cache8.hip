@@ -1164,6 +1164,11 @@ extern "C" size_t ldx_cache8_attention_workspace_bytes(const ldx_cache8_attentio
   return check_attention(p) == LDX_OK ? split_bytes(p, plan_of(p).splits) : 0;
 }
 
+extern "C" int ldx_cache8_attention_rows(const ldx_cache8_attention_args* p) {
+  if (int rc = check_attention(p)) return rc;
+  return plan_of(p).wide ? kWideRows : 16;
+}
+
 extern "C" int ldx_cache8_attention(const ldx_cache8_attention_args* p, void* stream) {
   if (int rc = check_attention(p)) return rc;
   Plan plan = plan_of(p);

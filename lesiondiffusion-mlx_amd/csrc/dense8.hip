@@ -541,10 +541,8 @@ inline double estimate(const Cost& c, bool act, int64_t M, int64_t O, int kb, in
          (act ? c.act * rounds + c.act_tile * full : 0.0);
 }
 
-template <typename T>
-int launch(const Dense8Args& a, hipStream_t st) {
-  constexpr bool EXACT = sizeof(T) == 4;
-  const bool act = a.act != LDX_ACT_NONE;
+template <bool EXACT>
+int choose(bool act, int64_t M, int64_t O, int kb) {
   constexpr Cost big4 = EXACT ? Cost{9.80f, 2.11f, 2.267f, 0.298f, 14.97f, 15.5f, 3.4f}
                               : Cost{10.78f, 1.97f, 0.981f, 0.299f, 9.03f, 15.5f, 3.4f};
   constexpr Cost big2 = EXACT ? Cost{5.22f, 0.f, 0.740f, 0.654f, 9.33f, 2.8f, 4.4f}
@@ -555,17 +553,22 @@ int launch(const Dense8Args& a, hipStream_t st) {
                               : Cost{3.10f, 1.60f, 0.677f, 0.192f, 0.80f, 0.9f, 0.1f};
   constexpr Cost split1 = EXACT ? Cost{3.66f, 0.f, 0.468f, 0.267f, 1.16f, 0.5f, 0.f}
                               : Cost{3.65f, 0.01f, 0.339f, 0.327f, 0.91f, 0.5f, 0.f};
-  const double t[5] = {estimate(split1, act, a.M, a.O, a.kb, 32, 32, 512, 4), estimate(split2, act, a.M, a.O, a.kb, 64, 64, 256, 4),
-                       estimate(big1, act, a.M, a.O, a.kb, 64, 64, 512, 1), estimate(big2, act, a.M, a.O, a.kb, 128, 128, 512, 1),
-                       estimate(big4, act, a.M, a.O, a.kb, 256, 256, 256, 1)};
+  const double t[5] = {estimate(split1, act, M, O, kb, 32, 32, 512, 4), estimate(split2, act, M, O, kb, 64, 64, 256, 4),
+                       estimate(big1, act, M, O, kb, 64, 64, 512, 1), estimate(big2, act, M, O, kb, 128, 128, 512, 1),
+                       estimate(big4, act, M, O, kb, 256, 256, 256, 1)};
   int best = 0;
   for (int i = 1; i < 5; i++)
     if (t[i] < t[best]) best = i;
-  switch (best) {
-    case 0: return launch_split<T, 1, 1, 4, 2>(a, st);
-    case 1: return launch_split<T, 2, 2, 4, 2>(a, st);
-    case 2: return launch_big<T, 1, 1, 4>(a, st);
-    case 3: return launch_big<T, 2, 2, 2>(a, st);
+  return best;
+}
+
+template <typename T>
+int launch(const Dense8Args& a, hipStream_t st) {
+  switch (choose<sizeof(T) == 4>(a.act != LDX_ACT_NONE, a.M, a.O, a.kb)) {
+    case LDX_DENSE8_OWN_32: return launch_split<T, 1, 1, 4, 2>(a, st);
+    case LDX_DENSE8_OWN_64: return launch_split<T, 2, 2, 4, 2>(a, st);
+    case LDX_DENSE8_SHARED_64: return launch_big<T, 1, 1, 4>(a, st);
+    case LDX_DENSE8_SHARED_128: return launch_big<T, 2, 2, 2>(a, st);
     default: return launch_big<T, 4, 4, 2>(a, st);
   }
 }
@@ -579,12 +582,7 @@ int check_operand(const char* name, const void* codes, int64_t cp, const void* s
   return LDX_OK;
 }
 
-}  // namespace
-}  // namespace ldx
-
-using namespace ldx;
-
-extern "C" int ldx_dense8(const ldx_dense8_args* p, void* stream) {
+int check_call(const ldx_dense8_args* p) {
   if (!p || !p->y) return fail("dense8: null pointer");
   if (p->rows < 1 || p->rows > 0x7fffffff || p->features < 1 || p->features > (1 << 22) || p->out_features < 1 ||
       p->out_features > (1 << 28))
@@ -599,6 +597,24 @@ extern "C" int ldx_dense8(const ldx_dense8_args* p, void* stream) {
   if (int rc = check_operand("w", p->w_codes, p->w_pitch, p->w_scales, p->w_scales_pitch, kb)) return rc;
   if (p->y_pitch < p->out_features || (p->residual && p->residual_pitch < p->out_features))
     return fail("dense8: row pitch below %d outputs", p->out_features);
+  return LDX_OK;
+}
+
+}  // namespace
+}  // namespace ldx
+
+using namespace ldx;
+
+extern "C" int ldx_dense8_kernel(const ldx_dense8_args* p) {
+  if (int rc = check_call(p)) return rc;
+  const int kb = (p->features + kBlock8 - 1) / kBlock8;
+  return p->dtype == LDX_DTYPE_F32 ? choose<true>(p->act != LDX_ACT_NONE, p->rows, p->out_features, kb)
+                                   : choose<false>(p->act != LDX_ACT_NONE, p->rows, p->out_features, kb);
+}
+
+extern "C" int ldx_dense8(const ldx_dense8_args* p, void* stream) {
+  if (int rc = check_call(p)) return rc;
+  const int kb = (p->features + kBlock8 - 1) / kBlock8;
   const Dense8Args a = {(const uint8_t*)p->x_codes, p->x_pitch, (const uint8_t*)p->x_scales, p->x_scales_pitch,
                         (const uint8_t*)p->w_codes, p->w_pitch, (const uint8_t*)p->w_scales, p->w_scales_pitch,
                         p->bias, p->residual, p->residual_pitch, p->y, p->y_pitch, p->rows, p->out_features, kb,

@@ -545,6 +545,58 @@ def test_dense8_tiles(pkg, dev, m, k, o, t) -> None:
         assert ((part - y).abs() <= allowed)[~inf].all(), ((part - y).abs() / allowed)[~inf].max()
 
 
+# Sizes, ragged in both directions, for each kernel of dense8, whatever the result's type and the activation.
+KERNELS = [(0, 45, 300, 71), (1, 673, 4507, 1435), (2, 165, 576, 7223), (3, 3619, 1700, 1735), (4, 6081, 4873, 8139)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize(("kernel", "m", "k", "o"), KERNELS)
+def test_dense8_kernels_of_the_tested_sizes(pkg, kernel, m, k, o, t) -> None:
+    """The sizes of test_dense8_of_every_kernel take the kernels that they are there for."""
+    lib, kb = pkg._lib, -(-k // 128)
+    for act in (0, 1, 2):
+        a = lib.Dense8Args(rows=m, features=k, out_features=o, x_codes=16, x_pitch=kb * 128, x_scales=16,
+                           x_scales_pitch=-(-kb // 4) * 4, w_codes=16, w_pitch=kb * 128, w_scales=16,
+                           w_scales_pitch=-(-kb // 4) * 4, y=16, y_pitch=o, act=act, dtype=pkg.ops.ALL_DTYPES[t])
+        assert lib.lib.ldx_dense8_kernel(ctypes.byref(a)) == kernel, act
+    a.rows = 0
+    refused(pkg, lib.lib.ldx_dense8_kernel(ctypes.byref(a)), "dense8")
+
+
+@gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", [None, "gelu", "silu"])
+@pytest.mark.parametrize(("kernel", "m", "k", "o"), KERNELS)
+def test_dense8_of_every_kernel(pkg, dev, kernel, m, k, o, act, t) -> None:
+    """Each kernel with a bias, a residual and an output that are column ranges at odd offsets, and an activation:
+    all rows of some outputs and all outputs of some rows, the last ones among them, against the bound of the small
+    cases; what stands beside the output stays."""
+    g, gd = torch.Generator().manual_seed(k), torch.Generator(device=dev).manual_seed(k)
+    x = pkg.ops.quantize8(torch.randn(m, k, generator=gd, device=dev))
+    w = pkg.ops.quantize8(torch.randn(o, k, generator=gd, device=dev) / math.sqrt(k))
+    b = torch.randn(o, generator=gd, device=dev)
+    r = torch.randn(m, o + 4, generator=gd, device=dev).to(t)[:, 1:1 + o]
+    base = torch.full((m, o + 3), 7.0, dtype=t, device=dev)
+    got = pkg.ops.dense8(x, w, b, residual=r, act=act, out=base[:, 2:2 + o], dtype=t)
+    assert (base[:, :2] == 7).all() and (base[:, 2 + o:] == 7).all()
+    xs, ws = (q.codes.double().unflatten(-1, (-1, 128)) * q.scales.double()[:, :q.codes.shape[1] // 128, None] for q in (x, w))
+    xs, ws = xs.flatten(1)[:, :k], ws.flatten(1)[:, :k]
+    rows = torch.cat((torch.randperm(m, generator=g)[:20], torch.tensor([0, m - 1]))).to(dev)
+    cols = torch.cat((torch.randperm(o, generator=g)[:20], torch.tensor([0, o - 1]))).to(dev)
+    every = slice(None)
+    for i, j in ((every, cols), (rows, every)):
+        add = (b.double()[j], r.double()[i][:, j])
+        y = torch.mm(xs[i], ws[j].t().contiguous())
+        allowed = dense_bound(xs[i], ws[j], k, t)
+        for extra in add:
+            y = y + extra
+            allowed = allowed + 2.0 ** -23 * (y.abs() + extra.abs())
+        z = activate(y, act)
+        allowed = 1.13 * allowed + z.abs() * (half_step(t) + 8 * 2.0 ** -23) + tiny(t) + (2.0 ** -23 * y.abs() if act else 0)
+        err = (got.double()[i][:, j] - z).abs()
+        assert (err <= allowed).all(), (err / allowed).max()
+
+
 @gpu
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("m", [2, 700])
@@ -863,6 +915,23 @@ LONG = {64: 14000, 128: 2600, 256: 1300}
 def longer(table: torch.Tensor, width: int | None) -> torch.Tensor:
     """``table`` followed by columns that name no page."""
     return table if width is None else torch.nn.functional.pad(table, (0, width - table.shape[1]), value=-1)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_attention_kernels_of_the_tested_widths(pkg, d) -> None:
+    """From 128 rows of a cache head on a table of LONG columns takes the kernel that shares pages, for any number of
+    heads and sequences; fewer rows, the tests' short tables and heads of 32 the streaming one."""
+    lib = pkg._lib
+
+    def rows(batch, heads, group, q_len, width):
+        a = lib.Cache8AttentionArgs(cache=_cache_args(lib, heads=heads, head_dim=d), batch=batch, q_heads=heads * group,
+                                    q_len=q_len, q=16, o=16, scale=1.0, table=16, table_pitch=width, width=width, lengths=16)
+        return lib.lib.ldx_cache8_attention_rows(ctypes.byref(a))
+
+    for batch, heads, group, q_len in ((1, 1, 1, 128), (7, 1, 3, 50), (1, 1, 2, 70), (4, 2, 1, 150), (2, 2, 2, 100), (1, 1, 1, 300)):
+        assert rows(batch, heads, group, q_len, LONG.get(d, 14000)) == (16 if d == 32 else 128)
+        assert rows(1, heads, group, q_len, 8) == rows(batch, heads, group, 127 // group, LONG.get(d, 14000)) == 16
+    assert rows(1, 3, 1, 0, 8) == lib.LDX_EINVAL
 
 
 def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, seed=0, scale=None, long=None, spread=9):
