@@ -35,7 +35,8 @@ __all__ = [
 class count_flops:
     """Context manager tallying the algorithmic FLOPs (2 x real multiply-adds, no
     padding; a folded upsample conv counts its 8 taps) of the convs, dense layers and
-    attention launched inside it -- for throughput figures."""
+    attention launched inside it -- for throughput figures. ``cache8_attention`` is not counted: how
+    many tokens its queries see stands on the device alone."""
 
     active: "count_flops | None" = None
 
@@ -1160,8 +1161,10 @@ def cache8_attention(q: torch.Tensor, cache: Cache8, table: torch.Tensor, length
     ``j`` reads the cache's head ``j // group``). With ``starts`` query ``i`` sees tokens up to position
     ``starts[b] + i`` (causal); without, all ``lengths[b]``. A query that sees no token gives 0; tokens that
     it does not see, and pages behind the length, do not touch its result. A page that the cache does
-    not have, or a length past the table, gives NaN. Returns ``(B, heads, L, D)`` in ``q``'s type (into
-    ``out`` when given, which may be ``q``); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
+    not have, or a length past the table, gives NaN. Scores, softmax and sums are fp32; probabilities are
+    rounded to fp16 (2^-11 of each, those below 2^-21 of a query's largest to 2^-32 of it). Returns
+    ``(B, heads, L, D)`` in ``q``'s type (into ``out`` when given, which may be ``q``); ``table``,
+    ``lengths`` and ``starts`` are int32 on the device."""
     block, dev = _cache_block(cache, "cache8_attention")
     _need(q, "q", _ELEM, dev)
     shape = q.shape
