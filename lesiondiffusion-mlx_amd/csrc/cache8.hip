@@ -214,11 +214,14 @@ __device__ __forceinline__ float soft_scale(const Attend8Args& a) { return a.sca
 // A page's scale, any E8M0 byte (append writes 1 to 254); infinity for 255.
 __device__ __forceinline__ float any_scale(int byte) { return byte ? scale_of(byte) : __int_as_float(0x00400000); }
 
-// That and the keys' scale go onto the scores inside the exponential. Kept a number larger than 0, so that a masked
-// score stays minus infinity and a score of 0 stays 0; least scales make it a subnormal number, which the fused
-// multiply-add takes as it is.
-__device__ __forceinline__ float score_scale(float c, int byte) {
-  return fminf(fmaxf(c * any_scale(byte), 1.4e-45f), 3.0e38f);
+// That and the keys' scale (c and a wave's byte) go onto the scores inside the exponential: an exponent more on c, in
+// scalar arithmetic, but where it leaves the normal numbers. Kept a number larger than 0, so that a masked score stays
+// minus infinity and a score of 0 stays 0; least scales make it a subnormal number, which the fused multiply-add takes
+// as it is.
+__device__ __forceinline__ float score_scale(int c, int byte) {
+  const int e = (c >> 23) + byte - 127;
+  if (c >= 0x00800000 && e >= 1 && e <= 253) return __int_as_float(c + (byte - 127) * (1 << 23));
+  return fminf(fmaxf(__int_as_float(c) * any_scale(byte), 1.4e-45f), 3.0e38f);
 }
 
 // A query's reference for its exponentials is 2^kRaise below its maximum, and follows it only where that passes it by
@@ -230,21 +233,12 @@ constexpr float kSlack = 8.f, kRaise = 7.f, kLower = 0x1p-7f;
 
 // A score times its scale goes into the exponential unrounded, its reference does not: what the reference's rounding
 // left out, up to 2^-24 of it, moves all probabilities of a query by one factor, which beyond scores of 2^28 leaves
-// fp16. Pages that may hold scores of kFarScore (by the queries' sums of magnitudes and the largest code) have them
-// multiplied, and rounded, first, and have no slack (7 less is rounded, too: to 8 less, or to nothing from 2^27 on).
-constexpr float kFarScore = 4194304.f;
-__device__ __forceinline__ bool far_page(float most, float grow) { return most * grow > kFarScore; }
-
-// The wave's largest score at a scale of 1, or more: 448 times the sum of a query's magnitudes, of which a lane holds
-// one of `lanes` parts.
-template <typename V, int N>
-__device__ __forceinline__ float most_score(const V (&q)[N], int lanes) {
-  float sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < N; j++)
-#pragma unroll
-    for (int e = 0; e < 8; e++) sum += fabsf((float)q[j][e]);
-  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(wave_max(sum) * (448.f * lanes))));
+// fp16. Pages that may hold scores of 2^22 and more have them multiplied, and rounded, first, and have no slack (7 less
+// is rounded, too: to 8 less, or to nothing from 2^27 on). This is the least scale byte of such a page, by the largest
+// code and the sums of the wave's queries' magnitudes, of which a lane holds one of `lanes` parts.
+__device__ __forceinline__ int far_byte(float sum, int lanes, float c) {
+  const float most = wave_max(sum) * (448.f * lanes) * c;   // below 2^(e - 126)
+  return 127 + 22 + 127 - (__builtin_amdgcn_readfirstlane(__float_as_int(most)) >> 23);
 }
 
 // l and eight probabilities: as the products take them, in fp16 (their sum in fp32), so that rounding moves
@@ -259,15 +253,18 @@ __device__ __forceinline__ float sum8(f16x8 p, float l) {
 // A value page's scale; 1 for 255, NaN, whose queries get NaN by their sum.
 __device__ __forceinline__ float page_scale(int byte) { return byte == 255 ? 1.f : any_scale(byte); }
 
-// Channels at .. at + 7 of a query, with the softmax scale's sign.
+// Channels at .. at + 7 of a query, with the softmax scale's sign; their magnitudes are added to sum.
 template <typename T>
-__device__ __forceinline__ typename Vec8<T>::V query8(const Attend8Args& a, const T* q, int at, bool real) {
+__device__ __forceinline__ typename Vec8<T>::V query8(const Attend8Args& a, const T* q, int at, bool real, float& sum) {
   float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (real) load8(q + at, f);
   const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;
   typename Vec8<T>::V v;
 #pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = (T)(f[e] * sign);
+  for (int e = 0; e < 8; e++) {
+    v[e] = (T)(f[e] * sign);
+    sum += fabsf(f[e]);
+  }
   return v;
 }
 
@@ -318,13 +315,15 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
   if (p0 >= p1 && split > 0) return;   // the join knows that there is no such part
 
   const float c = soft_scale(a);
+  const int c_bits = __builtin_amdgcn_readfirstlane(__float_as_int(c));
   V8 q[NK];
+  float q_sum = 0.f;
   {
     const T* qp = (const T*)a.q + b * a.qs[0] + (int64_t)(row / a.G) * a.qs[1] + (int64_t)(h * a.G + row % a.G) * a.qs[2];
     // D >= 64: the products 2 j and 2 j + 1 take channels 64 j + 16 g + 0..7 and + 8..15, so that a
     // key's bytes are read 16 at a time.
 #pragma unroll
-    for (int j = 0; j < NK; j++) q[j] = query8<T>(a, qp, D == 32 ? 8 * g : 64 * (j / 2) + 16 * g + 8 * (j % 2), real);
+    for (int j = 0; j < NK; j++) q[j] = query8<T>(a, qp, D == 32 ? 8 * g : 64 * (j / 2) + 16 * g + 8 * (j % 2), real, q_sum);
   }
 
   float acc[ND][4];   // single numbers: as vectors, every branch that changes them copies them
@@ -384,10 +383,11 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
   int after = entry(p + 2 * kAttendWaves);
   load_k(now, p);
   load_v(now, p);
-  const float most_q = most_score(q, 4);
+  const int far_from = far_byte(q_sum, 4, c);
   for (; p < p1; p += kAttendWaves) {
-    float grow = score_scale(c, ks);
-    const bool none_k = ks == 255;
+    const int ksb = __builtin_amdgcn_readfirstlane(ks);
+    const bool none_k = ksb == 255, far = ksb >= far_from;
+    const float scale = score_scale(c_bits, ksb), grow = far ? 1.f : scale;
     const int base = p * kPage8 + 16 * g;   // the lane's first token
     float s[16];
 #pragma unroll
@@ -416,14 +416,12 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
     const float vscale = page_scale(vs) * kLower;
     if ((now.missing || none_k || vs == 255) && p * kPage8 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
     const bool cut = p * kPage8 + kPage8 > least;   // some query does not see the whole page
-    const bool far = __any(far_page(most_q, grow));
     if (cut || far) {
       int left = limit - base;
       pin_value(left);
-      const float first = far ? grow : 1.f;
+      const float first = far ? scale : 1.f;
 #pragma unroll
       for (int i = 0; i < 16; i++) s[i] = i < left ? s[i] * first : -__builtin_inff();
-      grow = far ? 1.f : grow;
     }
     float mx = s[0];
 #pragma unroll
@@ -639,13 +637,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
   if (p0 >= p1 && split > 0) return;   // the join knows that there is no such part
 
   const float c = soft_scale(a);
+  const int c_bits = __builtin_amdgcn_readfirstlane(__float_as_int(c));
   V8 q[NJ];
+  float q_sum = 0.f;
   {
     const T* qp = (const T*)a.q + b * a.qs[0] + (int64_t)(row / a.G) * a.qs[1] + (int64_t)(h * a.G + row % a.G) * a.qs[2];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) q[j] = query8<T>(a, qp, 16 * j + 8 * hh, real);
+    for (int j = 0; j < NJ; j++) q[j] = query8<T>(a, qp, 16 * j + 8 * hh, real, q_sum);
   }
-  float most_q = 0.f;
+  int far_from = 0;
   f32x16 acc[NT];
 #pragma unroll
   for (int d = 0; d < NT; d++)
@@ -756,17 +756,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
       for (int e = 0; e < 16; e++) s[t][e] = sv[t][e];
     const int base = p * kPage8 + 16 * hh;   // score e of tile t is token base + 32 t + e
     if (missing && p * kPage8 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
-    float kc = score_scale(c, ksb);
-    const bool far = far_page(most_q, kc);
+    const bool far = ksb >= far_from;
+    const float scale = score_scale(c_bits, ksb), kc = far ? 1.f : scale;
     if (p * kPage8 + kPage8 > least || far) {
       int left = limit - base;
       pin_value(left);
-      const float first = far ? kc : 1.f;
+      const float first = far ? scale : 1.f;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) s[t][e] = 32 * t + e < left ? s[t][e] * first : -__builtin_inff();
-      kc = far ? 1.f : kc;
     }
     float mx = max3_f(s[0][0], s[1][0], s[0][1]);
     mx = max3_f(mx, s[1][1], s[1][1]);
@@ -843,7 +842,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attend8_
     int page = entry(p0), next = entry(p0 + 1);
     int64_t at = place(page);
     load(at);
-    most_q = most_score(q, 2);
+    far_from = far_byte(q_sum, 2, c);
     const int first = __builtin_amdgcn_readfirstlane(vs);
     unit = top = max(first == 255 ? 127 : first, 1);
     sums = unit;
