@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
   int to = scale_byte(amax);
   const bool rises = lo > 0 && to > was;
   if (lo > 0 && to < was) to = was;
-  // (254, which no append writes by itself, may be an older page's: its inverse, 2^-127, is a subnormal number.)
+  // (254, which no append makes, may be an older page's: its inverse, 2^-127, is a subnormal number.)
   const float inv = to < 254 ? inverse_of(to) : __int_as_float(0x00400000);
   if (tid == 0) *scale = (uint8_t)to;
   if (which == 0) {
@@ -211,7 +211,7 @@ __device__ __forceinline__ int key_limit(const Attend8Args& a, int len, int64_t 
 // The softmax scale's size, in powers of two (1 for a scale of 0); its sign, or 0, is the queries'.
 __device__ __forceinline__ float soft_scale(const Attend8Args& a) { return a.scale == 0.f ? 1.f : fabsf(a.scale); }
 
-// A page's scale, any E8M0 byte (append writes 1 to 254); infinity for 255.
+// A page's scale, any E8M0 byte (append makes 1 to 247); infinity for 255.
 __device__ __forceinline__ float any_scale(int byte) { return byte ? scale_of(byte) : __int_as_float(0x00400000); }
 
 // That and the keys' scale (c and a wave's byte) go onto the scores inside the exponential: an exponent more on c, in
@@ -286,7 +286,7 @@ __device__ __forceinline__ unsigned nan_bytes(int w) {
 // the scores are done, the next values when the sums are. (Two whole pages in registers left one wave a
 // SIMD at head width 128.) The loads go through buffer descriptors that end at the page, or at nothing
 // behind the last page, so that every round issues the same loads and waits for the older half only. (One
-// query of 8 x 4 heads of 128 for each of 32 sequences of up to 8,192 tokens 64 us and 5 to join the parts,
+// query of 8 x 4 heads of 128 for each of 32 sequences of up to 8,192 tokens 63 us and 5 to join the parts,
 // 5.4 TB/s; with a page's loads issued where they are used 108.)
 constexpr int kAttendWaves = 4;
 
@@ -584,7 +584,8 @@ __global__ __launch_bounds__(64 * kAttendWaves, D == 256 ? 1 : D == 128 ? 2 : 3)
 // The keys' scale goes with the softmax's into the exponential's argument (whose sign goes into the queries).
 // The values' goes into their widening, exactly (see `unit` below), so that the products add to the running
 // sums themselves. (Scaled and added behind each page's products: 2,048 causal queries of 8 x 4 heads of 128
-// at the end of 8,192 tokens 396 us, so 348 to 365, 870 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 140 and 129.)
+// behind 8,192 tokens 396 us, so 345 to 360, 860 to 900 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 140 and 129,
+// 118 with the join now; of 256 510 and 580 TF/s.)
 //
 // What bounds it is issue: at head width 64 a page of 32 rows takes a SIMD 1,560 cycles, of which products 512
 // and 32 exponentials, their arguments, maxima, sums and conversions 880, only 150 of them at once -- with two

@@ -127,7 +127,8 @@ __device__ __forceinline__ void tile_of(unsigned l, unsigned nt, unsigned mt, un
 // latencies, not by any rate. Here a workgroup's W waves take blocks of k of their own: each has a ring of
 // S blocks (32 FN outputs + 32 FM rows of 128 bytes, swizzled as below), no barrier until the end, and the
 // sums of the whole tile, which are added through LDS in wave order.
-// (64 x 4,096 x 4,096 7.4 us, 18 with the shared blocks of the next kernel; 77 x 768 x 512 4.6 and 5.7.)
+// (64 x 4,096 x 4,096 7.4 us, 18 with the shared blocks of the next kernel; 77 x 768 x 512 4.6 and 5.7. With a few rows
+// most of a block's places are empty, and 4,096 outputs are 128 workgroups, on half of the CUs: 4 x 4,096 x 4,096 6.0.)
 template <int FN, int FM, int W, int S>
 struct SplitTile {
   static constexpr int TN = 32 * FN, TM = 32 * FM;
