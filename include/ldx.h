@@ -421,10 +421,10 @@ int ldx_group_norm_source_half(const void* x, int64_t x_batch_stride, int64_t x_
 #define LDX_PAGE8 64
 
 /* s = T(x + residual) (without a residual x itself); y = s / sqrt(mean(s^2) + eps) * gamma,
- * squares summed in fp32, at most 32 at a time, and those sums in fp64; rounded to T (y) or written as 8-bit rows (codes, scales): one of the
- * two. sum (may be NULL) receives s and may be x or residual; y may be x. x, residual, sum
- * and y are of type dtype (T) with contiguous features, any alignment; gamma fp32, eps at
- * least 1e-30. Rows whose squares pass fp32 although their values do not are normalised from
+ * squares summed in fp32, at most 32 at a time, and those sums in fp64; rounded to T (y) or
+ * written as 8-bit rows (codes, scales): one of the two. sum (may be NULL) receives s and may
+ * be x or residual; y may be x. x, residual, sum and y are of type dtype (T) with contiguous
+ * features, any alignment; gamma fp32, eps at least 1e-30. Rows whose squares pass fp32 although their values do not are normalised from
  * scaled squares. */
 typedef struct ldx_rms_norm_args {
   int64_t rows;
@@ -452,7 +452,8 @@ int ldx_quantize8(const void* x, int64_t x_pitch, int64_t rows, int32_t features
  * the terms' magnitudes (about 1.5e-5 of the result's size for ordinary data). An fp32 y is
  * summed from the operands as bf16 values, which hold them exactly but for digits below 2^-133
  * and values of 2^128 and more (infinite). Scale bytes may be any: 0 is 2^-127, 255 makes NaN
- * of its row's or output's results. residual and y are of type dtype; bias fp32. At most 2^22 features; pitches of codes and scales at most 2^22. */
+ * of its row's or output's results. residual and y are of type dtype; bias fp32. At most 2^22
+ * features; pitches of codes and scales at most 2^22. */
 typedef struct ldx_dense8_args {
   int64_t rows;
   int32_t features, out_features;
@@ -518,7 +519,8 @@ int ldx_cache8_append(const ldx_cache8_append_args* args, void* stream);
  * that sees no token gets 0. Tokens that a query does not see do not touch its result, NaN
  * among them. A page that the cache does not have, or with a scale of NaN, gives NaN to the
  * queries that see it, a length past the table to the whole sequence. Where pages' value scales
- * are more than 2^63 apart, what is below 2^-83 of the largest values may be lost. o may be q.
+ * are more than 2^63 apart, what is below 2^-83 of the largest values may be lost; values are
+ * summed before they are divided, so that sums past fp32 are infinite. o may be q.
  * Workspace: partial results where a sequence is split over workgroups,
  * ldx_cache8_attention_workspace_bytes of them, 256 MiB at most; with less nothing is split. */
 typedef struct ldx_cache8_attention_args {
