@@ -541,6 +541,118 @@ int ldx_cache8_attention(const ldx_cache8_attention_args* args, void* stream);
  * alone: 16, each wave reading pages of its own, or 128, which share them. */
 int ldx_cache8_attention_rows(const ldx_cache8_attention_args* args);
 
+/* ------------------------------------------------------------ rotation of heads ------
+ * No counterpart in the reference.
+ *
+ * Queries and keys before an attention: for each head the root-mean-square norm of its channels
+ * where a gamma is given, f = x / sqrt(mean(x^2) + eps) * gamma, then the position rotation: the
+ * head's channels are sections, one for each axis of positions (axis_dims[i] channels, even, in
+ * order; what is left behind them stays as it is), and pair i of a section, channels (i, i + dim /
+ * 2) of it, or (2 i, 2 i + 1) where interleaved, turns by positions[axis] * turns[pair] full
+ * turns, turns holding all sections' pairs one after another (fp64; theta^(-2 i / dim) / (2 pi) for
+ * the usual frequencies). Angles are reduced in fp64, so that any position has its own; norm and
+ * rotation are fp32, rounded once to dtype. q, k and outputs: (batch, token, head) strides in
+ * elements, contiguous channels; an output may be its input. positions: int32, device, (axis,
+ * batch, token) strides. k_heads may be 0. head_dim even, at most 512; eps at least 1e-30. Heads
+ * whose squares pass fp32 although their values do not are normalised from scaled squares. */
+#define LDX_ROTARY_AXES 4
+typedef struct ldx_rotate_heads_args {
+  int32_t batch, tokens, q_heads, k_heads, head_dim, dtype;
+  const void* q; int64_t q_stride[3];
+  void* q_out; int64_t q_out_stride[3];
+  const void* k; int64_t k_stride[3];
+  void* k_out; int64_t k_out_stride[3];
+  const float* q_gamma;
+  const float* k_gamma;
+  float eps;
+  int32_t axes;
+  int32_t axis_dims[LDX_ROTARY_AXES];
+  int32_t interleaved;
+  const int32_t* positions; int64_t position_stride[3];
+  const double* turns;
+} ldx_rotate_heads_args;
+int ldx_rotate_heads(const ldx_rotate_heads_args* args, void* stream);
+
+/* ------------------------------------------------------------ 4-bit cache ------------
+ * No counterpart in the reference.
+ *
+ * A cache of keys and values in pages of LDX_PAGE4 tokens: OCP e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6, sign in the top bit), two channels in a byte, the even one in its lower half, and one scale
+ * byte b (E8M0, 2^(b - 127), 255 NaN) for each LDX_BLOCK4 channels of a token. k and v: codes (pages,
+ * heads, 64, head_dim / 2), scales (pages, heads, head_dim / 32, 64). All contiguous and aligned to
+ * 16 bytes. head_dim 32, 64, 128 or 256. A sequence's pages stand in its row of `table` (int32,
+ * device; `width` pages a row), its token t in page table[b][t / 64] at t % 64. */
+#define LDX_BLOCK4 32
+#define LDX_PAGE4 64
+typedef struct ldx_cache4 {
+  void* k; void* v;
+  void* k_scales; void* v_scales;
+  int32_t pages, heads, head_dim;
+} ldx_cache4;
+
+/* Writes tokens 0..counts[b] (counts NULL: all `tokens`) of k and v (batch, token, head strides
+ * in elements, contiguous channels, type dtype) at positions starts[b].. of each sequence. A
+ * block takes the least scale b from 1 to 252 with which its largest magnitude is at most 6 * 2^(b -
+ * 127), 127 if it is zero; codes are rounded to nearest even, magnitudes past 6 * 2^125 are held
+ * as that. A block with a NaN or an infinity gets 255. Other tokens stay as they are, so sequences may
+ * share a page as long as they write different tokens of it. Nothing is written of a sequence with starts[b] < 0, past the
+ * table's width, or in a page that the cache does not have. */
+typedef struct ldx_cache4_append_args {
+  ldx_cache4 cache;
+  int32_t batch, tokens;
+  const void* k; int64_t k_stride[3];
+  const void* v; int64_t v_stride[3];
+  int32_t dtype;
+  const int32_t* table; int64_t table_pitch; int32_t width;
+  const int32_t* starts;
+  const int32_t* counts;
+} ldx_cache4_append_args;
+int ldx_cache4_append(const ldx_cache4_append_args* args, void* stream);
+
+/* Reads tokens starts[b] .. starts[b] + tokens (starts NULL: from 0) of each sequence into k and v
+ * (batch, token, head strides, contiguous channels, type dtype), rounded to it. Rows of tokens
+ * before 0 or from lengths[b] on are zeros with `fill`, left as they were without; rows in a page that
+ * the cache does not have or past the table's width are NaN. */
+typedef struct ldx_cache4_read_args {
+  ldx_cache4 cache;
+  int32_t batch, tokens;
+  void* k; int64_t k_stride[3];
+  void* v; int64_t v_stride[3];
+  int32_t dtype;
+  const int32_t* table; int64_t table_pitch; int32_t width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int32_t fill;
+} ldx_cache4_read_args;
+int ldx_cache4_read(const ldx_cache4_read_args* args, void* stream);
+
+/* o = softmax(q k^T * scale) v over a sequence's first lengths[b] tokens of the cache; with
+ * starts, query i sees no token behind starts[b] + i (causal for queries at starts[b]..). q and
+ * o: (batch, token, head) strides, contiguous channels, fp16 or bf16; q_heads a multiple of
+ * the cache's heads, query head j reads the cache's head j / (q_heads / heads). Scores, softmax and
+ * sums are fp32; keys and values enter the products exactly, queries too, probabilities with 16 bits.
+ * A query that sees no token gets 0. Tokens that a query does not see do not touch its result, NaN
+ * among them. A page that the cache does not have, or a key of NaN, gives NaN to the queries that see
+ * it, a value of NaN to their channels of its block, a length past the table to the whole
+ * sequence. Scale bytes of 253 and 254, which append does not write, may count as NaN. Values are summed before
+ * they are divided, with weights of up to 2^8, so that sums past fp32 are infinite. o may be q.
+ * Workspace: partial results where a sequence is split over workgroups,
+ * ldx_cache4_attention_workspace_bytes of them, 256 MiB at most; with less nothing is split. */
+typedef struct ldx_cache4_attention_args {
+  ldx_cache4 cache;
+  int32_t batch, q_heads, q_len;
+  const void* q; int64_t q_stride[3];
+  void* o; int64_t o_stride[3];
+  int32_t dtype;
+  float scale;
+  const int32_t* table; int64_t table_pitch; int32_t width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  void* workspace; size_t workspace_bytes;
+} ldx_cache4_attention_args;
+size_t ldx_cache4_attention_workspace_bytes(const ldx_cache4_attention_args* args);
+int ldx_cache4_attention(const ldx_cache4_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

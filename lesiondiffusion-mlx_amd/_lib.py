@@ -24,6 +24,9 @@ DTYPE_F32 = 1
 DTYPE_BF16 = 2
 BLOCK8 = 128                         # LDX_BLOCK8
 PAGE8 = 64                           # LDX_PAGE8
+BLOCK4 = 32                          # LDX_BLOCK4
+PAGE4 = 64                           # LDX_PAGE4
+ROTARY_AXES = 4                      # LDX_ROTARY_AXES
 GROUP_NORM_SCRATCH_BYTES = 4 << 20   # LDX_GROUP_NORM_SCRATCH_BYTES
 
 c_i32 = ctypes.c_int32
@@ -145,6 +148,48 @@ class Cache8AttentionArgs(ctypes.Structure):
     ]
 
 
+class RotateHeadsArgs(ctypes.Structure):
+    """Mirror of ``ldx_rotate_heads_args``."""
+
+    _fields_ = [
+        ("batch", c_i32), ("tokens", c_i32), ("q_heads", c_i32), ("k_heads", c_i32), ("head_dim", c_i32), ("dtype", c_i32),
+        ("q", c_vp), ("q_stride", c_i64 * 3), ("q_out", c_vp), ("q_out_stride", c_i64 * 3),
+        ("k", c_vp), ("k_stride", c_i64 * 3), ("k_out", c_vp), ("k_out_stride", c_i64 * 3),
+        ("q_gamma", c_vp), ("k_gamma", c_vp), ("eps", c_f32),
+        ("axes", c_i32), ("axis_dims", c_i32 * ROTARY_AXES), ("interleaved", c_i32),
+        ("positions", c_vp), ("position_stride", c_i64 * 3), ("turns", c_vp),
+    ]
+
+
+class Cache4Block(ctypes.Structure):
+    """Mirror of ``ldx_cache4``."""
+
+    _fields_ = list(Cache8Block._fields_)
+
+
+class Cache4AppendArgs(ctypes.Structure):
+    """Mirror of ``ldx_cache4_append_args``."""
+
+    _fields_ = [("cache", Cache4Block), *Cache8AppendArgs._fields_[1:]]
+
+
+class Cache4ReadArgs(ctypes.Structure):
+    """Mirror of ``ldx_cache4_read_args``."""
+
+    _fields_ = [
+        ("cache", Cache4Block), ("batch", c_i32), ("tokens", c_i32),
+        ("k", c_vp), ("k_stride", c_i64 * 3), ("v", c_vp), ("v_stride", c_i64 * 3), ("dtype", c_i32),
+        ("table", c_vp), ("table_pitch", c_i64), ("width", c_i32),
+        ("lengths", c_vp), ("starts", c_vp), ("fill", c_i32),
+    ]
+
+
+class Cache4AttentionArgs(ctypes.Structure):
+    """Mirror of ``ldx_cache4_attention_args``."""
+
+    _fields_ = [("cache", Cache4Block), *Cache8AttentionArgs._fields_[1:]]
+
+
 # name -> (restype, argtypes); every function declared in include/ldx.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ldx_last_error": (ctypes.c_char_p, []),
@@ -202,9 +247,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ldx_cache8_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Cache8AttentionArgs)]),
     "ldx_cache8_attention_rows": (c_i32, [ctypes.POINTER(Cache8AttentionArgs)]),
     "ldx_cache8_attention": (c_i32, [ctypes.POINTER(Cache8AttentionArgs), c_vp]),
+    "ldx_rotate_heads": (c_i32, [ctypes.POINTER(RotateHeadsArgs), c_vp]),
+    "ldx_cache4_append": (c_i32, [ctypes.POINTER(Cache4AppendArgs), c_vp]),
+    "ldx_cache4_read": (c_i32, [ctypes.POINTER(Cache4ReadArgs), c_vp]),
+    "ldx_cache4_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Cache4AttentionArgs)]),
+    "ldx_cache4_attention": (c_i32, [ctypes.POINTER(Cache4AttentionArgs), c_vp]),
 }
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 
 def _load() -> ctypes.CDLL:

@@ -1,0 +1,648 @@
+// A cache of keys and values held in 4 bits, in pages of 64 tokens: OCP e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6
+// and their negatives) with a power of two (E8M0) for each 32 channels of a token. Writing new tokens, reading
+// them back, and the attention that reads the cache.
+//
+// Keys and values lie alike: codes (pages, H, 64, D / 2), two channels in a byte, the even one in its lower half,
+// and scales (pages, H, D / 32, 64), a block's tokens side by side: a lane of the attention reads those of 16
+// tokens at once. A scale per token is what lets a token be written without touching older ones, which in 4 bits
+// would lose too much by being rounded again.
+#include "attend_parts.h"
+
+namespace ldx {
+namespace {
+
+constexpr int kPage4 = LDX_PAGE4;
+constexpr int kBlock4 = LDX_BLOCK4;
+static_assert(kPage4 == kPage8, "attend_parts.h counts pages of 64 tokens");
+
+// The scale byte of a block with largest magnitude amax = 1.m * 2^(E - 127): the least b from 1 on with amax <= 6 *
+// 2^(b - 127) = 1.5 * 2^(b - 125). Zeros get 127. At most 252: values past 6 * 2^125, which the next scale's larger
+// codes would round to 2^128, are held as that. NaN and infinite blocks get 255, which is NaN.
+__device__ __forceinline__ int scale4_byte(float amax) {
+  const int bits = __float_as_int(amax);
+  if (bits >= 0x7f800000) return 255;
+  if (bits == 0) return 127;
+  const int b = (bits >> 23) - 2 + ((bits & 0x7fffff) > 0x400000 ? 1 : 0);
+  return min(max(b, 1), 252);
+}
+
+// Eight values times the inverse scale as eight codes (round to nearest even, magnitudes past 6 as 6).
+__device__ __forceinline__ unsigned encode8(const float (&f)[8], float inv) {
+  unsigned w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0] * inv, f[1] * inv, 1.f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2] * inv, f[3] * inv, 1.f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4] * inv, f[5] * inv, 1.f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6] * inv, f[7] * inv, 1.f, 3);
+}
+
+// The widening conversions take a scale's exponent bits alone, as E8M0 (0 is 2^-127, 255 gives NaN): a scale byte goes
+// there by one rotation of the word that holds it, whatever lands beside it.
+__device__ __forceinline__ float scale_at(int word, int byte) {
+  return __int_as_float((int)__builtin_amdgcn_alignbit((unsigned)word, (unsigned)word, 8 * byte + 9));
+}
+
+// ------------------------------------------------------------------------------ append and read
+
+struct Store4Args {
+  uint8_t* codes[2];     // keys, values (pages, H, 64, D / 2)
+  uint8_t* scales[2];    // (pages, H, D / 32, 64)
+  void* x[2];            // what is appended, or where it is read to
+  int64_t st[2][3];      // its batch, token, head strides
+  int pages, H, tokens;
+  const int32_t* table; int64_t tp; int width;
+  const int32_t* starts;
+  const int32_t* counts;   // append: tokens of each sequence
+  const int32_t* lengths;  // read: tokens that a sequence holds
+  bool fill;               // read: zeros behind them
+};
+
+// A page's part of the tokens that a workgroup (a head's keys or values) takes.
+struct Span {
+  int64_t first;   // position of the page's first token
+  int lo, hi;      // places of it
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void append4_kernel(Store4Args a) {
+  constexpr int UNITS = D / 8;   // eight channels, a lane each; four lanes hold a block
+  const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, tid = threadIdx.x;
+  const int start = a.starts[b];
+  const int n = a.counts ? min(a.counts[b], a.tokens) : a.tokens;
+  if (start < 0 || n <= 0) return;
+  const int64_t end = (int64_t)start + n, slot = start / kPage4 + (int64_t)blockIdx.x, first = slot * kPage4;
+  if (first >= end || slot >= a.width) return;
+  const int page = a.table[b * a.tp + slot];
+  if ((unsigned)page >= (unsigned)a.pages) return;
+  const int lo = (int)max(start - first, (int64_t)0), hi = (int)min(end - first, (int64_t)kPage4);
+  const int64_t at = (int64_t)page * a.H + h, tok = a.st[which][1];
+  uint8_t* codes = a.codes[which] + at * (kPage4 * D / 2);
+  uint8_t* scales = a.scales[which] + at * (kPage4 * D / kBlock4);
+  const T* src = (const T*)a.x[which] + b * a.st[which][0] + (first + lo - start) * tok + h * a.st[which][2];
+  for (int c = tid; c < (hi - lo) * UNITS; c += 256) {
+    const int t = c / UNITS, u = c % UNITS;
+    float f[8];
+    load8(src + t * tok + u * 8, f);
+    float amax = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      amax = fmaxf(amax, fabsf(f[i]));
+      nan |= f[i] != f[i];
+    }
+    if (nan) amax = __builtin_inff();
+    amax = fmaxf(amax, dpp_f<0xB1>(amax));   // quad_perm 1 0 3 2
+    amax = fmaxf(amax, dpp_f<0x4E>(amax));   // quad_perm 2 3 0 1
+    const int s = scale4_byte(amax);
+    *reinterpret_cast<unsigned*>(codes + (lo + t) * (D / 2) + u * 4) = s == 255 ? 0u : encode8(f, inverse_of(s));
+    if (u % 4 == 0) scales[u / 4 * kPage4 + lo + t] = (uint8_t)s;
+  }
+}
+
+// Eight codes times their scale in T.
+__device__ __forceinline__ void decode8(unsigned w, float s, f16* p) {
+  f16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1),
+                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3)};
+  __builtin_memcpy(p, v, sizeof(v));
+}
+__device__ __forceinline__ void decode8(unsigned w, float s, bf16* p) {
+  bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1),
+                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3)};
+  __builtin_memcpy(p, v, sizeof(v));
+}
+__device__ __forceinline__ void decode8(unsigned w, float s, float* p) {
+  f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1),
+                __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3)};
+  __builtin_memcpy(p, v, sizeof(v));
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void read4_kernel(Store4Args a) {
+  constexpr int UNITS = D / 8;
+  const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, tid = threadIdx.x;
+  const int64_t start = a.starts ? a.starts[b] : 0;
+  // Row i is token start + i; the workgroup takes rows of one page, the first of them maybe less than whole.
+  const int64_t slot = (start >= 0 ? start / kPage4 : -((-start + kPage4 - 1) / kPage4)) + blockIdx.x, first = slot * kPage4;
+  const int64_t lo = max(start, first), hi = min(start + a.tokens, first + kPage4);
+  if (lo >= hi) return;
+  const int64_t len = a.lengths[b];
+  const bool within = slot >= 0 && slot < a.width;
+  const int page = within ? a.table[b * a.tp + slot] : -1;
+  const bool missing = (unsigned)page >= (unsigned)a.pages;
+  const int64_t at = (int64_t)(missing ? 0 : page) * a.H + h, tok = a.st[which][1];
+  const uint8_t* codes = a.codes[which] + at * (kPage4 * D / 2);
+  const uint8_t* scales = a.scales[which] + at * (kPage4 * D / kBlock4);
+  T* dst = (T*)a.x[which] + b * a.st[which][0] + h * a.st[which][2];
+  for (int c = tid; c < (int)(hi - lo) * UNITS; c += 256) {
+    const int u = c % UNITS;
+    const int64_t t = lo + c / UNITS;
+    const bool held = t >= 0 && t < len;
+    if (!held && !a.fill) continue;
+    const int place = (int)(t - first);
+    const unsigned w = held && !missing ? *reinterpret_cast<const unsigned*>(codes + place * (D / 2) + u * 4) : 0u;
+    const int s = !held ? 127 : missing ? 255 : scales[u / 4 * kPage4 + place];
+    T v[8];
+    decode8(w, __int_as_float(s << 23), v);
+    __builtin_memcpy(dst + (t - start) * tok + u * 8, v, sizeof(v));
+  }
+}
+
+template <typename T, bool READ>
+void launch_store(const Store4Args& a, int D, dim3 grid, hipStream_t st) {
+  if constexpr (READ) {
+    if (D == 32) hipLaunchKernelGGL((read4_kernel<T, 32>), grid, dim3(256), 0, st, a);
+    else if (D == 64) hipLaunchKernelGGL((read4_kernel<T, 64>), grid, dim3(256), 0, st, a);
+    else if (D == 128) hipLaunchKernelGGL((read4_kernel<T, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((read4_kernel<T, 256>), grid, dim3(256), 0, st, a);
+  } else {
+    if (D == 32) hipLaunchKernelGGL((append4_kernel<T, 32>), grid, dim3(256), 0, st, a);
+    else if (D == 64) hipLaunchKernelGGL((append4_kernel<T, 64>), grid, dim3(256), 0, st, a);
+    else if (D == 128) hipLaunchKernelGGL((append4_kernel<T, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((append4_kernel<T, 256>), grid, dim3(256), 0, st, a);
+  }
+}
+
+// ------------------------------------------------------------------------------------- attention
+
+struct Attend4Args {
+  const uint8_t* k; const uint8_t* v;
+  const uint8_t* ks; const uint8_t* vs;
+  int pages, H;
+  const void* q; int64_t qs[3];
+  void* o; int64_t os[3];
+  int G, lq, rows;       // query heads per cache head; queries; G * lq
+  float scale;           // times log2(e)
+  const int32_t* table; int64_t tp; int width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int splits, chunk;     // parts of a sequence; least pages of a part
+  int tile;              // rows of a workgroup
+  float* part;           // splits > 1: [b][h][row][split] of D sums, then of (m, l)
+};
+
+__device__ __forceinline__ f32x4 mfma16b(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// Eight codes times a scale as bf16, which holds them exactly.
+__device__ __forceinline__ bf16x8 widen8(unsigned w, float s) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
+  return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Two codes (byte SEL of a word) times a scale, as a word of two bf16.
+template <int SEL>
+__device__ __forceinline__ unsigned widen2(unsigned w, float s) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, SEL));
+}
+__device__ __forceinline__ unsigned widen2(unsigned w, float s, int sel) {
+  return sel == 0 ? widen2<0>(w, s) : sel == 1 ? widen2<1>(w, s) : sel == 2 ? widen2<2>(w, s) : widen2<3>(w, s);
+}
+
+// A number as two bf16: its upper half, cut off, and what is left, rounded: 16 bits of it.
+__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
+  const unsigned a = (unsigned)__float_as_int(x), b = (unsigned)__float_as_int(y);
+  hi = __builtin_amdgcn_perm(b, a, 0x07060302);
+  const bf16x2 l = {(bf16)(x - __int_as_float((int)(a & 0xffff0000u))), (bf16)(y - __int_as_float((int)(b & 0xffff0000u)))};
+  lo = __builtin_bit_cast(unsigned, l);
+}
+
+// The 0x80 bit of every scale byte of 253 and more: NaN, and blocks whose values may pass fp32.
+__device__ __forceinline__ unsigned beyond_bytes(int w) {
+  return (((unsigned)w & 0x7f7f7f7fu) + 0x03030303u) & (unsigned)w & 0x80808080u;
+}
+
+// A query's reference for its exponentials follows its maximum only where that passes it by more than this (in
+// powers of two): the sums are seldom multiplied then.
+constexpr float kLag = 8.f;
+constexpr int kWaves4 = 4;
+
+// S^T = K Q^T per page on 16 x 16 x 32 products: lane l holds query column l % 16, g = l / 16. Key row m of key tile t
+// is the page's token 16 (m / 4) + 4 t + m % 4, so that the scores a lane receives (rows 4 g + i, tiles t) are those
+// of tokens 16 g + 4 t + i, sixteen in a row, and the probabilities go into the second product as they lie. There lane l
+// holds the values of the same tokens for channels l % 16 * (D / 16) .. of each, D / 32 bytes a token, of which tile d
+// of O^T takes the d-th: eight tokens' bytes are widened and their 16-bit halves sorted by channel.
+//
+// Operands are bf16, which holds a code times any scale exactly; a 16-bit query of more digits and the probabilities
+// go in as two of them, 16 bits in all. Sums are fp32.
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves4, D == 256 ? 1 : 2) void attend4_kernel(Attend4Args a) {
+  constexpr int ND = D / 16;              // channel tiles; channels of a lane's values
+  constexpr int NK = D / 32;              // products per key tile; words of a lane's part of a key
+  constexpr int QP = sizeof(T) == 2 && __is_same(T, f16) ? 2 : 1;   // parts of a query
+  constexpr int NB = D == 256 ? 2 : 1;    // blocks of a lane's part of a key
+  constexpr int VW = D == 256 ? 2 : 1;    // words of a lane's part of a token's values
+  __shared__ float sm[kWaves4][16], sl[kWaves4][16];
+  __shared__ __align__(16) float sacc[kWaves4][16][D + 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int b = blockIdx.z, split = blockIdx.x % a.splits, tiles = (a.rows + 15) / 16, tile = blockIdx.x / a.splits;
+  const int h = tile / tiles, row0 = tile % tiles * 16;
+  const int row = row0 + r;
+  const bool real = row < a.rows;
+  const int raw = a.lengths[b];
+  const bool too_long = raw > (int64_t)a.width * kPage4;
+  const int len = too_long || raw < 0 ? 0 : raw;
+  const int64_t start = a.starts ? a.starts[b] : 0;
+  const int limit = real ? key_limit(a, len, start, row) : 0;
+  const int least = key_limit(a, len, start, row0);                                // the tile's first row
+  const int most = key_limit(a, len, start, min(row0 + 15, a.rows - 1));           // and its last
+  const int npages = (most + kPage4 - 1) / kPage4;
+  const int chunk = max((npages + a.splits - 1) / a.splits, a.chunk);
+  const int p0 = a.splits > 1 ? split * chunk : 0, p1 = a.splits > 1 ? min(p0 + chunk, npages) : npages;
+  if (p0 >= p1 && split > 0) return;   // the join knows that there is no such part
+
+  bf16x8 q[QP][NK];
+  {
+    const T* qp = (const T*)a.q + b * a.qs[0] + (int64_t)(row / a.G) * a.qs[1] + (int64_t)(h * a.G + row % a.G) * a.qs[2];
+#pragma unroll
+    for (int j = 0; j < NK; j++) {
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (real) load8(qp + D / 4 * g + 8 * j, f);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const bf16 hi = (bf16)f[e];
+        q[0][j][e] = hi;
+        if constexpr (QP == 2) q[1][j][e] = (bf16)(f[e] - (float)hi);
+      }
+    }
+  }
+
+  float acc[ND][4];
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[d][i] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;
+  int poison = 0;   // bit i: the lane's query sees a value of NaN in block i of its channels' ones
+
+  const int32_t* table = a.table + b * a.tp;
+  const unsigned koff = (unsigned)(16 * (r >> 2) + (r & 3)) * (D / 2) + (D / 8) * g;
+  const unsigned voff = (unsigned)(16 * g) * (D / 2) + (D / 32) * r;
+  const unsigned ksoff = (unsigned)(D / 4 * g / kBlock4) * kPage4 + 16 * (r >> 2);
+  const unsigned vsoff = (unsigned)(ND * r / kBlock4) * kPage4 + 16 * g;
+  const int kbyte = r & 3;
+  unsigned kc[4][NK];   // a page's keys
+  i32x4 ks[NB], vs;
+  unsigned vc[16][VW];  // and its values
+  struct Place {
+    int64_t at;
+    bool missing;
+  };
+  const auto place = [&](int page) {
+    const bool missing = (unsigned)page >= (unsigned)a.pages;
+    return Place{(int64_t)(missing ? 0 : page) * a.H + h, missing};
+  };
+  const auto load_k = [&](Place t, int p) {
+    const __amdgpu_buffer_rsrc_t kr = make_rsrc(a.k + t.at * (kPage4 * D / 2), p < p1 ? (unsigned)(kPage4 * D / 2) : 0u);
+    const __amdgpu_buffer_rsrc_t sr = make_rsrc(a.ks + t.at * (kPage4 * NK), p < p1 ? (unsigned)(kPage4 * NK) : 0u);
+#pragma unroll
+    for (int i = 0; i < NB; i++) ks[i] = buffer_load16<i32x4>(sr, ksoff, i * kPage4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (NK == 1) {
+        kc[i][0] = __builtin_amdgcn_raw_buffer_load_b32(kr, koff, 4 * i * (D / 2), 0);
+      } else if constexpr (NK == 2) {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(kr, koff, 4 * i * (D / 2), 0);
+        kc[i][0] = w[0];
+        kc[i][1] = w[1];
+      } else {
+#pragma unroll
+        for (int j = 0; j < NK / 4; j++) {
+          const u32x4 w = buffer_load16<u32x4>(kr, koff, 4 * i * (D / 2) + 16 * j);
+#pragma unroll
+          for (int x = 0; x < 4; x++) kc[i][4 * j + x] = w[x];
+        }
+      }
+    }
+  };
+  const auto load_v = [&](Place t, int p) {
+    const __amdgpu_buffer_rsrc_t vr = make_rsrc(a.v + t.at * (kPage4 * D / 2), p < p1 ? (unsigned)(kPage4 * D / 2) : 0u);
+    const __amdgpu_buffer_rsrc_t sr = make_rsrc(a.vs + t.at * (kPage4 * NK), p < p1 ? (unsigned)(kPage4 * NK) : 0u);
+    vs = buffer_load16<i32x4>(sr, vsoff);
+#pragma unroll
+    for (int x = 0; x < 16; x++) {
+      if constexpr (D == 32) vc[x][0] = __builtin_amdgcn_raw_buffer_load_b8(vr, voff, x * (D / 2), 0);
+      else if constexpr (D == 64) vc[x][0] = __builtin_amdgcn_raw_buffer_load_b16(vr, voff, x * (D / 2), 0);
+      else if constexpr (D == 128) vc[x][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, voff, x * (D / 2), 0);
+      else {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(vr, voff, x * (D / 2), 0);
+        vc[x][0] = w[0];
+        vc[x][VW - 1] = w[1];
+      }
+    }
+  };
+
+  // Page numbers are known two rounds ahead; behind the last page the last one's is read again.
+  const int last = max(p1 - 1, 0);
+  const auto entry = [&](int p) { return table_entry(table, min(p, last)); };
+  int p = p0 + wave;
+  Place now = place(entry(p)), next = place(entry(p + kWaves4));
+  int after = entry(p + 2 * kWaves4);
+  load_k(now, p);
+  load_v(now, p);
+  for (; p < p1; p += kWaves4) {
+    const int base = p * kPage4 + 16 * g;   // the lane's first token
+    float s[16];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NK; j++) {
+        const float f = __int_as_float((int)__builtin_amdgcn_alignbit((unsigned)ks[j * NB / NK][t], (unsigned)ks[j * NB / NK][t], 8 * kbyte + 9));
+        const bf16x8 kv = widen8(kc[t][j], f);
+#pragma unroll
+        for (int x = 0; x < QP; x++) o = mfma16b(kv, q[x][j], o);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[4 * t + i] = o[i] * a.scale;
+      __builtin_amdgcn_sched_barrier(0);   // one tile's widened codes at a time
+    }
+    load_k(next, p + kWaves4);
+    __builtin_amdgcn_sched_barrier(0);
+    if (now.missing && p * kPage4 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
+    const bool cut = p * kPage4 + kPage4 > least;   // some query does not see the whole page
+    if (cut) {
+      int left = limit - base;
+      pin_value(left);
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[i] = i < left ? s[i] : -__builtin_inff();
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 15; i += 2) mx = max3_f(mx, s[i], s[i + 1]);
+    mx = max3_f(mx, s[15], s[15]);
+    const auto x16 = __builtin_amdgcn_permlane16_swap(__float_as_int(mx), __float_as_int(mx), false, false);
+    mx = max3_f(__int_as_float(x16[0]), __int_as_float(x16[1]), __int_as_float(x16[1]));
+    const auto x32 = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
+    const float mn = max3_f(m, __int_as_float(x32[0]), __int_as_float(x32[1]));
+    float ref = m == -__builtin_inff() ? 0.f : m;
+    if (__any(mn - m > kLag)) {
+      ref = mn == -__builtin_inff() ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[d][i] *= alpha;
+      m = mn;
+    }
+    u32x4 ph[2], pl[2];
+    float lp = 0.f;   // the page's own sum, so that small ones do not go one by one into a large one
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float e0 = __builtin_amdgcn_exp2f(s[i] - ref), e1 = __builtin_amdgcn_exp2f(s[i + 1] - ref);
+      lp += e0 + e1;
+      unsigned hi, lo;
+      split2(e0, e1, hi, lo);
+      ph[i / 8][i % 8 / 2] = hi;
+      pl[i / 8][i % 8 / 2] = lo;
+    }
+    l += lp;
+    if (cut) {
+      // Tokens that only some of the queries see may have values of NaN, and those behind the sequence anything; zero
+      // times NaN is not zero. Such blocks get a scale of 1, and the queries that see them NaN, at the end.
+      unsigned beyond = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) beyond |= beyond_bytes(vs[i]);
+      if (__any(beyond != 0)) {
+        const uint8_t* sp = a.vs + now.at * (kPage4 * NK) + (D / 4 * g / kBlock4) * kPage4;
+#pragma unroll 1
+        for (int t = 0; t < kPage4; t++)
+#pragma unroll
+          for (int i = 0; i < NB; i++)
+            if (sp[i * kPage4 + t] >= 253 && p * kPage4 + t < limit) poison |= 1 << i;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const unsigned mask = (beyond_bytes(vs[i]) >> 7) * 255u;
+          vs[i] = (int)(((unsigned)vs[i] & ~mask) | (0x7f7f7f7fu & mask));
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < ND; d += 2) {   // the two channels of a byte
+      f32x4 o0 = {acc[d][0], acc[d][1], acc[d][2], acc[d][3]}, o1 = {acc[d + 1][0], acc[d + 1][1], acc[d + 1][2], acc[d + 1][3]};
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        u32x4 v0, v1;
+#pragma unroll
+        for (int x = 0; x < 8; x += 2) {
+          const int t = 8 * u + x;
+          const unsigned e = widen2(vc[t][d / 8], scale_at(vs[t / 4], t % 4), d % 8 / 2);
+          const unsigned f = widen2(vc[t + 1][d / 8], scale_at(vs[(t + 1) / 4], (t + 1) % 4), d % 8 / 2);
+          v0[x / 2] = __builtin_amdgcn_perm(f, e, 0x05040100);
+          v1[x / 2] = __builtin_amdgcn_perm(f, e, 0x07060302);
+        }
+        const bf16x8 hi = __builtin_bit_cast(bf16x8, ph[u]), lo = __builtin_bit_cast(bf16x8, pl[u]);
+        o0 = mfma16b(__builtin_bit_cast(bf16x8, v0), hi, o0);
+        o1 = mfma16b(__builtin_bit_cast(bf16x8, v1), hi, o1);
+        o0 = mfma16b(__builtin_bit_cast(bf16x8, v0), lo, o0);
+        o1 = mfma16b(__builtin_bit_cast(bf16x8, v1), lo, o1);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        acc[d][i] = o0[i];
+        acc[d + 1][i] = o1[i];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    load_v(next, p + kWaves4);
+    __builtin_amdgcn_sched_barrier(0);
+    now = next;
+    next = place(after);
+    after = entry(p + 3 * kWaves4);
+  }
+
+  // Lane (r, g) holds channels (4 g + i) ND + d of query r.
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const bool bad = poison >> (NB == 1 ? 0 : i / 2) & 1;
+      sacc[wave][r][(4 * g + i) * ND + d] = bad ? __builtin_nanf("") : acc[d][i];
+    }
+  // l over the four lane groups of a query, then the waves' states through LDS.
+  const auto l16 = __builtin_amdgcn_permlane16_swap(__float_as_int(l), __float_as_int(l), false, false);
+  l = __int_as_float(l16[0]) + __int_as_float(l16[1]);
+  const auto l32 = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
+  l = __int_as_float(l32[0]) + __int_as_float(l32[1]);
+  if (g == 0) {
+    sm[wave][r] = m;
+    sl[wave][r] = l;
+  }
+  __syncthreads();
+  const int64_t bh = (int64_t)b * a.H + h;
+  for (int e = threadIdx.x; e < 16 * D / 4; e += 64 * kWaves4) {
+    const int er = e / (D / 4), ec = e % (D / 4) * 4, orow = row0 + er;
+    if (orow >= a.rows) continue;
+    float mt = sm[0][er];
+#pragma unroll
+    for (int w = 1; w < kWaves4; w++) mt = fmaxf(mt, sm[w][er]);
+    const float ref = mt == -__builtin_inff() ? 0.f : mt;
+    float lt = 0.f;
+    f32x4 ot = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves4; w++) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][er] - ref);
+      lt += sl[w][er] * f;
+      ot += *reinterpret_cast<const f32x4*>(&sacc[w][er][ec]) * f;
+    }
+    if (too_long) lt = __builtin_nanf("");
+    if (a.splits > 1) {
+      const int64_t at = (bh * a.rows + orow) * a.splits + split;
+      const int64_t all = (int64_t)gridDim.z * a.H * a.rows * a.splits;
+      *reinterpret_cast<f32x4*>(a.part + at * D + ec) = ot;
+      if (ec == 0) {
+        a.part[all * D + 2 * at] = ref;
+        a.part[all * D + 2 * at + 1] = lt;
+      }
+      continue;
+    }
+    put4<T>(a, b, h, orow, ec, ot, lt);
+  }
+}
+
+template <typename T, int D>
+int launch_d(const Attend4Args& a, int batch, hipStream_t st) {
+  const dim3 grid((unsigned)a.splits * (unsigned)(a.H * ((a.rows + a.tile - 1) / a.tile)), 1, (unsigned)batch);
+  hipLaunchKernelGGL((attend4_kernel<T, D>), grid, dim3(64 * kWaves4), 0, st, a);
+  launch_join<T, D>(a, (int64_t)batch * a.H * a.rows, st);
+  return check_launch("cache4_attention");
+}
+
+template <typename T>
+int launch_t(const Attend4Args& a, int D, int batch, hipStream_t st) {
+  if (D == 32) return launch_d<T, 32>(a, batch, st);
+  if (D == 64) return launch_d<T, 64>(a, batch, st);
+  if (D == 128) return launch_d<T, 128>(a, batch, st);
+  return launch_d<T, 256>(a, batch, st);
+}
+
+int check_cache(const char* what, const ldx_cache4& c) {
+  if (!c.k || !c.v || !c.k_scales || !c.v_scales) return fail("%s: null pointer", what);
+  if (c.pages < 1 || c.heads < 1 || c.heads > 8192) return fail("%s: %d pages, %d heads", what, c.pages, c.heads);
+  if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
+    return fail("%s: head_dim %d is not 32, 64, 128 or 256", what, c.head_dim);
+  if ((uintptr_t)c.k % 16 || (uintptr_t)c.v % 16 || (uintptr_t)c.k_scales % 16 || (uintptr_t)c.v_scales % 16)
+    return fail("%s: codes and scales must be aligned to 16 bytes", what);
+  return LDX_OK;
+}
+
+int check_store(const char* what, const ldx_cache4& c, int batch, int tokens, int dtype, int64_t table_pitch, int width) {
+  if (int rc = check_cache(what, c)) return rc;
+  if (dtype != LDX_DTYPE_F16 && dtype != LDX_DTYPE_BF16 && dtype != LDX_DTYPE_F32)
+    return fail("%s: dtype %d is not LDX_DTYPE_F16, LDX_DTYPE_BF16 or LDX_DTYPE_F32", what, dtype);
+  if (batch < 1 || batch > 65535 || tokens < 1 || tokens > 1 << 28 || width < 1 || width > (1 << 24))
+    return fail("%s: batch %d, %d tokens, %d pages a sequence", what, batch, tokens, width);
+  if (table_pitch < width) return fail("%s: table pitch below %d", what, width);
+  return LDX_OK;
+}
+
+// Pages that `tokens` tokens from any place on may touch, by a head's keys and values, by sequences.
+dim3 store_grid(const ldx_cache4& c, int batch, int tokens) {
+  return dim3((unsigned)((tokens + 2 * (int64_t)kPage4 - 2) / kPage4), 2 * (unsigned)c.heads, (unsigned)batch);
+}
+
+// How a call is laid out. The host knows only how many pages a table's row holds; the kernels divide the
+// pages that a sequence has.
+struct Plan {
+  int splits;   // parts that a sequence's pages may be spread over
+};
+
+constexpr int kLeastChunk = 8;   // pages of a part at least: two for each wave
+
+size_t split_bytes(const ldx_cache4_attention_args* p, int splits) {
+  if (splits < 2) return 0;
+  const size_t rows = (size_t)p->q_len * (p->q_heads / p->cache.heads);
+  return (size_t)p->batch * p->cache.heads * rows * splits * (p->cache.head_dim + 2) * sizeof(float);
+}
+
+// What partial results may take at most. (It bounds the join's launch, too.)
+constexpr size_t kMostPartBytes = (size_t)256 << 20;
+
+Plan plan_of(const ldx_cache4_attention_args* p) {
+  const int64_t heads = (int64_t)p->batch * p->cache.heads, rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
+  const int64_t most = (p->width + kLeastChunk - 1) / kLeastChunk;
+  int64_t s = 512 / (heads * ((rows + 15) / 16));
+  if (s > most) s = most;
+  if (p->width <= 32) s = 1;
+  Plan plan;
+  plan.splits = (int)(s < 1 ? 1 : s > kMostParts ? kMostParts : s);
+  return plan;
+}
+
+int check_attention(const ldx_cache4_attention_args* p) {
+  if (!p || !p->q || !p->o || !p->table || !p->lengths) return fail("cache4_attention: null pointer");
+  if (int rc = check_cache("cache4_attention", p->cache)) return rc;
+  if (p->dtype != LDX_DTYPE_F16 && p->dtype != LDX_DTYPE_BF16)
+    return fail("cache4_attention: dtype %d is not LDX_DTYPE_F16 or LDX_DTYPE_BF16", p->dtype);
+  if (p->batch < 1 || p->batch > 65535 || p->q_len < 1 || p->width < 1 || p->width > (1 << 24))
+    return fail("cache4_attention: batch %d, %d queries, %d pages a sequence", p->batch, p->q_len, p->width);
+  if (p->q_heads < 1 || p->q_heads % p->cache.heads)
+    return fail("cache4_attention: %d query heads over %d cache heads", p->q_heads, p->cache.heads);
+  const int64_t rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
+  if (rows * p->cache.heads * p->batch > 0x7fffffff || (rows + 15) / 16 * p->cache.heads > 1 << 23)   // 2^31 threads
+    return fail("cache4_attention: %d x %d queries of %d heads are more than one launch takes", p->batch, p->q_len,
+                p->q_heads);
+  if (p->table_pitch < p->width) return fail("cache4_attention: table pitch below %d", p->width);
+  if (!(p->scale > -1e30f && p->scale < 1e30f)) return fail("cache4_attention: scale %g", (double)p->scale);
+  return LDX_OK;
+}
+
+}  // namespace
+}  // namespace ldx
+
+using namespace ldx;
+
+extern "C" int ldx_cache4_append(const ldx_cache4_append_args* p, void* stream) {
+  if (!p || !p->k || !p->v || !p->table || !p->starts) return fail("cache4_append: null pointer");
+  if (int rc = check_store("cache4_append", p->cache, p->batch, p->tokens, p->dtype, p->table_pitch, p->width)) return rc;
+  const ldx_cache4& c = p->cache;
+  const Store4Args a = {{(uint8_t*)c.k, (uint8_t*)c.v}, {(uint8_t*)c.k_scales, (uint8_t*)c.v_scales},
+                        {(void*)p->k, (void*)p->v},
+                        {{p->k_stride[0], p->k_stride[1], p->k_stride[2]}, {p->v_stride[0], p->v_stride[1], p->v_stride[2]}},
+                        c.pages, c.heads, p->tokens, p->table, p->table_pitch, p->width, p->starts, p->counts, nullptr, false};
+  const dim3 grid = store_grid(c, p->batch, p->tokens);
+  if (p->dtype == LDX_DTYPE_F16) launch_store<f16, false>(a, c.head_dim, grid, as_stream(stream));
+  else if (p->dtype == LDX_DTYPE_BF16) launch_store<bf16, false>(a, c.head_dim, grid, as_stream(stream));
+  else launch_store<float, false>(a, c.head_dim, grid, as_stream(stream));
+  return check_launch("cache4_append");
+}
+
+extern "C" int ldx_cache4_read(const ldx_cache4_read_args* p, void* stream) {
+  if (!p || !p->k || !p->v || !p->table || !p->lengths) return fail("cache4_read: null pointer");
+  if (int rc = check_store("cache4_read", p->cache, p->batch, p->tokens, p->dtype, p->table_pitch, p->width)) return rc;
+  const ldx_cache4& c = p->cache;
+  const Store4Args a = {{(uint8_t*)c.k, (uint8_t*)c.v}, {(uint8_t*)c.k_scales, (uint8_t*)c.v_scales}, {p->k, p->v},
+                        {{p->k_stride[0], p->k_stride[1], p->k_stride[2]}, {p->v_stride[0], p->v_stride[1], p->v_stride[2]}},
+                        c.pages, c.heads, p->tokens, p->table, p->table_pitch, p->width, p->starts, nullptr, p->lengths,
+                        p->fill != 0};
+  const dim3 grid = store_grid(c, p->batch, p->tokens);
+  if (p->dtype == LDX_DTYPE_F16) launch_store<f16, true>(a, c.head_dim, grid, as_stream(stream));
+  else if (p->dtype == LDX_DTYPE_BF16) launch_store<bf16, true>(a, c.head_dim, grid, as_stream(stream));
+  else launch_store<float, true>(a, c.head_dim, grid, as_stream(stream));
+  return check_launch("cache4_read");
+}
+
+extern "C" size_t ldx_cache4_attention_workspace_bytes(const ldx_cache4_attention_args* p) {
+  return check_attention(p) == LDX_OK ? split_bytes(p, plan_of(p).splits) : 0;
+}
+
+extern "C" int ldx_cache4_attention(const ldx_cache4_attention_args* p, void* stream) {
+  if (int rc = check_attention(p)) return rc;
+  Plan plan = plan_of(p);
+  if (plan.splits > 1 && (!p->workspace || p->workspace_bytes < split_bytes(p, plan.splits))) plan.splits = 1;
+  if (plan.splits > 1 && (uintptr_t)p->workspace % 16) return fail("cache4_attention: workspace not aligned");
+  const int G = p->q_heads / p->cache.heads;
+  const Attend4Args a = {(const uint8_t*)p->cache.k, (const uint8_t*)p->cache.v, (const uint8_t*)p->cache.k_scales,
+                         (const uint8_t*)p->cache.v_scales, p->cache.pages, p->cache.heads,
+                         p->q, {p->q_stride[0], p->q_stride[1], p->q_stride[2]},
+                         p->o, {p->o_stride[0], p->o_stride[1], p->o_stride[2]},
+                         G, p->q_len, G * p->q_len, p->scale * 1.4426950408889634f,
+                         p->table, p->table_pitch, p->width, p->lengths, p->starts, plan.splits, kLeastChunk, 16,
+                         (float*)p->workspace};
+  hipStream_t st = as_stream(stream);
+  return p->dtype == LDX_DTYPE_F16 ? launch_t<f16>(a, p->cache.head_dim, p->batch, st)
+                                   : launch_t<bf16>(a, p->cache.head_dim, p->batch, st);
+}

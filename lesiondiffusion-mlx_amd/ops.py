@@ -20,23 +20,25 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from ._lib import (ACT_GELU, ACT_NONE, ACT_SILU, BLOCK8, PAGE8, AttnArgs, Cache8AppendArgs, Cache8AttentionArgs,
-                   Cache8Block, ConvArgs, Dense8Args, RmsNormArgs, SourceConvArgs, check, lib)
+from ._lib import (ACT_GELU, ACT_NONE, ACT_SILU, BLOCK4, BLOCK8, PAGE4, PAGE8, ROTARY_AXES, AttnArgs, Cache4AppendArgs,
+                   Cache4AttentionArgs, Cache4Block, Cache4ReadArgs, Cache8AppendArgs, Cache8AttentionArgs, Cache8Block,
+                   ConvArgs, Dense8Args, RmsNormArgs, RotateHeadsArgs, SourceConvArgs, check, lib)
 
 __all__ = [
     "PackedWeight", "pack_weight", "pack_upsample_weight", "nax_conv3d", "conv3d", "dense",
     "group_norm_affine", "layer_norm", "attention", "flash_attention", "timestep_embedding",
     "silu", "upsample_nearest2", "resize_nearest", "output_extent", "count_flops", "squared_norms4",
     "nearest_codebook4", "conv3d_half", "group_norm_half", "Quantized8", "quantize8", "rms_norm", "dense8",
-    "Cache8", "cache8_append", "cache8_attention",
+    "Cache8", "cache8_append", "cache8_attention", "Rotary", "rotate_heads", "Cache4", "cache4_append", "cache4_read",
+    "cache4_attention",
 ]
 
 
 class count_flops:
     """Context manager tallying the algorithmic FLOPs (2 x real multiply-adds, no
     padding; a folded upsample conv counts its 8 taps) of the convs, dense layers and
-    attention launched inside it -- for throughput figures. ``cache8_attention`` is not counted: how
-    many tokens its queries see stands on the device alone."""
+    attention launched inside it -- for throughput figures. ``cache8_attention`` and
+    ``cache4_attention`` are not counted: how many tokens their queries see stands on the device alone."""
 
     active: "count_flops | None" = None
 
@@ -1193,6 +1195,262 @@ def cache8_attention(q: torch.Tensor, cache: Cache8, table: torch.Tensor, length
         ws = q.new_empty(ws_bytes, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws_bytes
     _launch8(lib.ldx_cache8_attention, (ref,), dev, "cache8_attention")
+    if given:
+        _wrote(out)
+    return out
+
+
+# ------------------------------------------------------------------ rotation of heads, 4-bit cache
+
+@dataclass
+class Rotary:
+    """The plan of a position rotation: ``axes`` are the widths (even) of a head's sections, one for each
+    axis of positions, in order; what a head has behind them is not turned. ``turns`` (fp64, on the device)
+    holds every pair's full turns per position, the sections' one after another. Pair ``i`` of a section of
+    ``w`` channels is its channels ``(i, i + w / 2)``, or ``(2 i, 2 i + 1)`` where ``interleaved``."""
+
+    turns: torch.Tensor
+    axes: tuple[int, ...]
+    interleaved: bool = False
+
+    @staticmethod
+    def make(axes: tuple[int, ...] | int, *, theta: float = 10000.0, interleaved: bool = False,
+             scale: float | tuple[float, ...] = 1.0, device: torch.device | str = "cuda") -> "Rotary":
+        """The usual frequencies, ``theta^(-2 i / w)`` for pair ``i`` of an axis of ``w`` channels, times ``scale``
+        (of every axis, or one each: positions of a finer or coarser grid than the model's)."""
+        axes = (axes,) if isinstance(axes, int) else tuple(axes)
+        scales = scale if isinstance(scale, tuple) else (scale,) * len(axes)
+        if not axes or len(scales) != len(axes) or any(w < 2 or w % 2 for w in axes):
+            raise ValueError(f"Rotary: axes {axes} must be even widths, with a scale each, got {scales}")
+        turns = [s * theta ** (-2.0 * i / w) / (2 * math.pi) for w, s in zip(axes, scales) for i in range(w // 2)]
+        return Rotary(torch.tensor(turns, dtype=torch.float64, device=device), axes, interleaved)
+
+
+def _heads_out(out: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Tensor:
+    """``out``, checked, or a new (B, H, L, D) tensor whose tokens hold their heads side by side."""
+    if out is None:
+        b, h, l, d = x.shape
+        return x.new_empty((b, l, h, d)).transpose(1, 2)
+    _need(out, name, x.dtype, x.get_device())
+    if out.shape != x.shape:
+        raise ValueError(f"{name} shape {tuple(out.shape)} != {tuple(x.shape)}")
+    if not out.is_contiguous():
+        _distinct(out, name)
+    return out
+
+
+def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, *,
+                 q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, eps: float = 1e-6,
+                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Queries and keys before an attention, in one launch: each head divided by its root mean square and
+    times ``q_gamma`` / ``k_gamma`` (D,) where given, then turned by its token's position. ``q`` (B, H, L, D)
+    and ``k`` (B, H', L, D; or None) are fp16, bf16 or fp32, any strides with contiguous channels (slices of one
+    projection, say); D is even and at most 512. ``positions`` is int32 on the device, (B, L) for one axis,
+    (axes, B, L) for several (a volume's depth, height and width), any strides, so that one row expanded serves
+    the batch; ``rotary`` says how an axis turns (at most four). Angles are reduced in fp64: position 10^9
+    has its own. Norm and rotation are fp32, rounded once. Returns ``(q, k)``, or ``q`` without keys, in the
+    inputs' type: into ``q_out`` and ``k_out`` when given, which may be the inputs, else with a token's heads
+    side by side in memory (``(B, L, H * D)`` is a view)."""
+    _need(q, "q", _ALL, -1)
+    dev, shape = q.get_device(), q.shape
+    if len(shape) != 4 or not q.numel():
+        raise ValueError(f"q {tuple(shape)} must be (B, heads, L, D)")
+    b, h, l, d = shape
+    if not isinstance(rotary, Rotary):
+        raise ValueError("rotate_heads: rotary must be a Rotary")
+    turns, axes = rotary.turns, rotary.axes
+    n = len(axes)
+    _need(turns, "rotary turns", torch.float64, dev)
+    if not 1 <= n <= ROTARY_AXES or sum(axes) > d or turns.shape != (sum(axes) // 2,) or not turns.is_contiguous():
+        raise ValueError(f"rotary: axes {axes} (at most {ROTARY_AXES}) with {tuple(turns.shape)} turns do not fit heads of {d}")
+    _need(positions, "positions", torch.int32, dev)
+    at = positions[None] if positions.dim() == 2 and n == 1 else positions
+    if at.shape != (n, b, l):
+        raise ValueError(f"positions {tuple(positions.shape)} must be ({n}, {b}, {l})")
+    if b > _MOST or h > _MOST or l > _MOST:
+        raise ValueError(f"rotate_heads: {b} x {h} x {l} heads")
+    for g, name in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+        if g is not None:
+            _need(g, name, None, dev)
+            if g.shape != (d,):
+                raise ValueError(f"{name} shape {tuple(g.shape)} != ({d},)")
+    qg = None if q_gamma is None else _f32(q_gamma)
+    kg = None if k_gamma is None else _f32(k_gamma)
+    qo = _heads_out(q_out, q, "q_out")
+    ko, kh, ks, kos = None, 0, (0, 0, 0), (0, 0, 0)
+    if k is None:
+        if k_out is not None or k_gamma is not None:
+            raise ValueError("rotate_heads: k_out and k_gamma need keys")
+    else:
+        _need(k, "k", q.dtype, dev)
+        if k.dim() != 4 or k.shape[0] != b or k.shape[2:] != shape[2:] or not 0 < k.shape[1] <= _MOST:
+            raise ValueError(f"k {tuple(k.shape)} does not fit q {tuple(shape)}")
+        ko, kh = _heads_out(k_out, k, "k_out"), k.shape[1]
+        if ko.data_ptr() == qo.data_ptr():
+            raise ValueError("rotate_heads: q_out and k_out are the same tensor")
+        ks, kos = _head_strides(k, "k"), _head_strides(ko, "k_out")
+    a = RotateHeadsArgs(b, l, h, kh, d, ALL_DTYPES[q.dtype], q.data_ptr(), _head_strides(q, "q"), qo.data_ptr(),
+                        _head_strides(qo, "q_out"), _ptr(k), ks, _ptr(ko), kos, _ptr(qg), _ptr(kg), eps, n, axes,
+                        rotary.interleaved, at.data_ptr(), at.stride(), turns.data_ptr())
+    _launch8(lib.ldx_rotate_heads, (ctypes.byref(a),), dev, "rotate_heads")
+    if q_out is not None:
+        _wrote(q_out)
+    if k_out is not None:
+        _wrote(k_out)
+    return qo if k is None else (qo, ko)
+
+
+@dataclass
+class Cache4:
+    """Keys and values in 4 bits, in pages of 64 tokens: e2m1 codes ``k`` and ``v`` (pages, heads, 64, D / 2; uint8, two
+    channels in a byte, the even one in its lower half) and E8M0 scales ``k_scales``, ``v_scales`` (pages, heads, D /
+    32, 64), one for each 32 channels of a token, all contiguous: 17 bytes for 32 values. Pages belong to no
+    sequence by themselves: an int32 ``table`` (batch, pages per sequence) says which hold a sequence's tokens, in
+    order."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+    @staticmethod
+    def empty(pages: int, heads: int, head_dim: int, device: torch.device | str = "cuda") -> "Cache4":
+        """A cache of zeros."""
+        codes = [torch.zeros((pages, heads, PAGE4, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.full((pages, heads, head_dim // BLOCK4, PAGE4), 127, dtype=torch.uint8, device=device).view(E8M0)
+                  for _ in range(2)]
+        return Cache4(*codes, *scales)
+
+
+def _cache4_block(cache: Cache4, what: str) -> tuple[Cache4Block, int]:
+    """The C view of a cache and its device."""
+    if not isinstance(cache, Cache4):
+        raise ValueError(f"{what}: cache must be a Cache4")
+    k, v, ks, vs = cache.k, cache.v, cache.k_scales, cache.v_scales
+    if not (type(k) is type(v) is type(ks) is type(vs) is torch.Tensor and k.dtype is v.dtype is torch.uint8
+            and ks.dtype is vs.dtype is E8M0 and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() >= 0):
+        _need(k, "cache k", torch.uint8, -1)
+        _need(v, "cache v", torch.uint8, k.get_device())
+        _need(ks, "cache k_scales", E8M0, k.get_device())
+        _need(vs, "cache v_scales", E8M0, k.get_device())
+    dev, shape = k.get_device(), k.shape
+    if len(shape) != 4 or shape[2] != PAGE4:
+        raise ValueError(f"cache k must be (pages, heads, {PAGE4}, D / 2), got {tuple(shape)}")
+    pages, heads, _, half = shape
+    each = (pages, heads, half // (BLOCK4 // 2), PAGE4)
+    if v.shape != shape or ks.shape != each or vs.shape != each:
+        raise ValueError(f"cache v {tuple(v.shape)} or scales {tuple(ks.shape)}, {tuple(vs.shape)} do not fit k "
+                         f"{tuple(shape)}")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("cache tensors must be contiguous")
+    if not 0 < pages <= _MOST or not 0 < heads <= _MOST:
+        raise ValueError(f"{what}: {pages} pages of {heads} heads")
+    return Cache4Block(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, 2 * half), dev
+
+
+def cache4_append(cache: Cache4, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, *,
+                  counts: torch.Tensor | None = None) -> None:
+    """Write ``k``, ``v`` (B, heads, L, D; fp16, bf16 or fp32, any strides with contiguous channels) into
+    ``cache`` at positions ``starts[b] ..`` of each sequence: its first ``counts[b]`` tokens (all ``L``
+    without). Each 32 channels of a token get the least power of two (up to 2^125) with which their largest
+    magnitude does not pass 6, and codes rounded to nearest even; 32 channels with a NaN or an infinity among them
+    become NaN. No other token changes. Tokens past the table's width, of a negative start or in a page that the
+    cache does not have are left out; no token is written by two sequences. ``table``, ``starts`` and ``counts``
+    are int32 on the device, so a captured graph appends where they say at each replay."""
+    block, dev = _cache4_block(cache, "cache4_append")
+    _need(k, "k", _ALL, dev)
+    _need(v, "v", k.dtype, dev)
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[1] != block.heads or shape[3] != block.head_dim or not shape[0] \
+            or not shape[2]:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must be (B, {block.heads}, L, {block.head_dim})")
+    b, _, n, _ = shape
+    if b > _MOST or n > _MOST:
+        raise ValueError(f"cache4_append: {b} x {n} tokens")
+    a = Cache4AppendArgs(block, b, n, k.data_ptr(), _head_strides(k, "k"), v.data_ptr(), _head_strides(v, "v"),
+                         ALL_DTYPES[k.dtype], *_cache_table(table, b, dev), _cache_ints(starts, "starts", b, dev),
+                         None if counts is None else _cache_ints(counts, "counts", b, dev))
+    _launch8(lib.ldx_cache4_append, (ctypes.byref(a),), dev, "cache4_append")
+    if not cache.k.is_inference():
+        increment_version((cache.k, cache.v, cache.k_scales, cache.v_scales))
+
+
+def cache4_read(cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, tokens: int, *,
+                starts: torch.Tensor | None = None, dtype: torch.dtype = torch.float16,
+                out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """What ``cache`` holds of ``tokens`` tokens of each sequence, from ``starts[b]`` on (from its first one without):
+    ``(k, v)``, (B, heads, tokens, D) each, in ``dtype`` (fp16, bf16 or fp32; rounded to it). Rows from ``lengths[b]``
+    on, and before token 0, are zeros; with ``out``, a pair of that type and shape (any strides with contiguous
+    channels), they are left as they were. A page that the cache does not have, or a token past the table, gives
+    NaN. ``table``, ``lengths`` and ``starts`` are int32 on the device."""
+    block, dev = _cache4_block(cache, "cache4_read")
+    if dtype not in ALL_DTYPES:
+        raise ValueError(f"dtype must be fp16, bf16 or fp32, not {dtype}")
+    if not isinstance(tokens, int) or not 0 < tokens <= _MOST:
+        raise ValueError(f"cache4_read: {tokens} tokens")
+    b = lengths.shape[0] if isinstance(lengths, torch.Tensor) and lengths.dim() == 1 else 0
+    if not 0 < b <= _MOST:
+        raise ValueError("lengths must be int32 (B,)")
+    shape = (b, block.heads, tokens, block.head_dim)
+    if out is None:
+        k, v = (cache.k.new_empty(shape, dtype=dtype) for _ in range(2))
+    else:
+        k, v = out
+        for t, name in ((k, "out k"), (v, "out v")):
+            _need(t, name, dtype, dev)
+            if t.shape != shape:
+                raise ValueError(f"{name} shape {tuple(t.shape)} != {shape}")
+            if not t.is_contiguous():
+                _distinct(t, name)
+        if k.data_ptr() == v.data_ptr():
+            raise ValueError("cache4_read: out's k and v are the same tensor")
+    a = Cache4ReadArgs(block, b, tokens, k.data_ptr(), _head_strides(k, "out k"), v.data_ptr(), _head_strides(v, "out v"),
+                       ALL_DTYPES[dtype], *_cache_table(table, b, dev), _cache_ints(lengths, "lengths", b, dev),
+                       None if starts is None else _cache_ints(starts, "starts", b, dev), out is None)
+    _launch8(lib.ldx_cache4_read, (ctypes.byref(a),), dev, "cache4_read")
+    if out is not None:
+        _wrote(k)
+        _wrote(v)
+    return k, v
+
+
+def cache4_attention(q: torch.Tensor, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, scale: float, *,
+                     starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``softmax(q k^T * scale) v`` over the first ``lengths[b]`` tokens that ``cache`` holds of each
+    sequence. ``q`` is fp16 or bf16 ``(B, heads, L, D)``, its heads a multiple of the cache's (query head
+    ``j`` reads the cache's head ``j // group``). With ``starts`` query ``i`` sees tokens up to position
+    ``starts[b] + i`` (causal); without, all ``lengths[b]``. A query that sees no token gives 0; tokens that
+    it does not see, and pages behind the length, do not touch its result. A page that the cache does
+    not have, or a length past the table, gives NaN. Scores, softmax and sums are fp32; probabilities enter their
+    product with 16 bits. Returns ``(B, heads, L, D)`` in ``q``'s type (into ``out`` when given, which may be
+    ``q``); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
+    block, dev = _cache4_block(cache, "cache4_attention")
+    _need(q, "q", _ELEM, dev)
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != block.head_dim or shape[1] % block.heads or not q.numel():
+        raise ValueError(f"q {tuple(shape)} must be (B, a multiple of {block.heads}, L, {block.head_dim})")
+    b, hq, lq, _ = shape
+    if b > _MOST or hq > _MOST or lq > _MOST:
+        raise ValueError(f"cache4_attention: {b} x {hq} x {lq} queries")
+    given = out is not None
+    if given:
+        _need(out, "out", q.dtype, dev)
+        if out.shape != shape:
+            raise ValueError(f"out shape {tuple(out.shape)} != {tuple(shape)}")
+        if not out.is_contiguous():
+            _distinct(out, "out")
+    else:
+        out = q.new_empty(shape)
+    a = Cache4AttentionArgs(block, b, hq, lq, q.data_ptr(), _head_strides(q, "q"), out.data_ptr(),
+                            _head_strides(out, "out"), ALL_DTYPES[q.dtype], scale, *_cache_table(table, b, dev),
+                            _cache_ints(lengths, "lengths", b, dev),
+                            None if starts is None else _cache_ints(starts, "starts", b, dev))
+    ref = ctypes.byref(a)
+    ws_bytes = lib.ldx_cache4_attention_workspace_bytes(ref)
+    if ws_bytes:
+        ws = q.new_empty(ws_bytes, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws_bytes
+    _launch8(lib.ldx_cache4_attention, (ref,), dev, "cache4_attention")
     if given:
         _wrote(out)
     return out
