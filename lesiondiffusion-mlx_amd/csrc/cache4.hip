@@ -98,21 +98,32 @@ __global__ __launch_bounds__(256) void append4_kernel(Store4Args a) {
   }
 }
 
-// Eight codes times their scale in T.
-__device__ __forceinline__ void decode8(unsigned w, float s, f16* p) {
-  f16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1),
-                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3)};
-  __builtin_memcpy(p, v, sizeof(v));
-}
-__device__ __forceinline__ void decode8(unsigned w, float s, bf16* p) {
-  bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1),
-                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3)};
-  __builtin_memcpy(p, v, sizeof(v));
-}
-__device__ __forceinline__ void decode8(unsigned w, float s, float* p) {
-  f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1),
-                __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3)};
-  __builtin_memcpy(p, v, sizeof(v));
+// Eight codes times their scale in T, to memory of any alignment, past the caches' retention.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<f16> {
+  template <int SEL>
+  static __device__ __forceinline__ f16x2 of(unsigned w, float s) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, SEL); }
+};
+template <>
+struct Pair<bf16> {
+  template <int SEL>
+  static __device__ __forceinline__ bf16x2 of(unsigned w, float s) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, SEL); }
+};
+template <>
+struct Pair<float> {
+  template <int SEL>
+  static __device__ __forceinline__ f32x2 of(unsigned w, float s) { return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, SEL); }
+};
+template <typename T>
+__device__ __forceinline__ void decode8(unsigned w, float s, T* p) {
+  typedef T V __attribute__((ext_vector_type(8)));
+  typedef V Unaligned __attribute__((aligned(sizeof(T))));
+  const auto a = Pair<T>::template of<0>(w, s), b = Pair<T>::template of<1>(w, s), c = Pair<T>::template of<2>(w, s),
+             d = Pair<T>::template of<3>(w, s);
+  const V v = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  __builtin_nontemporal_store(v, reinterpret_cast<Unaligned*>(p));
 }
 
 template <typename T, int D>
@@ -140,9 +151,7 @@ __global__ __launch_bounds__(256) void read4_kernel(Store4Args a) {
     const int place = (int)(t - first);
     const unsigned w = held && !missing ? *reinterpret_cast<const unsigned*>(codes + place * (D / 2) + u * 4) : 0u;
     const int s = !held ? 127 : missing ? 255 : scales[u / 4 * kPage4 + place];
-    T v[8];
-    decode8(w, __int_as_float(s << 23), v);
-    __builtin_memcpy(dst + (t - start) * tok + u * 8, v, sizeof(v));
+    decode8(w, __int_as_float(s << 23), dst + (t - start) * tok + u * 8);
   }
 }
 

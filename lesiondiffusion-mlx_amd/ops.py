@@ -1226,11 +1226,19 @@ class Rotary:
         return Rotary(torch.tensor(turns, dtype=torch.float64, device=device), axes, interleaved)
 
 
+def _head_gamma(gamma: torch.Tensor, name: str, d: int, device: int) -> torch.Tensor:
+    """A head's ``d`` factors as contiguous fp32."""
+    _need(gamma, name, None, device)
+    if gamma.shape != (d,):
+        raise ValueError(f"{name} shape {tuple(gamma.shape)} != ({d},)")
+    return _f32(gamma)
+
+
 def _heads_out(out: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Tensor:
     """``out``, checked, or a new (B, H, L, D) tensor whose tokens hold their heads side by side."""
     if out is None:
         b, h, l, d = x.shape
-        return x.new_empty((b, l, h, d)).transpose(1, 2)
+        return x.new_empty_strided((b, h, l, d), (l * h * d, d, h * d, 1))
     _need(out, name, x.dtype, x.get_device())
     if out.shape != x.shape:
         raise ValueError(f"{name} shape {tuple(out.shape)} != {tuple(x.shape)}")
@@ -1252,46 +1260,46 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     inputs' type: into ``q_out`` and ``k_out`` when given, which may be the inputs, else with a token's heads
     side by side in memory (``(B, L, H * D)`` is a view)."""
     _need(q, "q", _ALL, -1)
-    dev, shape = q.get_device(), q.shape
+    dev, shape, dtype = q.get_device(), q.shape, q.dtype
     if len(shape) != 4 or not q.numel():
         raise ValueError(f"q {tuple(shape)} must be (B, heads, L, D)")
     b, h, l, d = shape
     if not isinstance(rotary, Rotary):
         raise ValueError("rotate_heads: rotary must be a Rotary")
     turns, axes = rotary.turns, rotary.axes
-    n = len(axes)
+    n, turned = len(axes), sum(axes)
     _need(turns, "rotary turns", torch.float64, dev)
-    if not 1 <= n <= ROTARY_AXES or sum(axes) > d or turns.shape != (sum(axes) // 2,) or not turns.is_contiguous():
+    if not 1 <= n <= ROTARY_AXES or turned > d or turns.shape != (turned // 2,) or not turns.is_contiguous():
         raise ValueError(f"rotary: axes {axes} (at most {ROTARY_AXES}) with {tuple(turns.shape)} turns do not fit heads of {d}")
     _need(positions, "positions", torch.int32, dev)
-    at = positions[None] if positions.dim() == 2 and n == 1 else positions
-    if at.shape != (n, b, l):
-        raise ValueError(f"positions {tuple(positions.shape)} must be ({n}, {b}, {l})")
+    ps, at = positions.shape, positions.stride()
+    if n == 1 and ps == (b, l):
+        at = (0, *at)
+    elif ps != (n, b, l):
+        raise ValueError(f"positions {tuple(ps)} must be ({n}, {b}, {l})")
     if b > _MOST or h > _MOST or l > _MOST:
         raise ValueError(f"rotate_heads: {b} x {h} x {l} heads")
-    for g, name in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
-        if g is not None:
-            _need(g, name, None, dev)
-            if g.shape != (d,):
-                raise ValueError(f"{name} shape {tuple(g.shape)} != ({d},)")
-    qg = None if q_gamma is None else _f32(q_gamma)
-    kg = None if k_gamma is None else _f32(k_gamma)
+    if q_gamma is not None:
+        q_gamma = _head_gamma(q_gamma, "q_gamma", d, dev)
+    if k_gamma is not None:
+        k_gamma = _head_gamma(k_gamma, "k_gamma", d, dev)
     qo = _heads_out(q_out, q, "q_out")
     ko, kh, ks, kos = None, 0, (0, 0, 0), (0, 0, 0)
     if k is None:
         if k_out is not None or k_gamma is not None:
             raise ValueError("rotate_heads: k_out and k_gamma need keys")
     else:
-        _need(k, "k", q.dtype, dev)
-        if k.dim() != 4 or k.shape[0] != b or k.shape[2:] != shape[2:] or not 0 < k.shape[1] <= _MOST:
-            raise ValueError(f"k {tuple(k.shape)} does not fit q {tuple(shape)}")
-        ko, kh = _heads_out(k_out, k, "k_out"), k.shape[1]
+        _need(k, "k", dtype, dev)
+        kshape = k.shape
+        if len(kshape) != 4 or kshape[0] != b or kshape[2] != l or kshape[3] != d or not 0 < kshape[1] <= _MOST:
+            raise ValueError(f"k {tuple(kshape)} does not fit q {tuple(shape)}")
+        ko, kh = _heads_out(k_out, k, "k_out"), kshape[1]
         if ko.data_ptr() == qo.data_ptr():
             raise ValueError("rotate_heads: q_out and k_out are the same tensor")
         ks, kos = _head_strides(k, "k"), _head_strides(ko, "k_out")
-    a = RotateHeadsArgs(b, l, h, kh, d, ALL_DTYPES[q.dtype], q.data_ptr(), _head_strides(q, "q"), qo.data_ptr(),
-                        _head_strides(qo, "q_out"), _ptr(k), ks, _ptr(ko), kos, _ptr(qg), _ptr(kg), eps, n, axes,
-                        rotary.interleaved, at.data_ptr(), at.stride(), turns.data_ptr())
+    a = RotateHeadsArgs(b, l, h, kh, d, ALL_DTYPES[dtype], q.data_ptr(), _head_strides(q, "q"), qo.data_ptr(),
+                        _head_strides(qo, "q_out"), _ptr(k), ks, _ptr(ko), kos, _ptr(q_gamma), _ptr(k_gamma), eps, n, axes,
+                        rotary.interleaved, positions.data_ptr(), at, turns.data_ptr())
     _launch8(lib.ldx_rotate_heads, (ctypes.byref(a),), dev, "rotate_heads")
     if q_out is not None:
         _wrote(q_out)

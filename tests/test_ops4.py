@@ -75,7 +75,8 @@ def refused(pkg, rc: int, word: str) -> None:
     {"q": None}, {"q_out": None}, {"positions": None}, {"turns": None}, {"k": None}, {"k_out": None}, {"k_heads": -1},
     {"dtype": 3}, {"head_dim": 0}, {"head_dim": 33}, {"head_dim": 514}, {"q_heads": 0}, {"q_heads": 70000}, {"batch": 0},
     {"tokens": 0}, {"batch": 70000, "tokens": 70000}, {"axes": 0}, {"axes": 5}, {"axis_dims": (16, 20)}, {"axis_dims": (3, 4)},
-    {"axis_dims": (0, 4)}, {"axis_dims": (-2, 4)}, {"q_gamma": 16, "eps": 0.0}, {"k_gamma": 16, "eps": NAN},
+    {"axis_dims": (0, 4)}, {"axis_dims": (-2, 4)},
+    {"batch": 0x7fff, "tokens": 0xffff, "head_dim": 512}, {"q_gamma": 16, "eps": 0.0}, {"k_gamma": 16, "eps": NAN},
 ])
 def test_rotate_heads_refuses(pkg, bad) -> None:
     a = pkg._lib.RotateHeadsArgs(batch=1, tokens=1, q_heads=1, k_heads=1, head_dim=32, dtype=0, q=16, q_out=16, k=16, k_out=16,
