@@ -630,12 +630,14 @@ int ldx_cache4_read(const ldx_cache4_read_args* args, void* stream);
  * starts, query i sees no token behind starts[b] + i (causal for queries at starts[b]..). q and
  * o: (batch, token, head) strides, contiguous channels, fp16 or bf16; q_heads a multiple of
  * the cache's heads, query head j reads the cache's head j / (q_heads / heads). Scores, softmax and
- * sums are fp32; keys and values enter the products exactly, queries too, probabilities with 16 bits.
+ * sums are fp32; keys, values and queries enter the products exactly, probabilities rounded: to 16 bits,
+ * or, where many queries share pages, to fp16 in both of the quotient's sums (2^-11 of themselves, those
+ * below 2^-21 of a query's largest 2^-32 of it).
  * A query that sees no token gets 0. Tokens that a query does not see do not touch its result, NaN
  * among them. A page that the cache does not have, or a key of NaN, gives NaN to the queries that see
  * it, a value of NaN to their channels of its block, a length past the table to the whole
  * sequence. Scale bytes of 253 and 254, which append does not write, may count as NaN. Values are summed before
- * they are divided, with weights of up to 2^8, so that sums past fp32 are infinite. o may be q.
+ * they are divided, with weights of up to 2^15, so that sums past fp32 are infinite. o may be q.
  * Workspace: partial results where a sequence is split over workgroups,
  * ldx_cache4_attention_workspace_bytes of them, 256 MiB at most; with less nothing is split. */
 typedef struct ldx_cache4_attention_args {
@@ -652,6 +654,9 @@ typedef struct ldx_cache4_attention_args {
 } ldx_cache4_attention_args;
 size_t ldx_cache4_attention_workspace_bytes(const ldx_cache4_attention_args* args);
 int ldx_cache4_attention(const ldx_cache4_attention_args* args, void* stream);
+/* Rows (queries x heads of a cache head) that a workgroup of such a call takes, on the host
+ * alone: 16, each wave reading pages of its own, or 128, which share them. */
+int ldx_cache4_attention_rows(const ldx_cache4_attention_args* args);
 
 #ifdef __cplusplus
 }

@@ -251,6 +251,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ldx_cache4_append": (c_i32, [ctypes.POINTER(Cache4AppendArgs), c_vp]),
     "ldx_cache4_read": (c_i32, [ctypes.POINTER(Cache4ReadArgs), c_vp]),
     "ldx_cache4_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Cache4AttentionArgs)]),
+    "ldx_cache4_attention_rows": (c_i32, [ctypes.POINTER(Cache4AttentionArgs)]),
     "ldx_cache4_attention": (c_i32, [ctypes.POINTER(Cache4AttentionArgs), c_vp]),
 }
 

@@ -512,10 +512,561 @@ __global__ __launch_bounds__(64 * kWaves4, D == 256 ? 1 : 2) void attend4_kernel
   }
 }
 
+// ------------------------------------------------------------------- many queries of a cache head
+//
+// A workgroup takes 128 rows (queries x grouped heads), a wave 32 of them, and shares each page through LDS as 16-bit
+// operands, so that a code is widened once for all of them. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: lane
+// l holds query column l % 32, h = l / 32. Row 8 q + 4 h + i of a 32-token key tile is its token 16 h + 4 q + i, so that
+// the scores a lane receives are 16 tokens in a row and the probabilities go into the second product as they lie. Row 8 q +
+// 4 h + i of a value tile is its channel 16 (q / 2) + 8 h + 4 (q % 2) + i, so that a lane's results are eight channels in a
+// row.
+//
+// Keys are widened to the queries' type and values to fp16, which holds a code times 2^-23 to 2^8 exactly; probabilities
+// are rounded to fp16. A page with scales outside of that (of its keys only where queries are fp16) is widened to bf16
+// instead, with fp16 queries and the probabilities in two parts.
+//
+// A round takes the probabilities of page p between the products that make page p + 1's scores, and page p's values'
+// products between the widening of later pages' codes, an instruction of the matrix units and some of the vector units in
+// turn, so that a wave keeps both busy by itself. (One after the other, 2,048 causal queries of 8 x 4 heads of 128 behind
+// 8,192 tokens 445 us, so 345 to 380, 820 to 900 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 tokens 130 and 7 for the join,
+// of 256 1,160 and 540.) Matrix units, vector units and LDS are each busy half of the time then, at the 2.0 GHz that the
+// power allows.
+constexpr int kWideRows = 128;
+// A query's reference is this much below its maximum, and lags kLag behind it: probabilities reach 2^15, and fp16 holds
+// those from 2^-21 of the largest on to 2^-11 of themselves and smaller ones to 2^-32 of it, so that many small ones
+// beside a dominant one keep their weight.
+constexpr float kRaise = 7.f;
+
+__device__ __forceinline__ f32x16 mfma_w(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma_w(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Whether a word holds only scale bytes 104 to 135, whose codes fp16 holds: their upper three bits, 24 more. (A byte of 232
+// and more carries into its neighbour, but gives itself away.)
+__device__ __forceinline__ bool within_fp16(int w) { return (((unsigned)w + 0x18181818u) & 0xe0e0e0e0u) == 0x80808080u; }
+
+// l and eight probabilities, as the products take them (their sum in fp32), so that rounding moves both sides of the
+// quotient alike. Two at a time: half the additions of fp32 numbers.
+__device__ __forceinline__ float sum8(f16x8 p, float l) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    l = __builtin_amdgcn_fdot2((f16x2){p[i], p[i + 1]}, (f16x2){(f16)1.f, (f16)1.f}, l, false);
+  return l;
+}
+
+// Two codes (byte sel of a word) times a scale, as a word of two T.
+template <typename T>
+__device__ __forceinline__ unsigned pair_of(unsigned w, float s, int sel) {
+  return sel == 0   ? __builtin_bit_cast(unsigned, Pair<T>::template of<0>(w, s))
+         : sel == 1 ? __builtin_bit_cast(unsigned, Pair<T>::template of<1>(w, s))
+         : sel == 2 ? __builtin_bit_cast(unsigned, Pair<T>::template of<2>(w, s))
+                    : __builtin_bit_cast(unsigned, Pair<T>::template of<3>(w, s));
+}
+
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
+
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<f16> { typedef f16x8 V; };
+template <>
+struct Vec8<bf16> { typedef bf16x8 V; };
+
+// LDS holds keys in fragment order (a lane's 16 bytes at its place): 16 widening lanes write pieces j of 256 / D keys, and a
+// fragment's pad moves its 16-byte places by 256 / D a piece. Values lie as they do in the cache, a token's channels in a
+// row, and are turned as they are read, four tokens of 32 channels by 32 lanes (rows of 64 bytes past a multiple of 256, or
+// 64 short of one, so that the four meet all banks once).
+template <int D>
+struct WideLds {
+  static constexpr int KF = 1024 + 4096 / D, KEYS = 2 * (D / 16) * KF, VROW = 2 * D + 64;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Attend4Args a) {
+  typedef typename Vec8<T>::V V8;
+  constexpr int NJ = D / 16;               // products per key tile
+  constexpr int NT = D / 32;               // channel tiles; blocks
+  constexpr int RAW = D / 64;              // 8-byte pieces of a page's keys (values) that a thread widens
+  constexpr int CHECK = D == 256 ? 2 : 1;  // words of a page's key (value) scales that a lane looks at
+  typedef WideLds<D> L;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
+  const int b = blockIdx.z, split = blockIdx.x % a.splits, tiles = (a.rows + kWideRows - 1) / kWideRows;
+  const int tile = blockIdx.x / a.splits;
+  const int h = tile / tiles, row0 = (tiles - 1 - tile % tiles) * kWideRows;   // causal: longest first
+  const int wrow = row0 + 32 * wave, row = wrow + r;
+  const bool real = row < a.rows;
+  const int raw = a.lengths[b];
+  const bool too_long = raw > (int64_t)a.width * kPage4;
+  const int len = too_long || raw < 0 ? 0 : raw;
+  const int64_t start = a.starts ? a.starts[b] : 0;
+  const int limit = real ? key_limit(a, len, start, row) : 0;
+  const int least = wrow < a.rows ? key_limit(a, len, start, wrow) : 0;                             // of the wave
+  const int wmost = wrow < a.rows ? key_limit(a, len, start, min(wrow + 31, a.rows - 1)) : 0;
+  const int most = key_limit(a, len, start, min(row0 + kWideRows, a.rows) - 1);                     // of the tile
+  const int npages = (most + kPage4 - 1) / kPage4;
+  const int chunk = max((npages + a.splits - 1) / a.splits, a.chunk);
+  const int p0 = a.splits > 1 ? split * chunk : 0, p1 = a.splits > 1 ? min(p0 + chunk, npages) : npages;
+  if (p0 >= p1 && split > 0) return;   // the join knows that there is no such part
+
+  V8 q[NJ];
+  {
+    const T* qp = (const T*)a.q + b * a.qs[0] + (int64_t)(row / a.G) * a.qs[1] + (int64_t)(h * a.G + row % a.G) * a.qs[2];
+    const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;   // the size goes into the exponentials
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (real) load8(qp + 16 * j + 8 * hh, f);
+#pragma unroll
+      for (int e = 0; e < 8; e++) q[j][e] = (T)(f[e] * sign);
+    }
+  }
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale);
+  f32x16 acc[NT];
+#pragma unroll
+  for (int d = 0; d < NT; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;
+  unsigned poison = 0;   // bit d: the lane's query sees a value of NaN in channel tile d
+
+  const int32_t* table = a.table + b * a.tp;
+  const auto entry = [&](int p) { return table_entry(table, min(p, p1 - 1)); };
+  const auto place = [&](int page) { return (int64_t)((unsigned)page >= (unsigned)a.pages ? 0 : page) * a.H + h; };
+
+  // A thread's pieces of a page's keys, and of another's values.
+  struct Raw {
+    i32x2 codes[RAW];
+    int scale[RAW];
+  };
+  Raw kraw, vraw;
+  const unsigned soff = tid % NJ / 2 * kPage4 + tid / NJ;   // (256 / NJ tokens on for the next piece)
+  const auto load = [&](const uint8_t* codes, const uint8_t* scales, int64_t at, Raw& raw) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t cr = make_rsrc(codes + at * (kPage4 * D / 2), kPage4 * D / 2);
+    const __amdgpu_buffer_rsrc_t sr = make_rsrc(scales + at * (kPage4 * NT), kPage4 * NT);
+#pragma unroll
+    for (int i = 0; i < RAW; i++) {
+      raw.codes[i] = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(cr, tid * 8, 2048 * i, 0));
+      raw.scale[i] = __builtin_amdgcn_raw_buffer_load_b8(sr, soff, 256 / NJ * i, 0);
+    }
+  };
+  // A page's scales, which every wave looks at, so that all take the page alike. (At head width 64 half of the lanes read
+  // behind them, zeros, which stand for nothing.)
+  struct Check {
+    int word[CHECK];
+  };
+  const auto ask = [&](const uint8_t* scales, int64_t at, Check& c) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t sr = make_rsrc(scales + at * (kPage4 * NT), kPage4 * NT);
+#pragma unroll
+    for (int i = 0; i < CHECK; i++) c.word[i] = __builtin_amdgcn_raw_buffer_load_b32(sr, lane * 4, 256 * i, 0);
+  };
+  // Whether page p needs more than fp16. Tokens behind all that the rows see say nothing.
+  const auto is_odd = [&](int p, Check& c) __attribute__((always_inline)) {
+    if (p * kPage4 + kPage4 > most) {
+      const int mine = most - p * kPage4 - lane * 4 % kPage4;
+      const unsigned keep = mine >= 4 ? ~0u : mine <= 0 ? 0u : ~0u >> (32 - 8 * mine);
+#pragma unroll
+      for (int i = 0; i < CHECK; i++) c.word[i] = (int)(((unsigned)c.word[i] & keep) | (0x7f7f7f7fu & ~keep));
+    }
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < CHECK; i++) bad |= !within_fp16(c.word[i]);
+    return (bool)__any(bad && (D > 64 || lane < 32));
+  };
+  const auto times = [&](float f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[d][e] *= f;
+  };
+  // Widen half x of a thread's piece i of the keys, or the values, into buffer `to`.
+  const auto widen_key = [&](uint8_t* to, int i, int x, auto kt) __attribute__((always_inline)) {
+    typedef decltype(kt) KT;
+    const int e = tid + 256 * i, key = e / NJ, j = e % NJ;
+    const int t = key & 31, at = 8 * (t >> 2 & 3) + 4 * (t >> 4) + (t & 3);   // the token's row of its tile
+    const float s = __int_as_float(kraw.scale[i] << 23);
+    u32x4 w;
+#pragma unroll
+    for (int y = 0; y < 4; y++) w[y] = pair_of<KT>((unsigned)kraw.codes[i][x], s, y);
+    *reinterpret_cast<u32x4*>(to + ((key >> 5) * NJ + j) * L::KF + at * 16 + 512 * x) = w;
+  };
+  const auto widen_value = [&](uint8_t* to, int left, int i, int x, auto vt) __attribute__((always_inline)) {
+    typedef decltype(vt) VT;
+    const int e = tid + 256 * i, key = e / NJ, j = e % NJ;
+    // Values of tokens that none of the rows sees get a scale of 1: probabilities of 0 times anything finite; in bf16
+    // those of NaN (and past fp32), too, see below.
+    const bool one = key >= left || (__is_same(VT, bf16) && vraw.scale[i] >= 253);
+    const float s = __int_as_float((one ? 127 : vraw.scale[i]) << 23);
+    const int flip = (D == 256 ? j >> 3 : D == 128 ? j >> 2 : key) & 1;   // 16 lanes write 16 bytes each, half of them first halves
+    const int c0 = vraw.codes[i][x], c1 = vraw.codes[i][1 - x];
+    const unsigned codes = (unsigned)(flip ? c1 : c0);
+    u32x4 w;
+#pragma unroll
+    for (int y = 0; y < 4; y++) w[y] = pair_of<VT>(codes, s, y);
+    *reinterpret_cast<u32x4*>(to + key * L::VROW + j * 32 + 16 * (x ^ flip)) = w;
+  };
+  const auto widen_keys = [&](uint8_t* to, auto kt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2 * RAW; i++) widen_key(to, i / 2, i % 2, kt);
+  };
+  const auto widen_values = [&](uint8_t* to, int left, auto vt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2 * RAW; i++) widen_value(to, left, i / 2, i % 2, vt);
+  };
+  // Eight tokens, 32 t + 16 h + 8 u .., of the channel that is row r of tile d, in 16 bits: lane l % 16 of 16 hands in
+  // where four channels of a token stand and gets a channel of four tokens.
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  typedef __attribute__((address_space(3))) s16x4* lds4;
+  const unsigned turned = (16 * hh + (lane & 15) / 4) * L::VROW + 2 * (16 * (lane >> 4 & 1) + 8 * (lane & 1) + 4 * (lane >> 1 & 1));
+  const auto values = [&](const uint8_t* vb, int d, int t, int u) __attribute__((always_inline)) {
+    const unsigned at = lds_offset(vb) + turned + (32 * t + 8 * u) * L::VROW + 64 * d;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)at);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(at + 4 * L::VROW));
+    return (s16x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  };
+
+  struct Scores {
+    f32x16 t[2];   // tiles of 32 tokens
+  };
+  const auto product = [&](const uint8_t* kb, Scores& sv) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) sv.t[t][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+        sv.t[t] = mfma_w(*reinterpret_cast<const V8*>(kb + lane * 16 + (t * NJ + j) * L::KF), q[j], sv.t[t]);
+      if (j % 2) __builtin_amdgcn_sched_barrier(0);   // bounds the operands read ahead
+    }
+  };
+  // The same of keys in bf16, and queries in two parts, made anew for each such page so that they do not stay in registers.
+  const auto product_odd = [&](const uint8_t* kb, Scores& sv) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) sv.t[t][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      V8 w = q[j];
+      pin_value(w);
+      bf16x8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        hi[e] = (bf16)(float)w[e];
+        lo[e] = (bf16)((float)w[e] - (float)hi[e]);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb + lane * 16 + (t * NJ + j) * L::KF);
+        sv.t[t] = mfma_w(kv, lo, mfma_w(kv, hi, sv.t[t]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // A page's scores as exponents below the lane's reference, which is moved where it has to be.
+  const auto exponents = [&](int p, bool missing, Scores& s, float& kc) __attribute__((always_inline)) {
+    const int base = p * kPage4 + 16 * hh;   // score e of tile t is token base + 32 t + e
+    if (missing && p * kPage4 < limit) l = __builtin_nanf("");   // (page 0 was read in a missing one's place)
+    if (p * kPage4 + kPage4 > least) {
+      int left = limit - base;
+      pin_value(left);
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s.t[t][e] = 32 * t + e < left ? s.t[t][e] : -__builtin_inff();
+    }
+    float mx = max3_f(s.t[0][0], s.t[1][0], s.t[0][1]);
+    mx = max3_f(mx, s.t[1][1], s.t[1][1]);
+#pragma unroll
+    for (int e = 2; e < 16; e++) mx = max3_f(mx, s.t[0][e], s.t[1][e]);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
+    const float mn = max3_f(m, __builtin_fmaf(__int_as_float(x[0]), scale, -kRaise),
+                            __builtin_fmaf(__int_as_float(x[1]), scale, -kRaise));
+    // A score goes into the exponential times the scale and unrounded, its reference does not: what the reference's
+    // rounding left out, up to 2^-24 of it, moves a query's probabilities by one factor, which must not leave fp16.
+    // Beyond 2^20 scores are rounded first, and the reference never lags.
+    const bool far = __any(fabsf(mn) >= 0x1p20f && mn != -__builtin_inff());
+    kc = far ? 1.f : scale;
+    if (__builtin_expect(far, 0)) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s.t[t][e] *= scale;
+    }
+    float ref = m == -__builtin_inff() ? 0.f : m;
+    if (__any(mn - m > (far ? 0.f : kLag))) {
+      ref = mn == -__builtin_inff() ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+      l *= alpha;
+      times(alpha);
+      m = mn;
+    }
+    return ref;
+  };
+  const auto two = [&](const Scores& s, int i, float kc, float ref) __attribute__((always_inline)) {   // probabilities 2 i, 2 i + 1
+    const f16x2 p = {(f16)__builtin_amdgcn_exp2f(__builtin_fmaf(s.t[i / 8][2 * i % 16], kc, -ref)),
+                     (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(s.t[i / 8][2 * i % 16 + 1], kc, -ref))};
+    return p;
+  };
+  const auto probabilities = [&](const Scores& s, float kc, float ref, f16x8 (&pr)[4]) __attribute__((always_inline)) {
+    float lp = 0.f;   // the page's own sum, so that small ones do not go one by one into a large one
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const f16x2 p = two(s, 4 * i + e, kc, ref);
+        pr[i][2 * e] = p[0], pr[i][2 * e + 1] = p[1];
+      }
+      lp = sum8(pr[i], lp);
+      pin_value(lp);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l += lp;
+  };
+  const auto add_values = [&](const uint8_t* vb, const f16x8 (&pr)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int d = 0; d < NT; d++) {
+        acc[d] = mfma_w(__builtin_bit_cast(f16x8, values(vb, d, i / 2, i % 2)), pr[i], acc[d]);
+        if (d % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  // A page's probabilities between the next page's products, and its values' products between the widening of codes, to
+  // kto and vto (of the page's `left` tokens that count). A product's operand is read two products ahead.
+  const auto both = [&](const Scores& now, Scores& next, float kc, float ref, const uint8_t* kb, const uint8_t* vb, uint8_t* kto,
+                        uint8_t* vto, int left) __attribute__((always_inline)) {
+    constexpr int NK = 2 * NJ, NV = 4 * NT, AHEAD = D == 64 ? 3 : 2;
+    const auto key = [&](int i) __attribute__((always_inline)) {
+      return *reinterpret_cast<const V8*>(kb + lane * 16 + (i % 2 * NJ + i / 2) * L::KF);
+    };
+    const auto value = [&](int i) __attribute__((always_inline)) { return values(vb, i % NT, i / NT / 2, i / NT % 2); };
+    f16x8 pr[4];
+    float lp = 0.f;
+    V8 k[AHEAD];
+    s16x8 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) k[i] = key(i);
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) next.t[t][e] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      next.t[i % 2] = mfma_w(k[i % AHEAD], q[i / 2], next.t[i % 2]);
+      if (i + AHEAD < NK) k[i % AHEAD] = key(i + AHEAD);
+      else v[i + AHEAD - NK] = value(i + AHEAD - NK);
+#pragma unroll
+      for (int x = i * 16 / NK; x < (i + 1) * 16 / NK; x++) {   // sixteen pairs
+        const f16x2 p = two(now, x, kc, ref);
+        pr[x / 4][2 * x % 8] = p[0], pr[x / 4][2 * x % 8 + 1] = p[1];
+        lp = __builtin_amdgcn_fdot2(p, (f16x2){(f16)1.f, (f16)1.f}, lp, false);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l += lp;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      acc[i % NT] = mfma_w(__builtin_bit_cast(f16x8, v[i % AHEAD]), pr[i / NT], acc[i % NT]);
+      if (i + AHEAD < NV) v[i % AHEAD] = value(i + AHEAD);
+      if (i % 2) {   // D / 16 halves of pieces
+        const int x = i / 2;
+        if (x < 2 * RAW) widen_key(kto, x / 2, x % 2, T());
+        else widen_value(vto, left, (x - 2 * RAW) / 2, x % 2, f16());
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // The same of values in bf16. Those of NaN were left out of LDS: the queries that see them get it at the end.
+  const auto add_odd = [&](int p, int64_t at, const uint8_t* vb, const Scores& s, float kc, float ref) __attribute__((always_inline)) {
+    float lp = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        u32x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s.t[t][8 * u + e], kc, -ref));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s.t[t][8 * u + e + 1], kc, -ref));
+          lp += x + y;
+          unsigned xy, left;
+          split2(x, y, xy, left);
+          hi[e / 2] = xy;
+          lo[e / 2] = left;
+        }
+#pragma unroll
+        for (int d = 0; d < NT; d++) {
+          const bf16x8 v = __builtin_bit_cast(bf16x8, values(vb, d, t, u));
+          acc[d] = mfma_w(v, __builtin_bit_cast(bf16x8, lo), mfma_w(v, __builtin_bit_cast(bf16x8, hi), acc[d]));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    l += lp;
+    const uint8_t* vs = a.vs + at * (kPage4 * NT);
+#pragma unroll 1
+    for (int i = 0; i < kPage4 * NT; i++)
+      if (vs[i] >= 253 && p * kPage4 + i % kPage4 < limit) poison |= 1u << i / kPage4;
+  };
+
+  if (p0 < p1) {
+    // Round p takes the exponentials of page p's scores, made in the round before, while the matrix units make page p + 1's,
+    // and adds its values while page p + 2's keys and p + 1's values are widened. Keys of p + 3 and values of p + 2 are on
+    // their way.
+    uint8_t* const keys[2] = {lds, lds + L::KEYS};
+    uint8_t* const vals[2] = {lds + 2 * L::KEYS, lds + 2 * L::KEYS + kPage4 * L::VROW};
+    int pages[5];   // numbers of pages p .. p + 4
+#pragma unroll
+    for (int i = 0; i < 5; i++) pages[i] = entry(p0 + i);
+    constexpr bool EXACT = __is_same(T, bf16);   // keys of any scale are what they are
+    const auto keys_at = [&](int i) __attribute__((always_inline)) { load(a.k, a.ks, place(pages[i]), kraw); };
+    const auto values_at = [&](int i) __attribute__((always_inline)) { load(a.v, a.vs, place(pages[i]), vraw); };
+    int p = p0;
+    Scores s0, s1;
+    Check kc0, kc1, vc0, vc1;   // of the keys and values that this round and the next one widen
+    keys_at(0);
+    values_at(0);
+    ask(a.ks, place(pages[0]), kc0);
+    ask(a.ks, place(pages[1]), kc1);
+    ask(a.vs, place(pages[0]), vc0);
+    bool odd = (!EXACT && (is_odd(p0, kc0) | is_odd(p0 + 1, kc1))) | is_odd(p0, vc0);
+    if (__builtin_expect(!odd, 1)) {
+      widen_keys(keys[0], T());
+      widen_values(vals[0], most - p0 * kPage4, f16());
+      keys_at(1);
+      ring_barrier();
+      product(keys[0], s0);
+      widen_keys(keys[1], T());
+      if (!EXACT) ask(a.ks, place(pages[2]), kc0);
+      ask(a.vs, place(pages[1]), vc0);
+      keys_at(2);
+      values_at(1);
+      if (!EXACT) ask(a.ks, place(pages[3]), kc1);
+      ask(a.vs, place(pages[2]), vc1);
+      const auto round = [&](auto parity, Scores& now, Scores& next, Check& kcheck, Check& vcheck) __attribute__((always_inline)) {
+        constexpr int P = decltype(parity)::value;
+        // Page p + 1's keys and page p's values stand in LDS, and every wave is done with page p's keys and p - 1's
+        // values. (__syncthreads would wait for the codes asked for, too.)
+        ring_barrier();
+        odd |= (!EXACT && is_odd(p + 2, kcheck)) | is_odd(p + 1, vcheck);
+        if (__builtin_expect(odd, 0)) return;
+        const int left = most - (p + 1) * kPage4;
+        if (p * kPage4 < wmost) {
+          float kc;
+          const float ref = exponents(p, (unsigned)pages[0] >= (unsigned)a.pages, now, kc);
+          both(now, next, kc, ref, keys[1 - P], vals[P], keys[P], vals[1 - P], left);
+        } else {
+          widen_keys(keys[P], T());
+          widen_values(vals[1 - P], left, f16());
+        }
+        keys_at(3);
+        values_at(2);
+        if (!EXACT) ask(a.ks, place(pages[4]), kcheck);
+        ask(a.vs, place(pages[3]), vcheck);
+#pragma unroll
+        for (int i = 0; i < 4; i++) pages[i] = pages[i + 1];
+        p++;
+        pages[4] = entry(p + 4);
+      };
+      while (p < p1 && !odd) {
+        round(Const<0>(), s0, s1, kc0, vc0);
+        if (p < p1 && !odd) round(Const<1>(), s1, s0, kc1, vc1);
+      }
+    }
+    // From the first page that fp16 does not hold on (and the few before it that are on their way) a page at a time.
+    for (; p < p1; p++) {
+      pages[0] = entry(p);
+      const int64_t at = place(pages[0]);
+      keys_at(0);
+      values_at(0);
+      ask(a.ks, at, kc0);
+      ask(a.vs, at, vc0);
+      const bool kodd = !EXACT && is_odd(p, kc0), vodd = is_odd(p, vc0);
+      const int left = most - p * kPage4;
+      ring_barrier();
+      if (kodd) widen_keys(keys[0], bf16());
+      else widen_keys(keys[0], T());
+      if (vodd) widen_values(vals[0], left, bf16());
+      else widen_values(vals[0], left, f16());
+      ring_barrier();
+      if (p * kPage4 >= wmost) continue;
+      if (kodd) product_odd(keys[0], s0);
+      else product(keys[0], s0);
+      float kc;
+      const float ref = exponents(p, (unsigned)pages[0] >= (unsigned)a.pages, s0, kc);
+      if (vodd) {
+        add_odd(p, at, vals[0], s0, kc, ref);
+      } else {
+        f16x8 pr[4];
+        probabilities(s0, kc, ref, pr);
+        add_values(vals[0], pr);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int d = 0; d < NT; d++)
+    if (poison >> d & 1)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[d][e] = __builtin_nanf("");
+  const auto l32 = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
+  l = __int_as_float(l32[0]) + __int_as_float(l32[1]);
+  if (too_long) l = __builtin_nanf("");
+  if (!real) return;
+  const int64_t bh = (int64_t)b * a.H + h, place8 = (bh * a.rows + row) * a.splits + split;
+  const int64_t all = (int64_t)gridDim.z * a.H * a.rows * a.splits;
+  const float inv = a.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  T* op = (T*)a.o + b * a.os[0] + (int64_t)(row / a.G) * a.os[1] + (int64_t)(h * a.G + row % a.G) * a.os[2];
+#pragma unroll
+  for (int d = 0; d < NT; d++)
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+      float f[8];
+#pragma unroll
+      for (int c = 0; c < 8; c++) f[c] = acc[d][8 * g + c] * inv;
+      const int channel = 32 * d + 16 * g + 8 * hh;
+      if (a.splits > 1) {
+        float* to = a.part + place8 * D + channel;
+        *reinterpret_cast<f32x4*>(to) = (f32x4){f[0], f[1], f[2], f[3]};
+        *reinterpret_cast<f32x4*>(to + 4) = (f32x4){f[4], f[5], f[6], f[7]};
+      } else {
+        store8(op + channel, f);
+      }
+    }
+  if (a.splits > 1 && hh == 0) {
+    a.part[all * D + 2 * place8] = m == -__builtin_inff() ? 0.f : m;
+    a.part[all * D + 2 * place8 + 1] = l;
+  }
+}
+
+template <typename T, int D>
+int launch_wide(const Attend4Args& a, dim3 grid, hipStream_t st) {
+  constexpr int LDS = 2 * (WideLds<D>::KEYS + kPage4 * WideLds<D>::VROW);
+  const auto kern = attend4_wide_kernel<T, D>;
+  if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+    return check_launch("cache4_attention: set LDS size");
+  hipLaunchKernelGGL(kern, grid, dim3(256), LDS, st, a);
+  return LDX_OK;
+}
+
 template <typename T, int D>
 int launch_d(const Attend4Args& a, int batch, hipStream_t st) {
   const dim3 grid((unsigned)a.splits * (unsigned)(a.H * ((a.rows + a.tile - 1) / a.tile)), 1, (unsigned)batch);
-  hipLaunchKernelGGL((attend4_kernel<T, D>), grid, dim3(64 * kWaves4), 0, st, a);
+  if (a.tile == 16) {
+    hipLaunchKernelGGL((attend4_kernel<T, D>), grid, dim3(64 * kWaves4), 0, st, a);
+  } else if constexpr (D >= 64) {
+    if (int rc = launch_wide<T, D>(a, grid, st)) return rc;
+  }
   launch_join<T, D>(a, (int64_t)batch * a.H * a.rows, st);
   return check_launch("cache4_attention");
 }
@@ -556,6 +1107,7 @@ dim3 store_grid(const ldx_cache4& c, int batch, int tokens) {
 // How a call is laid out. The host knows only how many pages a table's row holds; the kernels divide the
 // pages that a sequence has.
 struct Plan {
+  bool wide;    // pages shared through LDS by 128 rows of a cache head, or streamed by 16
   int splits;   // parts that a sequence's pages may be spread over
 };
 
@@ -573,10 +1125,32 @@ constexpr size_t kMostPartBytes = (size_t)256 << 20;
 Plan plan_of(const ldx_cache4_attention_args* p) {
   const int64_t heads = (int64_t)p->batch * p->cache.heads, rows = (int64_t)p->q_len * (p->q_heads / p->cache.heads);
   const int64_t most = (p->width + kLeastChunk - 1) / kLeastChunk;
-  int64_t s = 512 / (heads * ((rows + 15) / 16));
-  if (s > most) s = most;
-  if (p->width <= 32) s = 1;
   Plan plan;
+  const int D = p->cache.head_dim;
+  // A page of 16 rows is a unit of work. Sharing pages is ahead from about 40,000 of them on, at head width 256 from half of
+  // that where there are groups of rows enough to fill the card: 4 heads of 2,048 rows behind 4,096 tokens (37,000) 36 and
+  // 35 us shared at 64, 50 and 51 at 128, behind 16,384 118 and 68 at 64; 8 heads of 2,048 behind 1,024 (25,000) 27 and 30,
+  // 38 and 40, 88 and 72 at 256, 512 rows of 4 heads behind 16,384 (33,000) 39 and 46, 51 and 67, 110 and 130. At 32 the
+  // codes of a page are so few that there is nothing to share.
+  const int64_t groups = heads * ((rows + kWideRows - 1) / kWideRows), work = heads * ((rows + 15) / 16) * p->width;
+  plan.wide = D >= 64 && rows >= kWideRows && work >= (D == 256 && groups >= 64 ? 20000 : 40000);
+  int64_t s = 1;
+  if (plan.wide) {
+    // Rounds of workgroups on the CUs' places, the pages of a round, and what a part more costs: 3 pages of a round
+    // to join, or what it writes and the join reads, at 4.5 TB/s and 2.2 us a page of a round.
+    const int64_t places = D <= 128 ? 512 : 256;
+    const double traffic = 8e-7 * (double)(heads * rows) * (D + 2), part = traffic > 3.0 ? traffic : 3.0;
+    double best = 1e30;
+    for (int64_t i = 1; i <= kFewParts && i <= most; i++) {
+      if (split_bytes(p, (int)i) > kMostPartBytes) break;
+      const double cost = (double)((groups * i + places - 1) / places) * ((p->width + i - 1) / i) + part * i;
+      if (cost < best) best = cost, s = i;
+    }
+  } else {
+    s = 512 / (heads * ((rows + 15) / 16));
+    if (s > most) s = most;
+    if (p->width <= 32) s = 1;
+  }
   plan.splits = (int)(s < 1 ? 1 : s > kMostParts ? kMostParts : s);
   return plan;
 }
@@ -638,6 +1212,11 @@ extern "C" size_t ldx_cache4_attention_workspace_bytes(const ldx_cache4_attentio
   return check_attention(p) == LDX_OK ? split_bytes(p, plan_of(p).splits) : 0;
 }
 
+extern "C" int ldx_cache4_attention_rows(const ldx_cache4_attention_args* p) {
+  if (int rc = check_attention(p)) return rc;
+  return plan_of(p).wide ? kWideRows : 16;
+}
+
 extern "C" int ldx_cache4_attention(const ldx_cache4_attention_args* p, void* stream) {
   if (int rc = check_attention(p)) return rc;
   Plan plan = plan_of(p);
@@ -649,7 +1228,8 @@ extern "C" int ldx_cache4_attention(const ldx_cache4_attention_args* p, void* st
                          p->q, {p->q_stride[0], p->q_stride[1], p->q_stride[2]},
                          p->o, {p->o_stride[0], p->o_stride[1], p->o_stride[2]},
                          G, p->q_len, G * p->q_len, p->scale * 1.4426950408889634f,
-                         p->table, p->table_pitch, p->width, p->lengths, p->starts, plan.splits, kLeastChunk, 16,
+                         p->table, p->table_pitch, p->width, p->lengths, p->starts, plan.splits, kLeastChunk,
+                         plan.wide ? kWideRows : 16,
                          (float*)p->workspace};
   hipStream_t st = as_stream(stream);
   return p->dtype == LDX_DTYPE_F16 ? launch_t<f16>(a, p->cache.head_dim, p->batch, st)

@@ -1429,8 +1429,9 @@ def cache4_attention(q: torch.Tensor, cache: Cache4, table: torch.Tensor, length
     ``j`` reads the cache's head ``j // group``). With ``starts`` query ``i`` sees tokens up to position
     ``starts[b] + i`` (causal); without, all ``lengths[b]``. A query that sees no token gives 0; tokens that
     it does not see, and pages behind the length, do not touch its result. A page that the cache does
-    not have, or a length past the table, gives NaN. Scores, softmax and sums are fp32; probabilities enter their
-    product with 16 bits. Returns ``(B, heads, L, D)`` in ``q``'s type (into ``out`` when given, which may be
+    not have, or a length past the table, gives NaN. Scores, softmax and sums are fp32; probabilities are
+    rounded to 16 bits, or to fp16 (2^-11 of each, those below 2^-21 of a query's largest to 2^-32 of it) where
+    many queries share pages. Returns ``(B, heads, L, D)`` in ``q``'s type (into ``out`` when given, which may be
     ``q``); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
     block, dev = _cache4_block(cache, "cache4_attention")
     _need(q, "q", _ELEM, dev)

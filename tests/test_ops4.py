@@ -605,7 +605,34 @@ def test_read_says_when_a_page_is_wrong(pkg, dev) -> None:
 
 # ------------------------------------------------------------------ attention
 
-def attention_reference(ref, q, table, lengths, scale, starts, bits=16):
+# Columns of a page table with which 128 rows and more of one cache head share pages through LDS (the host decides by
+# the table's width); a table that is longer than its sequences is what serving keeps anyway.
+LONG = 5000
+
+
+def longer(table: torch.Tensor, width: int | None) -> torch.Tensor:
+    """``table`` followed by columns that name no page."""
+    return table if width is None else torch.nn.functional.pad(table, (0, width - table.shape[1]), value=-1)
+
+
+@pytest.mark.parametrize("d", DIMS)
+def test_attention_kernels_of_the_tested_widths(pkg, d) -> None:
+    """From 128 rows of a cache head on a table of LONG columns takes the kernel that shares pages, for any number of
+    heads and sequences; fewer rows, the tests' short tables and heads of 32 the streaming one."""
+    lib = pkg._lib
+
+    def rows(batch, heads, group, q_len, width):
+        a = lib.Cache4AttentionArgs(cache=_cache_args(lib, heads=heads, head_dim=d), batch=batch, q_heads=heads * group,
+                                    q_len=q_len, q=16, o=16, scale=1.0, table=16, table_pitch=width, width=width, lengths=16)
+        return lib.lib.ldx_cache4_attention_rows(ctypes.byref(a))
+
+    for batch, heads, group, q_len in ((1, 1, 1, 128), (7, 1, 3, 50), (1, 1, 2, 70), (4, 2, 1, 150), (2, 2, 2, 100), (1, 1, 1, 300)):
+        assert rows(batch, heads, group, q_len, LONG) == (16 if d == 32 else 128)
+        assert rows(1, heads, group, q_len, 8) == rows(batch, heads, group, 127 // group, LONG) == 16
+    assert rows(1, 3, 1, 0, 8) == lib.LDX_EINVAL
+
+
+def attention_reference(ref, q, table, lengths, scale, starts, shared=False):
     """(result, error allowed before the rounding to q's type) in float64."""
     b, hq, lq, d = q.shape
     out, allowed = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
@@ -629,12 +656,16 @@ def attention_reference(ref, q, table, lengths, scale, starts, bits=16):
         safe = torch.where(l > 0, l, 1.0)
         out[i] = p @ vz / safe
         mass = p @ vz.abs() / safe
-        # A probability enters the values' product with `bits` bits and their sum whole: 2^-bits of the mass. Scores are
-        # off by `off`; fp32 sums of n terms on both sides; the hardware's exponential (2^-22). One below fp32's normal
-        # numbers, 2^-126 of the largest, is 0: of a result of 1e-39 beside a dominant value of 0 that is a part.
+        # A probability enters the values' product with 16 bits and their sum whole: 2^-16 of the mass. Where pages are
+        # shared it is rounded to fp16 in both sums, p (1 + e) + u, |e| <= 2^-11, |u| <= 2^-32 of the largest: with o the
+        # exact result the quotient is off by sum (p e + u) (v - o) / sum p (1 + e), at most 2^-11 (mass + |o|) and 2^-32
+        # (sum |v| + n |o|) / sum p, times 1 + 2^-10 for the divisor. Scores are off by `off`; fp32 sums of n terms on
+        # both sides; the hardware's exponential (2^-22). One below fp32's normal numbers, 2^-126 of the largest, is 0: of
+        # a result of 1e-39 beside a dominant value of 0 that is a part.
         o = out[i].abs()
-        under = 2.0 ** -126 * (seen.double() @ vz.abs() + seen.sum(-1, keepdim=True) * o) / safe
-        allowed[i] = mass * 2.0 ** -bits + mass * (2.2 * off) + (mass + o) * (n + 40) * 2.0 ** -23 + under
+        least = (seen.double() @ vz.abs() + seen.sum(-1, keepdim=True) * o) / safe
+        rounded = ((mass + o) * 2.0 ** -11 + 2.0 ** -32 * least) * (1 + 2.0 ** -10) if shared else mass * 2.0 ** -16
+        allowed[i] = rounded + mass * (2.2 * off) + (mass + o) * (n + 40) * 2.0 ** -23 + 2.0 ** -126 * least
     return out, allowed
 
 
@@ -657,18 +688,25 @@ def filled(pkg, dev, b, heads, d, width, seed=0, lengths=None, spread=9):
     return cache, Pages(cache), table
 
 
-def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, seed=0, scale=None, spread=9):
+def agree(got, want, allowed):
+    """``got`` is ``want`` within ``allowed`` and the rounding to its type, past which numbers are infinite."""
+    t = got.dtype
+    bar = allowed * (1 + half_step(t)) + want.abs() * half_step(t) + tiny(t)
+    got = got.cpu().double()
+    past = got.isinf() & (got.sign() == want.sign()) & (want.abs() + bar >= torch.finfo(t).max * (1 + half_step(t) / 2))
+    err = (got - want).abs()
+    assert ((err <= bar) | past).all(), ((err / bar).max(), (~((err <= bar) | past)).nonzero()[:5])
+
+
+def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, seed=0, scale=None, spread=9, long=None):
     scale = d ** -0.5 if scale is None else scale
     cache, ref, table = filled(pkg, dev, b, heads, d, width, seed, lengths, spread)
     q = rand((b, heads * group, lq, d), seed + 7, t)
-    got = pkg.ops.cache4_attention(q.to(dev), cache, table.to(dev), lengths.to(dev), scale,
+    got = pkg.ops.cache4_attention(q.to(dev), cache, longer(table, long).to(dev), lengths.to(dev), scale,
                                    starts=None if starts is None else starts.to(dev))
     assert got.dtype == t and got.shape == q.shape
-    want, allowed = attention_reference(ref, q, table, lengths, scale, starts)
-    err = (got.cpu().double() - want).abs()
-    bar = allowed * (1 + half_step(t)) + want.abs() * half_step(t) + tiny(t)
-    assert (err <= bar).all(), ((err / bar).max(), (err > bar).nonzero()[:5])
-    return got
+    want, allowed = attention_reference(ref, q, table, lengths, scale, starts, long is not None)
+    agree(got, want, allowed)
 
 
 @gpu
@@ -694,6 +732,70 @@ def test_attention_causal(pkg, dev, heads, group, lq, d, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("t", HALF)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize(("heads", "group", "lq"), [(1, 1, 128), (2, 1, 129), (1, 3, 50), (2, 4, 65)])
+def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
+    """128 rows of a cache head and more: the last tile with one row, or full; lengths and starts as above; values whose
+    scales fp16 holds in all pages, and in some."""
+    starts = ints(0, 1, 100, -3, 250, 63)
+    lengths = ints(lq, lq + 1, 100 + lq, lq, 250 + max(lq // 2, 1), 63 + lq)
+    for spread in (5, 30):
+        attention_case(pkg, dev, t, 7, heads, group, d, lq, ints(0, 1, 63, 64, 65, 300, 448), None, 7, seed=d + lq, long=LONG, spread=spread)
+        attention_case(pkg, dev, t, 6, heads, group, d, lq, lengths, starts, 8, seed=d + lq, long=LONG, spread=spread)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_of_many_rows_in_parts(pkg, dev, d) -> None:
+    """Sequences of unequal lengths spread over several workgroups, some of which find nothing to do."""
+    attention_case(pkg, dev, torch.float16, 3, 1, 2, d, 70, ints(5000, 700, 1), None, 80, long=LONG)
+    attention_case(pkg, dev, torch.bfloat16, 3, 1, 1, d, 200, ints(5000, 700, 200), ints(4800, 500, 0), 80, long=LONG)
+
+
+@gpu
+@pytest.mark.parametrize("t", HALF)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_of_pages_beyond_fp16(pkg, dev, d, t) -> None:
+    """Single blocks whose scales fp16 does not hold, of keys or values, in the first, a middle or the last page: shared
+    pages go another way from there on."""
+    for slot, which in ((0, "k"), (1, "v"), (3, "k"), (4, "v"), (6, "v"), (6, "k")):
+        cache, _, table = filled(pkg, dev, 1, 1, d, 7, seed=slot, spread=3)
+        scales = (cache.k_scales if which == "k" else cache.v_scales).view(torch.uint8)
+        scales[int(table[0, slot]), 0, d // 32 - 1, 17 * slot % 50] = 60 if which == "k" else 150
+        ref, q = Pages(cache), rand((1, 2, 130, d), 7, t)
+        got = pkg.ops.cache4_attention(q.to(dev), cache, longer(table, LONG).to(dev), ints(440).to(dev), d ** -0.5, starts=ints(310).to(dev))
+        want, allowed = attention_reference(ref, q, table, ints(440), d ** -0.5, ints(310), True)
+        agree(got, want, allowed)
+
+
+@gpu
+@pytest.mark.parametrize("t", HALF)
+@pytest.mark.parametrize("d", DIMS)
+def test_attention_does_not_feel_what_stands_behind_a_sequence(pkg, dev, d, t) -> None:
+    """Any codes and any scales behind the length and in the table's other pages: the same bits."""
+    cache, _, table = filled(pkg, dev, 2, 1, d, 7, seed=1, spread=3)
+    lengths = ints(300, 64)
+    for lq, long in ((1, None), (150, None), (150, LONG)):
+        q = rand((2, 2, lq, d), 7, t).to(dev)
+        for starts in (None, (lengths - lq).to(dev)):
+            results = []
+            for seed in range(3):
+                g = torch.Generator().manual_seed(seed)
+                for i, n in enumerate(lengths.tolist()):
+                    for slot in range(n // 64, 7):
+                        page, lo = int(table[i, slot]), max(n - 64 * slot, 0)
+                        for x in (cache.k, cache.v):
+                            x[page, :, lo:] = torch.randint(0, 256, x[page, :, lo:].shape, dtype=torch.uint8, generator=g).to(dev)
+                        for x in (cache.k_scales, cache.v_scales):
+                            x = x.view(torch.uint8)[page, :, :, lo:]
+                            x.copy_(torch.randint(0, 256, x.shape, dtype=torch.uint8, generator=g))
+                results.append(pkg.ops.cache4_attention(q, cache, longer(table, long).to(dev), lengths.to(dev), 0.1, starts=starts))
+            assert results[0].isfinite().all()
+            assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+
+
+@gpu
 @pytest.mark.parametrize(("b", "heads", "group", "d", "n"), [(2, 1, 2, 32, 9000), (1, 1, 1, 64, 20000), (2, 2, 8, 128, 9001), (1, 1, 4, 256, 5000)])
 def test_attention_long(pkg, dev, b, heads, group, d, n) -> None:
     lengths = ints(*[n - 77 * i for i in range(b)])
@@ -714,9 +816,10 @@ def test_cache_beyond_4_gib(pkg, dev) -> None:
     n = ints(1203).to(dev)
     for mine, theirs in zip(pkg.ops.cache4_read(small, low, n, 1203), pkg.ops.cache4_read(big, high, n, 1203)):
         assert torch.equal(mine, theirs)
-    for lq in (1, 150):
+    for lq, long in ((1, None), (150, LONG)):
         q = rand((1, 8, lq, d), 3, torch.bfloat16).to(dev)
-        assert torch.equal(pkg.ops.cache4_attention(q, big, high, n, 0.1), pkg.ops.cache4_attention(q, small, low, n, 0.1))
+        got = pkg.ops.cache4_attention(q, big, longer(high, long), n, 0.1)
+        assert torch.equal(got, pkg.ops.cache4_attention(q, small, longer(low, long), n, 0.1))
 
 
 @gpu
@@ -725,7 +828,7 @@ def test_cache_beyond_4_gib(pkg, dev) -> None:
 def test_attention_in_place(pkg, dev, d, lq) -> None:
     cache, _, table = filled(pkg, dev, 2, 2, d, 60)
     q = rand((2, lq, 4, d), 3, torch.bfloat16).to(dev).transpose(1, 2)
-    args = cache, table.to(dev), ints(3800, 640).to(dev), 0.1
+    args = cache, longer(table, LONG if lq > 100 else None).to(dev), ints(3800, 640).to(dev), 0.1
     want = pkg.ops.cache4_attention(q, *args)
     got = pkg.ops.cache4_attention(q, *args, out=q)
     assert got is q and torch.equal(got, want)
@@ -736,8 +839,9 @@ def test_attention_in_place(pkg, dev, d, lq) -> None:
 @pytest.mark.parametrize("d", DIMS)
 def test_attention_value_scales_far_apart(pkg, dev, d, lq) -> None:
     """Values up to 2^80 apart, in both orders."""
-    attention_case(pkg, dev, torch.bfloat16, 2, 1, 1, d, lq, ints(1000, 640), None, 16, spread=40)
-    attention_case(pkg, dev, torch.bfloat16, 2, 1, 1, d, lq, ints(1000, 640), ints(1000 - lq, 500), 16, seed=5, spread=40)
+    long = LONG if lq > 100 and d > 32 else None
+    attention_case(pkg, dev, torch.bfloat16, 2, 1, 1, d, lq, ints(1000, 640), None, 16, spread=40, long=long)
+    attention_case(pkg, dev, torch.bfloat16, 2, 1, 1, d, lq, ints(1000, 640), ints(1000 - lq, 500), 16, seed=5, spread=40, long=long)
 
 
 @gpu
@@ -747,6 +851,10 @@ def test_attention_scores_far_apart(pkg, dev, lq) -> None:
     attention_case(pkg, dev, torch.float16, 2, 2, 2, 64, lq, ints(300, 129), None, 5, scale=3.0)
     attention_case(pkg, dev, torch.bfloat16, 2, 2, 2, 128, lq, ints(300, 129), ints(200, 100), 5, scale=-2.0)
     attention_case(pkg, dev, torch.float16, 2, 1, 2, 64, lq, ints(300, 129), None, 5, scale=0.0)
+    if lq == 100:
+        attention_case(pkg, dev, torch.float16, 2, 2, 2, 64, lq, ints(300, 129), None, 5, scale=3.0, long=LONG)
+        attention_case(pkg, dev, torch.bfloat16, 2, 2, 2, 128, lq, ints(300, 129), ints(200, 100), 5, scale=-2.0, long=LONG)
+        attention_case(pkg, dev, torch.float16, 2, 1, 2, 64, lq, ints(300, 129), None, 5, scale=0.0, long=LONG)
 
 
 @gpu
@@ -769,7 +877,7 @@ def test_attention_of_huge_scores(pkg, dev, lq, d, t) -> None:
         sure = top.values[..., 0] - top.values[..., 1] > 2 * off + 40      # ahead by more than fp32 scores are off
         assert sure.double().mean() > 0.9
         want = torch.stack([vv[h, top.indices[h, :, 0]] for h in range(2)])
-        got = pkg.ops.cache4_attention(q.to(dev), cache, table.to(dev), ints(n).to(dev), scale).cpu().double()
+        got = pkg.ops.cache4_attention(q.to(dev), cache, longer(table, LONG if lq > 100 else None).to(dev), ints(n).to(dev), scale).cpu().double()
         bad = (got[0] - want).abs() > want.abs() * (half_step(t) + 2.0 ** -10) + tiny(t)
         assert not (bad & sure[..., None]).any(), scale
 
@@ -799,7 +907,7 @@ def test_attention_keeps_the_weight_of_a_long_tail(pkg, dev, b, n, lq, d, first,
     allowed = off + 2200 * 2.0 ** -24 * (mass + o.abs())
     for t in HALF:
         q = torch.ones(b, 1, lq, d, dtype=t, device=dev)
-        got = pkg.ops.cache4_attention(q, cache, table.expand(b, -1).contiguous().to(dev),
+        got = pkg.ops.cache4_attention(q, cache, longer(table, LONG if lq > 100 else None).expand(b, -1).contiguous().to(dev),
                                        torch.full((b,), n + 1, dtype=torch.int32, device=dev), x * math.log(2.0) / (16 * d))
         err = (got.cpu().double() - o).abs()
         bar = allowed * (1 + half_step(t)) + o.abs() * half_step(t) + tiny(t)
@@ -819,8 +927,8 @@ def test_attention_of_small_scales(pkg, dev, lq, d, byte) -> None:
     q = ((torch.randint(0, 2, (1, 1, lq, d), generator=g) * 2.0 - 1) * 2.0 ** big).to(torch.bfloat16)
     ref = Pages(cache)
     for scale in (2.0 ** -8, 0.4, 3.0):
-        got = pkg.ops.cache4_attention(q.to(dev), cache, table.to(dev), ints(190).to(dev), scale).cpu().double()
-        want, allowed = attention_reference(ref, q, table, ints(190), scale, None)
+        got = pkg.ops.cache4_attention(q.to(dev), cache, longer(table, LONG if lq > 100 else None).to(dev), ints(190).to(dev), scale).cpu().double()
+        want, allowed = attention_reference(ref, q, table, ints(190), scale, None, lq > 100)
         bar = allowed * (1 + half_step(q.dtype)) + want.abs() * half_step(q.dtype) + tiny(q.dtype) + 2.0 ** -126
         assert ((got - want).abs() <= bar).all(), (scale, ((got - want).abs() / bar).max())
 
@@ -836,58 +944,71 @@ def test_attention_loud_tokens_of_small_weight(pkg, dev, lq, d) -> None:
     k[:, :, 64:128] = -16.0
     v[:, :, 64:128, :32] *= 2.0 ** 30
     pkg.ops.cache4_append(cache, k, v, table.to(dev), ints(0).to(dev))
-    got = pkg.ops.cache4_attention(q, cache, table.to(dev), ints(256).to(dev), 1.0).cpu().double()
+    got = pkg.ops.cache4_attention(q, cache, longer(table, LONG if lq > 100 else None).to(dev), ints(256).to(dev), 1.0).cpu().double()
     want, _ = attention_reference(Pages(cache), q.cpu(), table, ints(256), 1.0, None)
     # equal probabilities of 1: their rounding is exact, the sums are fp32
     assert ((got - want).abs() <= want.abs() * half_step(torch.float16) + 300 * 2.0 ** -23 * 4).all()
 
 
 @gpu
-@pytest.mark.parametrize(("lq", "group", "d"), [(4, 1, 64), (70, 1, 64), (33, 4, 128), (200, 1, 32), (100, 2, 256), (200, 1, 64), (130, 2, 128), (300, 1, 256)])
+@pytest.mark.parametrize(("lq", "group", "d", "long"), [
+    (4, 1, 64, None), (70, 1, 64, None), (33, 4, 128, None), (200, 1, 32, None), (100, 2, 256, None), (200, 1, 64, LONG),
+    (130, 2, 128, LONG), (300, 1, 256, LONG)])
 @pytest.mark.parametrize("byte", [255, 254, 253])
-def test_attention_nan_in_tokens_that_a_query_does_not_see(pkg, dev, lq, group, d, byte) -> None:
+def test_attention_nan_in_tokens_that_a_query_does_not_see(pkg, dev, lq, group, d, long, byte) -> None:
     """A NaN key and a NaN value: queries before them are untouched, queries from them on are NaN (in that block of channels,
-    for a value); scales whose values pass fp32 touch no query that does not see them either."""
-    cache, _, table = filled(pkg, dev, 1, 1, d, 7, seed=1)
-    q = rand((1, group, lq, d), 2, torch.float16).to(dev)
-    args = (table.to(dev), ints(100 + lq).to(dev), d ** -0.5)
-    starts = ints(100).to(dev)
-    clean = pkg.ops.cache4_attention(q, cache, *args, starts=starts)
+    for a value); scales whose values pass fp32 touch no query that does not see them either. Where pages are shared the
+    others' probabilities are rounded to 16 bits instead of to fp16, as everywhere beside such scales."""
+    cache, _, table = filled(pkg, dev, 1, 1, d, 7, seed=1, spread=3)
+    q = rand((1, group, lq, d), 2, torch.float16)
+    args = (longer(table, long).to(dev), ints(100 + lq).to(dev), d ** -0.5)
+    starts = ints(100)
+    run = lambda: pkg.ops.cache4_attention(q.to(dev), cache, *args, starts=starts.to(dev)).cpu()
+    clean = run()
+    want, allowed = attention_reference(Pages(cache), q, table, ints(100 + lq), d ** -0.5, starts, long is not None)
+    bar = allowed * (1 + half_step(q.dtype)) + want.abs() * half_step(q.dtype) + tiny(q.dtype)
+
+    def untouched(got, *where):
+        if long is None:
+            assert torch.equal(got[where], clean[where])
+        assert ((got.double() - want).abs() <= bar)[where].all()
+
     at, blk = 100 + lq // 2, d // 32 - 1
     page, slot = int(table[0, at // 64]), at % 64
     mine = list(range(32 * blk, 32 * blk + 32))
     rest = [i for i in range(d) if i not in mine]
-    was = cache.v_scales.view(torch.uint8)[page, 0, blk, slot].clone()
-    cache.v_scales.view(torch.uint8)[page, 0, blk, slot] = byte
-    got = pkg.ops.cache4_attention(q, cache, *args, starts=starts)
-    assert torch.equal(got[:, :, :lq // 2], clean[:, :, :lq // 2])
-    assert torch.equal(got[..., rest], clean[..., rest])
+    scales = cache.v_scales.view(torch.uint8)
+    was = scales[page, 0, blk, slot].clone()
+    scales[page, 0, blk, slot] = byte
+    got = run()
+    untouched(got, slice(None), slice(None), slice(0, lq // 2))
+    untouched(got, Ellipsis, rest)
     if byte == 255:
         assert got[:, :, lq // 2:, mine].isnan().all()
-    cache.v_scales.view(torch.uint8)[page, 0, blk, slot] = was
+    scales[page, 0, blk, slot] = was
     cache.k_scales.view(torch.uint8)[page, 0, blk, slot] = byte
-    got = pkg.ops.cache4_attention(q, cache, *args, starts=starts)
-    assert torch.equal(got[:, :, :lq // 2], clean[:, :, :lq // 2])
+    got = run()
+    untouched(got, slice(None), slice(None), slice(0, lq // 2))
     if byte == 255:
         assert got[:, :, lq // 2:].isnan().all()
 
 
 @gpu
-@pytest.mark.parametrize("lq", [1, 90, 150])
-def test_attention_says_when_a_page_or_a_length_is_wrong(pkg, dev, lq) -> None:
+@pytest.mark.parametrize(("lq", "long"), [(1, None), (90, None), (150, None), (150, LONG)])
+def test_attention_says_when_a_page_or_a_length_is_wrong(pkg, dev, lq, long) -> None:
     cache, _, table = filled(pkg, dev, 4, 2, 64, 5, seed=1)
     q = rand((4, 2, lq, 64), 2, torch.float16).to(dev)
     lengths = ints(320, 320, 130, 320)
-    good = pkg.ops.cache4_attention(q, cache, table.to(dev), lengths.to(dev), 0.1)
+    good = pkg.ops.cache4_attention(q, cache, longer(table, long).to(dev), lengths.to(dev), 0.1)
     table[1, 3], table[2, 3], table[3, 1] = 1 << 30, -7, -1      # sequence 2 does not reach its bad page
-    got = pkg.ops.cache4_attention(q, cache, table.to(dev), lengths.to(dev), 0.1)
+    got = pkg.ops.cache4_attention(q, cache, longer(table, long).to(dev), lengths.to(dev), 0.1)
     assert torch.equal(got[[0, 2]], good[[0, 2]]) and got[[1, 3]].isnan().all()
-    got = pkg.ops.cache4_attention(q, cache, table.to(dev), ints(320, -4, 321, 1 << 30).to(dev), 0.1)
+    got = pkg.ops.cache4_attention(q, cache, longer(table, long).to(dev), ints(320, -4, (long or 5) * 64 + 1, 1 << 30).to(dev), 0.1)
     assert torch.equal(got[0], good[0]) and (got[1] == 0).all() and got[2:].isnan().all()
 
 
 @gpu
-@pytest.mark.parametrize(("lq", "width"), [(1, 9), (70, 9), (140, 9), (1, 300)])
+@pytest.mark.parametrize(("lq", "width"), [(1, 9), (70, 9), (140, LONG), (1, 300)])
 def test_attention_layouts(pkg, dev, lq, width) -> None:
     """Head-interleaved q and out, a table that is part of a wider one, out given."""
     cache, _, table = filled(pkg, dev, 2, 2, 64, 5, seed=1)
