@@ -11,6 +11,10 @@
 // sines, which the heads share, then a lane takes a part of a head, and the lanes of a head add their squares. Where pairs
 // are neighbours, or the halves of all sections whole fours, a lane holds both ends of its pairs; else it takes channels
 // as they lie, so that every access to memory is of whole lines, and gets the other ends through LDS.
+//
+// Bound by memory: 51,200 tokens of 16 query and 16 key heads of 32 in fp16, three axes, 45 us, 4.7 TB/s; 16,384 of 32 and 8
+// heads of 128 in bf16 64, 5.2. Few heads are bound by the launch (a token's 3.3 us). Queries and keys in the same
+// workgroups, without the next head asked for ahead, took 104 and 78.
 #include "quant8.h"
 
 namespace ldx {

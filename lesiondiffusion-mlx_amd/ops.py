@@ -1247,6 +1247,12 @@ def _heads_out(out: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Te
     return out
 
 
+def _in_place(out: torch.Tensor, x: torch.Tensor, name: str) -> None:
+    """An output that begins where its input does is that input, value for value."""
+    if out.data_ptr() == x.data_ptr() and any(n > 1 and s != t for n, s, t in zip(x.shape, out.stride(), x.stride())):
+        raise ValueError(f"{name} stands in its input's place with strides {out.stride()}, not {x.stride()}")
+
+
 def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, *,
                  q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, eps: float = 1e-6,
                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
@@ -1257,7 +1263,7 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     (axes, B, L) for several (a volume's depth, height and width), any strides, so that one row expanded serves
     the batch; ``rotary`` says how an axis turns (at most four). Angles are reduced in fp64: position 10^9
     has its own. Norm and rotation are fp32, rounded once. Returns ``(q, k)``, or ``q`` without keys, in the
-    inputs' type: into ``q_out`` and ``k_out`` when given, which may be the inputs, else with a token's heads
+    inputs' type: into ``q_out`` and ``k_out`` when given, each of which may be its own input, else with a token's heads
     side by side in memory (``(B, L, H * D)`` is a view)."""
     _need(q, "q", _ALL, -1)
     dev, shape, dtype = q.get_device(), q.shape, q.dtype
@@ -1284,6 +1290,8 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if k_gamma is not None:
         k_gamma = _head_gamma(k_gamma, "k_gamma", d, dev)
     qo = _heads_out(q_out, q, "q_out")
+    if q_out is not None:
+        _in_place(qo, q, "q_out")
     ko, kh, ks, kos = None, 0, (0, 0, 0), (0, 0, 0)
     if k is None:
         if k_out is not None or k_gamma is not None:
@@ -1294,8 +1302,13 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if len(kshape) != 4 or kshape[0] != b or kshape[2] != l or kshape[3] != d or not 0 < kshape[1] <= _MOST:
             raise ValueError(f"k {tuple(kshape)} does not fit q {tuple(shape)}")
         ko, kh = _heads_out(k_out, k, "k_out"), kshape[1]
-        if ko.data_ptr() == qo.data_ptr():
+        if k_out is not None:
+            _in_place(ko, k, "k_out")
+        at_q, at_k = qo.data_ptr(), ko.data_ptr()
+        if at_k == at_q:
             raise ValueError("rotate_heads: q_out and k_out are the same tensor")
+        if at_q == k.data_ptr() or at_k == q.data_ptr():
+            raise ValueError("rotate_heads: an output may be its own input, not the other")
         ks, kos = _head_strides(k, "k"), _head_strides(ko, "k_out")
     a = RotateHeadsArgs(b, l, h, kh, d, ALL_DTYPES[dtype], q.data_ptr(), _head_strides(q, "q"), qo.data_ptr(),
                         _head_strides(qo, "q_out"), _ptr(k), ks, _ptr(ko), kos, _ptr(q_gamma), _ptr(k_gamma), eps, n, axes,
@@ -1448,6 +1461,7 @@ def cache4_attention(q: torch.Tensor, cache: Cache4, table: torch.Tensor, length
             raise ValueError(f"out shape {tuple(out.shape)} != {tuple(shape)}")
         if not out.is_contiguous():
             _distinct(out, "out")
+        _in_place(out, q, "out")
     else:
         out = q.new_empty(shape)
     a = Cache4AttentionArgs(block, b, hq, lq, q.data_ptr(), _head_strides(q, "q"), out.data_ptr(),

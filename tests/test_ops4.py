@@ -380,7 +380,11 @@ def test_rotate_refuses_on_the_device(pkg, dev) -> None:
                  lambda: ops.rotate_heads(q, None, at, rotary, q_gamma=torch.ones(64, device=dev), eps=0.0),
                  lambda: ops.rotate_heads(q, None, at, rotary, q_out=q[:, :1]),
                  lambda: ops.rotate_heads(q, None, at, rotary, q_out=q[:, :1].expand(1, 2, 3, 64)),
-                 lambda: ops.rotate_heads(q, q, at, rotary, q_out=q, k_out=q)):
+                 lambda: ops.rotate_heads(q, q, at, rotary, q_out=q, k_out=q),
+                 lambda: ops.rotate_heads(q, q, at, rotary, q_out=q),
+                 lambda: ops.rotate_heads(q, q.clone(), at, rotary, k_out=q),
+                 lambda: ops.rotate_heads(q, None, at, rotary, q_out=q.view(1, 3, 2, 64).transpose(1, 2)),
+                 lambda: ops.rotate_heads(q.clone(), q, at, rotary, k_out=q.view(1, 3, 2, 64).transpose(1, 2))):
         with pytest.raises(ValueError):
             call()
 
@@ -1048,6 +1052,7 @@ def test_cache_refuses_on_the_device(pkg, dev) -> None:
                  lambda: ops.cache4_attention(q, cache, table, n, NAN),
                  lambda: ops.cache4_attention(q, cache, table, n, 1.0, out=q[:, :, :2]),
                  lambda: ops.cache4_attention(q, cache, table, n, 1.0, out=q[:, :, :1].expand(-1, -1, 3, -1)),
+                 lambda: ops.cache4_attention(q, cache, table, n, 1.0, out=q.view(1, 3, 2, 64).transpose(1, 2)),
                  lambda: ops.cache4_attention(q, cache, table, n, 1.0, starts=n.cpu()),
                  lambda: ops.cache4_append(cache, q, q[:, :, :1], table, n),
                  lambda: ops.cache4_append(cache, q, q.float(), table, n),
