@@ -21,8 +21,8 @@ from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import (ACT_GELU, ACT_NONE, ACT_SILU, BLOCK4, BLOCK8, PAGE4, PAGE8, ROTARY_AXES, AttnArgs, Cache4AppendArgs,
-                   Cache4AttentionArgs, Cache4Block, Cache4ReadArgs, Cache8AppendArgs, Cache8AttentionArgs, Cache8Block,
-                   ConvArgs, Dense8Args, RmsNormArgs, RotateHeadsArgs, SourceConvArgs, check, lib)
+                   Cache4AttentionArgs, Cache4ReadArgs, Cache8AppendArgs, Cache8AttentionArgs, Cache8Block,
+                   ConvArgs, Dense8Args, RmsNormArgs, RotateHeadsArgs, SourceConvArgs, check, filler, lib)
 
 __all__ = [
     "PackedWeight", "pack_weight", "pack_upsample_weight", "nax_conv3d", "conv3d", "dense",
@@ -1247,6 +1247,10 @@ def _heads_out(out: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Te
     return out
 
 
+_rotate_heads_args = filler(RotateHeadsArgs)
+_NO_KEYS, _NO_AXES = (0,) * 8, (0,) * ROTARY_AXES
+
+
 def _in_place(out: torch.Tensor, x: torch.Tensor, name: str) -> None:
     """An output that begins where its input does is that input, value for value."""
     if out.data_ptr() == x.data_ptr() and any(n > 1 and s != t for n, s, t in zip(x.shape, out.stride(), x.stride())):
@@ -1292,7 +1296,7 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     qo = _heads_out(q_out, q, "q_out")
     if q_out is not None:
         _in_place(qo, q, "q_out")
-    ko, kh, ks, kos = None, 0, (0, 0, 0), (0, 0, 0)
+    ko, kh, keys = None, 0, _NO_KEYS
     if k is None:
         if k_out is not None or k_gamma is not None:
             raise ValueError("rotate_heads: k_out and k_gamma need keys")
@@ -1309,10 +1313,11 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             raise ValueError("rotate_heads: q_out and k_out are the same tensor")
         if at_q == k.data_ptr() or at_k == q.data_ptr():
             raise ValueError("rotate_heads: an output may be its own input, not the other")
-        ks, kos = _head_strides(k, "k"), _head_strides(ko, "k_out")
-    a = RotateHeadsArgs(b, l, h, kh, d, ALL_DTYPES[dtype], q.data_ptr(), _head_strides(q, "q"), qo.data_ptr(),
-                        _head_strides(qo, "q_out"), _ptr(k), ks, _ptr(ko), kos, _ptr(q_gamma), _ptr(k_gamma), eps, n, axes,
-                        rotary.interleaved, positions.data_ptr(), at, turns.data_ptr())
+        keys = (k.data_ptr(), *_head_strides(k, "k"), at_k, *_head_strides(ko, "k_out"))
+    a = _rotate_heads_args(b, l, h, kh, d, ALL_DTYPES[dtype], q.data_ptr(), *_head_strides(q, "q"), qo.data_ptr(),
+                           *_head_strides(qo, "q_out"), *keys, 0 if q_gamma is None else q_gamma.data_ptr(),
+                           0 if k_gamma is None else k_gamma.data_ptr(), eps, n, *axes, *_NO_AXES[n:],
+                           rotary.interleaved, positions.data_ptr(), *at, turns.data_ptr())
     _launch8(lib.ldx_rotate_heads, (ctypes.byref(a),), dev, "rotate_heads")
     if q_out is not None:
         _wrote(q_out)
@@ -1343,8 +1348,12 @@ class Cache4:
         return Cache4(*codes, *scales)
 
 
-def _cache4_block(cache: Cache4, what: str) -> tuple[Cache4Block, int]:
-    """The C view of a cache and its device."""
+_cache4_append_args, _cache4_read_args = filler(Cache4AppendArgs), filler(Cache4ReadArgs)
+_cache4_attention_args = filler(Cache4AttentionArgs)
+
+
+def _cache4_block(cache: Cache4, what: str) -> tuple[tuple[int, ...], int]:
+    """What the C view of a cache holds (its pointers, pages, heads and head width), and its device."""
     if not isinstance(cache, Cache4):
         raise ValueError(f"{what}: cache must be a Cache4")
     k, v, ks, vs = cache.k, cache.v, cache.k_scales, cache.v_scales
@@ -1366,7 +1375,7 @@ def _cache4_block(cache: Cache4, what: str) -> tuple[Cache4Block, int]:
         raise ValueError("cache tensors must be contiguous")
     if not 0 < pages <= _MOST or not 0 < heads <= _MOST:
         raise ValueError(f"{what}: {pages} pages of {heads} heads")
-    return Cache4Block(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, 2 * half), dev
+    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, 2 * half), dev
 
 
 def cache4_append(cache: Cache4, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, *,
@@ -1379,18 +1388,19 @@ def cache4_append(cache: Cache4, k: torch.Tensor, v: torch.Tensor, table: torch.
     cache does not have are left out; no token is written by two sequences. ``table``, ``starts`` and ``counts``
     are int32 on the device, so a captured graph appends where they say at each replay."""
     block, dev = _cache4_block(cache, "cache4_append")
+    heads, d = block[5:]
     _need(k, "k", _ALL, dev)
     _need(v, "v", k.dtype, dev)
     shape = k.shape
-    if len(shape) != 4 or shape != v.shape or shape[1] != block.heads or shape[3] != block.head_dim or not shape[0] \
+    if len(shape) != 4 or shape != v.shape or shape[1] != heads or shape[3] != d or not shape[0] \
             or not shape[2]:
-        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must be (B, {block.heads}, L, {block.head_dim})")
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must be (B, {heads}, L, {d})")
     b, _, n, _ = shape
     if b > _MOST or n > _MOST:
         raise ValueError(f"cache4_append: {b} x {n} tokens")
-    a = Cache4AppendArgs(block, b, n, k.data_ptr(), _head_strides(k, "k"), v.data_ptr(), _head_strides(v, "v"),
-                         ALL_DTYPES[k.dtype], *_cache_table(table, b, dev), _cache_ints(starts, "starts", b, dev),
-                         None if counts is None else _cache_ints(counts, "counts", b, dev))
+    a = _cache4_append_args(*block, b, n, k.data_ptr(), *_head_strides(k, "k"), v.data_ptr(), *_head_strides(v, "v"),
+                            ALL_DTYPES[k.dtype], *_cache_table(table, b, dev), _cache_ints(starts, "starts", b, dev),
+                            0 if counts is None else _cache_ints(counts, "counts", b, dev))
     _launch8(lib.ldx_cache4_append, (ctypes.byref(a),), dev, "cache4_append")
     if not cache.k.is_inference():
         increment_version((cache.k, cache.v, cache.k_scales, cache.v_scales))
@@ -1405,6 +1415,7 @@ def cache4_read(cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, token
     channels), they are left as they were. A page that the cache does not have, or a token past the table, gives
     NaN. ``table``, ``lengths`` and ``starts`` are int32 on the device."""
     block, dev = _cache4_block(cache, "cache4_read")
+    heads, d = block[5:]
     if dtype not in ALL_DTYPES:
         raise ValueError(f"dtype must be fp16, bf16 or fp32, not {dtype}")
     if not isinstance(tokens, int) or not 0 < tokens <= _MOST:
@@ -1412,7 +1423,7 @@ def cache4_read(cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, token
     b = lengths.shape[0] if isinstance(lengths, torch.Tensor) and lengths.dim() == 1 else 0
     if not 0 < b <= _MOST:
         raise ValueError("lengths must be int32 (B,)")
-    shape = (b, block.heads, tokens, block.head_dim)
+    shape = (b, heads, tokens, d)
     if out is None:
         k, v = (cache.k.new_empty(shape, dtype=dtype) for _ in range(2))
     else:
@@ -1425,9 +1436,10 @@ def cache4_read(cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, token
                 _distinct(t, name)
         if k.data_ptr() == v.data_ptr():
             raise ValueError("cache4_read: out's k and v are the same tensor")
-    a = Cache4ReadArgs(block, b, tokens, k.data_ptr(), _head_strides(k, "out k"), v.data_ptr(), _head_strides(v, "out v"),
-                       ALL_DTYPES[dtype], *_cache_table(table, b, dev), _cache_ints(lengths, "lengths", b, dev),
-                       None if starts is None else _cache_ints(starts, "starts", b, dev), out is None)
+    a = _cache4_read_args(*block, b, tokens, k.data_ptr(), *_head_strides(k, "out k"), v.data_ptr(),
+                          *_head_strides(v, "out v"), ALL_DTYPES[dtype], *_cache_table(table, b, dev),
+                          _cache_ints(lengths, "lengths", b, dev),
+                          0 if starts is None else _cache_ints(starts, "starts", b, dev), out is None)
     _launch8(lib.ldx_cache4_read, (ctypes.byref(a),), dev, "cache4_read")
     if out is not None:
         _wrote(k)
@@ -1447,10 +1459,11 @@ def cache4_attention(q: torch.Tensor, cache: Cache4, table: torch.Tensor, length
     many queries share pages. Returns ``(B, heads, L, D)`` in ``q``'s type (into ``out`` when given, which may be
     ``q``); ``table``, ``lengths`` and ``starts`` are int32 on the device."""
     block, dev = _cache4_block(cache, "cache4_attention")
+    heads, d = block[5:]
     _need(q, "q", _ELEM, dev)
     shape = q.shape
-    if len(shape) != 4 or shape[3] != block.head_dim or shape[1] % block.heads or not q.numel():
-        raise ValueError(f"q {tuple(shape)} must be (B, a multiple of {block.heads}, L, {block.head_dim})")
+    if len(shape) != 4 or shape[3] != d or shape[1] % heads or not q.numel():
+        raise ValueError(f"q {tuple(shape)} must be (B, a multiple of {heads}, L, {d})")
     b, hq, lq, _ = shape
     if b > _MOST or hq > _MOST or lq > _MOST:
         raise ValueError(f"cache4_attention: {b} x {hq} x {lq} queries")
@@ -1464,10 +1477,10 @@ def cache4_attention(q: torch.Tensor, cache: Cache4, table: torch.Tensor, length
         _in_place(out, q, "out")
     else:
         out = q.new_empty(shape)
-    a = Cache4AttentionArgs(block, b, hq, lq, q.data_ptr(), _head_strides(q, "q"), out.data_ptr(),
-                            _head_strides(out, "out"), ALL_DTYPES[q.dtype], scale, *_cache_table(table, b, dev),
-                            _cache_ints(lengths, "lengths", b, dev),
-                            None if starts is None else _cache_ints(starts, "starts", b, dev))
+    a = _cache4_attention_args(*block, b, hq, lq, q.data_ptr(), *_head_strides(q, "q"), out.data_ptr(),
+                               *_head_strides(out, "out"), ALL_DTYPES[q.dtype], scale, *_cache_table(table, b, dev),
+                               _cache_ints(lengths, "lengths", b, dev),
+                               0 if starts is None else _cache_ints(starts, "starts", b, dev), 0, 0)
     ref = ctypes.byref(a)
     ws_bytes = lib.ldx_cache4_attention_workspace_bytes(ref)
     if ws_bytes:

@@ -66,6 +66,23 @@ def test_structs_match_c_layout(pkg, tmp_path) -> None:
         assert int(val) == want, line
 
 
+def test_fillers_put_each_value_where_its_field_is(pkg) -> None:
+    import ctypes
+    flat = lambda v: [x for i in v for x in flat(i)] if isinstance(v, ctypes.Array) else \
+        [x for name, _ in v._fields_ for x in flat(getattr(v, name))] if isinstance(v, ctypes.Structure) else [v]
+    for kind in (pkg._lib.RotateHeadsArgs, pkg._lib.Cache4AppendArgs, pkg._lib.Cache4ReadArgs, pkg._lib.Cache4AttentionArgs):
+        fill, values = pkg._lib.filler(kind), list(range(1, len(flat(kind())) + 1))
+        assert flat(fill(*values)) == values
+        for bad in (values[:-1], [*values, 1], [1 << 64, *values[1:]], [*values[:-1], None], [*values[:-1], 1.5]):
+            with pytest.raises(ValueError, match=kind.__name__):
+                fill(*bad)
+    for scale in (1e300, "1"):
+        values = list(range(1, len(flat(pkg._lib.Cache4AttentionArgs())) + 1))
+        values[19] = scale
+        with pytest.raises(ValueError, match="Cache4AttentionArgs"):
+            pkg.ops._cache4_attention_args(*values)
+
+
 def refused(pkg, rc: int, word: str) -> None:
     assert rc == pkg._lib.LDX_EINVAL
     assert word in pkg._lib.last_error(), pkg._lib.last_error()
@@ -214,7 +231,7 @@ def test_sizes_beyond_the_abi_fields_are_refused(pkg, monkeypatch) -> None:
         ops.cache4_read(big, ints32(1, 1), ints32(1), 3)
     monkeypatch.undo()
     monkeypatch.setattr(ops, "_need", lambda *a: None)
-    monkeypatch.setattr(ops, "_cache4_block", lambda c, what: (pkg._lib.Cache4Block(16, 16, 16, 16, 2, 1, 32), 0))
+    monkeypatch.setattr(ops, "_cache4_block", lambda c, what: ((16, 16, 16, 16, 2, 1, 32), 0))
     for word, call in (
             ("tokens", lambda: ops.cache4_append(cache, kv, kv, ints32(1, 1), ints32(1))),
             ("tokens", lambda: ops.cache4_append(cache, many, many, ints32(huge, 1), ints32(huge))),
