@@ -533,7 +533,7 @@ __global__ __launch_bounds__(64 * kWaves4, D == 256 ? 1 : 2) void attend4_kernel
 // products between the widening of later pages' codes, an instruction of the matrix units and some of the vector units in
 // turn, so that a wave keeps both busy by itself. (One after the other, 2,048 causal queries of 8 x 4 heads of 128 behind
 // 8,192 tokens 445 us, so 345 to 380, 820 to 900 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 tokens 130 and 7 for the join,
-// of 256 1,160 and 540.) Matrix units, vector units and LDS are each busy half of the time then, at the 2.0 GHz that the
+// of 256 1,160 and 540, of 32 97 and 6, with three waves a SIMD (two 109, four, which spill registers, 160).) Matrix units, vector units and LDS are each busy half of the time then, at the 2.0 GHz that the
 // power allows.
 constexpr int kWideRows = 128;
 // A query's reference is this much below its maximum, and lags kLag behind it: probabilities reach 2^15, and fp16 holds
@@ -588,15 +588,15 @@ struct Vec8<bf16> { typedef bf16x8 V; };
 // 64 short of one, so that the four meet all banks once).
 template <int D>
 struct WideLds {
-  static constexpr int KF = 1024 + 4096 / D, KEYS = 2 * (D / 16) * KF, VROW = 2 * D + 64;
+  static constexpr int KF = 1024 + 4096 / D, KEYS = 2 * (D / 16) * KF, VROW = D == 32 ? 64 : 2 * D + 64;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Attend4Args a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 32 ? 3 : 2) void attend4_wide_kernel(Attend4Args a) {
   typedef typename Vec8<T>::V V8;
   constexpr int NJ = D / 16;               // products per key tile
   constexpr int NT = D / 32;               // channel tiles; blocks
-  constexpr int RAW = D / 64;              // 8-byte pieces of a page's keys (values) that a thread widens
+  constexpr int RAW = D == 32 ? 1 : D / 64;   // 8-byte pieces of a page's keys (values) that a thread widens
   constexpr int CHECK = D == 256 ? 2 : 1;  // words of a page's key (value) scales that a lane looks at
   typedef WideLds<D> L;
   extern __shared__ __align__(16) uint8_t lds[];
@@ -650,18 +650,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Att
     int scale[RAW];
   };
   Raw kraw, vraw;
-  const unsigned soff = tid % NJ / 2 * kPage4 + tid / NJ;   // (256 / NJ tokens on for the next piece)
-  const auto load = [&](const uint8_t* codes, const uint8_t* scales, int64_t at, Raw& raw) __attribute__((always_inline)) {
+  // At head width 32 there are 128 pieces, for two waves: the others have the values'.
+  const int vid = D == 32 ? tid ^ 128 : tid;
+  const auto load = [&](const uint8_t* codes, const uint8_t* scales, int64_t at, int id, Raw& raw) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t cr = make_rsrc(codes + at * (kPage4 * D / 2), kPage4 * D / 2);
     const __amdgpu_buffer_rsrc_t sr = make_rsrc(scales + at * (kPage4 * NT), kPage4 * NT);
+    const unsigned soff = id % NJ / 2 * kPage4 + id / NJ;   // (256 / NJ tokens on for the next piece)
 #pragma unroll
     for (int i = 0; i < RAW; i++) {
-      raw.codes[i] = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(cr, tid * 8, 2048 * i, 0));
+      raw.codes[i] = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(cr, id * 8, 2048 * i, 0));
       raw.scale[i] = __builtin_amdgcn_raw_buffer_load_b8(sr, soff, 256 / NJ * i, 0);
     }
   };
-  // A page's scales, which every wave looks at, so that all take the page alike. (At head width 64 half of the lanes read
-  // behind them, zeros, which stand for nothing.)
+  // A page's scales, which every wave looks at, so that all take the page alike. (At head widths 64 and 32 the other lanes
+  // read behind them, zeros, which stand for nothing.)
   struct Check {
     int word[CHECK];
   };
@@ -681,7 +683,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Att
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < CHECK; i++) bad |= !within_fp16(c.word[i]);
-    return (bool)__any(bad && (D > 64 || lane < 32));
+    return (bool)__any(bad && lane < 16 * NT);
   };
   const auto times = [&](float f) __attribute__((always_inline)) {
 #pragma unroll
@@ -692,6 +694,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Att
   // Widen half x of a thread's piece i of the keys, or the values, into buffer `to`.
   const auto widen_key = [&](uint8_t* to, int i, int x, auto kt) __attribute__((always_inline)) {
     typedef decltype(kt) KT;
+    if (D == 32 && wave >= 2) return;
     const int e = tid + 256 * i, key = e / NJ, j = e % NJ;
     const int t = key & 31, at = 8 * (t >> 2 & 3) + 4 * (t >> 4) + (t & 3);   // the token's row of its tile
     const float s = __int_as_float(kraw.scale[i] << 23);
@@ -702,12 +705,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Att
   };
   const auto widen_value = [&](uint8_t* to, int left, int i, int x, auto vt) __attribute__((always_inline)) {
     typedef decltype(vt) VT;
-    const int e = tid + 256 * i, key = e / NJ, j = e % NJ;
+    if (D == 32 && wave < 2) return;
+    const int e = vid + 256 * i, key = e / NJ, j = e % NJ;
     // Values of tokens that none of the rows sees get a scale of 1: probabilities of 0 times anything finite; in bf16
     // those of NaN (and past fp32), too, see below.
     const bool one = key >= left || (__is_same(VT, bf16) && vraw.scale[i] >= 253);
     const float s = __int_as_float((one ? 127 : vraw.scale[i]) << 23);
-    const int flip = (D == 256 ? j >> 3 : D == 128 ? j >> 2 : key) & 1;   // 16 lanes write 16 bytes each, half of them first halves
+    const int flip = (D == 256 ? j >> 3 : D == 128 ? j >> 2 : D == 64 ? key : key >> 2) & 1;   // 16 lanes write 16 bytes each, half of them first halves
     const int c0 = vraw.codes[i][x], c1 = vraw.codes[i][1 - x];
     const unsigned codes = (unsigned)(flip ? c1 : c0);
     u32x4 w;
@@ -849,7 +853,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Att
   // kto and vto (of the page's `left` tokens that count). A product's operand is read two products ahead.
   const auto both = [&](const Scores& now, Scores& next, float kc, float ref, const uint8_t* kb, const uint8_t* vb, uint8_t* kto,
                         uint8_t* vto, int left) __attribute__((always_inline)) {
-    constexpr int NK = 2 * NJ, NV = 4 * NT, AHEAD = D == 64 ? 3 : 2;
+    constexpr int NK = 2 * NJ, NV = 4 * NT, AHEAD = D <= 64 ? 3 : 2;
     const auto key = [&](int i) __attribute__((always_inline)) {
       return *reinterpret_cast<const V8*>(kb + lane * 16 + (i % 2 * NJ + i / 2) * L::KF);
     };
@@ -883,8 +887,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Att
     for (int i = 0; i < NV; i++) {
       acc[i % NT] = mfma_w(__builtin_bit_cast(f16x8, v[i % AHEAD]), pr[i / NT], acc[i % NT]);
       if (i + AHEAD < NV) v[i % AHEAD] = value(i + AHEAD);
-      if (i % 2) {   // D / 16 halves of pieces
-        const int x = i / 2;
+#pragma unroll
+      for (int x = i * 4 * RAW / NV; x < (i + 1) * 4 * RAW / NV; x++) {   // halves of pieces
         if (x < 2 * RAW) widen_key(kto, x / 2, x % 2, T());
         else widen_value(vto, left, (x - 2 * RAW) / 2, x % 2, f16());
       }
@@ -933,8 +937,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend4_wide_kernel(Att
 #pragma unroll
     for (int i = 0; i < 5; i++) pages[i] = entry(p0 + i);
     constexpr bool EXACT = __is_same(T, bf16);   // keys of any scale are what they are
-    const auto keys_at = [&](int i) __attribute__((always_inline)) { load(a.k, a.ks, place(pages[i]), kraw); };
-    const auto values_at = [&](int i) __attribute__((always_inline)) { load(a.v, a.vs, place(pages[i]), vraw); };
+    const auto keys_at = [&](int i) __attribute__((always_inline)) { load(a.k, a.ks, place(pages[i]), tid, kraw); };
+    const auto values_at = [&](int i) __attribute__((always_inline)) { load(a.v, a.vs, place(pages[i]), vid, vraw); };
     int p = p0;
     Scores s0, s1;
     Check kc0, kc1, vc0, vc1;   // of the keys and values that this round and the next one widen
@@ -1068,8 +1072,8 @@ int launch_d(const Attend4Args& a, int batch, hipStream_t st) {
   const dim3 grid((unsigned)a.splits * (unsigned)(a.H * ((a.rows + a.tile - 1) / a.tile)), 1, (unsigned)batch);
   if (a.tile == 16) {
     hipLaunchKernelGGL((attend4_kernel<T, D>), grid, dim3(64 * kWaves4), 0, st, a);
-  } else if constexpr (D >= 64) {
-    if (int rc = launch_wide<T, D>(a, grid, st)) return rc;
+  } else if (int rc = launch_wide<T, D>(a, grid, st)) {
+    return rc;
   }
   launch_join<T, D>(a, (int64_t)batch * a.H * a.rows, st);
   return check_launch("cache4_attention");
@@ -1133,16 +1137,16 @@ Plan plan_of(const ldx_cache4_attention_args* p) {
   const int D = p->cache.head_dim;
   // A page of 16 rows is a unit of work. Sharing pages is ahead from about 40,000 of them on, at head width 256 from half of
   // that where there are groups of rows enough to fill the card: 4 heads of 2,048 rows behind 4,096 tokens (37,000) 36 and
-  // 35 us shared at 64, 50 and 51 at 128, behind 16,384 118 and 68 at 64; 8 heads of 2,048 behind 1,024 (25,000) 27 and 30,
-  // 38 and 40, 88 and 72 at 256, 512 rows of 4 heads behind 16,384 (33,000) 39 and 46, 51 and 67, 110 and 130. At 32 the
-  // codes of a page are so few that there is nothing to share.
+  // 35 us shared at 64, 50 and 51 at 128, 30 and 28 at 32, behind 16,384 118 and 68 at 64, 98 and 57 at 32; 8 heads of 2,048
+  // behind 1,024 (25,000) 27 and 30, 38 and 40, 23 and 23, 88 and 72 at 256, 512 rows of 4 heads behind 16,384 (33,000) 39
+  // and 46, 51 and 67, 33 and 41, 110 and 130.
   const int64_t groups = heads * ((rows + kWideRows - 1) / kWideRows), work = heads * ((rows + 15) / 16) * p->width;
-  plan.wide = D >= 64 && rows >= kWideRows && work >= (D == 256 && groups >= 64 ? 20000 : 40000);
+  plan.wide = rows >= kWideRows && work >= (D == 256 && groups >= 64 ? 20000 : 40000);
   int64_t s = 1;
   if (plan.wide) {
     // Rounds of workgroups on the CUs' places, the pages of a round, and what a part more costs: 3 pages of a round
     // to join, or what it writes and the join reads, at 4.5 TB/s and 2.2 us a page of a round.
-    const int64_t places = D <= 128 ? 512 : 256;
+    const int64_t places = D == 32 ? 768 : D <= 128 ? 512 : 256;
     const double traffic = 8e-7 * (double)(heads * rows) * (D + 2), part = traffic > 3.0 ? traffic : 3.0;
     double best = 1e30;
     for (int64_t i = 1; i <= kFewParts && i <= most; i++) {

@@ -639,7 +639,7 @@ def longer(table: torch.Tensor, width: int | None) -> torch.Tensor:
 @pytest.mark.parametrize("d", DIMS)
 def test_attention_kernels_of_the_tested_widths(pkg, d) -> None:
     """From 128 rows of a cache head on a table of LONG columns takes the kernel that shares pages, for any number of
-    heads and sequences; fewer rows, the tests' short tables and heads of 32 the streaming one."""
+    heads and sequences; fewer rows and the tests' short tables the streaming one."""
     lib = pkg._lib
 
     def rows(batch, heads, group, q_len, width):
@@ -648,7 +648,7 @@ def test_attention_kernels_of_the_tested_widths(pkg, d) -> None:
         return lib.lib.ldx_cache4_attention_rows(ctypes.byref(a))
 
     for batch, heads, group, q_len in ((1, 1, 1, 128), (7, 1, 3, 50), (1, 1, 2, 70), (4, 2, 1, 150), (2, 2, 2, 100), (1, 1, 1, 300)):
-        assert rows(batch, heads, group, q_len, LONG) == (16 if d == 32 else 128)
+        assert rows(batch, heads, group, q_len, LONG) == 128
         assert rows(1, heads, group, q_len, 8) == rows(batch, heads, group, 127 // group, LONG) == 16
     assert rows(1, 3, 1, 0, 8) == lib.LDX_EINVAL
 
@@ -754,7 +754,7 @@ def test_attention_causal(pkg, dev, heads, group, lq, d, t) -> None:
 
 @gpu
 @pytest.mark.parametrize("t", HALF)
-@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("d", DIMS)
 @pytest.mark.parametrize(("heads", "group", "lq"), [(1, 1, 128), (2, 1, 129), (1, 3, 50), (2, 4, 65)])
 def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
     """128 rows of a cache head and more: the last tile with one row, or full; lengths and starts as above; values whose
@@ -767,7 +767,7 @@ def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
 
 
 @gpu
-@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("d", DIMS)
 def test_attention_of_many_rows_in_parts(pkg, dev, d) -> None:
     """Sequences of unequal lengths spread over several workgroups, some of which find nothing to do."""
     attention_case(pkg, dev, torch.float16, 3, 1, 2, d, 70, ints(5000, 700, 1), None, 80, long=LONG)
@@ -776,7 +776,7 @@ def test_attention_of_many_rows_in_parts(pkg, dev, d) -> None:
 
 @gpu
 @pytest.mark.parametrize("t", HALF)
-@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("d", DIMS)
 def test_attention_of_pages_beyond_fp16(pkg, dev, d, t) -> None:
     """Single blocks whose scales fp16 does not hold, of keys or values, in the first, a middle or the last page: shared
     pages go another way from there on."""
