@@ -1029,21 +1029,22 @@ def test_attention_says_when_a_page_or_a_length_is_wrong(pkg, dev, lq, long) -> 
 
 
 @gpu
+@pytest.mark.parametrize("d", [32, 64])
 @pytest.mark.parametrize(("lq", "width"), [(1, 9), (70, 9), (140, LONG), (1, 300)])
-def test_attention_layouts(pkg, dev, lq, width) -> None:
+def test_attention_layouts(pkg, dev, lq, width, d) -> None:
     """Head-interleaved q and out, a table that is part of a wider one, out given."""
-    cache, _, table = filled(pkg, dev, 2, 2, 64, 5, seed=1)
-    q = rand((2, 4, lq, 64), 2, torch.bfloat16).to(dev)
+    cache, _, table = filled(pkg, dev, 2, 2, d, 5, seed=1)
+    q = rand((2, 4, lq, d), 2, torch.bfloat16).to(dev)
     lengths = ints(300, 90).to(dev)
     wide = torch.full((2, width), -1, dtype=torch.int32)
     wide[:, 2:7] = table
     want = pkg.ops.cache4_attention(q, cache, wide.to(dev)[:, 2:width - 2].contiguous(), lengths, 0.1)
     inter = q.transpose(1, 2).contiguous().transpose(1, 2)
-    buf = torch.zeros(2, lq, 4, 64 + 3, dtype=torch.bfloat16, device=dev)
-    out = buf[..., 1:65].transpose(1, 2)
+    buf = torch.zeros(2, lq, 4, d + 3, dtype=torch.bfloat16, device=dev)
+    out = buf[..., 1:d + 1].transpose(1, 2)
     got = pkg.ops.cache4_attention(inter, cache, wide.to(dev)[:, 2:width - 2], lengths, 0.1, out=out)
     assert got is out and torch.equal(out, want)
-    assert (buf[..., 0] == 0).all() and (buf[..., 65:] == 0).all()
+    assert (buf[..., 0] == 0).all() and (buf[..., d + 1:] == 0).all()
 
 
 @gpu
@@ -1188,6 +1189,36 @@ def test_captured_step_replays_with_new_inputs(pkg, dev) -> None:
         want = step(caches[0], x[:, 130 + i:131 + i], now, now + 1)
         assert torch.equal(y, want[0]) and torch.equal(held, want[1]), i
         assert torch.equal(caches[0].v, caches[1].v) and torch.equal(caches[0].k, caches[1].k)
+
+
+@gpu
+@pytest.mark.parametrize("d", [32, 128])
+def test_captured_prompt_replays_at_other_places(pkg, dev, d) -> None:
+    """Two graphs of the kernel that shares pages, with and without parts, replayed in turn: queries, starts and lengths
+    come from device memory."""
+    cache, _, table = filled(pkg, dev, 2, 1, d, 40, seed=2)
+    tables2 = [longer(table, LONG).to(dev), longer(table[:1], LONG).to(dev)]
+    queries = [rand((b, 2, 150, d), 3 + b, torch.float16).to(dev) for b in (2, 1)]
+    starts = [torch.zeros(b, dtype=torch.int32, device=dev) for b in (2, 1)]
+    ends = [s + 150 for s in starts]
+    run = lambda i: pkg.ops.cache4_attention(queries[i], cache, tables2[i], ends[i], 0.1, starts=starts[i])
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        run(0), run(1)
+    torch.cuda.current_stream().wait_stream(warm)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], [None, None]
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], pool=graphs[0].pool() if i else None):
+            outs[i] = run(i)
+    for n, at in enumerate((0, 700, 2400, 63, -20)):
+        for i in range(2):
+            starts[i].fill_(at)
+            ends[i].fill_(max(at, 0) + 150 - n)
+            queries[i].mul_(-1.5 if n % 2 else 0.75)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], run(i)), (n, i)
 
 
 @gpu
