@@ -1135,13 +1135,14 @@ Plan plan_of(const ldx_cache4_attention_args* p) {
   const int64_t most = (p->width + kLeastChunk - 1) / kLeastChunk;
   Plan plan;
   const int D = p->cache.head_dim;
-  // A page of 16 rows is a unit of work. Sharing pages is ahead from about 40,000 of them on, at head width 256 from half of
-  // that where there are groups of rows enough to fill the card: 4 heads of 2,048 rows behind 4,096 tokens (37,000) 36 and
-  // 35 us shared at 64, 50 and 51 at 128, 30 and 28 at 32, behind 16,384 118 and 68 at 64, 98 and 57 at 32; 8 heads of 2,048
-  // behind 1,024 (25,000) 27 and 30, 38 and 40, 23 and 23, 88 and 72 at 256, 512 rows of 4 heads behind 16,384 (33,000) 39
-  // and 46, 51 and 67, 33 and 41, 110 and 130.
+  // A page of 16 rows is a unit of work. Sharing pages is ahead from about 40,000 of them on, at head width 256, where a page
+  // costs more to widen, earlier the more groups of rows there are for the CUs. A causal call's us shared and streamed at head
+  // widths 32, 64, 128 and 256: 8 heads of 512 rows behind 8,000 tokens (34,000 units, 32 groups) 31 32, 38 38, 51 51, 96 103;
+  // 4 of 1,900 behind 2,000 (29,000, 60) 27 26, 31 30, 45 41, 84 89, behind 4,000 (44,000) 34 35, 41 43, 57 59, 109 124;
+  // 15 of 1,024 behind 500 (23,000, 120) 22 22, 28 25, 39 37, 70 80; 1 of 1,900 behind 16,000 (33,000, 15) 45 34, 50 39,
+  // 69 52, 140 109.
   const int64_t groups = heads * ((rows + kWideRows - 1) / kWideRows), work = heads * ((rows + 15) / 16) * p->width;
-  plan.wide = rows >= kWideRows && work >= (D == 256 && groups >= 64 ? 20000 : 40000);
+  plan.wide = rows >= kWideRows && work >= (D < 256 || groups < 32 ? 40000 : groups < 64 ? 28000 : 20000);
   int64_t s = 1;
   if (plan.wide) {
     // Rounds of workgroups on the CUs' places, the pages of a round, and what a part more costs: 3 pages of a round
@@ -1157,9 +1158,12 @@ Plan plan_of(const ldx_cache4_attention_args* p) {
   } else {
     // Two workgroups for each CU: a query of 8 x 4 heads for each of 32 sequences of up to 16,384 tokens 83 us with the join
     // at 128 and 56 at 64, with four 84 and 57, with eight 86 and 54, with one 97 and 73; 16 of 256 behind 8,192 55, 58, 67
-    // and 86. Below 32 pages a join costs more than it saves: a query of 8 heads behind 2,040 tokens 10.5 us at 64 and 12 at
-    // 128 in parts, 12.7 and 16 in one; behind 1,000 tokens 9.7 and 11.6, 8.8 and 10.7.
-    s = 512 / (heads * ((rows + 15) / 16));
+    // and 86. Where that leaves one to some CUs and two to others, each in two parts, three to a CU: 300 heads behind up to
+    // 5,000 tokens 45 and 40 us at 128, 31 and 30 at 64, 95 and 87 at 256, 400 52 and 50, 37 and 33, 106 and 100, 470 52 and 54,
+    // 37 and 39, 118 and 125. Below 32 pages a join costs more than it saves: a query of 8 heads behind 2,040 tokens 10.5 us
+    // at 64 and 12 at 128 in parts, 12.7 and 16 in one; behind 1,000 tokens 9.7 and 11.6, 8.8 and 10.7.
+    const int64_t units = heads * ((rows + 15) / 16);
+    s = units > 256 && units <= 400 ? 2 : 512 / units;
     if (s > most) s = most;
     if (p->width < 32) s = 1;
   }
