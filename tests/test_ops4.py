@@ -376,6 +376,23 @@ def test_rotate_of_extreme_heads(pkg, dev, t) -> None:
 
 
 @gpu
+@pytest.mark.parametrize(("d", "axes"), [(128, (128,)), (36, (12, 10, 14))])
+def test_rotate_beyond_4_gib(pkg, dev, d, axes) -> None:
+    """Offsets past 32 bits, of values and of bytes: the last tokens are those of a call of their own."""
+    ops, l, heads = pkg.ops, 70_001, 36 * 1024 // d
+    rotary, gamma = ops.Rotary.make(axes, device=dev), torch.linspace(0.5, 2, d, device=dev)
+    q = torch.zeros(1, l, heads, d, dtype=torch.float16, device=dev).transpose(1, 2)
+    assert q.numel() > 2 ** 31
+    tail = rand((1, heads, 40, d), 1, torch.float16).to(dev)
+    q[:, :, -40:] = tail
+    at = torch.arange(l, dtype=torch.int32, device=dev).expand(len(axes), 1, l)
+    at = at[0] if len(axes) == 1 else at
+    want = ops.rotate_heads(tail, None, at[..., -40:], rotary, q_gamma=gamma)
+    got = ops.rotate_heads(q, None, at, rotary, q_gamma=gamma, q_out=q)
+    assert got is q and torch.equal(got[:, :, -40:], want) and not got[:, :, :-40].any()
+
+
+@gpu
 def test_rotate_refuses_on_the_device(pkg, dev) -> None:
     ops = pkg.ops
     q = torch.zeros(1, 2, 3, 64, dtype=torch.float16, device=dev)
@@ -733,7 +750,7 @@ def attention_case(pkg, dev, t, b, heads, group, d, lq, lengths, starts, width, 
 @gpu
 @pytest.mark.parametrize("t", HALF)
 @pytest.mark.parametrize("d", DIMS)
-@pytest.mark.parametrize(("heads", "group", "lq"), [(1, 1, 1), (2, 4, 1), (3, 1, 5), (1, 8, 3), (2, 2, 40), (1, 3, 150)])
+@pytest.mark.parametrize(("heads", "group", "lq"), [(1, 1, 1), (2, 4, 1), (3, 1, 5), (1, 8, 3), (2, 2, 40), (1, 3, 150), (1, 40, 1)])
 def test_attention_matches_float64(pkg, dev, heads, group, lq, d, t) -> None:
     """Lengths of none, one, page ends and their neighbours; NaN behind every length."""
     lengths = ints(0, 1, 63, 64, 65, 300, 448)
@@ -755,7 +772,7 @@ def test_attention_causal(pkg, dev, heads, group, lq, d, t) -> None:
 @gpu
 @pytest.mark.parametrize("t", HALF)
 @pytest.mark.parametrize("d", DIMS)
-@pytest.mark.parametrize(("heads", "group", "lq"), [(1, 1, 128), (2, 1, 129), (1, 3, 50), (2, 4, 65)])
+@pytest.mark.parametrize(("heads", "group", "lq"), [(1, 1, 128), (2, 1, 129), (1, 3, 50), (2, 4, 65), (1, 130, 1)])
 def test_attention_of_many_rows(pkg, dev, heads, group, lq, d, t) -> None:
     """128 rows of a cache head and more: the last tile with one row, or full; lengths and starts as above; values whose
     scales fp16 holds in all pages, and in some."""
