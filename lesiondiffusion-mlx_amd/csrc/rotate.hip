@@ -180,8 +180,10 @@ __device__ __forceinline__ void section_of(const RotateArgs& a, int pair, int& l
     }
 }
 
-// 1 / sqrt(mean(x^2) + eps) of a head whose N values a lane's f are a part of. Values whose squares pass fp32 are made
-// 2^-66 of themselves first.
+// 1 / sqrt(mean(x^2) + eps) of a head whose N values a lane's f are a part of. Where the sum of squares passes fp32, values
+// are squared at 2^-70 of themselves (512 squares of fp32's largest number make 2^125; the largest value is 2^59 or more, so
+// what is lost below does not count), and the values, which the root goes to, are made 2^-16 of themselves, so that the root
+// stays a normal number: it is at least 2^-128 of fp32's largest value, 2^-112 then.
 template <int N>
 __device__ __forceinline__ float root_of(const RotateArgs& a, float (&f)[N]) {
   float sum = 0.f;
@@ -192,10 +194,11 @@ __device__ __forceinline__ float root_of(const RotateArgs& a, float (&f)[N]) {
   sum = 0.f;   // (or NaN)
 #pragma unroll
   for (int i = 0; i < N; i++) {
-    f[i] *= 0x1p-66f;
-    sum = __builtin_fmaf(f[i], f[i], sum);
+    const float x = f[i] * 0x1p-70f;
+    sum = __builtin_fmaf(x, x, sum);
+    f[i] *= 0x1p-16f;
   }
-  return __builtin_amdgcn_rsqf(head_sum(sum, a.lanes) * a.per);
+  return __builtin_amdgcn_rsqf(head_sum(sum, a.lanes) * a.per) * 0x1p-54f;
 }
 
 // Pairs that lie well: lane u of a head takes pairs (u + i * lanes) V .., i < NU; neighbours (NEAR) or halves of a section.

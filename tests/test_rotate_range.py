@@ -1,0 +1,35 @@
+"""``rotate_heads`` at the ends of its types' ranges, compared with float64: heads of the largest values."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_ops4 import check_rotated, ints, rand
+
+gpu = pytest.mark.gpu
+WIDE = [torch.bfloat16, torch.float32]   # the types whose values' squares pass fp32
+
+# Heads whose halves, or whose sections' halves, divide by 8, 4, 2 and nothing, of one unit a lane and of several.
+PLANS = [((2,), 2), ((32,), 32), ((8, 12, 12), 32), ((36,), 36), ((64,), 64), ((16, 30, 30), 80), ((128,), 128),
+         ((256,), 256), ((512,), 512), ((254, 6, 250), 510), ((252, 8, 248), 508)]
+
+
+@gpu
+@pytest.mark.parametrize("t", WIDE)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize(("axes", "d"), PLANS)
+def test_norm_of_heads_of_the_largest_values(pkg, dev, axes, d, interleaved, t) -> None:
+    """Every channel the type's largest number of either sign; 2^127, 2^126, 2^64 and 2^60 (squares that pass fp32 only in a
+    wide head) times ordinary numbers, held at the type's end; one large channel among ordinary ones."""
+    rotary, most = pkg.ops.Rotary.make(axes, interleaved=interleaved), torch.finfo(t).max
+    x = rand((1, 7, 3, d), 1).double()
+    x[0, 0] = torch.where(x[0, 0] < 0, -most, most)
+    for i, e in enumerate((127, 126, 64, 60)):
+        x[0, 1 + i] *= 2.0 ** e
+    x[0, 5, :, d // 2] = -most
+    x = x.clamp(-most, most).to(t)
+    at = ints(0, 3, -1000).expand(len(axes), 1, 3)
+    gamma = 1 + rand((d,), 3, scale=0.2)
+    got = pkg.ops.rotate_heads(x.to(dev), None, at.to(dev), rotary, q_gamma=gamma.to(dev))
+    check_rotated(got, x, gamma, 1e-6, at, rotary)
