@@ -180,8 +180,8 @@ __device__ __forceinline__ void section_of(const RotateArgs& a, int pair, int& l
     }
 }
 
-// 1 / sqrt(mean(x^2) + eps) of a head whose N values a lane's f are a part of. Where the sum of squares passes fp32, values
-// are squared at 2^-70 of themselves (512 squares of fp32's largest number make 2^125; the largest value is 2^59 or more, so
+// 1 / sqrt(mean(x^2) + eps) of a head whose N values a lane's f are a part of. Where that sum passes fp32, values are squared
+// at 2^-70 of themselves (512 squares of fp32's largest number make 2^125; values, or the root of eps, are 2^59 or more, so
 // what is lost below does not count), and the values, which the root goes to, are made 2^-16 of themselves, so that the root
 // stays a normal number: it is at least 2^-128 of fp32's largest value, 2^-112 then.
 template <int N>
@@ -189,8 +189,8 @@ __device__ __forceinline__ float root_of(const RotateArgs& a, float (&f)[N]) {
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; i++) sum = __builtin_fmaf(f[i], f[i], sum);
-  sum = head_sum(sum, a.lanes);
-  if (sum <= 3.0e38f) return __builtin_amdgcn_rsqf(__builtin_fmaf(sum, a.per, a.eps));
+  const float mean = __builtin_fmaf(head_sum(sum, a.lanes), a.per, a.eps);
+  if (mean < __builtin_inff()) return __builtin_amdgcn_rsqf(mean);
   sum = 0.f;   // (or NaN)
 #pragma unroll
   for (int i = 0; i < N; i++) {
@@ -198,7 +198,7 @@ __device__ __forceinline__ float root_of(const RotateArgs& a, float (&f)[N]) {
     sum = __builtin_fmaf(x, x, sum);
     f[i] *= 0x1p-16f;
   }
-  return __builtin_amdgcn_rsqf(head_sum(sum, a.lanes) * a.per) * 0x1p-54f;
+  return __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum(sum, a.lanes), a.per, a.eps * 0x1p-70f * 0x1p-70f)) * 0x1p-54f;
 }
 
 // Pairs that lie well: lane u of a head takes pairs (u + i * lanes) V .., i < NU; neighbours (NEAR) or halves of a section.

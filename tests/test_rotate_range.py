@@ -33,3 +33,19 @@ def test_norm_of_heads_of_the_largest_values(pkg, dev, axes, d, interleaved, t) 
     gamma = 1 + rand((d,), 3, scale=0.2)
     got = pkg.ops.rotate_heads(x.to(dev), None, at.to(dev), rotary, q_gamma=gamma.to(dev))
     check_rotated(got, x, gamma, 1e-6, at, rotary)
+
+
+@gpu
+@pytest.mark.parametrize("t", WIDE)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize(("axes", "d"), PLANS)
+def test_norm_with_an_eps_beside_large_squares(pkg, dev, axes, d, interleaved, t) -> None:
+    """An eps of the size of the mean square, where the squares' sum, or the mean with eps, passes fp32."""
+    rotary = pkg.ops.Rotary.make(axes, interleaved=interleaved)
+    x = rand((1, 5, 3, d), 1)
+    for i, e in enumerate((0, 60, 62.5, 63.5, 66)):
+        x[0, i] *= 2.0 ** e
+    x, at, gamma = x.to(t), ints(0, 3, -1000).expand(len(axes), 1, 3), 1 + rand((d,), 3, scale=0.2)
+    for eps in (1e36, 3e38):
+        got = pkg.ops.rotate_heads(x.to(dev), None, at.to(dev), rotary, q_gamma=gamma.to(dev), eps=eps)
+        check_rotated(got, x, gamma, torch.tensor(eps, dtype=torch.float32).double(), at, rotary)
