@@ -180,10 +180,11 @@ __device__ __forceinline__ void section_of(const RotateArgs& a, int pair, int& l
     }
 }
 
-// 1 / sqrt(mean(x^2) + eps) of a head whose N values a lane's f are a part of. Where that sum passes fp32, values are squared
-// at 2^-70 of themselves (512 squares of fp32's largest number make 2^125; values, or the root of eps, are 2^59 or more, so
-// what is lost below does not count), and the values, which the root goes to, are made 2^-16 of themselves, so that the root
-// stays a normal number: it is at least 2^-128 of fp32's largest value, 2^-112 then.
+// 1 / sqrt(mean(x^2) + eps) of a head whose N values a lane's f are a part of; it goes to the values before gamma does, since
+// it may leave fp32 with gamma alone. Where the mean with eps passes fp32, values are squared at 2^-70 of themselves (512
+// squares of fp32's largest number make 2^125; values, or the root of eps, are 2^59 or more, so what is lost below does not
+// count), and the values, which the root goes to, are made 2^-16 of themselves, so that the root stays a normal number: it is
+// at least 2^-128 of fp32's largest value, 2^-112 then.
 template <int N>
 __device__ __forceinline__ float root_of(const RotateArgs& a, float (&f)[N]) {
   float sum = 0.f;
@@ -260,8 +261,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
       for (int i = 0; i < NU; i++)
 #pragma unroll
         for (int v = 0; v < V; v++) {
-          f[2 * i * V + v] *= root * gamma[i].a.v[v];
-          f[(2 * i + 1) * V + v] *= root * gamma[i].b.v[v];
+          f[2 * i * V + v] = f[2 * i * V + v] * root * gamma[i].a.v[v];
+          f[(2 * i + 1) * V + v] = f[(2 * i + 1) * V + v] * root * gamma[i].b.v[v];
         }
     }
     T* q = y + base[1][n] + h * a.ys[w.which][2];
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(256) void rotate_mixed_kernel(RotateArgs a) {
     if (norm) {
       const float root = root_of(a, f);
 #pragma unroll
-      for (int i = 0; i < NU * C; i++) f[i] *= root * gamma[i / C].v[i % C];
+      for (int i = 0; i < NU * C; i++) f[i] = f[i] * root * gamma[i / C].v[i % C];
     }
 #pragma unroll
     for (int i = 0; i < NU * C; i++) mine[i * 64 + lane] = f[i];

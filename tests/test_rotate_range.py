@@ -49,3 +49,18 @@ def test_norm_with_an_eps_beside_large_squares(pkg, dev, axes, d, interleaved, t
     for eps in (1e36, 3e38):
         got = pkg.ops.rotate_heads(x.to(dev), None, at.to(dev), rotary, q_gamma=gamma.to(dev), eps=eps)
         check_rotated(got, x, gamma, torch.tensor(eps, dtype=torch.float32).double(), at, rotary)
+
+
+@gpu
+@pytest.mark.parametrize("t", WIDE)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize(("axes", "d"), PLANS)
+def test_norm_with_gammas_far_from_one(pkg, dev, axes, d, interleaved, t) -> None:
+    """Small heads times a large gamma and large ones times a small gamma: the root times gamma leaves fp32, the result does
+    not."""
+    rotary = pkg.ops.Rotary.make(axes, interleaved=interleaved)
+    at = ints(0, 3, -1000).expand(len(axes), 1, 3)
+    for size, factor in ((2.0 ** -60, 2.0 ** 90), (2.0 ** 60, 2.0 ** -90), (2.0 ** 120, 2.0 ** -50), (1.0, 2.0 ** 120)):
+        x, gamma = (rand((1, 2, 3, d), 1) * size).to(t), (1 + rand((d,), 3, scale=0.2)) * factor
+        got = pkg.ops.rotate_heads(x.to(dev), None, at.to(dev), rotary, q_gamma=gamma.to(dev), eps=1e-30)
+        check_rotated(got, x, gamma, torch.tensor(1e-30, dtype=torch.float32).double(), at, rotary)
