@@ -134,6 +134,10 @@ struct Ends {
   }
 };
 
+// In a cosine's place for channels behind the sections. They are passed through: 0 times an infinity or a NaN of the channel
+// that is paired with them is not 0, and zeros keep their sign.
+constexpr float kStay = 2.f;
+
 // What a workgroup is to do: a part of the tokens, all heads of the queries or of the keys.
 struct Part {
   int which, heads, count;
@@ -157,7 +161,7 @@ __device__ __forceinline__ void prepare(const RotateArgs& a, const Part& w, int6
   for (int e = threadIdx.x; e < w.count * a.pairs; e += 256) {
     const int n = udiv(e, a.by_pairs), pair = e - n * a.pairs;
     const int b = udiv((int)(w.first + n), a.by_L), l = (int)(w.first + n) - b * a.L;
-    float c = 1.f, s = 0.f;
+    float c = kStay, s = 0.f;
     if (pair < a.section[a.axes]) {
       int axis = 0;
 #pragma unroll
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     table[1][n * a.pairs + pair] = s;
   });
   Ends<float, V, NEAR> gamma[NU];
-  const bool norm = a.gamma[w.which] != nullptr;
+  const bool norm = a.gamma[w.which] != nullptr, stay = a.section[a.axes] < a.pairs;
   if (norm)
 #pragma unroll
     for (int i = 0; i < NU; i++) gamma[i].load(a.gamma[w.which], at[i], to[i]);
@@ -280,6 +284,10 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
         o.a.v[v] = (T)__builtin_fmaf(p, c[v], -(r * s[v]));
         o.b.v[v] = (T)__builtin_fmaf(r, c[v], p * s[v]);
       }
+      if (__builtin_expect(stay, 0))
+#pragma unroll
+        for (int v = 0; v < V; v++)
+          if (c[v] == kStay) o.a.v[v] = (T)f[2 * i * V + v], o.b.v[v] = (T)f[(2 * i + 1) * V + v];
       o.store(q, at[i], to[i]);
     }
 #pragma unroll
@@ -294,9 +302,9 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
 // over the lanes, so that lanes of a section meet different banks).
 template <typename T, int C, int NU>
 __global__ __launch_bounds__(256) void rotate_mixed_kernel(RotateArgs a) {
-  __shared__ __align__(16) float table[2][2 * kMostPairs];   // cosines, sines, by channel
+  constexpr int TABLE = 2 * kMostPairs, OWN = NU * C * 64;
+  __shared__ __align__(16) float lds[2 * TABLE + 4 * OWN];   // cosines and sines by channel, the waves' values
   __shared__ int64_t base[2][kMostPlaces];
-  __shared__ float swap[4][NU * C][64];
   __shared__ int16_t other[512];
   const int tid = threadIdx.x, lane = tid & 63, u = tid & (a.lanes - 1), step = 256 / a.lanes, D = 2 * a.pairs;
   const Part w(a);
@@ -304,10 +312,13 @@ __global__ __launch_bounds__(256) void rotate_mixed_kernel(RotateArgs a) {
     int low, size;
     section_of(a, pair, low, size);
     const int at = low + pair;
-    table[0][n * D + at] = table[0][n * D + at + size] = c;
-    table[1][n * D + at] = -s;
-    table[1][n * D + at + size] = s;
-    if (n == 0) other[at] = (int16_t)(at + size), other[at + size] = (int16_t)at;
+    // A channel that stays is one time itself and its cosine, 1, times -0, which added leaves every number, -0 too, as it is.
+    const bool stay = c == kStay;
+    float* token = lds + n * D;
+    token[at] = token[at + size] = stay ? 1.f : c;
+    token[TABLE + at] = -s;
+    token[TABLE + at + size] = stay ? -s : s;
+    if (n == 0) other[at] = (int16_t)(stay ? -1 : at + size), other[at + size] = (int16_t)(stay ? -1 : at);
   });
   bool in[NU];
   int at[NU];
@@ -322,12 +333,13 @@ __global__ __launch_bounds__(256) void rotate_mixed_kernel(RotateArgs a) {
 #pragma unroll
     for (int i = 0; i < NU; i++) __builtin_memcpy(&gamma[i], a.gamma[w.which] + at[i], sizeof(gamma[i]));
   __syncthreads();
-  float* mine = &swap[tid >> 6][0][0];
+  const int own = 2 * TABLE + (tid >> 6) * OWN;
+  const int log = __builtin_ctz(a.lanes);
   int from[NU * C];   // where the other end of a channel stands
 #pragma unroll
   for (int i = 0; i < NU * C; i++) {
-    const int c = other[at[i / C] + i % C], unit = c / C;
-    from[i] = (unit / a.lanes * C + c % C) * 64 + (lane - u) + unit % a.lanes;
+    const int mine = at[i / C] + i % C, c = other[mine], unit = c / C;
+    from[i] = c < 0 ? mine : own + ((unit >> log) * C + c % C) * 64 + (lane - u) + (unit & (a.lanes - 1));
   }
 
   const T* x = (const T*)a.x[w.which];
@@ -354,18 +366,18 @@ __global__ __launch_bounds__(256) void rotate_mixed_kernel(RotateArgs a) {
       for (int i = 0; i < NU * C; i++) f[i] = f[i] * root * gamma[i / C].v[i % C];
     }
 #pragma unroll
-    for (int i = 0; i < NU * C; i++) mine[i * 64 + lane] = f[i];
+    for (int i = 0; i < NU * C; i++) lds[own + i * 64 + lane] = f[i];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     T* q = y + base[1][n] + h * a.ys[w.which][2];
 #pragma unroll
     for (int i = 0; i < NU; i++) {
       if (!in[i]) continue;
       float c[C], s[C];
-      table_n<C>(&table[0][n * D + at[i]], c);
-      table_n<C>(&table[1][n * D + at[i]], s);
+      table_n<C>(lds + n * D + at[i], c);
+      table_n<C>(lds + TABLE + n * D + at[i], s);
       Run<T, C> o;
 #pragma unroll
-      for (int v = 0; v < C; v++) o.v[v] = (T)__builtin_fmaf(f[i * C + v], c[v], mine[from[i * C + v]] * s[v]);
+      for (int v = 0; v < C; v++) o.v[v] = (T)__builtin_fmaf(f[i * C + v], c[v], lds[from[i * C + v]] * s[v]);
       o.stream(q + at[i]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -1,6 +1,9 @@
-"""``rotate_heads`` at the ends of its types' ranges, compared with float64: heads of the largest values."""
+"""``rotate_heads`` at the ends of its types' ranges, compared with float64: heads of the largest values, gammas
+and an eps far from one, and channels that are not turned."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -8,6 +11,7 @@ import torch
 from tests.test_ops4 import check_rotated, ints, rand
 
 gpu = pytest.mark.gpu
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
 WIDE = [torch.bfloat16, torch.float32]   # the types whose values' squares pass fp32
 
 # Heads whose halves, or whose sections' halves, divide by 8, 4, 2 and nothing, of one unit a lane and of several.
@@ -64,3 +68,41 @@ def test_norm_with_gammas_far_from_one(pkg, dev, axes, d, interleaved, t) -> Non
         x, gamma = (rand((1, 2, 3, d), 1) * size).to(t), (1 + rand((d,), 3, scale=0.2)) * factor
         got = pkg.ops.rotate_heads(x.to(dev), None, at.to(dev), rotary, q_gamma=gamma.to(dev), eps=1e-30)
         check_rotated(got, x, gamma, torch.tensor(1e-30, dtype=torch.float32).double(), at, rotary)
+
+
+# Sections that leave channels behind them: in both kernels, of a lane's unit as a whole and in its middle.
+PARTS = [((8,), 24), ((16, 16), 64), ((32,), 128), ((16, 30, 30), 80), ((10, 6), 18), ((24, 24, 16), 72), ((6,), 36),
+         ((2, 2, 2, 2), 14), ((254, 6, 248), 510), ((252, 8, 240), 512), ((2,), 4)]
+
+
+@gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize(("axes", "d"), PARTS)
+def test_channels_behind_the_sections_stay(pkg, dev, axes, d, interleaved, t) -> None:
+    """NaN, infinities and zeros of both signs in channels that are not turned stay in their own; with a norm an infinity
+    makes the other channels zeros, and a NaN all of them NaN."""
+    rotary, w = pkg.ops.Rotary.make(axes, interleaved=interleaved), sum(axes)
+    q, at = rand((1, 9, 3, d), 1, t), ints(0, 3, -1000).expand(len(axes), 1, 3)
+    q[0, 0, :, w], q[0, 1, :, d - 1], q[0, 2, :, (w + d) // 2] = math.inf, -math.inf, math.nan
+    q[0, 3, :, w:] = -0.0
+    q[0, 4, :, w::2] = -0.0
+    q[0, 5, :, w], q[0, 5, :, d - 1] = math.inf, math.nan
+    q[0, 6, :, w:] = torch.finfo(t).max
+    got = pkg.ops.rotate_heads(q.to(dev), None, at.to(dev), rotary).cpu()
+    assert torch.equal(got[..., w:].nan_to_num(7.0, 8.0, 9.0), q[..., w:].nan_to_num(7.0, 8.0, 9.0))
+    there = ~q[..., w:].isnan()
+    assert torch.equal(got[..., w:].signbit()[there], q[..., w:].signbit()[there])
+    finite = torch.where(q.isfinite(), q, 0.0)
+    want = pkg.ops.rotate_heads(finite.to(dev), None, at.to(dev), rotary).cpu()
+    assert torch.equal(got[..., :w], want[..., :w])
+    check_rotated(want, finite, None, 1e-6, at, rotary)
+
+    normed = pkg.ops.rotate_heads(q.to(dev), None, at.to(dev), rotary, q_gamma=torch.ones(d, device=dev)).cpu()
+    assert normed[0, [2, 5]].isnan().all()
+    for h, c in ((0, w), (1, d - 1)):
+        others = [i for i in range(d) if i != c]
+        assert normed[0, h, :, c].isnan().all() and (normed[0, h][:, others] == 0).all()
+    keep = [3, 4, 7, 8] + [6] * (t == torch.float16)   # (beside other types' largest numbers the turned channels are subnormal)
+    check_rotated(normed[:, keep], q[:, keep], torch.ones(d), 1e-6, at, rotary)
+    assert torch.equal(normed[0, 3:5, :, w:].signbit(), q[0, 3:5, :, w:].signbit())
