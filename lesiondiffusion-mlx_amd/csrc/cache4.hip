@@ -797,11 +797,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 32 ? 3 : 2) void attend4_w
 #pragma unroll
     for (int e = 2; e < 16; e++) mx = max3_f(mx, s.t[0][e], s.t[1][e]);
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
-    const float mn = max3_f(m, __builtin_fmaf(__int_as_float(x[0]), scale, -kRaise),
-                            __builtin_fmaf(__int_as_float(x[1]), scale, -kRaise));
+    float mn = max3_f(m, __builtin_fmaf(__int_as_float(x[0]), scale, -kRaise),
+                      __builtin_fmaf(__int_as_float(x[1]), scale, -kRaise));
     // A score goes into the exponential times the scale and unrounded, its reference does not: what the reference's
     // rounding left out, up to 2^-24 of it, moves a query's probabilities by one factor, which must not leave fp16.
-    // Beyond 2^20 scores are rounded first, and the reference never lags.
+    // Beyond 2^20 scores are rounded first, the reference never lags, and it is taken from the largest score as that is
+    // rounded, so that the two are at most 8 apart, whatever number scores are multiples of. (Rounded by itself it would be 16
+    // below, and the probability infinite in fp16, for 7 in 16 of the largest scores from 2^27 to 2^28.)
     const bool far = __any(fabsf(mn) >= 0x1p20f && mn != -__builtin_inff());
     kc = far ? 1.f : scale;
     if (__builtin_expect(far, 0)) {
@@ -809,6 +811,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 32 ? 3 : 2) void attend4_w
       for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) s.t[t][e] *= scale;
+      float a0 = __int_as_float(x[0]) * scale, a1 = __int_as_float(x[1]) * scale;
+      pin_value(a0);   // (or the compiler makes one rounding of the two)
+      pin_value(a1);
+      mn = max3_f(m, a0 - kRaise, a1 - kRaise);
     }
     float ref = m == -__builtin_inff() ? 0.f : m;
     if (__any(mn - m > (far ? 0.f : kLag))) {
