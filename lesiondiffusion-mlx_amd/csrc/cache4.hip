@@ -531,10 +531,14 @@ __global__ __launch_bounds__(64 * kWaves4, D == 256 ? 1 : 2) void attend4_kernel
 //
 // A round takes the probabilities of page p between the products that make page p + 1's scores, and page p's values'
 // products between the widening of later pages' codes, an instruction of the matrix units and some of the vector units in
-// turn, so that a wave keeps both busy by itself. (One after the other, 2,048 causal queries of 8 x 4 heads of 128 behind
-// 8,192 tokens 445 us, so 345 to 380, 820 to 900 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 tokens 130 and 7 for the join,
-// of 256 1,160 and 540, of 32 97 and 6, with three waves a SIMD (two 109, four, which spill registers, 160).) Matrix units, vector units and LDS are each busy half of the time then, at the 2.0 GHz that the
-// power allows.
+// turn. (One after the other, 2,048 causal queries of 8 x 4 heads of 128 behind 8,192 tokens 445 us, so 345 to 380, 820 to
+// 900 TF/s; 2,000 of 4 x 4 heads of 64 behind 8,000 tokens 130 and 7 for the join, of 256 1,160 and 540, of 32 97 and 6, with
+// three waves a SIMD (two 109, four, which spill registers, 160).)
+//
+// At head width 64 a page takes a SIMD 1,650 cycles for 32 rows, 515 of which its matrix units work and 880 its vector units. Of
+// the time that a CU is busy its vector units, matrix units and LDS work 67, 20 and 20 % at head width 32, 53, 31 and 27 at 64,
+// 50, 52 and 45 at 128, 33, 27 and 24 at 256 (one wave a SIMD): but at 128 no more than one after the other would. The waves of a
+// workgroup meet at a barrier each page and so run the same part of it at the same time.
 constexpr int kWideRows = 128;
 // A query's reference is this much below its maximum, and lags kLag behind it: probabilities reach 2^15, and fp16 holds
 // those from 2^-21 of the largest on to 2^-11 of themselves and smaller ones to 2^-32 of it, so that many small ones
@@ -1007,7 +1011,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 32 ? 3 : 2) void attend4_w
         if (p < p1 && !odd) round(Const<1>(), s1, s0, kc1, vc1);
       }
     }
-    // From the first page that fp16 does not hold on (and the few before it that are on their way) a page at a time.
+    // From the first page that fp16 does not hold on (and the few before it that are on their way) a page at a time, nothing on
+    // its way: 2,000 fp16 queries of 4 x 4 heads behind 8,000 tokens with such a block of values in none of the pages, the middle
+    // one, the first and all at head width 32 100, 101, 101 and 128 us, at 64 119, 129, 150 and 210, at 128 179, 194, 232 and
+    // 335, at 256 510, 617, 682 and 1,030; of keys the same, and 121, 192, 307 and 870 in all.
     for (; p < p1; p++) {
       pages[0] = entry(p);
       const int64_t at = place(pages[0]);
