@@ -6,7 +6,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_ops4 import DIMS, HALF, LONG, Pages, half_step, ints, longer, rand, tables, tiny
+from tests.test_ops4 import (DIMS, HALF, LONG, Pages, agree, attention_reference, filled, half_step, ints, longer, rand, tables,
+                             tiny)
 
 gpu = pytest.mark.gpu
 
@@ -69,3 +70,36 @@ def test_huge_scores_of_all_channels(pkg, dev, lq, d, t) -> None:
         bar = want.abs() * (half_step(t) + 2.0 ** -10) + tiny(t)
         assert (((got - want).abs() <= bar) | ~sure[..., None]).all(), (scale, got.isnan().any(-1).sum())
         assert (got.abs() <= most * (1 + 2 * half_step(t) + 2.0 ** -10)).all(), scale
+
+
+@gpu
+@pytest.mark.parametrize("t", HALF)
+@pytest.mark.parametrize("d", DIMS)
+@pytest.mark.parametrize(("lq", "long"), [(40, None), (130, LONG)])
+def test_ordinary_queries_beside_those_of_huge_scores(pkg, dev, lq, long, d, t) -> None:
+    """Every third query's scores are 2^21 times the others', and the first page's and a middle one's keys are zeros: the ordinary
+    queries come out as they do alone, the others take their largest key's value."""
+    cache, _, table = filled(pkg, dev, 1, 1, d, 6, seed=d, spread=5)
+    zeros, values = torch.zeros(1, 1, 64, d, device=dev), rand((1, 1, 64, d), 5).to(dev)
+    for slot in (0, 3):
+        pkg.ops.cache4_append(cache, zeros, values, table.to(dev), ints(64 * slot).to(dev))
+    ref, n = Pages(cache), 370
+    q = rand((1, 2, lq, d), 7, t)
+    q[:, :, ::3] *= 2.0 ** 13
+    k, v = ref.read(table[0], n)
+    ordinary = [i for i in range(lq) if i % 3]
+    for scale in (2.0 ** 8, -(2.0 ** 8)):
+        x = q.clone()
+        x[:, :, ordinary] *= 2.0 ** -8
+        got = pkg.ops.cache4_attention(x.to(dev), cache, longer(table, long).to(dev), ints(n).to(dev), scale)
+        want, allowed = attention_reference(ref, x, table, ints(n), scale, None, long is not None)
+        agree(got[:, :, ordinary], want[:, :, ordinary], allowed[:, :, ordinary])
+        s = x[0, :, ::3].double() @ k[0].t().contiguous() * scale
+        off = (2 * d + 6) * 2.0 ** -24 * (x[0, :, ::3].double().abs() @ k[0].t().contiguous().abs() * abs(scale)).amax(-1)
+        top = s.topk(2, -1)
+        sure = top.values[..., 0] - top.values[..., 1] > 2 * off + 40
+        assert sure.double().mean() > 0.9
+        want = v[0][top.indices[..., 0]]
+        bar = want.abs() * (half_step(t) + 2.0 ** -10) + tiny(t)
+        err = (got[0, :, ::3].cpu().double() - want).abs()
+        assert ((err <= bar) | ~sure[..., None]).all() and got.isfinite().all()
