@@ -552,7 +552,7 @@ int ldx_cache8_attention_rows(const ldx_cache8_attention_args* args);
  * turns, turns holding all sections' pairs one after another (fp64; theta^(-2 i / dim) / (2 pi) for
  * the usual frequencies). Angles are reduced in fp64, so that any position has its own; norm and
  * rotation are fp32, rounded once to dtype. q, k and outputs: (batch, token, head) strides in
- * elements, contiguous channels; an output may be its input. positions: int32, device, (axis,
+ * elements, contiguous channels; an output may be its input, and overlaps nothing else. positions: int32, device, (axis,
  * batch, token) strides. k_heads may be 0. head_dim even, at most 512; eps at least 1e-30. Heads
  * whose squares pass fp32 although their values do not are normalised from scaled squares. */
 #define LDX_ROTARY_AXES 4

@@ -13,8 +13,8 @@
 // as they lie, so that every access to memory is of whole lines, and gets the other ends through LDS.
 //
 // Bound by memory: 51,200 tokens of 16 query and 16 key heads of 32 in fp16, three axes, 45 us, 4.7 TB/s; 16,384 of 32 and 8
-// heads of 128 in bf16 64, 5.3, in fp32 141, 4.8, with neighbours 64 and 131. Few heads are bound by the launch (a token's 3.3 us). Queries and keys in the same
-// workgroups, without the next head asked for ahead, took 104 and 78.
+// heads of 128 in bf16 64, 5.3, in fp32 141, 4.8, with neighbours 64 and 131. Few heads are bound by the launch (a token's 3.3
+// us). Queries and keys in the same workgroups, without the next head asked for ahead, took 104 and 78.
 #include "quant8.h"
 
 namespace ldx {

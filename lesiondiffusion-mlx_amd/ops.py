@@ -1219,9 +1219,11 @@ class Rotary:
         """The usual frequencies, ``theta^(-2 i / w)`` for pair ``i`` of an axis of ``w`` channels, times ``scale``
         (of every axis, or one each: positions of a finer or coarser grid than the model's)."""
         axes = (axes,) if isinstance(axes, int) else tuple(axes)
-        scales = scale if isinstance(scale, tuple) else (scale,) * len(axes)
+        scales = tuple(scale) if isinstance(scale, (tuple, list)) else (scale,) * len(axes)
         if not axes or len(scales) != len(axes) or any(w < 2 or w % 2 for w in axes):
             raise ValueError(f"Rotary: axes {axes} must be even widths, with a scale each, got {scales}")
+        if not theta > 0:
+            raise ValueError(f"Rotary: theta {theta} must be above 0")
         turns = [s * theta ** (-2.0 * i / w) / (2 * math.pi) for w, s in zip(axes, scales) for i in range(w // 2)]
         return Rotary(torch.tensor(turns, dtype=torch.float64, device=device), axes, interleaved)
 
@@ -1267,8 +1269,8 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     (axes, B, L) for several (a volume's depth, height and width), any strides, so that one row expanded serves
     the batch; ``rotary`` says how an axis turns (at most four). Angles are reduced in fp64: position 10^9
     has its own. Norm and rotation are fp32, rounded once. Returns ``(q, k)``, or ``q`` without keys, in the
-    inputs' type: into ``q_out`` and ``k_out`` when given, each of which may be its own input, else with a token's heads
-    side by side in memory (``(B, L, H * D)`` is a view)."""
+    inputs' type: into ``q_out`` and ``k_out`` when given, each of which may be its own input and overlaps nothing else of the
+    call, else with a token's heads side by side in memory (``(B, L, H * D)`` is a view)."""
     _need(q, "q", _ALL, -1)
     dev, shape, dtype = q.get_device(), q.shape, q.dtype
     if len(shape) != 4 or not q.numel():

@@ -14,6 +14,17 @@ gpu = pytest.mark.gpu
 TYPES = [torch.float16, torch.bfloat16, torch.float32]
 WIDE = [torch.bfloat16, torch.float32]   # the types whose values' squares pass fp32
 
+
+def test_plans_of_odd_arguments(pkg) -> None:
+    make = pkg.ops.Rotary.make
+    assert torch.equal(make([4, 6], scale=[1.0, 0.5], device="cpu").turns, make((4, 6), scale=(1.0, 0.5), device="cpu").turns)
+    for theta in (0.0, -2.0, math.nan):
+        with pytest.raises(ValueError, match="theta"):
+            make(8, theta=theta, device="cpu")
+    with pytest.raises(ValueError, match="scale"):
+        make((4, 6), scale=[1.0], device="cpu")
+
+
 # Heads whose halves, or whose sections' halves, divide by 8, 4, 2 and nothing, of one unit a lane and of several.
 PLANS = [((2,), 2), ((32,), 32), ((8, 12, 12), 32), ((36,), 36), ((64,), 64), ((16, 30, 30), 80), ((128,), 128),
          ((256,), 256), ((512,), 512), ((254, 6, 250), 510), ((252, 8, 248), 508)]
